@@ -3,6 +3,7 @@
 #include "../../include/kq4.h"
 #include "kq4_common.h"
 #include "kq4_internal.h"
+#include "kq4_kv.h"
 
 #include <stdarg.h>
 #include <stdio.h>
@@ -1217,7 +1218,184 @@ int kq4_moe_ffn_stages_dev(float *Y, const float *X, const int *sel, const float
                   (hipStream_t)stream);
 }
 
+}  // extern "C"
+
+// ---- the paged key/value cache, attention, log probabilities ---------------------------------
+
+namespace {
+
+int log2_of(int n) {   // of a power of two, else -1
+  if (n <= 0 || (n & (n - 1))) return -1;
+  int l = 0;
+  while ((1 << l) < n) ++l;
+  return l;
+}
+
+bool kv_shape_ok(int n_pages, int page_tokens, int kv_heads, int head_dim) {
+  const int lp = log2_of(page_tokens);
+  return n_pages >= 1 && lp >= 4 && lp <= 12 && kv_heads >= 1 && kv_heads <= 4096 &&
+         (head_dim == 64 || head_dim == 128);
+}
+
+// The checks that append and attention share; *log_pg = log2(groups of a page).
+int kv_check(const char *what, const kq4_kv *kv, int *log_pg) {
+  if (!kv) return fail(KQ4_EINVAL, "%s: null cache", what);
+  if (!kv_shape_ok(kv->n_pages, kv->page_tokens, kv->kv_heads, kv->head_dim))
+    return fail(KQ4_EINVAL, "%s: n_pages=%d page_tokens=%d (a power of two, 16..4096) kv_heads=%d head_dim=%d "
+                "(64 or 128)", what, kv->n_pages, kv->page_tokens, kv->kv_heads, kv->head_dim);
+  if (kv->n_seq < 0 || kv->n_tok < 0 || kv->table_pages < 1 ||
+      (long long)kv->table_pages * kv->page_tokens > 0x7fffffffLL - 65536)
+    return fail(KQ4_EINVAL, "%s: n_seq=%d n_tok=%d table_pages=%d", what, kv->n_seq, kv->n_tok,
+                kv->table_pages);
+  if ((kv->rope != nullptr) != (kv->rope_dim != 0) || kv->rope_dim < 0 || kv->rope_dim % 32 ||
+      kv->rope_dim > kv->head_dim || (kv->rope && kv->rope_rows < 1))
+    return fail(KQ4_EINVAL, "%s: rope_dim=%d (a multiple of 32, at most head_dim, 0 with a null table) "
+                "rope_rows=%d", what, kv->rope_dim, kv->rope_rows);
+  if (kv->n_seq && kv->n_tok) {
+    if (!kv->codes || !kv->scales || !kv->block_table || !kv->q_start || !kv->kv_len)
+      return fail(KQ4_EINVAL, "%s: null cache or batch pointer", what);
+    if ((uintptr_t)kv->codes % 16 || (uintptr_t)kv->scales % 8 || (uintptr_t)kv->rope % 8 ||
+        (uintptr_t)kv->block_table % 4 || (uintptr_t)kv->q_start % 4 || (uintptr_t)kv->kv_len % 4 ||
+        (uintptr_t)kv->rope_pos % 4)
+      return fail(KQ4_EINVAL, "%s: codes must be 16-byte, scales and rope 8-byte, indexes 4-byte aligned", what);
+  }
+  *log_pg = log2_of(kv->page_tokens) - 4;
+  return KQ4_OK;
+}
+
+// Rows of `width` floats at a stride.
+int rows_check(const char *what, const char *name, const float *p, long ld, long width) {
+  if (!p || (uintptr_t)p % 16 || ld < width || ld % 4)
+    return fail(KQ4_EINVAL, "%s: %s must be 16-byte aligned, its stride (%ld) a multiple of 4 and at least %ld",
+                what, name, ld, width);
+  return KQ4_OK;
+}
+
+size_t attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int heads, int head_dim, size_t *o_bytes) {
+  *o_bytes = 0;
+  if (p.ns <= 1) return 0;
+  const size_t rows = (size_t)p.ns * n_tok * heads;
+  *o_bytes = al256(rows * head_dim * sizeof(float));
+  return *o_bytes + al256(rows * 2 * sizeof(float));
+}
+
+size_t logprobs_bytes(int n, int vocab, int n_top, size_t *piece_bytes) {
+  const size_t np = (size_t)n * kq4_logprobs_pieces(vocab);
+  *piece_bytes = al256(np * kq4_logprobs_piece_bytes());
+  return *piece_bytes + al256(np * n_top * sizeof(unsigned long long));
+}
+
+bool logprobs_shape_ok(int n, int vocab, int n_top) {
+  return n >= 0 && vocab >= 1 && vocab <= KQ4_LOGPROBS_MAX_VOCAB && n_top >= 0 && n_top <= KQ4_LOGPROBS_MAX_TOP &&
+         n_top <= vocab && (long long)n * kq4_logprobs_pieces(vocab) <= 0x7fffffffLL;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kq4_kv_codes_bytes(int n_pages, int page_tokens, int kv_heads, int head_dim) {
+  if (!kv_shape_ok(n_pages, page_tokens, kv_heads, head_dim)) return 0;
+  return (size_t)n_pages * page_tokens * kv_heads * head_dim * 2;
+}
+
+size_t kq4_kv_scales_bytes(int n_pages, int page_tokens, int kv_heads, int head_dim) {
+  if (!kv_shape_ok(n_pages, page_tokens, kv_heads, head_dim)) return 0;
+  return (size_t)n_pages * (page_tokens / 16) * kv_heads * 2 * sizeof(float);
+}
+
+int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v, long ldv, void *stream) {
+  int log_pg = 0, rc = kv_check("kv_append", kv, &log_pg);
+  if (rc) return rc;
+  if (!kv->n_seq || !kv->n_tok) return KQ4_OK;
+  const long width = (long)kv->kv_heads * kv->head_dim;
+  if ((rc = rows_check("kv_append", "k", k, ldk, width)) || (rc = rows_check("kv_append", "v", v, ldv, width)))
+    return rc;
+  DevState *ds = nullptr;
+  if ((rc = cur_dev(&ds))) return rc;
+  KQ4_HIP((hipError_t)kq4_launch_kv_append(*kv, log_pg, k, ldk, v, ldv, (hipStream_t)stream));
+  return KQ4_OK;
+}
+
+int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_heads, float scale, int window,
+                 int max_q, int max_kv, void *stream) {
+  int log_pg = 0, rc = kv_check("attn", kv, &log_pg);
+  if (rc) return rc;
+  if (q_heads < 1 || q_heads % kv->kv_heads || window < 0 || max_q < 0 || max_kv < 0 || !(scale > 0.0f) ||
+      scale > 3.0e38f)
+    return fail(KQ4_EINVAL, "attn: q_heads=%d (a multiple of kv_heads=%d) scale=%g (> 0) window=%d max_q=%d "
+                "max_kv=%d", q_heads, kv->kv_heads, scale, window, max_q, max_kv);
+  if (!kv->n_seq || !kv->n_tok) return KQ4_OK;
+  const long width = (long)q_heads * kv->head_dim;
+  if ((rc = rows_check("attn", "q", q, ldq, width)) || (rc = rows_check("attn", "out", out, width, width)))
+    return rc;
+  if ((long long)kv->n_seq * kv->kv_heads > 0x7fffffffLL || (long long)kv->n_tok * q_heads > 0x7fffffffLL)
+    return fail(KQ4_EINVAL, "attn: n_seq=%d n_tok=%d q_heads=%d", kv->n_seq, kv->n_tok, q_heads);
+  const uintptr_t qa = (uintptr_t)q, qe = qa + ((kv->n_tok - 1) * (size_t)ldq + width) * sizeof(float);
+  const uintptr_t oa = (uintptr_t)out, oe = oa + (size_t)kv->n_tok * width * sizeof(float);
+  if (oa < qe && qa < oe) return fail(KQ4_EINVAL, "attn: out overlaps q");
+  DevState *ds = nullptr;
+  if ((rc = cur_dev(&ds))) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  const KQ4AttnPlan plan = kq4_attn_plan(kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, max_q, max_kv);
+  size_t o_bytes = 0;
+  const size_t bytes = attn_part_bytes(plan, kv->n_tok, q_heads, kv->head_dim, &o_bytes);
+  char *ws = nullptr;
+  if (bytes) {
+    if ((rc = ensure_ws(Ws{&ds->ws, ds}, bytes, s))) return rc;
+    ws = static_cast<char *>(ds->ws.p);
+  }
+  KQ4_HIP((hipError_t)kq4_launch_attn(out, *kv, log_pg, q, ldq, q_heads, scale, window, plan,
+                                      reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + o_bytes), s));
+  return KQ4_OK;
+}
+
+size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim, int max_q,
+                                int max_kv) {
+  if (n_tok < 1 || n_seq < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads ||
+      (head_dim != 64 && head_dim != 128) || max_q < 0 || max_kv < 0)
+    return 0;
+  size_t o_bytes = 0;
+  return attn_part_bytes(kq4_attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv), n_tok, q_heads, head_dim,
+                         &o_bytes);
+}
+
+int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *top_id, const float *logits, long ld,
+                     const int *token, int n, int vocab, int n_top, void *stream) {
+  if (!logprobs_shape_ok(n, vocab, n_top) || ld < vocab)
+    return fail(KQ4_EINVAL, "logprobs: n=%d vocab=%d (at most %d) ld=%ld n_top=%d (at most %d and vocab)", n, vocab,
+                KQ4_LOGPROBS_MAX_VOCAB, ld, n_top, KQ4_LOGPROBS_MAX_TOP);
+  if (n == 0) return KQ4_OK;
+  if (!logits || (logprob && !token) || (n_top != 0) != (top_logprob != nullptr) ||
+      (n_top != 0) != (top_id != nullptr) || (!logprob && !entropy && !n_top))
+    return fail(KQ4_EINVAL, "logprobs: logits, token with logprob, top_logprob and top_id with n_top, and one output at "
+                "least are needed");
+  if ((uintptr_t)logits % 4 || (uintptr_t)logprob % 4 || (uintptr_t)entropy % 4 || (uintptr_t)top_logprob % 4 ||
+      (uintptr_t)top_id % 4 || (uintptr_t)token % 4)
+    return fail(KQ4_EINVAL, "logprobs: pointers must be 4-byte aligned");
+  DevState *ds = nullptr;
+  int rc = cur_dev(&ds);
+  if (rc) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  size_t pb = 0;
+  if ((rc = ensure_ws(Ws{&ds->ws, ds}, logprobs_bytes(n, vocab, n_top, &pb), s))) return rc;
+  char *ws = static_cast<char *>(ds->ws.p);
+  KQ4_HIP((hipError_t)kq4_launch_logprobs(logits, ld, n, vocab, n_top, token, logprob, entropy, top_logprob, top_id, ws,
+                                          reinterpret_cast<unsigned long long *>(ws + pb), s));
+  return KQ4_OK;
+}
+
+size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top) {
+  if (n < 1 || !logprobs_shape_ok(n, vocab, n_top)) return 0;
+  size_t pb = 0;
+  return logprobs_bytes(n, vocab, n_top, &pb);
+}
+
+}  // extern "C"
+
 // ---- host-pointer drop-in API ----------------------------------------------------------------
+
+extern "C" {
 
 int kq4_weights_upload(uint64_t wkey, const uint8_t *w4x4, int rows, int cols) {
   if (!wkey || !w4x4 || !shape_ok(rows, cols)) {

@@ -180,3 +180,22 @@ int kq4_launch_moe_dbg(float *Y, const float *X, const int *sel, const float *pr
 int kq4_launch_moe(float *Y, const float *X, const int *sel, const float *pr, int T, int tk,
                    const uint8_t *G, const uint8_t *U, const uint8_t *D, int ne, int d, int ef,
                    const KQ4MoeWs &ws, hipStream_t stream);
+
+// Attention over a paged int8 cache, appending to it (kq4_kv.h has its layout) and the reading of logits.
+struct kq4_kv;
+int kq4_launch_kv_append(const kq4_kv &kv, int log_pg, const float *k, long ldk, const float *v, long ldv,
+                         hipStream_t s);
+// Keys per split and splits at most; part_o holds ns * n_tok * heads * head_dim floats, part_ml two per row
+// and split (none where ns is 1).
+struct KQ4AttnPlan {
+  int chunk, ns;
+};
+KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv);
+int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
+                    int window, const KQ4AttnPlan &plan, float *part_o, float *part_ml, hipStream_t s);
+// Pieces of a row, and a piece's bytes; best holds n * pieces * n_top keys.
+int kq4_logprobs_pieces(int vocab);
+size_t kq4_logprobs_piece_bytes();
+int kq4_launch_logprobs(const float *logits, long ld, int n, int vocab, int n_top, const int *token, float *logprob,
+                        float *entropy, float *top_logprob, int *top_id, void *pieces, unsigned long long *best,
+                        hipStream_t s);

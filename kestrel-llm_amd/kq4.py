@@ -67,6 +67,13 @@ SIGNATURES = [
     ("kq4_moe_layer_dev", _I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P]),
     ("kq4_moe_ffn_stages_dev", _I,
      [_P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P]),
+    ("kq4_kv_codes_bytes", ctypes.c_size_t, [_I, _I, _I, _I]),
+    ("kq4_kv_scales_bytes", ctypes.c_size_t, [_I, _I, _I, _I]),
+    ("kq4_kv_append_dev", _I, [_P, _P, ctypes.c_long, _P, ctypes.c_long, _P]),
+    ("kq4_attn_dev", _I, [_P, _P, _P, ctypes.c_long, _I, ctypes.c_float, _I, _I, _I, _P]),
+    ("kq4_attn_workspace_bytes", ctypes.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
+    ("kq4_logprobs_dev", _I, [_P, _P, _P, _P, _P, ctypes.c_long, _P, _I, _I, _I, _P]),
+    ("kq4_logprobs_workspace_bytes", ctypes.c_size_t, [_I, _I, _I]),
     # C11 op wrappers (include/kq4_ops.h)
     ("kq4_dyn_matvec_q4_q8", _I, [_P, _P, _P, _I, _I]),
     ("kq4_dyn_matvec_q4_q8_fused_gate_up", _I, [_P, _P, _P, _P, _P, _I, _I]),
@@ -711,3 +718,162 @@ class Vqf:
         key = _U64()
         check(lib().kq4_vqf_upload(self._h, proj, layer, ctypes.byref(key)), "kq4_vqf_upload")
         return key.value
+
+
+# ---- paged int8 key/value cache, attention, log probabilities ----------------------------------
+
+LOGPROBS_MAX_TOP, LOGPROBS_MAX_VOCAB = 32, 1 << 20
+
+
+class KV(ctypes.Structure):
+    """kq4_kv (include/kq4.h)."""
+    _fields_ = [("codes", _P), ("scales", _P), ("n_pages", _I), ("page_tokens", _I),
+                ("kv_heads", _I), ("head_dim", _I), ("block_table", _P), ("table_pages", _I),
+                ("q_start", _P), ("kv_len", _P), ("n_seq", _I), ("n_tok", _I), ("rope", _P),
+                ("rope_rows", _I), ("rope_dim", _I), ("rope_pos", _P)]
+
+
+def kv_codes_shape(n_pages, page_tokens, kv_heads, head_dim):
+    """Shape of a cache's uint8 codes; its fp32 scales are [:4] of it (include/kq4.h kq4_kv)."""
+    if lib().kq4_kv_codes_bytes(n_pages, page_tokens, kv_heads, head_dim) == 0:
+        raise KQ4Error(f"bad cache shape: {n_pages} pages of {page_tokens} tokens, {kv_heads} heads "
+                       f"of {head_dim}")
+    return (n_pages, kv_heads, page_tokens // 16, 2, 16 * head_dim)
+
+
+def kv_cache(n_pages, page_tokens, kv_heads, head_dim, device="cuda"):
+    """A new cache's (codes, scales); slots that hold no token are never read, so nothing is cleared."""
+    import torch
+    shape = kv_codes_shape(n_pages, page_tokens, kv_heads, head_dim)
+    return (torch.empty(shape, dtype=torch.uint8, device=device),
+            torch.empty(shape[:4], dtype=torch.float32, device=device))
+
+
+def rope_table(rows, dim, theta, device="cuda"):
+    """fp32 [rows][dim / 2][cos, sin] of the angles row * theta^(-2i / dim), formed in 64 bits (positions
+    far out lose their fraction in 32)."""
+    import torch
+    inv = theta ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    a = torch.arange(rows, dtype=torch.float64)[:, None] * inv
+    return torch.stack([a.cos(), a.sin()], 2).float().contiguous().to(device)
+
+
+def _here(t, name):
+    """Raises unless t is on the current device, which the call's launches go to."""
+    import torch
+    if t is not None and t.device.index != torch.cuda.current_device():
+        raise KQ4Error(f"{name}: on {t.device}, the current device is {torch.cuda.current_device()}")
+
+
+def _rows(t, name, n, width):
+    """Row stride of a [>= n][>= width] fp32 device tensor with unit column stride, checked."""
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise KQ4Error(f"{name}: not a device tensor")
+    if t.dtype != torch.float32:
+        raise KQ4Error(f"{name}: dtype {t.dtype}, expected torch.float32")
+    if t.dim() != 2 or t.shape[0] < n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise KQ4Error(f"{name}: expected [{n}, {width}] with unit column stride, got {tuple(t.shape)} "
+                       f"strides {t.stride()}")
+    _here(t, name)
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+class KVBatch:
+    """A layer's cache and the batch that a call works on (include/kq4.h kq4_kv), checked once: keep it as
+    long as its tensors' addresses and sizes stand, and change their contents (lengths, tables, cache)
+    between calls freely. codes / scales as kv_cache makes them; block_table int32 [n_seq][pages],
+    q_start int32 [n_seq + 1], kv_len int32 [n_seq]; rope as rope_table makes it, its columns the rotated
+    dimensions; rope_pos int32 [n_tok]."""
+
+    def __init__(self, codes, scales, page_tokens, block_table, q_start, kv_len, n_tok, rope=None,
+                 rope_pos=None):
+        import torch
+        if codes.dim() != 5 or codes.shape[4] % 16:
+            raise KQ4Error(f"codes: shape {tuple(codes.shape)}, expected as kv_codes_shape gives it")
+        n_pages, kv_heads, head_dim = codes.shape[0], codes.shape[1], codes.shape[4] // 16
+        shape = kv_codes_shape(n_pages, page_tokens, kv_heads, head_dim)
+        if tuple(codes.shape) != shape or tuple(scales.shape) != shape[:4]:
+            raise KQ4Error(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)}, expected {shape} "
+                           f"and {shape[:4]}")
+        if block_table.dim() != 2 or kv_len.dim() != 1 or kv_len.shape[0] != block_table.shape[0]:
+            raise KQ4Error("block_table [n_seq, pages] and kv_len [n_seq] differ in sequences")
+        n_seq = kv_len.shape[0]
+        _need(codes, "codes", torch.uint8, codes.numel())
+        _need(scales, "scales", torch.float32, scales.numel())
+        _need(block_table, "block_table", torch.int32, block_table.numel())
+        _need(q_start, "q_start", torch.int32, n_seq + 1)
+        _need(kv_len, "kv_len", torch.int32, n_seq)
+        _need(rope_pos, "rope_pos", torch.int32, n_tok, optional=True)
+        if rope is not None:
+            _need(rope, "rope", torch.float32, rope.numel())
+            if rope.dim() != 3 or rope.shape[2] != 2:
+                raise KQ4Error(f"rope: shape {tuple(rope.shape)}, expected [rows, dim / 2, 2]")
+        self.tensors = dict(codes=codes, scales=scales, block_table=block_table, q_start=q_start,
+                            kv_len=kv_len, rope=rope, rope_pos=rope_pos)
+        for name, t in self.tensors.items():
+            if t is not None and t.device != codes.device:
+                raise KQ4Error(f"{name}: on {t.device}, the cache is on {codes.device}")
+        self.n_tok, self.n_seq, self.kv_heads, self.head_dim = n_tok, n_seq, kv_heads, head_dim
+        self.device = codes.device.index
+        self.c = KV(_tp(codes), _tp(scales), n_pages, page_tokens, kv_heads, head_dim, _tp(block_table),
+                    block_table.shape[1], _tp(q_start), _tp(kv_len), n_seq, n_tok, _tp(rope),
+                    0 if rope is None else rope.shape[0], 0 if rope is None else 2 * rope.shape[1],
+                    _tp(rope_pos))
+        self.p = ctypes.addressof(self.c)
+
+
+def kv_append_dev(kv, k, v, stream=None):
+    """Appends the batch's keys (rotated) and values, [n_tok][kv_heads * head_dim] each, to its cache."""
+    width = kv.kv_heads * kv.head_dim
+    ldk, ldv = _rows(k, "k", kv.n_tok, width), _rows(v, "v", kv.n_tok, width)
+    _here(kv.tensors["codes"], "cache")
+    check(lib().kq4_kv_append_dev(kv.p, k.data_ptr(), ldk, v.data_ptr(), ldv, _stream_ptr(stream)),
+          "kq4_kv_append_dev")
+
+
+def attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv):
+    return lib().kq4_attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv)
+
+
+def attn_dev(out, q, kv, q_heads, scale, max_q, max_kv, window=0, stream=None):
+    """out [n_tok][q_heads * head_dim] = attention of q (rotated as it is read) over the batch's cache;
+    max_q / max_kv: the batch's most tokens of a sequence and longest kv_len, or bounds (speed only)."""
+    import torch
+    width = q_heads * kv.head_dim
+    ldq = _rows(q, "q", kv.n_tok, width)
+    _need(out, "out", torch.float32, kv.n_tok * width)
+    _here(out, "out")
+    _here(kv.tensors["codes"], "cache")
+    check(lib().kq4_attn_dev(out.data_ptr(), kv.p, q.data_ptr(), ldq, q_heads, scale, window, max_q,
+                             max_kv, _stream_ptr(stream)), "kq4_attn_dev")
+
+
+def logprobs_workspace_bytes(n, vocab, n_top):
+    return lib().kq4_logprobs_workspace_bytes(n, vocab, n_top)
+
+
+def logprobs_dev(logits, token=None, logprob=None, entropy=None, top_logprob=None, top_id=None,
+                 stream=None):
+    """Log probabilities of token (int32 [n]), entropy and the top alternatives of logits [n][vocab] (fp32,
+    unit column stride) into the outputs given: logprob and entropy [n], top_logprob and top_id [n][n_top]."""
+    import torch
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        raise KQ4Error("logits: expected a [n, vocab] device tensor")
+    n, vocab = logits.shape
+    ld = _rows(logits, "logits", n, vocab)
+    n_top = 0
+    if top_logprob is not None or top_id is not None:
+        if top_logprob is None or top_id is None or top_logprob.dim() != 2 or \
+                top_logprob.shape != top_id.shape or top_logprob.shape[0] != n:
+            raise KQ4Error("top_logprob and top_id: both [n, n_top]")
+        n_top = top_logprob.shape[1]
+    for name, t, dtype, numel in (("token", token, torch.int32, n), ("logprob", logprob, torch.float32, n),
+                                  ("entropy", entropy, torch.float32, n),
+                                  ("top_logprob", top_logprob, torch.float32, n * n_top),
+                                  ("top_id", top_id, torch.int32, n * n_top)):
+        _need(t, name, dtype, numel, optional=True)
+        _here(t, name)
+    check(lib().kq4_logprobs_dev(_tp(logprob), _tp(entropy), _tp(top_logprob), _tp(top_id),
+                                 logits.data_ptr(), ld, _tp(token), n, vocab, n_top,
+                                 _stream_ptr(stream)), "kq4_logprobs_dev")
