@@ -185,10 +185,10 @@ int kq4_launch_moe(float *Y, const float *X, const int *sel, const float *pr, in
 struct kq4_kv;
 int kq4_launch_kv_append(const kq4_kv &kv, int log_pg, const float *k, long ldk, const float *v, long ldv,
                          hipStream_t s);
-// Keys per split and splits at most; part_o holds ns * n_tok * heads * head_dim floats, part_ml two per row
+// Rows of a workgroup's tile (query tokens * heads per kv head), keys per split and splits at most; part_o holds ns * n_tok * heads * head_dim floats, part_ml two per row
 // and split (none where ns is 1).
 struct KQ4AttnPlan {
-  int chunk, ns;
+  int tile, chunk, ns;
 };
 KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv);
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
