@@ -214,7 +214,7 @@ int env_int(const char *name, int dflt) {
 enum OptId {
   kGemvKind, kGemvMfmaFrom, kGemvHs, kGemvRps, kGemvWaves, kGemvWpcu, kGemvMaxw,
   kGemvFq, kGemvFqWork, kGemvSiluFqWork, kGemvChunkMax, kGemmKind, kGemmTile, kGemmSplit,
-  kGemmPrio, kOptCount
+  kGemmPrio, kAttnTile, kAttnSplit, kOptCount
 };
 struct OptDef {
   const char *name, *env;
@@ -230,6 +230,7 @@ const OptDef kOpts[kOptCount] = {
     {"gemv_chunk_max", "KQ4_GEMV_CHUNK_MAX", 16},
     {"gemm_kind", "KQ4_GEMM_KIND", -1},          {"gemm_tile", "KQ4_GEMM_TILE", 0},
     {"gemm_split", "KQ4_GEMM_SPLIT", -1},        {"gemm_prio", "KQ4_GEMM_PRIO", -1},
+    {"attn_tile", "KQ4_ATTN_TILE", 0},           {"attn_split", "KQ4_ATTN_SPLIT", 0},
 };
 std::atomic<int> g_opt[kOptCount];
 int g_opt_init[kOptCount];   // each option's value at load: its environment variable or default
@@ -1271,6 +1272,10 @@ int rows_check(const char *what, const char *name, const float *p, long ld, long
   return KQ4_OK;
 }
 
+KQ4AttnPlan attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv) {
+  return kq4_attn_plan(n_tok, n_seq, heads, kv_heads, max_q, max_kv, opt(kAttnTile), opt(kAttnSplit));
+}
+
 size_t attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int heads, int head_dim, size_t *o_bytes) {
   *o_bytes = 0;
   if (p.ns <= 1) return 0;
@@ -1337,7 +1342,7 @@ int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_h
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;
   hipStream_t s = (hipStream_t)stream;
-  const KQ4AttnPlan plan = kq4_attn_plan(kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, max_q, max_kv);
+  const KQ4AttnPlan plan = attn_plan(kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, max_q, max_kv);
   size_t o_bytes = 0;
   const size_t bytes = attn_part_bytes(plan, kv->n_tok, q_heads, kv->head_dim, &o_bytes);
   char *ws = nullptr;
@@ -1356,7 +1361,7 @@ size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads,
       (head_dim != 64 && head_dim != 128) || max_q < 0 || max_kv < 0)
     return 0;
   size_t o_bytes = 0;
-  return attn_part_bytes(kq4_attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv), n_tok, q_heads, head_dim,
+  return attn_part_bytes(attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv), n_tok, q_heads, head_dim,
                          &o_bytes);
 }
 

@@ -17,10 +17,14 @@
 #include "kq4_kv.h"
 #include "kq4_internal.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4;
@@ -183,37 +187,54 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a)
     for (int d = 0; d < DT; ++d) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
     float M = kNegInf, l = 0.0f;
 
-    // group of this lane's key row (A operand) and of its key quarter (scales, values); -1: none
-    auto group_of = [&](int key, int sub) -> long {
+    // A step is 64 keys. Table entries are read two steps ahead, scales one; a register of keys or values is loaded
+    // again for the next step as soon as its codes are converted, so both are in flight for most of a step.
+    auto page_of = [&](int key, int sub) {   // of a lane's group among the step's 4; -1: none
+      const int g = (key >> 4) + sub, slot = g >> a.log_pg;
+      return key < end && g < g_end && slot < a.kv.table_pages ? table[slot] : -1;
+    };
+    auto group_of = [&](int page, int key, int sub) -> long {
       const int g = (key >> 4) + sub;
-      return key < end && g < g_end
-                 ? kq4_kv_group_at(table, a.kv.table_pages, g, h, a.kv.n_pages, a.kv.kv_heads, a.log_pg)
+      return (unsigned)page < (unsigned)a.kv.n_pages
+                 ? (((long)page * a.kv.kv_heads + h) << a.log_pg) | (g & ((1 << a.log_pg) - 1))
                  : -1;
     };
+    constexpr int kStep = 64 * kWaves;
+    const int ik = i16 >> 2;                 // this lane's key row's group; qd: that of its scales and values
     uint4 kr[4][TT], vr[DT];
-    float2 sc = make_float2(0.f, 0.f);
-    auto load_k = [&](long g) {
-      const uint8_t *p = a.kv.codes + (g < 0 ? 0 : g) * (32 * D) + 256 * qd + 16 * (i16 & 3);
+    int key = base + 64 * wave;
+    int page_k = page_of(key, ik), page_v = page_of(key, qd);
+    int next_k = page_of(key + kStep, ik), next_v = page_of(key + kStep, qd);
+    const uint8_t *kp, *vp;
+    auto point = [&](long gk, long gv) {
+      kp = a.kv.codes + (gk < 0 ? 0 : gk) * (32 * D) + 256 * qd + 16 * (i16 & 3);
+      vp = a.kv.codes + (gv < 0 ? 0 : gv) * (32 * D) + 16 * D + 16 * i16;
+    };
+    long gv = group_of(page_v, key, qd);
+    point(group_of(page_k, key, ik), gv);
+    float2 sc = *reinterpret_cast<const float2 *>(a.kv.scales + 2 * (gv < 0 ? 0 : gv));
+    if (key < end) {
 #pragma unroll
       for (int t4 = 0; t4 < 4; ++t4)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) kr[t4][t] = *reinterpret_cast<const uint4 *>(p + 1024 * t + 64 * t4);
-    };
-    auto load_v = [&](long g) {
-      const uint8_t *p = a.kv.codes + (g < 0 ? 0 : g) * (32 * D) + 16 * D + 16 * i16;
+        for (int t = 0; t < TT; ++t) kr[t4][t] = *reinterpret_cast<const uint4 *>(kp + 1024 * t + 64 * t4);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const uint4 *>(p + 256 * d);
-    };
+      for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const uint4 *>(vp + 256 * d);
+    }
 
-    int key = base + 64 * wave;
-    long gv = group_of(key, qd);
-    load_k(group_of(key, i16 >> 2));
-    load_v(gv);
-    if (gv >= 0) sc = *reinterpret_cast<const float2 *>(a.kv.scales + 2 * gv);
-    for (; key < end; key += 64 * kWaves) {
-      const int next = key + 64 * kWaves;
-      const long gk_n = group_of(next, i16 >> 2), gv_n = group_of(next, qd);
-
+    auto step = [&](auto more) {
+      const int next = key + kStep;
+      const bool there = gv >= 0;
+      const float2 scale = sc;
+      long gv_n = -1;
+      int page_k2 = -1, page_v2 = -1;
+      if constexpr (more.value) {
+        page_k2 = page_of(next + kStep, ik);
+        page_v2 = page_of(next + kStep, qd);
+        gv_n = group_of(next_v, next, qd);
+        point(group_of(next_k, next, ik), gv_n);
+        sc = *reinterpret_cast<const float2 *>(a.kv.scales + 2 * (gv_n < 0 ? 0 : gv_n));
+      }
       float4v s[4];
 #pragma unroll
       for (int t4 = 0; t4 < 4; ++t4) {
@@ -221,34 +242,37 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a)
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
           const half8 k0 = codes_f16(kr[t4][t].x, kr[t4][t].y), k1 = codes_f16(kr[t4][t].z, kr[t4][t].w);
+          if constexpr (more.value) kr[t4][t] = *reinterpret_cast<const uint4 *>(kp + 1024 * t + 64 * t4);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[t][0], s[t4], 0, 0, 0);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[t][0], s[t4], 0, 0, 0);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[t][1], s[t4], 0, 0, 0);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[t][1], s[t4], 0, 0, 0);
         }
       }
-      if (next < end) load_k(gk_n);
 
-      // this lane's 16 keys are tokens 4 t4 + r of group qd of the 64
-      const bool there = gv >= 0;
-      const float c = there ? sc.x * descale : 0.0f, lv = there ? __builtin_amdgcn_logf(sc.y) : 0.0f;
+      // this lane's 16 keys are tokens 4 t4 + j of group qd of the 64
+      float c = there ? scale.x * descale : 0.0f, lv = there ? __builtin_amdgcn_logf(scale.y) : 0.0f;
+      float rv = there ? __builtin_amdgcn_rcpf(scale.y) : 0.0f;
       const bool masked = key < all_lo || key + 64 > all_hi || __ballot(!there) != 0;
-      uint32_t off = 0;   // bit 4 t4 + r: this lane's row does not see the key
       if (masked) {
         const int k0 = key + 16 * qd;
         // slots [see_lo - k0, min(see_hi, end) - k0) of the 16
         const int b = see_lo - k0, e = (see_hi < end ? see_hi : end) - k0;
         const uint32_t from = b <= 0 ? 0xffffu : b >= 16 ? 0u : 0xffffu << b;
         const uint32_t to = e <= 0 ? 0u : e >= 16 ? 0xffffu : (1u << e) - 1u;
-        off = there ? ~(from & to) & 0xffffu : 0xffffu;
+        const uint32_t on = there ? from & to & 0xffffu : 0u;
+        // (a group of which this row sees nothing may hold any scale: 0, not 0 times it)
+        if (on == 0) c = lv = rv = 0.0f;
+#pragma unroll
+        for (int t4 = 0; t4 < 4; ++t4)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[t4][j] = (on >> (4 * t4 + j)) & 1u ? s[t4][j] : kNegInf;
       }
-      // (a group of which this row sees nothing may hold any scale: 0, not 0 times it)
-      const float rv = there && off != 0xffffu ? __builtin_amdgcn_rcpf(sc.y) : 0.0f;
-      float mx = kNegInf;
+      float mx = s[0][0];
 #pragma unroll
       for (int t4 = 0; t4 < 4; ++t4)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, (off >> (4 * t4 + j)) & 1u ? kNegInf : s[t4][j]);
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[t4][j]);
       float em = mx == kNegInf ? kNegInf : fmaf(mx, c, lv);
       em = max_xor32(max_xor16(em));
       if (__ballot(em > M + kSlack)) {
@@ -269,8 +293,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a)
           float p0 = __builtin_amdgcn_exp2f(fmaf(s[t4][j], c, shift));
           float p1 = __builtin_amdgcn_exp2f(fmaf(s[t4][j + 1], c, shift));
           if (masked) {
-            p0 = (off >> (4 * t4 + j)) & 1u ? 0.0f : p0;
-            p1 = (off >> (4 * t4 + j + 1)) & 1u ? 0.0f : p1;
+            p0 = s[t4][j] == kNegInf ? 0.0f : p0;
+            p1 = s[t4][j + 1] == kNegInf ? 0.0f : p1;
           }
           sum += p0 + p1;
           const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
@@ -282,15 +306,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const half8 v0 = codes_f16(vr[d].x, vr[d].y), v1 = codes_f16(vr[d].z, vr[d].w);
+        if constexpr (more.value) vr[d] = *reinterpret_cast<const uint4 *>(vp + 256 * d);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0].h, o[d], 0, 0, 0);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0].h, o[d], 0, 0, 0);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1].h, o[d], 0, 0, 0);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1].h, o[d], 0, 0, 0);
       }
-      if (next < end) load_v(gv_n);
-      if (gv_n >= 0) sc = *reinterpret_cast<const float2 *>(a.kv.scales + 2 * gv_n);
+      key = next;
       gv = gv_n;
-    }
+      next_k = page_k2;
+      next_v = page_v2;
+    };
+    while (key + kStep < end) step(std::true_type{});
+    if (key < end) step(std::false_type{});
 
     // join the waves
     l = kq4_xor_add<32>(kq4_xor_add<16>(l));
@@ -328,14 +356,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a)
 
 // ---- 32 rows a wave: prompts and chunks ------------------------------------------------------------
 // A workgroup is NW * 32 rows (query tokens * heads per kv head) of one sequence and kv head: its waves share
-// tiles of 64 keys, converted to f16 once on their way into LDS (two buffers, the next tile's loads in flight
-// meanwhile). LDS holds the operands in lane order, 16 bytes a lane without bank conflicts: keys as
-// [D/8][64 keys][8], values as [32-key tile][8-token half][group][D][8].
+// tiles of 32 keys, converted to f16 once on their way into a ring of 4 in LDS, the loads of the tile after next
+// in flight meanwhile. LDS holds the operands in lane order, 16 bytes a lane without bank conflicts: keys as
+// [D/8][32 keys][8], values as [8-token half][group][D][8]. The scores of tile n + 1 are formed while tile n's go
+// through the softmax, so matrix instructions and vector instructions of a wave are independent of each other.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
-  constexpr int NT = 64 * NW, TT = D / 32, DT = D / 32, NL = 8 * D / NT, TM = 32 * NW;
-  constexpr int KB = D / 8 * 64 * 16, VB = 8 * D * 16;   // bytes of a tile's keys, values
-  __shared__ __align__(16) uint8_t s_kv[2][KB + VB];
+  constexpr int NT = 64 * NW, TT = D / 32, DT = D / 32, TM = 32 * NW;
+  constexpr int L = 4 * D, NL = (L + NT - 1) / NT;      // 16-byte loads of a tile, of a thread
+  constexpr int KB = D / 8 * 32 * 16;                   // bytes of a tile's keys in LDS, and of its values
+  __shared__ __align__(16) uint8_t s_kv[4][2 * KB];
+  __shared__ float2v s_sc[4][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int i32 = lane & 31, hh = lane >> 5;
   const int h = blockIdx.x % a.kv.kv_heads, split = blockIdx.y;
@@ -378,17 +409,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
   const int g_end = (sp.len + 15) >> 4;
   const int *table = a.kv.block_table + (long)seq * a.kv.table_pages;
 
-  // this lane's query row; the keys that the wave's rows see, and those that all of them see
+  // this lane's query row; the keys it sees, and those that all of the wave's rows see
   const int w0 = r0 + 32 * wave, w1 = w0 + 31 < last ? w0 + 31 : last;
   const bool any = w0 <= last;
   const int r = w0 + i32 <= last ? w0 + i32 : last;
   const int tq = r / a.group, head = h * a.group + (r - tq * a.group);
-  int see_lo, see_hi, all_lo, all_hi, wave_lo, wave_hi;
+  int see_lo, see_hi, all_lo, all_hi, t_;
   kq4_kv_sees(sp.p0 + tq, sp.len, a.window, &see_lo, &see_hi);
-  kq4_kv_sees(sp.p0 + (any ? w1 : last) / a.group, sp.len, a.window, &all_lo, &wave_hi);
-  kq4_kv_sees(sp.p0 + (any ? w0 : last) / a.group, sp.len, a.window, &wave_lo, &all_hi);
-  if (wave_hi > end) wave_hi = end;
-  if (!any) wave_hi = 0;
+  kq4_kv_sees(sp.p0 + (any ? w1 : last) / a.group, sp.len, a.window, &all_lo, &t_);
+  kq4_kv_sees(sp.p0 + (any ? w0 : last) / a.group, sp.len, a.window, &t_, &all_hi);
+  if (see_hi > end) see_hi = end;
 
   half8 qh[TT][2], ql[TT][2];
   float descale;
@@ -424,105 +454,108 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   float M = kNegInf, l = 0.0f;
 
-  auto group_of = [&](int key, int sub) -> long {
-    const int g = (key >> 4) + sub;
-    return key < end && g < g_end
-               ? kq4_kv_group_at(table, a.kv.table_pages, g, h, a.kv.n_pages, a.kv.kv_heads, a.log_pg)
+  // Table entries are read a tile before the loads that they lead to, one per half of the wave; those loads two
+  // tiles before they go to LDS, there two tiles before use. A thread's load i is 16 bytes of group
+  // (i NT + 64 wave) / 2D of the tile, keys first; the first wave also carries the tile's scales.
+  struct Raw {
+    uint4v kv[NL];
+    float2v sc;
+    bool there;
+  };
+  const int tiles = (end - base + 31) >> 5;
+  auto entry = [&](int n) {
+    const int slot = (((base + 32 * n) >> 4) + hh) >> a.log_pg;
+    return table[slot < a.kv.table_pages ? slot : a.kv.table_pages - 1];
+  };
+  auto group_of = [&](int n, int half, int page) -> long {
+    const int g = ((base + 32 * n) >> 4) + half;
+    return g < g_end && (g >> a.log_pg) < a.kv.table_pages && (unsigned)page < (unsigned)a.kv.n_pages
+               ? (((long)page * a.kv.kv_heads + h) << a.log_pg) | (g & ((1 << a.log_pg) - 1))
                : -1;
   };
-  // load i of a thread: 16 bytes of group (64 i NW + 64 wave) / 2D, keys first; wave-uniform
-  uint4 raw[NL];
-  auto load = [&](int key) {
+  auto load = [&](int n, int entries, Raw &r) {
+    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(entries, 0));
+    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(entries, 32));
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int j = i * NT + 64 * wave;
-      const long g = group_of(key, j / (2 * D));
-      raw[i] = *reinterpret_cast<const uint4 *>(a.kv.codes + (g < 0 ? 0 : g) * (32 * D) +
-                                                16 * (j % (2 * D) + lane));
+      if (j < L) {
+        const long g = j / (2 * D) ? g1 : g0;
+        r.kv[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (g < 0 ? 0 : g) * (32 * D) +
+                                                    16 * (j % (2 * D)) + 16 * lane);
+      }
+    }
+    if (wave == 0) {
+      const long g = hh ? g1 : g0;
+      r.there = g >= 0;
+      r.sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (g < 0 ? 0 : g));
     }
   };
-  auto store = [&](uint8_t *buf) {
+  auto store = [&](int n, const Raw &r) {
+    uint8_t *buf = s_kv[n & 3];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int j = i * NT + 64 * wave, sub = j / (2 * D), part = j % (2 * D);
-      Frag f0, f1;
-      f0.h = codes_f16(raw[i].x, raw[i].y);
-      f1.h = codes_f16(raw[i].z, raw[i].w);
-      uint8_t *p0, *p1;
-      if (part < D) {   // keys: chunk, token -> pieces 2 chunk and 2 chunk + 1, the token's lane slot
-        const int c = (part + lane) >> 4, tok = lane & 15;
-        const int slot = 32 * (sub >> 1) + (tok & 3) + 4 * (sub & 1) + 8 * (tok >> 2);
-        p0 = buf + (2 * c * 64 + slot) * 16;
-        p1 = p0 + 64 * 16;
-      } else {          // values: dimension -> halves of 8 tokens
-        const int d = part - D + lane;
-        p0 = buf + KB + (((sub >> 1) * 4 + (sub & 1)) * D + d) * 16;
-        p1 = p0 + 2 * D * 16;
+      const int j = i * NT + 64 * wave, half = j / (2 * D), part = j % (2 * D);
+      if (j < L) {
+        const half8 f0 = codes_f16(r.kv[i][0], r.kv[i][1]), f1 = codes_f16(r.kv[i][2], r.kv[i][3]);
+        uint8_t *p0, *p1;
+        if (part < D) {   // keys: chunk, token -> pieces 2 chunk and 2 chunk + 1, the token's lane slot
+          const int c = (part + lane) >> 4, tok = lane & 15;
+          p0 = buf + (2 * c * 32 + (tok & 3) + 4 * half + 8 * (tok >> 2)) * 16;
+          p1 = p0 + 32 * 16;
+        } else {          // values: dimension -> halves of 8 tokens
+          p0 = buf + KB + (half * D + part - D + lane) * 16;
+          p1 = p0 + 2 * D * 16;
+        }
+        *reinterpret_cast<half8 *>(p0) = f0;
+        *reinterpret_cast<half8 *>(p1) = f1;
       }
-      *reinterpret_cast<uint4 *>(p0) = make_uint4(f0.u[0], f0.u[1], f0.u[2], f0.u[3]);
-      *reinterpret_cast<uint4 *>(p1) = make_uint4(f1.u[0], f1.u[1], f1.u[2], f1.u[3]);
     }
+    // (a group without a page: a value scale of 0, which no group has)
+    if (wave == 0 && i32 == 0) s_sc[n & 3][hh] = r.there ? r.sc : float2v{1.0f, 0.0f};
   };
 
-  load(base);
-  int buf = 0;
-  for (int key = base; key < end; key += 64, buf ^= 1) {
-    store(s_kv[buf]);
-    float c[2], lv[2], rv[2];
-    bool there[2];
+  const int k_at = (hh * 2 * 32 + i32) * 16, v_at = KB + (hh * D + i32) * 16;
+  auto scores = [&](int n, float16v &s) {
+    const uint8_t *kb = s_kv[n & 3] + k_at;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const long g0 = group_of(key, 2 * kt), g1 = group_of(key, 2 * kt + 1);
-      const long g = hh ? g1 : g0;
-      there[kt] = g >= 0;
-      const float2 sc = *reinterpret_cast<const float2 *>(a.kv.scales + 2 * (g < 0 ? 0 : g));
-      c[kt] = there[kt] ? sc.x * descale : 0.0f;
-      lv[kt] = there[kt] ? __builtin_amdgcn_logf(sc.y) : 0.0f;
-      rv[kt] = there[kt] ? __builtin_amdgcn_rcpf(sc.y) : 0.0f;
-    }
-    __syncthreads();
-    if (key + 64 < end) load(key + 64);
-    if (key >= wave_hi || key + 64 <= wave_lo) continue;   // (no barrier is left in this turn)
-
-    const uint8_t *kb = s_kv[buf] + (hh * 2 * 64 + i32) * 16, *vb = s_kv[buf] + KB + (hh * D + i32) * 16;
-    float16v s[2];
+    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const half8 k = *reinterpret_cast<const half8 *>(kb + ((4 * t + u) * 64 + 32 * kt) * 16);
-          s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t][u], s[kt], 0, 0, 0);
-          s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t][u], s[kt], 0, 0, 0);
-        }
-    }
-    // this lane's keys: 16 of group 2 kt + hh
-    const bool masked = key < all_lo || key + 64 > all_hi || __ballot(!(there[0] && there[1])) != 0;
-    float em = kNegInf;
-    if (masked) {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int k0 = key + 32 * kt + 16 * hh;
-        const int b = see_lo - k0, e = (see_hi < end ? see_hi : end) - k0;
-        const uint32_t from = b <= 0 ? 0xffffu : b >= 16 ? 0u : 0xffffu << b;
-        const uint32_t to = e <= 0 ? 0u : e >= 16 ? 0xffffu : (1u << e) - 1u;
-        const uint32_t on = there[kt] ? from & to & 0xffffu : 0u;
-        if (on == 0) c[kt] = lv[kt] = rv[kt] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[kt][j] = (on >> j) & 1u ? s[kt][j] : kNegInf;
+      for (int u = 0; u < 2; ++u) {
+        const half8 k = *reinterpret_cast<const half8 *>(kb + (4 * t + u) * 32 * 16);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t][u], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t][u], s, 0, 0, 0);
       }
-    }
+  };
+  // masks tile n's scores and raises the maximum where they pass it; c, lv, rv: the factors of its softmax
+  float c = 0.0f, lv = 0.0f, rv = 0.0f;
+  auto settle = [&](int n, float16v &s) {
+    const int key = base + 32 * n;
+    const float2v scale = s_sc[n & 3][hh];
+    const bool there = scale[1] != 0.0f;
+    c = scale[0] * descale;
+    lv = __builtin_amdgcn_logf(scale[1]);
+    rv = __builtin_amdgcn_rcpf(scale[1]);
+    c = c == 0.0f ? 1e-37f : c;   // (a masked score, -inf, stays that)
+    if (key < all_lo || key + 32 > all_hi || __ballot(!there) != 0) {
+      const int k0 = key + 16 * hh, b = see_lo - k0, e = see_hi - k0;
+      const uint32_t from = b <= 0 ? 0xffffu : b >= 16 ? 0u : 0xffffu << b;
+      const uint32_t to = e <= 0 ? 0u : e >= 16 ? 0xffffu : (1u << e) - 1u;
+      const uint32_t on = there ? from & to & 0xffffu : 0u;
+      // (a group of which this row sees nothing may hold any scale)
+      if (on == 0) {
+        c = 1.0f;
+        lv = rv = 0.0f;
+      }
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      float mx = s[kt][0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[kt][j]);
-      em = fmaxf(em, mx == kNegInf ? kNegInf : fmaf(mx, c[kt], lv[kt]));
+      for (int j = 0; j < 16; ++j) s[j] = (on >> j) & 1u ? s[j] : kNegInf;
     }
-    em = max_xor32(em);
+    float mx = s[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+    const float em = max_xor32(fmaf(mx, c, lv));
     if (__ballot(em > M + kSlack)) {
       const float m = em > M + kSlack ? em : M;
       const float f = M == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(M - m);
@@ -531,35 +564,74 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
       for (int d = 0; d < DT; ++d) o[d] *= f;
       M = m;
     }
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const float shift = (M == kNegInf ? 0.0f : lv[kt] - M) + kTop;
+  };
+
+  float16v s;
+  Raw ra, rb;
+  ra.there = rb.there = false;
+  int ent;
+  load(0, entry(0), ra);
+  load(1, entry(1), rb);
+  ent = entry(2);
+  store(0, ra);
+  store(1, rb);
+  load(2, ent, ra);
+  ent = entry(3);
+  load(3, ent, rb);
+  ent = entry(4);
+  __syncthreads();
+  if (any && tiles > 0) {
+    scores(0, s);
+    settle(0, s);
+  }
+  // (tiles past the last are loaded as group 0 and never used)
+  auto step = [&](int n, Raw &r, auto more) {
+    store(n + 2, r);
+    __syncthreads();
+    load(n + 4, ent, r);
+    ent = entry(n + 5);
+    if (any) {
+      float16v s_n;
+      if constexpr (more.value) scores(n + 1, s_n);
+      const float shift = (M == kNegInf ? 0.0f : lv - M) + kTop;
       Frag ph[2], pl[2];
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
-        float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][j], c[kt], shift));
-        float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][j + 1], c[kt], shift));
-        if (masked) {
-          p0 = s[kt][j] == kNegInf ? 0.0f : p0;
-          p1 = s[kt][j + 1] == kNegInf ? 0.0f : p1;
-        }
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c, shift));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c, shift));
         sum += p0 + p1;
         const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
         const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
         ph[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, hi);
         pl[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, lo);
       }
-      l = fmaf(sum, rv[kt], l);
+      l = fmaf(sum, rv, l);
+      const uint8_t *vb = s_kv[n & 3] + v_at;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const half8 v = *reinterpret_cast<const half8 *>(vb + ((kt * 4 + 2 * u) * D + 32 * d) * 16);
+          const half8 v = *reinterpret_cast<const half8 *>(vb + (2 * u * D + 32 * d) * 16);
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u].h, o[d], 0, 0, 0);
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u].h, o[d], 0, 0, 0);
         }
+      if constexpr (more.value) {
+        s = s_n;
+        settle(n + 1, s);
+      }
     }
+  };
+  int n = 0;
+  for (; n + 2 < tiles; n += 2) {
+    step(n, ra, std::true_type{});
+    step(n + 1, rb, std::true_type{});
+  }
+  if (n + 1 < tiles) {
+    step(n, ra, std::true_type{});
+    step(n + 1, rb, std::false_type{});
+  } else if (n < tiles) {
+    step(n, ra, std::false_type{});
   }
 
   if (!any || w0 + i32 > last) return;
@@ -576,13 +648,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
   if (used > 1 && hh == 0) a.part_ml[split * n_rows + row] = make_float2(M, l);
 }
 
-// Joins the splits of each row: one wave a row, 4 rows a workgroup.
+// Joins the splits of a row, 32 dimensions a workgroup: the factors 2^(M_s - M) of all splits into LDS, then 8
+// threads a dimension take splits in turn.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long row = blockIdx.x * 4L + (threadIdx.x >> 6), n_rows = (long)a.kv.n_tok * a.heads;
-  if (row >= n_rows) return;
+  __shared__ float s_f[KQ4_ATTN_MAX_SPLITS];
+  __shared__ float s_acc[8][32], s_m[4], s_l[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long row = blockIdx.x / (D / 32), n_rows = (long)a.kv.n_tok * a.heads;
+  const int d = 32 * (int)(blockIdx.x % (D / 32)) + (tid & 31);
   const int tok = (int)(row / a.heads), head = (int)(row - (long)tok * a.heads);
   KQ4KvSpan sp{0, 0, 0, 0};
   bool found = false;
@@ -606,56 +680,76 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile) {
   int base, end;
   const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, a.chunk, a.ns, &base, &end);
   if (used == 1) return;   // written by its only split
+
   float m = kNegInf;
-  for (int s = lane; s < used; s += 64) m = fmaxf(m, a.part_ml[s * n_rows + row].x);
+  for (int s = tid; s < used; s += 256) m = fmaxf(m, a.part_ml[s * n_rows + row].x);
 #pragma unroll
   for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  float sl = 0.0f, acc[E] = {};
-  for (int s = 0; s < used; ++s) {
+  if (lane == 0) s_m[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float sl = 0.0f;
+  for (int s = tid; s < used; s += 256) {
     const float2 ml = a.part_ml[s * n_rows + row];
-    const float f = ml.x == kNegInf && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x == kNegInf ? 0.0f : ml.x - m);
+    // (a split of which nothing was seen: 0; one whose scales were all NaN keeps its NaN)
+    const float f = ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
+    s_f[s] = f;
     sl = fmaf(ml.y, f, sl);
-    const float *p = a.part_o + (s * n_rows + row) * D + E * lane;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(p[e], f, acc[e]);
   }
-  const float f = sl == 0.0f ? 0.0f : 1.0f / sl;
 #pragma unroll
-  for (int e = 0; e < E; ++e) a.out[row * D + E * lane + e] = acc[e] * f;
+  for (int x = 32; x; x >>= 1) sl += __shfl_xor(sl, x);
+  if (lane == 0) s_l[wave] = sl;
+  __syncthreads();
+  float acc = 0.0f;
+  const float *p = a.part_o + row * D + d;
+#pragma unroll 8
+  for (int s = tid >> 5; s < used; s += 8) acc = fmaf(p[s * n_rows * D], s_f[s], acc);
+  s_acc[tid >> 5][tid & 31] = acc;
+  __syncthreads();
+  if (tid < 32) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) acc += s_acc[w][tid];
+    sl = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    a.out[row * D + d] = sl == 0.0f ? 0.0f : acc / sl;
+  }
 }
 
 template <int D>
 int launch(const AttnArgs &a, int tile, hipStream_t s) {
-  constexpr int NW = 8;
   if (tile == 16) {
     attn_rows16_kernel<D><<<dim3((unsigned)a.kv.n_seq * a.kv.kv_heads, a.ns), 64 * kWaves, 0, s>>>(a);
   } else {
-    const long items = (long)a.kv.n_tok * a.group / tile + a.kv.n_seq;
-    attn_rows32_kernel<D, NW><<<dim3((unsigned)(items * a.kv.kv_heads), a.ns), 64 * NW, 0, s>>>(a);
+    const dim3 grid((unsigned)(((long)a.kv.n_tok * a.group / tile + a.kv.n_seq) * a.kv.kv_heads), a.ns);
+    if (tile == 128)
+      attn_rows32_kernel<D, 4><<<grid, 256, 0, s>>>(a);
+    else
+      attn_rows32_kernel<D, 8><<<grid, 512, 0, s>>>(a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (a.ns > 1) {
     const long n_rows = (long)a.kv.n_tok * a.heads;
-    attn_join_kernel<D><<<(unsigned)((n_rows + 3) / 4), 256, 0, s>>>(a, tile);
+    attn_join_kernel<D><<<(unsigned)(n_rows * (D / 32)), 256, 0, s>>>(a, tile);
   }
   return (int)hipGetLastError();
 }
 
 }  // namespace
 
-KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv) {
+KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int force_tile,
+                          int force_split) {
   KQ4AttnPlan p;
   const long keys = max_kv < 1 ? 1 : max_kv;
   const int group = heads / kv_heads;
-  p.tile = (long)max_q * group <= 16 ? 16 : 256;
+  p.tile = force_tile == 16 || force_tile == 128 || force_tile == 256 ? force_tile : (long)max_q * group <= 16 ? 16 : 256;
   const long step = p.tile == 16 ? 64 * kWaves : 64;           // keys of a workgroup's turn
   const long items = p.tile == 16 ? n_seq : (long)n_tok * group / p.tile + n_seq;
   const long base = items * kv_heads;                          // workgroups of one split
   const long most = (keys + step - 1) / step;
   long ns = ((p.tile == 16 ? 512 : 256) + base - 1) / base;
+  if (force_split > 0) ns = force_split;
   if (ns > most) ns = most;
-  if (ns > 1024) ns = 1024;
+  if (ns > KQ4_ATTN_MAX_SPLITS) ns = KQ4_ATTN_MAX_SPLITS;
   if (ns < 1) ns = 1;
   p.chunk = (int)(((keys + ns - 1) / ns + step - 1) / step * step);
   p.ns = (int)((keys + p.chunk - 1) / p.chunk);

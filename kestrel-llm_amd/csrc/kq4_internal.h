@@ -190,7 +190,9 @@ int kq4_launch_kv_append(const kq4_kv &kv, int log_pg, const float *k, long ldk,
 struct KQ4AttnPlan {
   int tile, chunk, ns;
 };
-KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv);
+#define KQ4_ATTN_MAX_SPLITS 1024
+KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int force_tile,
+                          int force_split);
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
                     int window, const KQ4AttnPlan &plan, float *part_o, float *part_ml, hipStream_t s);
 // Pieces of a row, and a piece's bytes; best holds n * pieces * n_top keys.
