@@ -454,8 +454,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   float M = kNegInf, l = 0.0f;
 
-  // Table entries are read a tile before the loads that they lead to, one per half of the wave; those loads two
-  // tiles before they go to LDS, there two tiles before use. A thread's load i is 16 bytes of group
+  // Table entries are read a tile before the loads that they lead to, one per half of the wave; those loads a
+  // tile before they go to LDS, there a tile before use. A thread's load i is 16 bytes of group
   // (i NT + 64 wave) / 2D of the tile, keys first; the first wave also carries the tile's scales.
   struct Raw {
     uint4v kv[NL];
@@ -516,22 +516,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
   };
 
   const int k_at = (hh * 2 * 32 + i32) * 16, v_at = KB + (hh * D + i32) * 16;
-  auto scores = [&](int n, float16v &s) {
-    const uint8_t *kb = s_kv[n & 3] + k_at;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const half8 k = *reinterpret_cast<const half8 *>(kb + (4 * t + u) * 32 * 16);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[t][u], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[t][u], s, 0, 0, 0);
-      }
-  };
   // masks tile n's scores and raises the maximum where they pass it; c, lv, rv: the factors of its softmax
   float c = 0.0f, lv = 0.0f, rv = 0.0f;
-  auto settle = [&](int n, float16v &s) {
+  auto settle = [&](int n, float16v &s, float mx) {
     const int key = base + 32 * n;
     const float2v scale = s_sc[n & 3][hh];
     const bool there = scale[1] != 0.0f;
@@ -551,10 +538,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] = (on >> j) & 1u ? s[j] : kNegInf;
-    }
-    float mx = s[0];
+      mx = s[0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+    }
     const float em = max_xor32(fmaf(mx, c, lv));
     if (__ballot(em > M + kSlack)) {
       const float m = em > M + kSlack ? em : M;
@@ -566,75 +553,107 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
     }
   };
 
-  float16v s;
-  Raw ra, rb;
-  ra.there = rb.there = false;
-  int ent;
-  load(0, entry(0), ra);
-  load(1, entry(1), rb);
+  float16v sa, sb;
+  Raw raw;
+  raw.there = false;
+  int ent = entry(1);
+  load(0, entry(0), raw);
+  store(0, raw);
+  load(1, ent, raw);
   ent = entry(2);
-  store(0, ra);
-  store(1, rb);
-  load(2, ent, ra);
+  store(1, raw);
+  load(2, ent, raw);
   ent = entry(3);
-  load(3, ent, rb);
-  ent = entry(4);
   __syncthreads();
-  if (any && tiles > 0) {
-    scores(0, s);
-    settle(0, s);
-  }
-  // (tiles past the last are loaded as group 0 and never used)
-  auto step = [&](int n, Raw &r, auto more) {
-    store(n + 2, r);
+  auto stage = [&](int n) {
+    store(n + 2, raw);
     __syncthreads();
-    load(n + 4, ent, r);
-    ent = entry(n + 5);
-    if (any) {
-      float16v s_n;
-      if constexpr (more.value) scores(n + 1, s_n);
-      const float shift = (M == kNegInf ? 0.0f : lv - M) + kTop;
-      Frag ph[2], pl[2];
-      float sum = 0.0f;
+    load(n + 3, ent, raw);
+    ent = entry(n + 4);
+  };
+  if (!any) {   // (a wave without rows keeps up the others' tiles and barriers)
+    for (int n = 0; n < tiles; ++n) stage(n);
+    return;
+  }
+  constexpr int F = 2 * TT, AHEAD = 2;   // operand fragments of a product, read so many ahead of use
+  // Tile n's softmax and second product, and with `more` tile n + 1's scores; a fragment's two matrix instructions
+  // stand between those vector instructions, in this order, which the compiler is kept to.
+  // (tiles past the last are loaded as group 0 and never used)
+  auto step = [&](int n, float16v &s, float16v &s_n, auto has, auto more) {
+    if constexpr (has.value) stage(n);
+    half8 f[2 * F];   // keys of tile n + 1, values of tile n
+    auto fetch = [&](int i) {
+      if (i < F)
+        f[i] = *reinterpret_cast<const half8 *>(s_kv[(n + 1) & 3] + k_at + (4 * (i >> 1) + (i & 1)) * 32 * 16);
+      else
+        f[i] = *reinterpret_cast<const half8 *>(s_kv[n & 3] + v_at + (2 * ((i - F) / DT) * D + 32 * ((i - F) % DT)) * 16);
+    };
+    constexpr int first = more.value ? 0 : F, stop = has.value ? 2 * F : F;
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c, shift));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c, shift));
-        sum += p0 + p1;
-        const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-        const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
-        ph[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, hi);
-        pl[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, lo);
-      }
-      l = fmaf(sum, rv, l);
-      const uint8_t *vb = s_kv[n & 3] + v_at;
+    for (int i = 0; i < AHEAD; ++i) fetch(first + i);
+    if constexpr (more.value)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int e = 0; e < 16; ++e) s_n[e] = 0.0f;
+    const float shift = (M == kNegInf ? 0.0f : lv - M) + kTop;
+    Frag ph[2], pl[2];
+    float sum = 0.0f, mx = kNegInf;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const half8 v = *reinterpret_cast<const half8 *>(vb + (2 * u * D + 32 * d) * 16);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u].h, o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u].h, o[d], 0, 0, 0);
-        }
+    for (int i = 0; i < F; ++i) {
       if constexpr (more.value) {
-        s = s_n;
-        settle(n + 1, s);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + AHEAD < stop) fetch(i + AHEAD);
+        s_n = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], qh[i >> 1][i & 1], s_n, 0, 0, 0);
+        s_n = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], ql[i >> 1][i & 1], s_n, 0, 0, 0);
+      }
+      if constexpr (has.value) {
+#pragma unroll
+        for (int j = 16 / F * i; j < 16 / F * (i + 1); j += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c, shift));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c, shift));
+          sum += p0 + p1;
+          const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+          const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
+          ph[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, hi);
+          pl[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, lo);
+        }
       }
     }
+    if constexpr (has.value) {
+      l = fmaf(sum, rv, l);
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (F + i + AHEAD < 2 * F) fetch(F + i + AHEAD);
+        const int u = i / DT, d = i % DT;
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[F + i], ph[u].h, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[F + i], pl[u].h, o[d], 0, 0, 0);
+        if constexpr (more.value)
+#pragma unroll
+          for (int j = 16 / F * i; j < 16 / F * (i + 1); ++j) mx = fmaxf(mx, s_n[j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s_n[j]);
+    }
+    if constexpr (more.value) settle(n + 1, s_n, mx);
   };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
   int n = 0;
+  if (tiles > 0) step(-1, sb, sa, no, yes);
   for (; n + 2 < tiles; n += 2) {
-    step(n, ra, std::true_type{});
-    step(n + 1, rb, std::true_type{});
+    step(n, sa, sb, yes, yes);
+    step(n + 1, sb, sa, yes, yes);
   }
   if (n + 1 < tiles) {
-    step(n, ra, std::true_type{});
-    step(n + 1, rb, std::false_type{});
+    step(n, sa, sb, yes, yes);
+    step(n + 1, sb, sa, yes, no);
   } else if (n < tiles) {
-    step(n, ra, std::false_type{});
+    step(n, sa, sb, yes, no);
   }
 
-  if (!any || w0 + i32 > last) return;
+  if (w0 + i32 > last) return;
   l = kq4_xor_add<32>(l);
   const long row = (long)(sp.q0 + tq) * a.heads + head, n_rows = (long)a.kv.n_tok * a.heads;
   float *dst = used == 1 ? a.out + row * D : a.part_o + (split * n_rows + row) * D;
