@@ -118,6 +118,21 @@ KQ4_DEV int row_shift(float amax) {
   return 13 - ilogbf(amax);
 }
 
+// Two of a lane's keys of a 32-key tile: their weights, summed and as the second product's operand.
+KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float &sum, Frag (&ph)[2],
+                          Frag (&pl)[2]) {
+  const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c, shift));
+  const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c, shift));
+  sum += p0 + p1;
+  const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+  const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
+  uint32_t h = __builtin_bit_cast(uint32_t, hi), l = __builtin_bit_cast(uint32_t, lo);
+  // (no instruction: keeps the above from being moved towards its use, behind the matrix instructions it stands between)
+  asm volatile("" : "+v"(h), "+v"(l), "+v"(sum));
+  ph[j >> 3].u[(j & 7) >> 1] = h;
+  pl[j >> 3].u[(j & 7) >> 1] = l;
+}
+
 // ---- up to 16 rows (query tokens * heads per kv head) a tile: decode ---------------------------------
 // A workgroup is one sequence, kv head and split; its waves take 64 keys in turn straight from memory to
 // registers (nothing is shared between waves until they join), the next keys' loads in flight during the
@@ -456,12 +471,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
 
   // Table entries are read a tile before the loads that they lead to, one per half of the wave; those loads a
   // tile before they go to LDS, there a tile before use. A thread's load i is 16 bytes of group
-  // (i NT + 64 wave) / 2D of the tile, keys first; the first wave also carries the tile's scales.
-  struct Raw {
-    uint4v kv[NL];
-    float2v sc;
-    bool there;
-  };
+  // (i NT + 64 wave) / 2D of the tile, keys first.
   const int tiles = (end - base + 31) >> 5;
   auto entry = [&](int n) {
     const int slot = (((base + 32 * n) >> 4) + hh) >> a.log_pg;
@@ -473,114 +483,77 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
                ? (((long)page * a.kv.kv_heads + h) << a.log_pg) | (g & ((1 << a.log_pg) - 1))
                : -1;
   };
-  auto load = [&](int n, int entries, Raw &r) {
-    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(entries, 0));
-    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(entries, 32));
+  uint4v raw[NL];
+  float2v raw_sc = {1.0f, 0.0f};
+  bool raw_there = false;
+  int ent, put0[NL], put1[NL];   // table entries of the tile after raw's; where a load's halves go in LDS
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int j = i * NT + 64 * wave, half = j / (2 * D), part = j % (2 * D);
+    if (part < D) {   // keys: chunk, token -> pieces 2 chunk and 2 chunk + 1, the token's lane slot
+      const int c = (part + lane) >> 4, tok = lane & 15;
+      put0[i] = (2 * c * 32 + (tok & 3) + 4 * half + 8 * (tok >> 2)) * 16;
+      put1[i] = put0[i] + 32 * 16;
+    } else {          // values: dimension -> halves of 8 tokens
+      put0[i] = KB + (half * D + part - D + lane) * 16;
+      put1[i] = put0[i] + 2 * D * 16;
+    }
+  }
+  auto load = [&](int n) {
+    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(ent, 0));
+    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(ent, 32));
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int j = i * NT + 64 * wave;
       if (j < L) {
         const long g = j / (2 * D) ? g1 : g0;
-        r.kv[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (g < 0 ? 0 : g) * (32 * D) +
-                                                    16 * (j % (2 * D)) + 16 * lane);
+        raw[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (g < 0 ? 0 : g) * (32 * D) +
+                                                   16 * (j % (2 * D)) + 16 * lane);
       }
     }
-    if (wave == 0) {
-      const long g = hh ? g1 : g0;
-      r.there = g >= 0;
-      r.sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (g < 0 ? 0 : g));
-    }
+    const long g = hh ? g1 : g0;
+    raw_there = g >= 0;
+    raw_sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (g < 0 ? 0 : g));
+    ent = entry(n + 1);
   };
-  auto store = [&](int n, const Raw &r) {
+  auto store = [&](int n) {
     uint8_t *buf = s_kv[n & 3];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int j = i * NT + 64 * wave, half = j / (2 * D), part = j % (2 * D);
-      if (j < L) {
-        const half8 f0 = codes_f16(r.kv[i][0], r.kv[i][1]), f1 = codes_f16(r.kv[i][2], r.kv[i][3]);
-        uint8_t *p0, *p1;
-        if (part < D) {   // keys: chunk, token -> pieces 2 chunk and 2 chunk + 1, the token's lane slot
-          const int c = (part + lane) >> 4, tok = lane & 15;
-          p0 = buf + (2 * c * 32 + (tok & 3) + 4 * half + 8 * (tok >> 2)) * 16;
-          p1 = p0 + 32 * 16;
-        } else {          // values: dimension -> halves of 8 tokens
-          p0 = buf + KB + (half * D + part - D + lane) * 16;
-          p1 = p0 + 2 * D * 16;
-        }
-        *reinterpret_cast<half8 *>(p0) = f0;
-        *reinterpret_cast<half8 *>(p1) = f1;
+    for (int i = 0; i < NL; ++i)
+      if (i * NT + 64 * wave < L) {
+        *reinterpret_cast<half8 *>(buf + put0[i]) = codes_f16(raw[i][0], raw[i][1]);
+        *reinterpret_cast<half8 *>(buf + put1[i]) = codes_f16(raw[i][2], raw[i][3]);
       }
-    }
-    // (a group without a page: a value scale of 0, which no group has)
-    if (wave == 0 && i32 == 0) s_sc[n & 3][hh] = r.there ? r.sc : float2v{1.0f, 0.0f};
+    // (a group without a page: a value scale of 0, which no group has; every wave writes the same)
+    if (i32 == 0) s_sc[n & 3][hh] = raw_there ? raw_sc : float2v{1.0f, 0.0f};
   };
 
-  const int k_at = (hh * 2 * 32 + i32) * 16, v_at = KB + (hh * D + i32) * 16;
-  // masks tile n's scores and raises the maximum where they pass it; c, lv, rv: the factors of its softmax
-  float c = 0.0f, lv = 0.0f, rv = 0.0f;
-  auto settle = [&](int n, float16v &s, float mx) {
-    const int key = base + 32 * n;
-    const float2v scale = s_sc[n & 3][hh];
-    const bool there = scale[1] != 0.0f;
-    c = scale[0] * descale;
-    lv = __builtin_amdgcn_logf(scale[1]);
-    rv = __builtin_amdgcn_rcpf(scale[1]);
-    c = c == 0.0f ? 1e-37f : c;   // (a masked score, -inf, stays that)
-    if (key < all_lo || key + 32 > all_hi || __ballot(!there) != 0) {
-      const int k0 = key + 16 * hh, b = see_lo - k0, e = see_hi - k0;
-      const uint32_t from = b <= 0 ? 0xffffu : b >= 16 ? 0u : 0xffffu << b;
-      const uint32_t to = e <= 0 ? 0u : e >= 16 ? 0xffffu : (1u << e) - 1u;
-      const uint32_t on = there ? from & to & 0xffffu : 0u;
-      // (a group of which this row sees nothing may hold any scale)
-      if (on == 0) {
-        c = 1.0f;
-        lv = rv = 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = (on >> j) & 1u ? s[j] : kNegInf;
-      mx = s[0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
-    }
-    const float em = max_xor32(fmaf(mx, c, lv));
-    if (__ballot(em > M + kSlack)) {
-      const float m = em > M + kSlack ? em : M;
-      const float f = M == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(M - m);
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= f;
-      M = m;
-    }
-  };
-
-  float16v sa, sb;
-  Raw raw;
-  raw.there = false;
-  int ent = entry(1);
-  load(0, entry(0), raw);
-  store(0, raw);
-  load(1, ent, raw);
-  ent = entry(2);
-  store(1, raw);
-  load(2, ent, raw);
-  ent = entry(3);
-  __syncthreads();
-  auto stage = [&](int n) {
-    store(n + 2, raw);
-    __syncthreads();
-    load(n + 3, ent, raw);
-    ent = entry(n + 4);
-  };
+  ent = entry(0);
+  load(0);
+  store(0);
+  load(1);
+  store(1);
+  load(2);
   if (!any) {   // (a wave without rows keeps up the others' tiles and barriers)
-    for (int n = 0; n < tiles; ++n) stage(n);
+    __syncthreads();
+    for (int n = 0; n < tiles; ++n) {
+      __syncthreads();
+      store(n + 2);
+      load(n + 3);
+    }
     return;
   }
-  constexpr int F = 2 * TT, AHEAD = 2;   // operand fragments of a product, read so many ahead of use
-  // Tile n's softmax and second product, and with `more` tile n + 1's scores; a fragment's two matrix instructions
-  // stand between those vector instructions, in this order, which the compiler is kept to.
-  // (tiles past the last are loaded as group 0 and never used)
+
+  // A step: tile n's softmax and second product, and with `more` tile n + 1's scores. The matrix instructions
+  // of one operand fragment (F of each product, read AHEAD before use) and a share of the vector instructions
+  // make a block; the compiler is kept to the order of blocks. (Tiles past the last are loaded as group 0, or what
+  // follows it in the table, and never used.)
+  constexpr int F = 2 * TT, AHEAD = 2;
+  const int k_at = (hh * 2 * 32 + i32) * 16, v_at = KB + (hh * D + i32) * 16;
+  float16v sa, sb;
+  float c = 0.0f, lv = 0.0f, rv = 0.0f;   // of the tile whose scores are at hand: factor, log2 and 1 / value scale
   auto step = [&](int n, float16v &s, float16v &s_n, auto has, auto more) {
-    if constexpr (has.value) stage(n);
+    __syncthreads();
     half8 f[2 * F];   // keys of tile n + 1, values of tile n
     auto fetch = [&](int i) {
       if (i < F)
@@ -589,59 +562,97 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
         f[i] = *reinterpret_cast<const half8 *>(s_kv[n & 3] + v_at + (2 * ((i - F) / DT) * D + 32 * ((i - F) % DT)) * 16);
     };
     constexpr int first = more.value ? 0 : F, stop = has.value ? 2 * F : F;
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) fetch(first + i);
-    if constexpr (more.value)
+    float2v scale = {1.0f, 0.0f};
+    if constexpr (more.value) {
+      scale = s_sc[(n + 1) & 3][hh];
 #pragma unroll
       for (int e = 0; e < 16; ++e) s_n[e] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(first + i);
     const float shift = (M == kNegInf ? 0.0f : lv - M) + kTop;
     Frag ph[2], pl[2];
-    float sum = 0.0f, mx = kNegInf;
+    float sum = 0.0f, mx = kNegInf, c_n = 0.0f, lv_n = 0.0f, rv_n = 0.0f;
+    bool masked = false;
+    if constexpr (!more.value)
 #pragma unroll
-    for (int i = 0; i < F; ++i) {
-      if constexpr (more.value) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (i + AHEAD < stop) fetch(i + AHEAD);
+      for (int p = 0; p < 8; ++p) softmax_pair(s, 2 * p, c, shift, sum, ph, pl);
+#pragma unroll
+    for (int i = first; i < stop; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + AHEAD < stop) fetch(i + AHEAD);
+      if (i < F) {
         s_n = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], qh[i >> 1][i & 1], s_n, 0, 0, 0);
         s_n = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], ql[i >> 1][i & 1], s_n, 0, 0, 0);
+      } else {
+        const int u = (i - F) / DT, d = (i - F) % DT;
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], ph[u].h, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], pl[u].h, o[d], 0, 0, 0);
       }
-      if constexpr (has.value) {
+      if constexpr (has.value && more.value)
 #pragma unroll
-        for (int j = 16 / F * i; j < 16 / F * (i + 1); j += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c, shift));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c, shift));
-          sum += p0 + p1;
-          const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-          const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
-          ph[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, hi);
-          pl[j >> 3].u[(j & 7) >> 1] = __builtin_bit_cast(uint32_t, lo);
+        for (int p = 0; p < 8; ++p)   // pairs of keys: the first half before the second product starts
+          if (i == (p < 4 ? p : 2 * p - 4) * F / 8) softmax_pair(s, 2 * p, c, shift, sum, ph, pl);
+      if constexpr (more.value) {
+        if (i == F / 2 + 1) {
+          masked = (base + 32 * (n + 1) < all_lo) | (base + 32 * (n + 2) > all_hi) | (__ballot(scale[1] == 0.0f) != 0);
+          c_n = scale[0] * descale;
+          lv_n = __builtin_amdgcn_logf(scale[1]);
+          rv_n = __builtin_amdgcn_rcpf(scale[1]);
+          c_n = c_n == 0.0f ? 1e-37f : c_n;   // (a masked score, -inf, stays that)
+          asm volatile("" : "+v"(c_n), "+v"(lv_n), "+v"(rv_n));
+        }
+        if (has.value && i == F - 1) store(n + 2);
+        if (has.value && i == F) load(n + 3);
+        if (i >= F + F / 2) {
+          constexpr int each = 32 / F;
+#pragma unroll
+          for (int j = each * (i - F - F / 2); j < each * (i - F - F / 2 + 1); ++j) mx = fmaxf(mx, s_n[j]);
+          asm volatile("" : "+v"(mx));
         }
       }
     }
-    if constexpr (has.value) {
-      l = fmaf(sum, rv, l);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (has.value) l = fmaf(sum, rv, l);
+    if constexpr (more.value) {
+      if constexpr (!has.value)
 #pragma unroll
-      for (int i = 0; i < F; ++i) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (F + i + AHEAD < 2 * F) fetch(F + i + AHEAD);
-        const int u = i / DT, d = i % DT;
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[F + i], ph[u].h, o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[F + i], pl[u].h, o[d], 0, 0, 0);
-        if constexpr (more.value)
+        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s_n[j]);
+      c = c_n;
+      lv = lv_n;
+      rv = rv_n;
+      if (masked) {
+        const bool there = scale[1] != 0.0f;
+        const int k0 = base + 32 * (n + 1) + 16 * hh, b = see_lo - k0, e = see_hi - k0;
+        const uint32_t from = b <= 0 ? 0xffffu : b >= 16 ? 0u : 0xffffu << b;
+        const uint32_t to = e <= 0 ? 0u : e >= 16 ? 0xffffu : (1u << e) - 1u;
+        const uint32_t on = there ? from & to & 0xffffu : 0u;
+        if (on == 0) {   // (a group of which this row sees nothing may hold any scale)
+          c = 1.0f;
+          lv = rv = 0.0f;
+        }
+        mx = kNegInf;
 #pragma unroll
-          for (int j = 16 / F * i; j < 16 / F * (i + 1); ++j) mx = fmaxf(mx, s_n[j]);
+        for (int j = 0; j < 16; ++j) {
+          s_n[j] = (on >> j) & 1u ? s_n[j] : kNegInf;
+          mx = fmaxf(mx, s_n[j]);
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
-    } else {
+      const float em = max_xor32(fmaf(mx, c, lv));
+      if (__ballot(em > M + kSlack)) {
+        const float m = em > M + kSlack ? em : M;
+        const float x = M == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(M - m);
+        l *= x;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s_n[j]);
+        for (int d = 0; d < DT; ++d) o[d] *= x;
+        M = m;
+      }
     }
-    if constexpr (more.value) settle(n + 1, s_n, mx);
   };
   constexpr std::true_type yes;
   constexpr std::false_type no;
   int n = 0;
-  if (tiles > 0) step(-1, sb, sa, no, yes);
+  step(-1, sb, sa, no, yes);
   for (; n + 2 < tiles; n += 2) {
     step(n, sa, sb, yes, yes);
     step(n + 1, sb, sa, yes, yes);
