@@ -435,8 +435,8 @@ int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v
  * key axis: kq4_attn_workspace_bytes with the same numbers. */
 int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_heads, float scale, int window,
                  int max_q, int max_kv, void *stream);
-size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim, int max_q,
-                                int max_kv);
+size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim, int window,
+                                int max_q, int max_kv);
 
 /* Most alternatives and most logits of a row that kq4_logprobs_dev takes. */
 #define KQ4_LOGPROBS_MAX_TOP 32

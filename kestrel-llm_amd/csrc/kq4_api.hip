@@ -1272,14 +1272,15 @@ int rows_check(const char *what, const char *name, const float *p, long ld, long
   return KQ4_OK;
 }
 
-KQ4AttnPlan attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv) {
-  return kq4_attn_plan(n_tok, n_seq, heads, kv_heads, max_q, max_kv, opt(kAttnTile), opt(kAttnSplit));
+KQ4AttnPlan attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int window) {
+  return kq4_attn_plan(n_tok, n_seq, heads, kv_heads, max_q, max_kv, window, opt(kAttnTile), opt(kAttnSplit));
 }
 
 size_t attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int heads, int head_dim, size_t *o_bytes) {
   *o_bytes = 0;
-  if (p.ns <= 1) return 0;
-  const size_t rows = (size_t)p.ns * n_tok * heads;
+  const int ns = p.ns16 > p.ns32 ? p.ns16 : p.ns32;
+  if (ns <= 1) return 0;
+  const size_t rows = (size_t)ns * n_tok * heads;
   *o_bytes = al256(rows * head_dim * sizeof(float));
   return *o_bytes + al256(rows * 2 * sizeof(float));
 }
@@ -1342,7 +1343,12 @@ int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_h
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;
   hipStream_t s = (hipStream_t)stream;
-  const KQ4AttnPlan plan = attn_plan(kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, max_q, max_kv);
+  const KQ4AttnPlan plan = attn_plan(kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, max_q, max_kv, window);
+  const long long blocks = (long long)kv->n_seq * kv->kv_heads * plan.ns16 +
+                           (plan.tile32 ? ((long long)kv->n_tok * (q_heads / kv->kv_heads) / plan.tile32 +
+                                           kv->n_seq) * kv->kv_heads * plan.ns32 : 0);
+  if (blocks > 0x7fffffffLL)
+    return fail(KQ4_EINVAL, "attn: n_seq=%d n_tok=%d q_heads=%d", kv->n_seq, kv->n_tok, q_heads);
   size_t o_bytes = 0;
   const size_t bytes = attn_part_bytes(plan, kv->n_tok, q_heads, kv->head_dim, &o_bytes);
   char *ws = nullptr;
@@ -1355,13 +1361,13 @@ int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_h
   return KQ4_OK;
 }
 
-size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim, int max_q,
-                                int max_kv) {
+size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim, int window,
+                                int max_q, int max_kv) {
   if (n_tok < 1 || n_seq < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads ||
-      (head_dim != 64 && head_dim != 128) || max_q < 0 || max_kv < 0)
+      (head_dim != 64 && head_dim != 128) || window < 0 || max_q < 0 || max_kv < 0)
     return 0;
   size_t o_bytes = 0;
-  return attn_part_bytes(attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv), n_tok, q_heads, head_dim,
+  return attn_part_bytes(attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv, window), n_tok, q_heads, head_dim,
                          &o_bytes);
 }
 

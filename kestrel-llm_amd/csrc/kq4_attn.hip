@@ -17,6 +17,8 @@
 #include "kq4_kv.h"
 #include "kq4_internal.h"
 
+#include <limits.h>
+
 #include <type_traits>
 
 namespace {
@@ -28,6 +30,8 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4;
+constexpr int kCus = 256;      // compute units of an MI355X
+constexpr int kJoinFew = 16;   // splits up to which a wave joins a row alone
 constexpr float kNegInf = -__builtin_inff();
 // P is held at 2^kTop for the running maximum, which is raised only where a key passes it by 2^kSlack:
 // f16 holds 2^(kTop + kSlack), and lo's last bit at the maximum is 2^-31 of it.
@@ -42,9 +46,9 @@ struct AttnArgs {
   int heads, group;   // query heads, and those per kv head
   float scale2;       // softmax scale * log2(e)
   int window;
-  int chunk, ns;      // keys per split, splits at most
-  float *part_o;      // [ns][n_tok * heads][D], unnormalised
-  float2 *part_ml;    // [ns][n_tok * heads] maximum, sum
+  KQ4AttnPlan plan;
+  float *part_o;      // [splits][n_tok * heads][D], unnormalised
+  float2 *part_ml;    // [splits][n_tok * heads] maximum, sum
 };
 
 union Frag {
@@ -138,27 +142,30 @@ KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float 
 // registers (nothing is shared between waves until they join), the next keys' loads in flight during the
 // softmax and the second product.
 template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a) {
+constexpr int kLds16 = kWaves * 16 * ((D + 4) * 4 + 8);
+template <int D>
+KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) {
   constexpr int TT = D / 64, DT = D / 16, LD = D + 4;
-  __shared__ float s_o[kWaves][16][LD];
-  __shared__ float2 s_ml[kWaves][16];
+  float(*s_o)[16][LD] = reinterpret_cast<float(*)[16][LD]>(lds);
+  float2(*s_ml)[16] = reinterpret_cast<float2(*)[16]>(lds + kWaves * 16 * LD * 4);
+  const int chunk = a.plan.chunk16, ns = a.plan.ns16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i16 = lane & 15, qd = lane >> 4;
-  const int seq = blockIdx.x / a.kv.kv_heads, h = blockIdx.x - seq * a.kv.kv_heads;
-  const int split = blockIdx.y;
+  const int seq = block / a.kv.kv_heads, h = block - seq * a.kv.kv_heads;
   const KQ4KvSpan sp = kq4_kv_span(a.kv.q_start[seq], a.kv.q_start[seq + 1], a.kv.kv_len[seq], a.kv.n_tok,
                                    a.kv.table_pages << (a.log_pg + 4));
   const int rows = sp.nq * a.group;
+  if (rows > a.plan.max16) return;
   const int *table = a.kv.block_table + (long)seq * a.kv.table_pages;
   const long n_rows = (long)a.kv.n_tok * a.heads;
 
   for (int r0 = 0; r0 < rows; r0 += 16) {
     const int last = r0 + 15 < rows ? r0 + 15 : rows - 1;
     int base, end;
-    const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, a.chunk, a.ns, &base, &end);
+    const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, ns, &base, &end);
     if (split >= used) continue;
-    base += split * a.chunk;
-    if (split + 1 < used) end = base + a.chunk;
+    base += split * chunk;
+    if (split + 1 < used) end = base + chunk;
     const int g_end = (sp.len + 15) >> 4;      // groups that hold keys
 
     // this lane's query row, the keys it sees
@@ -375,27 +382,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a)
 // in flight meanwhile. LDS holds the operands in lane order, 16 bytes a lane without bank conflicts: keys as
 // [D/8][32 keys][8], values as [8-token half][group][D][8]. The scores of tile n + 1 are formed while tile n's go
 // through the softmax, so matrix instructions and vector instructions of a wave are independent of each other.
+template <int D>
+constexpr int kLds32 = 4 * 64 * D * 2 + 64;
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
+KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, uint8_t *lds) {
   constexpr int NT = 64 * NW, TT = D / 32, DT = D / 32, TM = 32 * NW;
   constexpr int L = 4 * D, NL = (L + NT - 1) / NT;      // 16-byte loads of a tile, of a thread
   constexpr int KB = D / 8 * 32 * 16;                   // bytes of a tile's keys in LDS, and of its values
-  __shared__ __align__(16) uint8_t s_kv[4][2 * KB];
-  __shared__ float2v s_sc[4][2];
+  uint8_t(*s_kv)[2 * KB] = reinterpret_cast<uint8_t(*)[2 * KB]>(lds);
+  float2v(*s_sc)[2] = reinterpret_cast<float2v(*)[2]>(lds + 8 * KB);
+  const int chunk = a.plan.chunk32, ns = a.plan.ns32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int i32 = lane & 31, hh = lane >> 5;
-  const int h = blockIdx.x % a.kv.kv_heads, split = blockIdx.y;
+  const int h = block % a.kv.kv_heads;
   const int room = a.kv.table_pages << (a.log_pg + 4);
 
   // the sequence and row tile of this item, last tiles first (those of a prompt see the most keys)
-  int item = (int)(gridDim.x / a.kv.kv_heads) - 1 - (int)(blockIdx.x / a.kv.kv_heads), seq = -1;
+  int item = blocks / a.kv.kv_heads - 1 - block / a.kv.kv_heads, seq = -1;
   KQ4KvSpan sp{0, 0, 0, 0};
   for (int b = 0; b < a.kv.n_seq; b += 64) {
     const int i = b + lane;
     KQ4KvSpan t{0, 0, 0, 0};
     if (i < a.kv.n_seq)
       t = kq4_kv_span(a.kv.q_start[i], a.kv.q_start[i + 1], a.kv.kv_len[i], a.kv.n_tok, room);
-    const int cnt = (t.nq * a.group + TM - 1) / TM;
+    const int cnt = t.nq * a.group > a.plan.max16 ? (t.nq * a.group + TM - 1) / TM : 0;
     int sum = cnt;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -417,10 +427,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
   const int rows = sp.nq * a.group, r0 = item * TM;
   const int last = r0 + TM - 1 < rows ? r0 + TM - 1 : rows - 1;
   int base, end;
-  const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, a.chunk, a.ns, &base, &end);
+  const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, ns, &base, &end);
   if (split >= used) return;
-  base += split * a.chunk;
-  if (split + 1 < used) end = base + a.chunk;
+  base += split * chunk;
+  if (split + 1 < used) end = base + chunk;
   const int g_end = (sp.len + 15) >> 4;
   const int *table = a.kv.block_table + (long)seq * a.kv.table_pages;
 
@@ -678,19 +688,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
   if (used > 1 && hh == 0) a.part_ml[split * n_rows + row] = make_float2(M, l);
 }
 
-// Joins the splits of a row, 32 dimensions a workgroup: the factors 2^(M_s - M) of all splits into LDS, then 8
-// threads a dimension take splits in turn.
 template <int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile) {
-  __shared__ float s_f[KQ4_ATTN_MAX_SPLITS];
-  __shared__ float s_acc[8][32], s_m[4], s_l[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long row = blockIdx.x / (D / 32), n_rows = (long)a.kv.n_tok * a.heads;
-  const int d = 32 * (int)(blockIdx.x % (D / 32)) + (tid & 31);
-  const int tok = (int)(row / a.heads), head = (int)(row - (long)tok * a.heads);
-  KQ4KvSpan sp{0, 0, 0, 0};
-  bool found = false;
-  for (int b = 0; b < a.kv.n_seq && !found; b += 64) {
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a) {
+  __shared__ __align__(16) uint8_t lds[kLds16<D>];
+  attn_rows16<D>(a, blockIdx.x, blockIdx.y, lds);
+}
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t dyn_lds[];
+  attn_rows32<D, NW>(a, blockIdx.x, gridDim.x, blockIdx.y, dyn_lds);
+}
+// Both in one launch, for batches of short and long runs of tokens: the first blocks16 * ns16 workgroups are
+// attn_rows16's, each kind returning for the other's sequences.
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_mixed_kernel(AttnArgs a, int blocks16, int blocks32) {
+  extern __shared__ __align__(16) uint8_t dyn_lds[];
+  const int b = blockIdx.x, n16 = blocks16 * a.plan.ns16;
+  if (b < n16)
+    attn_rows16<D>(a, b % blocks16, b / blocks16, dyn_lds);
+  else
+    attn_rows32<D, kWaves>(a, (b - n16) % blocks32, blocks32, (b - n16) / blocks32, dyn_lds);
+}
+
+// The split plan of a row's sequence and the splits its tile used; 0 for a row of no sequence. Wave-uniform tok.
+KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
+  for (int b = 0; b < a.kv.n_seq; b += 64) {
     const int i = b + lane;
     KQ4KvSpan t{0, 0, 0, 0};
     if (i < a.kv.n_seq)
@@ -699,17 +721,64 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile) {
     const unsigned long long at = __ballot(tok >= t.q0 && tok < t.q0 + t.nq);
     if (at) {
       const int l = __ffsll((long long)at) - 1;
-      sp = KQ4KvSpan{__builtin_amdgcn_readlane(t.q0, l), __builtin_amdgcn_readlane(t.nq, l),
-                     __builtin_amdgcn_readlane(t.p0, l), __builtin_amdgcn_readlane(t.len, l)};
-      found = true;
+      const KQ4KvSpan sp{__builtin_amdgcn_readlane(t.q0, l), __builtin_amdgcn_readlane(t.nq, l),
+                         __builtin_amdgcn_readlane(t.p0, l), __builtin_amdgcn_readlane(t.len, l)};
+      const int rows = sp.nq * a.group;
+      const bool small = rows <= a.plan.max16;
+      const int tile = small ? 16 : a.plan.tile32;
+      const int r = (tok - sp.q0) * a.group + head % a.group, r0 = r - r % tile;
+      const int last = r0 + tile - 1 < rows ? r0 + tile - 1 : rows - 1;
+      int base, end;
+      return kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, small ? a.plan.chunk16 : a.plan.chunk32,
+                           small ? a.plan.ns16 : a.plan.ns32, &base, &end);
     }
   }
-  if (!found) return;   // a row behind the last sequence
-  const int r = (tok - sp.q0) * a.group + head % a.group, r0 = r - r % tile;
-  const int rows = sp.nq * a.group, last = r0 + tile - 1 < rows ? r0 + tile - 1 : rows - 1;
-  int base, end;
-  const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, a.chunk, a.ns, &base, &end);
-  if (used == 1) return;   // written by its only split
+  return 0;
+}
+
+// The factor of a split's sums in the joined row (one of which nothing was seen: 0; one whose scales were all NaN
+// keeps its NaN).
+KQ4_DEV float split_factor(float2 ml, float m) {
+  return ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
+}
+
+// Joins the splits of a row, few of them: a wave a row.
+template <int D>
+__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long row = blockIdx.x * 4L + (threadIdx.x >> 6), n_rows = (long)a.kv.n_tok * a.heads;
+  if (row >= n_rows) return;
+  const int tok = __builtin_amdgcn_readfirstlane((int)(row / a.heads)), head = (int)(row - (long)tok * a.heads);
+  const int used = splits_used(a, tok, head, lane);
+  if (used <= 1) return;   // no sequence's row, or written by its only split
+  float m = kNegInf, sl = 0.0f, acc[E] = {};
+  for (int s = 0; s < used; ++s) m = fmaxf(m, a.part_ml[s * n_rows + row].x);
+#pragma unroll 4
+  for (int s = 0; s < used; ++s) {
+    const float2 ml = a.part_ml[s * n_rows + row];
+    const float f = split_factor(ml, m);
+    sl = fmaf(ml.y, f, sl);
+    const float *p = a.part_o + (s * n_rows + row) * D + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(p[e], f, acc[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) a.out[row * D + E * lane + e] = sl == 0.0f ? 0.0f : acc[e] / sl;
+}
+
+// Joins the splits of a row, many of them, 32 dimensions a workgroup: the factors of all splits into LDS, then 8
+// threads a dimension take splits in turn.
+template <int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  __shared__ float s_f[KQ4_ATTN_MAX_SPLITS];
+  __shared__ float s_acc[8][32], s_m[4], s_l[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long row = blockIdx.x / (D / 32), n_rows = (long)a.kv.n_tok * a.heads;
+  const int d = 32 * (int)(blockIdx.x % (D / 32)) + (tid & 31);
+  const int tok = (int)(row / a.heads), head = (int)(row - (long)tok * a.heads);
+  const int used = splits_used(a, tok, head, lane);
+  if (used <= 1) return;
 
   float m = kNegInf;
   for (int s = tid; s < used; s += 256) m = fmaxf(m, a.part_ml[s * n_rows + row].x);
@@ -721,8 +790,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile) {
   float sl = 0.0f;
   for (int s = tid; s < used; s += 256) {
     const float2 ml = a.part_ml[s * n_rows + row];
-    // (a split of which nothing was seen: 0; one whose scales were all NaN keeps its NaN)
-    const float f = ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
+    const float f = split_factor(ml, m);
     s_f[s] = f;
     sl = fmaf(ml.y, f, sl);
   }
@@ -745,50 +813,87 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile) {
 }
 
 template <int D>
-int launch(const AttnArgs &a, int tile, hipStream_t s) {
-  if (tile == 16) {
-    attn_rows16_kernel<D><<<dim3((unsigned)a.kv.n_seq * a.kv.kv_heads, a.ns), 64 * kWaves, 0, s>>>(a);
+int launch(const AttnArgs &a, hipStream_t s) {
+  const KQ4AttnPlan &p = a.plan;
+  const int blocks16 = a.kv.n_seq * a.kv.kv_heads;
+  const int blocks32 = p.tile32 ? (int)(((long)a.kv.n_tok * a.group / p.tile32 + a.kv.n_seq) * a.kv.kv_heads) : 0;
+  static std::atomic<unsigned long long> lds8{0}, lds4{0}, ldsm{0};
+  constexpr int lds = kLds32<D>;
+  hipError_t e = hipSuccess;
+  if (p.tile32 == 128 && p.max16) {
+    const void *fn = reinterpret_cast<const void *>(&attn_mixed_kernel<D>);
+    if ((e = kq4_lds_limit_once(fn, lds, ldsm)) != hipSuccess) return (int)e;
+    attn_mixed_kernel<D><<<blocks16 * p.ns16 + blocks32 * p.ns32, 256, lds, s>>>(a, blocks16, blocks32);
   } else {
-    const dim3 grid((unsigned)(((long)a.kv.n_tok * a.group / tile + a.kv.n_seq) * a.kv.kv_heads), a.ns);
-    if (tile == 128)
-      attn_rows32_kernel<D, 4><<<grid, 256, 0, s>>>(a);
-    else
-      attn_rows32_kernel<D, 8><<<grid, 512, 0, s>>>(a);
+    if (p.tile32 == 128) {
+      const void *fn = reinterpret_cast<const void *>(&attn_rows32_kernel<D, 4>);
+      if ((e = kq4_lds_limit_once(fn, lds, lds4)) != hipSuccess) return (int)e;
+      attn_rows32_kernel<D, 4><<<dim3(blocks32, p.ns32), 256, lds, s>>>(a);
+    } else if (p.tile32) {
+      const void *fn = reinterpret_cast<const void *>(&attn_rows32_kernel<D, 8>);
+      if ((e = kq4_lds_limit_once(fn, lds, lds8)) != hipSuccess) return (int)e;
+      attn_rows32_kernel<D, 8><<<dim3(blocks32, p.ns32), 512, lds, s>>>(a);
+    }
+    if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+    if (p.max16) attn_rows16_kernel<D><<<dim3(blocks16, p.ns16), 64 * kWaves, 0, s>>>(a);
   }
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
-  if (a.ns > 1) {
+  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  const int ns = p.ns16 > p.ns32 ? p.ns16 : p.ns32;
+  if (ns > 1) {
     const long n_rows = (long)a.kv.n_tok * a.heads;
-    attn_join_kernel<D><<<(unsigned)(n_rows * (D / 32)), 256, 0, s>>>(a, tile);
+    if (ns <= kJoinFew)
+      attn_join_few_kernel<D><<<(unsigned)((n_rows + 3) / 4), 256, 0, s>>>(a);
+    else
+      attn_join_kernel<D><<<(unsigned)(n_rows * (D / 32)), 256, 0, s>>>(a);
   }
   return (int)hipGetLastError();
 }
 
+// Splits of `keys` keys so that `base` workgroups become about `want`, each of at least min_chunk keys and at most
+// max_chunk (a split's workgroup walks its keys alone, however long other sequences are).
+void split_keys(long keys, long base, int want, int step, int min_chunk, int max_chunk, int force, int *chunk,
+                int *ns) {
+  long n = want / (base < 1 ? 1 : base);
+  const long most = (keys + min_chunk - 1) / min_chunk, least = (keys + max_chunk - 1) / max_chunk;
+  if (n > most) n = most;
+  if (n < least) n = least;
+  if (force > 0) n = force;
+  if (n > (keys + step - 1) / step) n = (keys + step - 1) / step;
+  if (n > KQ4_ATTN_MAX_SPLITS) n = KQ4_ATTN_MAX_SPLITS;
+  if (n < 1) n = 1;
+  *chunk = (int)(((keys + n - 1) / n + step - 1) / step * step);
+  *ns = (int)((keys + *chunk - 1) / *chunk);
+}
+
 }  // namespace
 
-KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int force_tile,
-                          int force_split) {
-  KQ4AttnPlan p;
-  const long keys = max_kv < 1 ? 1 : max_kv;
+KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int window,
+                          int force_tile, int force_split) {
   const int group = heads / kv_heads;
-  p.tile = force_tile == 16 || force_tile == 128 || force_tile == 256 ? force_tile : (long)max_q * group <= 16 ? 16 : 256;
-  const long step = p.tile == 16 ? 64 * kWaves : 64;           // keys of a workgroup's turn
-  const long items = p.tile == 16 ? n_seq : (long)n_tok * group / p.tile + n_seq;
-  const long base = items * kv_heads;                          // workgroups of one split
-  const long most = (keys + step - 1) / step;
-  long ns = ((p.tile == 16 ? 512 : 256) + base - 1) / base;
-  if (force_split > 0) ns = force_split;
-  if (ns > most) ns = most;
-  if (ns > KQ4_ATTN_MAX_SPLITS) ns = KQ4_ATTN_MAX_SPLITS;
-  if (ns < 1) ns = 1;
-  p.chunk = (int)(((keys + ns - 1) / ns + step - 1) / step * step);
-  p.ns = (int)((keys + p.chunk - 1) / p.chunk);
+  const long rows = (long)max_q * group;
+  // keys of a tile's queries, at most: the window's reach where that is less
+  long keys = max_kv < 1 ? 1 : max_kv;
+  if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
+  KQ4AttnPlan p{0, 256, 0, 0, 64, 0};
+  p.tile32 = force_tile == 16                                           ? 0
+             : force_tile == 128 || force_tile == 256                   ? force_tile
+             : rows <= 16                                               ? 0
+             : ((long)n_tok * group / 256 + n_seq) * kv_heads >= kCus   ? 256
+                                                                        : 128;
+  const bool mixed = p.tile32 && force_tile == 0 && n_seq > 1 && (long)n_tok != (long)n_seq * max_q;
+  p.max16 = !p.tile32 ? INT_MAX : mixed ? 16 : 0;
+  if (p.max16)
+    split_keys(keys, (long)n_seq * kv_heads, kCus, 64 * kWaves, 64 * kWaves, mixed ? 1024 : 8192, force_split,
+               &p.chunk16, &p.ns16);
+  if (p.tile32)
+    split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus, 64,
+               512, INT_MAX, force_split, &p.chunk32, &p.ns32);
   return p;
 }
 
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
                     int window, const KQ4AttnPlan &plan, float *part_o, float *part_ml, hipStream_t s) {
   AttnArgs a{kv, log_pg, q, ldq, out, heads, heads / kv.kv_heads, scale * 1.44269504088896340736f, window,
-             plan.chunk, plan.ns, part_o, reinterpret_cast<float2 *>(part_ml)};
-  return kv.head_dim == 128 ? launch<128>(a, plan.tile, s) : launch<64>(a, plan.tile, s);
+             plan, part_o, reinterpret_cast<float2 *>(part_ml)};
+  return kv.head_dim == 128 ? launch<128>(a, s) : launch<64>(a, s);
 }

@@ -8,12 +8,15 @@
 //
 // One pass: a workgroup holds 8192 logits of a row in registers (32 a thread), reduces its (m, z, t) and
 // picks its n_top best; a second launch joins a row's pieces. Candidates for the best are the elements that
-// reach the n_top-th largest of the threads' own maxima (there are at least n_top of those, and few more in
-// most rows), ordered by rank counting. Rows where many elements tie for it are selected exactly instead,
-// by bisection of the key and then of the index.
+// reach a threshold that at least n_top elements reach: the largest of the waves' n_top-th largest lane maxima, to 16
+// bits.
+// Few others reach it in most rows, and a thread whose own maximum does not is done. The candidates are ordered by
+// rank counting. Rows where too many elements reach it (many equal ones), and rows with a NaN, are selected
+// exactly instead, by bisection of the key and then of the index.
 // The order is that of the key: the logit's, ties to the lowest index; -inf is never a candidate.
 #include "kq4_common.h"
 #include "kq4_internal.h"
+#include "../../include/kq4.h"
 
 namespace {
 
@@ -32,15 +35,34 @@ KQ4_DEV float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// A wave's sum or maximum in every lane: DPP moves within rows of 16 lanes, then the swaps of rows and halves.
+template <int CTRL>
+KQ4_DEV uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+constexpr int kQuad1 = 0xB1, kQuad2 = 0x4E, kRow4 = 0x124, kRow8 = 0x128;   // xor 1, xor 2, rotate by 4, by 8
 KQ4_DEV float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+  v += __uint_as_float(dpp<kQuad1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp<kQuad2>(__float_as_uint(v)));
+  v += __uint_as_float(dpp<kRow4>(__float_as_uint(v)));
+  v += __uint_as_float(dpp<kRow8>(__float_as_uint(v)));
+  return kq4_xor_add<32>(kq4_xor_add<16>(v));
+}
+KQ4_DEV int wave_sum(int n) {
+  uint32_t v = (uint32_t)n;
+  v += dpp<kQuad1>(v);
+  v += dpp<kQuad2>(v);
+  v += dpp<kRow4>(v);
+  v += dpp<kRow8>(v);
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] + r[1];
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (int)(r[0] + r[1]);
 }
 KQ4_DEV float wave_max(float v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-  return v;
+  v = kq4_max32(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 struct Piece {   // of one row: maximum, z and t relative to it, whether it has a NaN
@@ -49,130 +71,149 @@ struct Piece {   // of one row: maximum, z and t relative to it, whether it has 
 };
 
 // Element i of a thread is logit base + at(i).
-template <bool V4>
-KQ4_DEV int at(int i) {
-  return V4 ? (i >> 2) * (4 * kThreads) + 4 * (int)threadIdx.x + (i & 3) : i * kThreads + (int)threadIdx.x;
-}
+KQ4_DEV int at(int i) { return (i >> 2) * (4 * kThreads) + 4 * (int)threadIdx.x + (i & 3); }
 
-template <bool V4>
+struct __attribute__((packed, aligned(4))) Four {   // 16 bytes at any 4-byte address
+  float v[4];
+};
+
 __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *__restrict__ logits, long ld,
-                                                                  int vocab, int n_pieces, int n_top, Piece *__restrict__ pieces,
+                                                                  int vocab, int n_pieces, int n_top,
+                                                                  Piece *__restrict__ pieces,
                                                                   unsigned long long *__restrict__ best) {
-  __shared__ float s_m[4], s_z[4], s_t[4];
-  __shared__ __align__(16) uint32_t s_keys[kThreads];
-  __shared__ uint32_t s_nan[4], s_thr;
+  __shared__ float s_m[4], s_z[4], s_t[4], s_thr[4];
   __shared__ int s_ones[4], s_count[4];
   __shared__ int s_n;
-  __shared__ unsigned long long s_cand[kCand];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) unsigned long long s_cand[kCand];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x / n_pieces, piece = blockIdx.x - row * n_pieces, base = piece * kPiece;
   const float *x = logits + row * ld + base;
   const int n = vocab - base < kPiece ? vocab - base : kPiece;
 
   float v[kPer];
-  if constexpr (V4) {
+  if (n == kPiece) {
 #pragma unroll
     for (int i = 0; i < kPer; i += 4) {
-      const int o = at<V4>(i);
-      float4 f = make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
-      if (o + 4 <= n) {
-        f = *reinterpret_cast<const float4 *>(x + o);
-      } else if (o < n) {
-        f.x = x[o];
-        if (o + 1 < n) f.y = x[o + 1];
-        if (o + 2 < n) f.z = x[o + 2];
-      }
-      v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+      const Four f = *reinterpret_cast<const Four *>(x + at(i));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + j] = f.v[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = at<V4>(i) < n ? x[at<V4>(i)] : kNegInf;
+    for (int i = 0; i < kPer; i += 4) {
+      const int o = at(i);
+      Four f = {{kNegInf, kNegInf, kNegInf, kNegInf}};
+      if (o + 4 <= n) {
+        f = *reinterpret_cast<const Four *>(x + o);
+      } else {
+        if (o < n) f.v[0] = x[o];
+        if (o + 1 < n) f.v[1] = x[o + 1];
+        if (o + 2 < n) f.v[2] = x[o + 2];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + j] = f.v[j];
+    }
   }
 
-  float mt = kNegInf;
-  bool nan = false;
+  float mt = v[0];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    mt = fmaxf(mt, v[i]);
-    nan |= v[i] != v[i];
-  }
+  for (int i = 1; i < kPer; ++i) mt = fmaxf(mt, v[i]);
   const float mw = wave_max(mt);
-  const bool nw = __ballot(nan) != 0;
-  if (lane == 0) {
-    s_m[wave] = mw;
-    s_nan[wave] = nw;
+  if (n_top > 0) {
+    // a value that n_top lanes' maxima reach, 16 bits of the largest such key (or -inf)
+    const uint32_t k = key_of(mt);
+    uint32_t reach = 0;
+#pragma unroll
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+      if ((int)__popcll(__ballot(k >= (reach | bit))) >= n_top) reach |= bit;
+    if (lane == 0) s_thr[wave] = reach > kKeyNegInf ? key_value(reach) : kNegInf;
   }
-  s_keys[tid] = nan ? 0xffffffffu : key_of(mt);
-  if (tid == 0) {
-    s_thr = 0;
-    s_n = 0;
-  }
+  if (lane == 0) s_m[wave] = mw;
+  if (tid == 0) s_n = 0;
   __syncthreads();
   const float m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
 
-  // the maximum's elements are counted, the others summed
+  // the maximum's elements are counted, the others summed (only a wave that has it looks for them)
   float z = 0.0f, t = 0.0f;
   int ones = 0;
   if (m > kNegInf) {
+    if (mw == m) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const float d = fmaxf(v[i] - m, kFar);
-      const float e = v[i] == m ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
-      ones += v[i] == m;
-      z += e;
-      t = fmaf(e, d, t);
+      for (int i = 0; i < kPer; ++i) {
+        const float d = v[i] - m;
+        const float e = d == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
+        ones += d == 0.0f;
+        z += e;
+        t = fmaf(e, fmaxf(d, kFar), t);
+      }
+      ones = wave_sum(ones);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float d = v[i] - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
+        z += e;
+        t = fmaf(e, fmaxf(d, kFar), t);
+      }
     }
-  }
-  z = wave_sum(z);
-  t = wave_sum(t);
+    z = wave_sum(z);   // (a NaN among the logits makes it NaN; the maxima pass over it)
+    t = wave_sum(t);
+  } else {
+    bool nan = false;
 #pragma unroll
-  for (int x2 = 32; x2; x2 >>= 1) ones += __shfl_xor(ones, x2);
+    for (int i = 0; i < kPer; ++i) nan |= v[i] != v[i];
+    if (__ballot(nan)) z = __uint_as_float(0x7fc00000u);
+  }
   if (lane == 0) {
     s_z[wave] = z;
     s_t[wave] = t;
     s_ones[wave] = ones;
   }
   unsigned long long *out = best + (long)blockIdx.x * n_top;
-
   if (n_top > 0) {
-    // the n_top-th largest of the threads' maxima
-    const uint32_t mine = s_keys[tid];
-    int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < kThreads; j += 4) {
-      const uint4 k = *reinterpret_cast<const uint4 *>(&s_keys[j]);
-      above += (k.x > mine || (k.x == mine && j < tid)) + (k.y > mine || (k.y == mine && j + 1 < tid)) +
-               (k.z > mine || (k.z == mine && j + 2 < tid)) + (k.w > mine || (k.w == mine && j + 3 < tid));
-    }
-    if (above == n_top - 1) s_thr = mine > kKeyNegInf ? mine : kKeyNegInf + 1;
-    __syncthreads();
-    const uint32_t thr = s_thr;
+    const float thr = fmaxf(fmaxf(s_thr[0], s_thr[1]), fmaxf(s_thr[2], s_thr[3]));
+    // (a threshold of -inf: fewer than n_top lanes of every wave have anything else; every such element, up to
+    // the limit)
+    const bool mine = thr > kNegInf ? mt >= thr : mt > kNegInf;
+    if (__ballot(mine)) {
+      int c = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t k = key_of(v[i]);
-      const unsigned long long in = __ballot(k >= thr);
-      if (in) {
-        int first = 0;
-        if (lane == 0) first = atomicAdd(&s_n, (int)__popcll(in));
-        first = __builtin_amdgcn_readfirstlane(first);
-        const int slot = first + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-        if (k >= thr && slot < kCand) s_cand[slot] = ((unsigned long long)k << 32) | (uint32_t)~(base + at<V4>(i));
+      for (int i = 0; i < kPer; ++i) c += (v[i] >= thr) & (v[i] > kNegInf);
+      int sum = c;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const int o = __shfl_up(sum, s);
+        if (lane >= s) sum += o;
+      }
+      int slot = 0;
+      if (lane == 63) slot = atomicAdd(&s_n, sum);
+      slot = __builtin_amdgcn_readlane(slot, 63) + sum - c;
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if ((v[i] >= thr) & (v[i] > kNegInf)) {
+            if (slot < kCand) s_cand[slot] = ((unsigned long long)key_of(v[i]) << 32) | (uint32_t)~(base + at(i));
+            ++slot;
+          }
       }
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  const bool has_nan = !(s_z[0] + s_z[1] + s_z[2] + s_z[3] >= 0.0f);
+  if (n_top > 0) {
     int nc = s_n;
-    if (nc > kCand) {
-      // too many ties: the n_top-th key by bisection, then how far into its equals
+    if (nc > kCand || has_nan) {
+      // the n_top-th key by bisection, then how far into its equals
       auto count = [&](auto pred) {
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) c += (int)__popcll(__ballot(pred(i)));
+        for (int i = 0; i < kPer; ++i) c += pred(i);
+        c = wave_sum(c);
         __syncthreads();
         if (lane == 0) s_count[wave] = c;
         __syncthreads();
         return s_count[0] + s_count[1] + s_count[2] + s_count[3];
       };
-      uint32_t lo = thr, hi = 0xffffffffu;   // the largest key that at least n_top elements reach
+      uint32_t lo = kKeyNegInf + 1, hi = 0xffffffffu;   // the largest key that at least n_top elements reach
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2 + 1;
         if (count([&](int i) { return key_of(v[i]) >= mid; }) >= n_top) lo = mid;
@@ -182,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
       int a = 0, b = kPiece - 1;             // the smallest end that leaves n_top - more equals
       while (a < b) {
         const int mid = (a + b) / 2;
-        if (count([&](int i) { return key_of(v[i]) == lo && at<V4>(i) <= mid; }) >= n_top - more) b = mid;
+        if (count([&](int i) { return key_of(v[i]) == lo && at(i) <= mid; }) >= n_top - more) b = mid;
         else a = mid + 1;
       }
       if (tid == 0) s_n = 0;
@@ -190,28 +231,23 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const uint32_t k = key_of(v[i]);
-        if (k > lo || (k == lo && at<V4>(i) <= a))
-          s_cand[atomicAdd(&s_n, 1)] = ((unsigned long long)k << 32) | (uint32_t)~(base + at<V4>(i));
+        if (k > lo || (k == lo && at(i) <= a))
+          s_cand[atomicAdd(&s_n, 1)] = ((unsigned long long)k << 32) | (uint32_t)~(base + at(i));
       }
       __syncthreads();
       nc = s_n;
     }
     for (int c = tid; c < nc; c += kThreads) {
-      const unsigned long long mine2 = s_cand[c];
+      const unsigned long long mine = s_cand[c];
       int rank = 0;
-      for (int j = 0; j < nc; ++j) rank += s_cand[j] > mine2;
-      if (rank < n_top) out[rank] = mine2;
+#pragma unroll 4
+      for (int j = 0; j < nc; ++j) rank += s_cand[j] > mine;
+      if (rank < n_top) out[rank] = mine;
     }
     for (int j = nc + tid; j < n_top; j += kThreads) out[j] = 0;
-  } else {
-    __syncthreads();
   }
   if (tid == 0) {
-    Piece p;
-    p.m = m;
-    p.z = 0.0f;
-    p.t = 0.0f;
-    p.nan = s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3];
+    Piece p{m, 0.0f, 0.0f, has_nan};
     if (m > kNegInf) {
       p.z = ((s_z[0] + s_z[1]) + (s_z[2] + s_z[3])) + (float)(s_ones[0] + s_ones[1] + s_ones[2] + s_ones[3] - 1);
       p.t = (s_t[0] + s_t[1]) + (s_t[2] + s_t[3]);
@@ -220,17 +256,28 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
   }
 }
 
-// Joins a row's pieces, one wave a row.
-__global__ __launch_bounds__(64) void logprobs_join_kernel(const float *__restrict__ logits, long ld, int vocab,
+// Joins a row's pieces, a workgroup a row (each wave forms the sums for itself).
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const float *__restrict__ logits, long ld, int vocab,
                                                            int n_pieces, int n_top, const int *__restrict__ token,
                                                            const Piece *__restrict__ pieces,
                                                            const unsigned long long *__restrict__ best,
                                                            float *logprob, float *entropy, float *top_logprob,
                                                            int *top_id) {
   extern __shared__ unsigned long long s_list[];
-  const int lane = threadIdx.x;
+  __shared__ int s_n;
+  __shared__ unsigned long long s_thr;
+  const int tid = threadIdx.x, lane = tid & 63;
   const long row = blockIdx.x;
   const Piece *p = pieces + row * n_pieces;
+  const int id = logprob ? token[row] : -1;
+  const float at_id = id >= 0 && id < vocab ? logits[row * ld + id] : 0.0f;
+  // the pieces' lists, each sorted (0: no element), behind the room for those that are kept
+  unsigned long long *s_all = s_list + n_pieces * n_top;
+  if (tid == 0) {
+    s_n = 0;
+    s_thr = 0;
+  }
+  for (int i = tid; i < n_pieces * n_top; i += kThreads) s_all[i] = best[row * n_pieces * n_top + i];
 
   float M = kNegInf;
   bool nan = false;
@@ -258,51 +305,48 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const float *__restri
   z = wave_sum(z);
   t = wave_sum(t);
   const float bad = __uint_as_float(0x7fc00000u), lz = log1pf(z);
-  if (lane == 0) {
+  if (tid == 0) {
     if (logprob) {
-      const int id = token[row];
       float r = bad;
-      if (id >= 0 && id < vocab && !nan) r = M > kNegInf ? (logits[row * ld + id] - M) - lz : kNegInf;
+      if (id >= 0 && id < vocab && !nan) r = M > kNegInf ? (at_id - M) - lz : kNegInf;
       logprob[row] = r;
     }
     if (entropy) entropy[row] = nan ? bad : M > kNegInf ? lz - t / (1.0f + z) : 0.0f;
   }
   if (n_top == 0) return;
 
-  // each of the pieces has ceil(n_top / n_pieces) elements that reach the least of those
-  const unsigned long long *l = best + row * n_pieces * n_top;
-  const int q = (n_top + n_pieces - 1) / n_pieces;
-  unsigned long long thr = ~0ull;
-  for (int i = lane; i < n_pieces; i += 64) {
-    const unsigned long long e = l[(long)i * n_top + q - 1];
-    thr = e < thr ? e : thr;
-  }
-#pragma unroll
-  for (int x = 32; x; x >>= 1) {
-    const unsigned long long o = __shfl_xor(thr, x);
-    thr = o < thr ? o : thr;
-  }
-  int nc = 0;
-  for (int b = 0; b < n_pieces * n_top; b += 64) {
-    const unsigned long long e = b + lane < n_pieces * n_top ? l[b + lane] : 0;
-    const bool in = e != 0 && e >= thr;
-    const unsigned long long all = __ballot(in);
-    if (in) s_list[nc + (int)__popcll(all & ((1ull << lane) - 1))] = e;
-    nc += (int)__popcll(all);
+  // at least n_top elements reach the `lists`-th largest of the lists' q-th elements
+  int q = n_top < 4 ? n_top : 4;
+  if (q * n_pieces < n_top) q = (n_top + n_pieces - 1) / n_pieces;
+  const int lists = (n_top + q - 1) / q;
+  __syncthreads();
+  if (tid < n_pieces) {
+    const unsigned long long e = s_all[tid * n_top + q - 1];
+    int above = 0;
+    for (int j = 0; j < n_pieces; ++j) above += s_all[j * n_top + q - 1] > e;
+    if (e != 0 && above == lists - 1) s_thr = e;
   }
   __syncthreads();
+  const unsigned long long thr = s_thr;
+  for (int i = tid; i < n_pieces * n_top; i += kThreads) {
+    const unsigned long long e = s_all[i];
+    if (e != 0 && e >= thr) s_list[atomicAdd(&s_n, 1)] = e;
+  }
+  __syncthreads();
+  const int nc = s_n;
   float *out_lp = top_logprob + row * n_top;
   int *out_id = top_id + row * n_top;
-  for (int c = lane; c < nc; c += 64) {
+  for (int c = tid; c < nc; c += kThreads) {
     const unsigned long long e = s_list[c];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < nc; ++j) rank += s_list[j] > e;
     if (rank < n_top) {
       out_lp[rank] = nan ? bad : (key_value((uint32_t)(e >> 32)) - M) - lz;
       out_id[rank] = (int)~(uint32_t)e;
     }
   }
-  if (nc < n_top) {   // the lowest ids of those at -inf (n_top <= 32: the first 64 ids hold enough)
+  if (nc < n_top && tid < 64) {   // the lowest ids of those at -inf (n_top <= 32: the first 64 ids hold enough)
     bool taken = lane >= vocab;
     for (int j = 0; j < nc; ++j) taken |= (int)~(uint32_t)s_list[j] == lane;
     const unsigned long long open = __ballot(!taken);
@@ -325,13 +369,13 @@ int kq4_launch_logprobs(const float *logits, long ld, int n, int vocab, int n_to
   const int np = kq4_logprobs_pieces(vocab);
   Piece *pc = static_cast<Piece *>(pieces);
   const unsigned grid = (unsigned)((long)n * np);
-  if ((uintptr_t)logits % 16 == 0 && ld % 4 == 0)
-    logprobs_piece_kernel<true><<<grid, kThreads, 0, s>>>(logits, ld, vocab, np, n_top, pc, best);
-  else
-    logprobs_piece_kernel<false><<<grid, kThreads, 0, s>>>(logits, ld, vocab, np, n_top, pc, best);
-  const hipError_t e = hipGetLastError();
+  logprobs_piece_kernel<<<grid, kThreads, 0, s>>>(logits, ld, vocab, np, n_top, pc, best);
+  static std::atomic<unsigned long long> limit{0};
+  constexpr int most = 2 * (KQ4_LOGPROBS_MAX_VOCAB / kPiece) * KQ4_LOGPROBS_MAX_TOP * (int)sizeof(unsigned long long);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) e = kq4_lds_limit_once(reinterpret_cast<const void *>(&logprobs_join_kernel), most, limit);
   if (e != hipSuccess) return (int)e;
-  logprobs_join_kernel<<<(unsigned)n, 64, (size_t)np * n_top * sizeof(unsigned long long), s>>>(
+  logprobs_join_kernel<<<(unsigned)n, kThreads, 2 * (size_t)np * n_top * sizeof(unsigned long long), s>>>(
       logits, ld, vocab, np, n_top, token, pc, best, logprob, entropy, top_logprob, top_id);
   return (int)hipGetLastError();
 }

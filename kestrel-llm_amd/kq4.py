@@ -71,7 +71,7 @@ SIGNATURES = [
     ("kq4_kv_scales_bytes", ctypes.c_size_t, [_I, _I, _I, _I]),
     ("kq4_kv_append_dev", _I, [_P, _P, ctypes.c_long, _P, ctypes.c_long, _P]),
     ("kq4_attn_dev", _I, [_P, _P, _P, ctypes.c_long, _I, ctypes.c_float, _I, _I, _I, _P]),
-    ("kq4_attn_workspace_bytes", ctypes.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
+    ("kq4_attn_workspace_bytes", ctypes.c_size_t, [_I] * 8),
     ("kq4_logprobs_dev", _I, [_P, _P, _P, _P, _P, ctypes.c_long, _P, _I, _I, _I, _P]),
     ("kq4_logprobs_workspace_bytes", ctypes.c_size_t, [_I, _I, _I]),
     # C11 op wrappers (include/kq4_ops.h)
@@ -832,8 +832,8 @@ def kv_append_dev(kv, k, v, stream=None):
           "kq4_kv_append_dev")
 
 
-def attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv):
-    return lib().kq4_attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv)
+def attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv, window=0):
+    return lib().kq4_attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, window, max_q, max_kv)
 
 
 def attn_dev(out, q, kv, q_heads, scale, max_q, max_kv, window=0, stream=None):

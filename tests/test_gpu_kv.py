@@ -200,6 +200,29 @@ def test_attention_bounds_change_no_result(kq4, torch_dev, max_q, max_kv):
     check_attn(kq4, torch_dev, b, rand(rng, b.n, 8, 128), 8, max_q=max_q, max_kv=max_kv)
 
 
+@pytest.mark.parametrize("tile", [16, 128, 256])
+@pytest.mark.parametrize("split", [1, 2, 5, 20])
+def test_attention_forms(kq4, torch_dev, tile, split):
+    """Every form and number of splits, also where the planner would take another."""
+    rng = np.random.default_rng(tile + split)
+    b = Batch(rng, [(1, 1400), (90, 90), (3, 700), (0, 9), (40, 1000)], 2, 64, 32, 64, pad=3)
+    b.fill(rng, upto="all", spread=1.0)
+    x = rand(rng, b.n, 6, 64)
+    with kq4.options(attn_tile=tile, attn_split=split):
+        check_attn(kq4, torch_dev, b, x, 6)
+        check_attn(kq4, torch_dev, b, x, 6, window=300)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [[(1, 9000)], [(1, 7000), (1, 50), (1, 4097)], [(30, 5000)], [(1, 6000), (70, 300)]])
+def test_attention_long_contexts(kq4, torch_dev, dim, lens):
+    """Many splits of the key axis, sequences that use few of them beside those that use all."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, lens, 1, dim, 64, dim)
+    b.fill(rng, upto="all", spread=1.0)
+    check_attn(kq4, torch_dev, b, rand(rng, b.n, 4, dim), 4)
+
+
 @pytest.mark.parametrize("lens", [[(1, 400), (1, 0), (5, 3), (1, 90)], [(70, 60), (64, 400), (1, 0)]])
 def test_attention_empty_rows_and_missing_pages(kq4, torch_dev, lens):
     """Sequences without keys, tokens before position 0, pages that the cache does not have, positions past the

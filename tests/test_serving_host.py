@@ -80,7 +80,7 @@ def test_workspace_of_captured_calls(standin):  # noqa: F811
     grow it, done after a reservation of the bytes they name."""
     res = standin(SETUP + """
 calls = [lambda: attn(kv(), max_q=1, max_kv=100000), lambda: logprobs()]
-need = [k.kq4_attn_workspace_bytes(7, 3, 32, 8, 128, 1, 100000), k.kq4_logprobs_workspace_bytes(4, 1000, 5)]
+need = [k.kq4_attn_workspace_bytes(7, 3, 32, 8, 128, 0, 1, 100000), k.kq4_logprobs_workspace_bytes(4, 1000, 5)]
 hip.standin_capture(1)
 before = [launched(f) for f in calls]
 hip.standin_capture(0)
