@@ -406,12 +406,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
     if (i < a.kv.n_seq)
       t = kq4_kv_span(a.kv.q_start[i], a.kv.q_start[i + 1], a.kv.kv_len[i], a.kv.n_tok, room);
     const int cnt = t.nq * a.group > a.plan.max16 ? (t.nq * a.group + TM - 1) / TM : 0;
-    int sum = cnt;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int o = __shfl_up(sum, m);
-      if (lane >= m) sum += o;
-    }
+    const int sum = kq4_scan_add(cnt);
     const unsigned long long at = __ballot(sum > item);
     if (at) {
       const int l = __ffsll((long long)at) - 1;

@@ -178,12 +178,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
       int c = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) c += (v[i] >= thr) & (v[i] > kNegInf);
-      int sum = c;
-#pragma unroll
-      for (int s = 1; s < 64; s <<= 1) {
-        const int o = __shfl_up(sum, s);
-        if (lane >= s) sum += o;
-      }
+      const int sum = kq4_scan_add(c);
       int slot = 0;
       if (lane == 63) slot = atomicAdd(&s_n, sum);
       slot = __builtin_amdgcn_readlane(slot, 63) + sum - c;
