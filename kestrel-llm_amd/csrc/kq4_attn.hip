@@ -77,31 +77,58 @@ KQ4_DEV float max_xor32(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Chunk c (16 dimensions) of a query row, rotated as the keys were (fp32 here: q is not rounded to a
-// grid afterwards). cs: the row's cosines and sines, nullptr without a rotation of the row.
-KQ4_DEV void load_q_chunk(const float *row, int c, int rp, const float2 *cs, bool bad, float (&x)[16]) {
-#pragma unroll
-  for (int e = 0; e < 16; e += 4) {
-    const float4 a = *reinterpret_cast<const float4 *>(row + 16 * c + e);
-    x[e] = a.x; x[e + 1] = a.y; x[e + 2] = a.z; x[e + 3] = a.w;
+// What a query row is rotated by: its row of the table, or none (rp: rotated chunk pairs).
+struct QRope {
+  int rp;
+  bool bad;
+  const float *cs;
+};
+KQ4_DEV QRope q_rope(const kq4_kv &kv, int token, int pos) {
+  QRope r{kv.rope_dim / 32, false, nullptr};
+  if (r.rp) {
+    const int row = kv.rope_pos ? kv.rope_pos[token] : pos;
+    r.bad = row < 0 || row >= kv.rope_rows;
+    r.cs = kv.rope + (long)(r.bad ? 0 : row) * kv.rope_dim;
   }
-  if (c >= 2 * rp) return;
-  if (bad) {
+  return r;
+}
+
+// Chunks c0, c0 + step, .. (16 dimensions each) of a query row, rotated as the keys were (in fp32 here: q is not
+// rounded to a grid afterwards). All loads first.
+template <int N>
+KQ4_DEV void load_q(const float *row, const QRope &r, int c0, int step, float (*x)[16]) {
+  float4v own[N][4], other[N][4], cs[N][8];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(0x7fc00000u);
-    return;
+  for (int k = 0; k < N; ++k) {
+    const int c = c0 + k * step;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[k][e] = reinterpret_cast<const float4v *>(row + 16 * c)[e];
+    if (r.rp) {   // (a chunk that is not rotated: itself and the table's first columns, not used)
+      const bool up = c >= r.rp, rot = c < 2 * r.rp;
+      const int o = !rot ? c : up ? c - r.rp : c + r.rp;
+      const float2v *t = reinterpret_cast<const float2v *>(r.cs) + (rot ? 16 * (up ? o : c) : 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) other[k][e] = reinterpret_cast<const float4v *>(row + 16 * o)[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2v f = t[2 * e], g = t[2 * e + 1];
+        cs[k][e] = float4v{f[0], f[1], g[0], g[1]};
+      }
+    }
   }
-  const bool up = c >= rp;             // the second of a pair: x2 c + x1 s, else x1 c - x2 s
-  const int o = up ? c - rp : c + rp;
-  const float2 *t = cs + 16 * (up ? o : c);
 #pragma unroll
-  for (int e = 0; e < 16; e += 4) {
-    const float4 a = *reinterpret_cast<const float4 *>(row + 16 * o + e);
-    const float y[4] = {a.x, a.y, a.z, a.w};
+  for (int k = 0; k < N; ++k) {
+    const int c = c0 + k * step;
+    const bool up = c >= r.rp, rot = c < 2 * r.rp;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = t[e + i];
-      x[e + i] = fmaf(x[e + i], f.x, up ? y[i] * f.y : -(y[i] * f.y));
+    for (int e = 0; e < 16; ++e) {
+      x[k][e] = own[k][e >> 2][e & 3];
+      if (r.rp) {
+        // the first of a pair: x1 c - x2 s, the second: x2 c + x1 s
+        const float co = cs[k][e >> 1][2 * (e & 1)], si = cs[k][e >> 1][2 * (e & 1) + 1];
+        const float y = fmaf(x[k][e], co, other[k][e >> 2][e & 3] * (up ? si : -si));
+        x[k][e] = !rot ? x[k][e] : r.bad ? __uint_as_float(0x7fc00000u) : y;
+      }
     }
   }
 }
@@ -177,33 +204,6 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
     kq4_kv_sees(sp.p0 + last / a.group, sp.len, a.window, &all_lo, &t_);
     kq4_kv_sees(sp.p0 + r0 / a.group, sp.len, a.window, &t_, &all_hi);
 
-    half8 qh[TT][2], ql[TT][2];
-    float descale;
-    {
-      const float *row = a.q + (sp.q0 + tq) * a.ldq + (long)head * D;
-      const int rp = a.kv.rope_dim / 32;
-      const float2 *cs = nullptr;
-      bool bad = false;
-      if (rp) {
-        const int pr = a.kv.rope_pos ? a.kv.rope_pos[sp.q0 + tq] : sp.p0 + tq;
-        bad = pr < 0 || pr >= a.kv.rope_rows;
-        cs = reinterpret_cast<const float2 *>(a.kv.rope) + (long)(bad ? 0 : pr) * (a.kv.rope_dim / 2);
-      }
-      float x[TT][16], amax = 0.0f;
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        load_q_chunk(row, 4 * t + qd, rp, cs, bad, x[t]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
-      }
-      const int sh = row_shift(max_xor32(max_xor16(amax)));
-      descale = ldexpf(a.scale2, -sh);
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) split_f16(&x[t][8 * u], sh, qh[t][u], ql[t][u]);
-    }
-
     float4v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -242,6 +242,23 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
         for (int t = 0; t < TT; ++t) kr[t4][t] = *reinterpret_cast<const uint4 *>(kp + 1024 * t + 64 * t4);
 #pragma unroll
       for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const uint4 *>(vp + 256 * d);
+    }
+
+    half8 qh[TT][2], ql[TT][2];
+    float descale;
+    {
+      float x[TT][16], amax = 0.0f;
+      load_q<TT>(a.q + (sp.q0 + tq) * a.ldq + (long)head * D, q_rope(a.kv, sp.q0 + tq, sp.p0 + tq), qd, 4, x);
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
+      const int sh = row_shift(max_xor32(max_xor16(amax)));
+      descale = ldexpf(a.scale2, -sh);
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) split_f16(&x[t][8 * u], sh, qh[t][u], ql[t][u]);
     }
 
     auto step = [&](auto more) {
@@ -444,21 +461,14 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   float descale;
   {
     const float *row = a.q + (sp.q0 + tq) * a.ldq + (long)head * D;
-    const int rp = a.kv.rope_dim / 32;
-    const float2 *cs = nullptr;
-    bool bad = false;
-    if (rp) {
-      const int pr = a.kv.rope_pos ? a.kv.rope_pos[sp.q0 + tq] : sp.p0 + tq;
-      bad = pr < 0 || pr >= a.kv.rope_rows;
-      cs = reinterpret_cast<const float2 *>(a.kv.rope) + (long)(bad ? 0 : pr) * (a.kv.rope_dim / 2);
-    }
+    const QRope rope = q_rope(a.kv, sp.q0 + tq, sp.p0 + tq);
     float x[TT][16], amax = 0.0f;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      load_q_chunk(row, 2 * t + hh, rp, cs, bad, x[t]);
+    for (int t = 0; t < TT; t += 2) load_q<2>(row, rope, 2 * t + hh, 2, x + t);
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
-    }
     const int sh = row_shift(max_xor32(amax));
     descale = ldexpf(a.scale2, -sh);
 #pragma unroll

@@ -758,25 +758,40 @@ def rope_table(rows, dim, theta, device="cuda"):
     return torch.stack([a.cos(), a.sin()], 2).float().contiguous().to(device)
 
 
-def _here(t, name):
-    """Raises unless t is on the current device, which the call's launches go to."""
+def _check_here(device, name):
+    """Raises unless `device` (an index) is the current one, which the call's launches go to."""
     import torch
-    if t is not None and t.device.index != torch.cuda.current_device():
-        raise KQ4Error(f"{name}: on {t.device}, the current device is {torch.cuda.current_device()}")
+    if device != torch.cuda.current_device():
+        raise KQ4Error(f"{name}: on device {device}, the current device is {torch.cuda.current_device()}")
 
 
-def _rows(t, name, n, width):
-    """Row stride of a [>= n][>= width] fp32 device tensor with unit column stride, checked."""
+def _rows(t, name, n, width, device):
+    """Row stride of a [>= n][width] fp32 tensor on `device` with unit column stride, checked."""
     import torch
+    if isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is torch.float32 and \
+            t.dim() == 2:
+        (rows, cols), (ld, step) = t.shape, t.stride()
+        if rows >= n and cols == width and (step == 1 or width <= 1):
+            return ld if rows > 1 else max(ld, width)
+    _need_on(t, name, torch.float32, device)
+    raise KQ4Error(f"{name}: expected [{n}, {width}] with unit column stride, got {tuple(t.shape)} "
+                   f"strides {t.stride()}")
+
+
+def _need_on(t, name, dtype, device, numel=0):
+    """_need for a tensor on `device`, of any strides with numel 0."""
+    import torch
+    if isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is dtype and \
+            (not numel or (t.is_contiguous() and t.numel() >= numel)):
+        return
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != device:
+        raise KQ4Error(f"{name}: on {t.device}, expected device {device}")
+    if numel:
+        _need(t, name, dtype, numel)
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise KQ4Error(f"{name}: not a device tensor")
-    if t.dtype != torch.float32:
-        raise KQ4Error(f"{name}: dtype {t.dtype}, expected torch.float32")
-    if t.dim() != 2 or t.shape[0] < n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
-        raise KQ4Error(f"{name}: expected [{n}, {width}] with unit column stride, got {tuple(t.shape)} "
-                       f"strides {t.stride()}")
-    _here(t, name)
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    if t.dtype != dtype:
+        raise KQ4Error(f"{name}: dtype {t.dtype}, expected {dtype}")
 
 
 class KVBatch:
@@ -825,9 +840,9 @@ class KVBatch:
 
 def kv_append_dev(kv, k, v, stream=None):
     """Appends the batch's keys (rotated) and values, [n_tok][kv_heads * head_dim] each, to its cache."""
-    width = kv.kv_heads * kv.head_dim
-    ldk, ldv = _rows(k, "k", kv.n_tok, width), _rows(v, "v", kv.n_tok, width)
-    _here(kv.tensors["codes"], "cache")
+    width, dev = kv.kv_heads * kv.head_dim, kv.device
+    ldk, ldv = _rows(k, "k", kv.n_tok, width, dev), _rows(v, "v", kv.n_tok, width, dev)
+    _check_here(dev, "cache")
     check(lib().kq4_kv_append_dev(kv.p, k.data_ptr(), ldk, v.data_ptr(), ldv, _stream_ptr(stream)),
           "kq4_kv_append_dev")
 
@@ -840,11 +855,10 @@ def attn_dev(out, q, kv, q_heads, scale, max_q, max_kv, window=0, stream=None):
     """out [n_tok][q_heads * head_dim] = attention of q (rotated as it is read) over the batch's cache;
     max_q / max_kv: the batch's most tokens of a sequence and longest kv_len, or bounds (speed only)."""
     import torch
-    width = q_heads * kv.head_dim
-    ldq = _rows(q, "q", kv.n_tok, width)
-    _need(out, "out", torch.float32, kv.n_tok * width)
-    _here(out, "out")
-    _here(kv.tensors["codes"], "cache")
+    width, dev = q_heads * kv.head_dim, kv.device
+    ldq = _rows(q, "q", kv.n_tok, width, dev)
+    _need_on(out, "out", torch.float32, dev, kv.n_tok * width)
+    _check_here(dev, "cache")
     check(lib().kq4_attn_dev(out.data_ptr(), kv.p, q.data_ptr(), ldq, q_heads, scale, window, max_q,
                              max_kv, _stream_ptr(stream)), "kq4_attn_dev")
 
@@ -860,20 +874,23 @@ def logprobs_dev(logits, token=None, logprob=None, entropy=None, top_logprob=Non
     import torch
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise KQ4Error("logits: expected a [n, vocab] device tensor")
-    n, vocab = logits.shape
-    ld = _rows(logits, "logits", n, vocab)
+    (n, vocab), dev = logits.shape, logits.get_device()
+    ld = _rows(logits, "logits", n, vocab, dev if dev >= 0 else None)
     n_top = 0
     if top_logprob is not None or top_id is not None:
         if top_logprob is None or top_id is None or top_logprob.dim() != 2 or \
                 top_logprob.shape != top_id.shape or top_logprob.shape[0] != n:
             raise KQ4Error("top_logprob and top_id: both [n, n_top]")
         n_top = top_logprob.shape[1]
-    for name, t, dtype, numel in (("token", token, torch.int32, n), ("logprob", logprob, torch.float32, n),
-                                  ("entropy", entropy, torch.float32, n),
-                                  ("top_logprob", top_logprob, torch.float32, n * n_top),
-                                  ("top_id", top_id, torch.int32, n * n_top)):
-        _need(t, name, dtype, numel, optional=True)
-        _here(t, name)
+        _need_on(top_logprob, "top_logprob", torch.float32, dev, n * n_top)
+        _need_on(top_id, "top_id", torch.int32, dev, n * n_top)
+    if token is not None:
+        _need_on(token, "token", torch.int32, dev, n)
+    if logprob is not None:
+        _need_on(logprob, "logprob", torch.float32, dev, n)
+    if entropy is not None:
+        _need_on(entropy, "entropy", torch.float32, dev, n)
+    _check_here(dev, "logits")
     check(lib().kq4_logprobs_dev(_tp(logprob), _tp(entropy), _tp(top_logprob), _tp(top_id),
                                  logits.data_ptr(), ld, _tp(token), n, vocab, n_top,
                                  _stream_ptr(stream)), "kq4_logprobs_dev")
