@@ -29,8 +29,8 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-constexpr int kWaves = 4;
 constexpr int kCus = 256;      // compute units of an MI355X
+constexpr int kMinChunk = 384; // keys that a split of the 32-row form has at least
 constexpr int kJoinFew = 16;   // splits up to which a wave joins a row alone
 constexpr float kNegInf = -__builtin_inff();
 // P is held at 2^kTop for the running maximum, which is raised only where a key passes it by 2^kSlack:
@@ -168,13 +168,13 @@ KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float 
 // A workgroup is one sequence, kv head and split; its waves take 64 keys in turn straight from memory to
 // registers (nothing is shared between waves until they join), the next keys' loads in flight during the
 // softmax and the second product.
-template <int D>
-constexpr int kLds16 = kWaves * 16 * ((D + 4) * 4 + 8);
-template <int D>
+template <int D, int NW>
+constexpr int kLds16 = NW * 16 * ((D + 4) * 4 + 8);
+template <int D, int NW>
 KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) {
   constexpr int TT = D / 64, DT = D / 16, LD = D + 4;
   float(*s_o)[16][LD] = reinterpret_cast<float(*)[16][LD]>(lds);
-  float2(*s_ml)[16] = reinterpret_cast<float2(*)[16]>(lds + kWaves * 16 * LD * 4);
+  float2(*s_ml)[16] = reinterpret_cast<float2(*)[16]>(lds + NW * 16 * LD * 4);
   const int chunk = a.plan.chunk16, ns = a.plan.ns16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i16 = lane & 15, qd = lane >> 4;
@@ -221,7 +221,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
                  ? (((long)page * a.kv.kv_heads + h) << a.log_pg) | (g & ((1 << a.log_pg) - 1))
                  : -1;
     };
-    constexpr int kStep = 64 * kWaves;
+    constexpr int kStep = 64 * NW;
     const int ik = i16 >> 2;                 // this lane's key row's group; qd: that of its scales and values
     uint4 kr[4][TT], vr[DT];
     int key = base + 64 * wave;
@@ -365,15 +365,15 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
     for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v *>(&s_o[wave][i16][16 * d + 4 * qd]) = o[d];
     if (qd == 0) s_ml[wave][i16] = make_float2(M, l);
     __syncthreads();
-    for (int i = threadIdx.x; i < (last - r0 + 1) * (D / 4); i += 64 * kWaves) {
+    for (int i = threadIdx.x; i < (last - r0 + 1) * (D / 4); i += 64 * NW) {
       const int rr = i / (D / 4), d = 4 * (i - rr * (D / 4));
       float m = kNegInf;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_ml[w][rr].x);
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, s_ml[w][rr].x);
       float sl = 0.0f;
       float4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float2 ml = s_ml[w][rr];
         const float f = ml.x == kNegInf && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x == kNegInf ? 0.0f : ml.x - m);
         sl = fmaf(ml.y, f, sl);
@@ -693,10 +693,10 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   if (used > 1 && hh == 0) a.part_ml[split * n_rows + row] = make_float2(M, l);
 }
 
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_rows16_kernel(AttnArgs a) {
-  __shared__ __align__(16) uint8_t lds[kLds16<D>];
-  attn_rows16<D>(a, blockIdx.x, blockIdx.y, lds);
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_rows16_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t dyn_lds[];
+  attn_rows16<D, NW>(a, blockIdx.x, blockIdx.y, dyn_lds);
 }
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
@@ -706,13 +706,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
 // Both in one launch, for batches of short and long runs of tokens: the first blocks16 * ns16 workgroups are
 // attn_rows16's, each kind returning for the other's sequences.
 template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_mixed_kernel(AttnArgs a, int blocks16, int blocks32) {
+__global__ __launch_bounds__(256, 2) void attn_mixed_kernel(AttnArgs a, int blocks16, int blocks32) {
   extern __shared__ __align__(16) uint8_t dyn_lds[];
   const int b = blockIdx.x, n16 = blocks16 * a.plan.ns16;
   if (b < n16)
-    attn_rows16<D>(a, b % blocks16, b / blocks16, dyn_lds);
+    attn_rows16<D, 4>(a, b % blocks16, b / blocks16, dyn_lds);
   else
-    attn_rows32<D, kWaves>(a, (b - n16) % blocks32, blocks32, (b - n16) / blocks32, dyn_lds);
+    attn_rows32<D, 4>(a, (b - n16) % blocks32, blocks32, (b - n16) / blocks32, dyn_lds);
 }
 
 // The split plan of a row's sequence and the splits its tile used; 0 for a row of no sequence. Wave-uniform tok.
@@ -840,7 +840,14 @@ int launch(const AttnArgs &a, hipStream_t s) {
       attn_rows32_kernel<D, 8><<<dim3(blocks32, p.ns32), 512, lds, s>>>(a);
     }
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-    if (p.max16) attn_rows16_kernel<D><<<dim3(blocks16, p.ns16), 64 * kWaves, 0, s>>>(a);
+    if (p.max16 && p.waves16 == 8) {
+      static std::atomic<unsigned long long> lds16{0};
+      const void *fn = reinterpret_cast<const void *>(&attn_rows16_kernel<D, 8>);
+      if ((e = kq4_lds_limit_once(fn, kLds16<D, 8>, lds16)) != hipSuccess) return (int)e;
+      attn_rows16_kernel<D, 8><<<dim3(blocks16, p.ns16), 512, kLds16<D, 8>, s>>>(a);
+    } else if (p.max16) {
+      attn_rows16_kernel<D, 4><<<dim3(blocks16, p.ns16), 256, kLds16<D, 4>, s>>>(a);
+    }
   }
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
   const int ns = p.ns16 > p.ns32 ? p.ns16 : p.ns32;
@@ -879,7 +886,7 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   // keys of a tile's queries, at most: the window's reach where that is less
   long keys = max_kv < 1 ? 1 : max_kv;
   if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
-  KQ4AttnPlan p{0, 256, 0, 0, 64, 0};
+  KQ4AttnPlan p{0, 0, 256, 0, 0, 64, 0};
   p.tile32 = force_tile == 16                                           ? 0
              : force_tile == 128 || force_tile == 256                   ? force_tile
              : rows <= 16                                               ? 0
@@ -887,12 +894,16 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
                                                                         : 128;
   const bool mixed = p.tile32 && force_tile == 0 && n_seq > 1 && (long)n_tok != (long)n_seq * max_q;
   p.max16 = !p.tile32 ? INT_MAX : mixed ? 16 : 0;
-  if (p.max16)
-    split_keys(keys, (long)n_seq * kv_heads, kCus, 64 * kWaves, 64 * kWaves, mixed ? 1024 : 8192, force_split,
-               &p.chunk16, &p.ns16);
+  if (p.max16) {
+    // 8 waves a workgroup, 4 where 64 keys a wave leave SIMDs idle (the shortest path then counts: one sequence of
+    // 1001 keys, 8 kv heads: 10.8 us in 4 splits of 4 waves, 11.9 in one of 8; one of 131072, 4 kv heads: 34.2 and 33.0)
+    p.waves16 = !mixed && keys / 64 * n_seq * kv_heads > 4 * kCus ? 8 : 4;
+    const int turn = 64 * p.waves16;
+    split_keys(keys, (long)n_seq * kv_heads, kCus, turn, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
+  }
   if (p.tile32)
     split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus, 64,
-               512, INT_MAX, force_split, &p.chunk32, &p.ns32);
+               kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
   return p;
 }
 

@@ -8,11 +8,10 @@
 //
 // One pass: a workgroup holds 8192 logits of a row in registers (32 a thread), reduces its (m, z, t) and
 // picks its n_top best; a second launch joins a row's pieces. Candidates for the best are the elements that
-// reach a threshold that at least n_top elements reach: the largest of the waves' n_top-th largest lane maxima, to 16
-// bits.
-// Few others reach it in most rows, and a thread whose own maximum does not is done. The candidates are ordered by
-// rank counting. Rows where too many elements reach it (many equal ones), and rows with a NaN, are selected
-// exactly instead, by bisection of the key and then of the index.
+// reach a threshold that at least n_top elements reach: the n_top-th largest of the threads' maxima, to 16 bits, by
+// bisection in one wave while the others sum. Few others reach it in most rows (of 8192 normal ones about 21 the
+// largest 20 of 256 maxima). They are ordered by rank counting. Rows where too many elements reach it (many equal
+// ones), and rows with a NaN, are selected exactly instead, by bisection of the key and then of the index.
 // The order is that of the key: the logit's, ties to the lowest index; -inf is never a candidate.
 #include "kq4_common.h"
 #include "kq4_internal.h"
@@ -20,7 +19,7 @@
 
 namespace {
 
-constexpr int kThreads = 256, kPer = 32, kPiece = kThreads * kPer, kCand = 512;
+constexpr int kThreads = 256, kPer = 32, kPiece = kThreads * kPer, kCand = 128;   // (kCand: a wave's)
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kFar = -1000.0f;   // e^d is 0 long before; no product of it with a 0 or a sum overflows
@@ -81,10 +80,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
                                                                   int vocab, int n_pieces, int n_top,
                                                                   Piece *__restrict__ pieces,
                                                                   unsigned long long *__restrict__ best) {
-  __shared__ float s_m[4], s_z[4], s_t[4], s_thr[4];
+  __shared__ float s_m[4], s_z[4], s_t[4], s_thr;
   __shared__ int s_ones[4], s_count[4];
   __shared__ int s_n;
-  __shared__ __align__(16) unsigned long long s_cand[kCand];
+  __shared__ __align__(16) uint32_t s_key[kThreads];
+  __shared__ __align__(16) unsigned long long s_cand[4][kCand];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x / n_pieces, piece = blockIdx.x - row * n_pieces, base = piece * kPiece;
   const float *x = logits + row * ld + base;
@@ -119,19 +119,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
 #pragma unroll
   for (int i = 1; i < kPer; ++i) mt = fmaxf(mt, v[i]);
   const float mw = wave_max(mt);
-  if (n_top > 0) {
-    // a value that n_top lanes' maxima reach, 16 bits of the largest such key (or -inf)
-    const uint32_t k = key_of(mt);
-    uint32_t reach = 0;
-#pragma unroll
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
-      if ((int)__popcll(__ballot(k >= (reach | bit))) >= n_top) reach |= bit;
-    if (lane == 0) s_thr[wave] = reach > kKeyNegInf ? key_value(reach) : kNegInf;
-  }
   if (lane == 0) s_m[wave] = mw;
-  if (tid == 0) s_n = 0;
+  s_key[tid] = key_of(mt);
   __syncthreads();
   const float m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  if (wave == 0 && n_top > 0) {
+    // a value that n_top threads' maxima reach, 16 bits of the largest such key (or the least number, where fewer have
+    // anything but -inf: then every such element, up to the limit)
+    const uint4 k = *reinterpret_cast<const uint4 *>(&s_key[4 * lane]);
+    uint32_t reach = 0;
+#pragma unroll
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+      const uint32_t c = reach | bit;
+      if ((int)(__popcll(__ballot(k.x >= c)) + __popcll(__ballot(k.y >= c)) + __popcll(__ballot(k.z >= c)) +
+                __popcll(__ballot(k.w >= c))) >= n_top)
+        reach = c;
+    }
+    if (lane == 0) s_thr = reach > kKeyNegInf ? key_value(reach) : -__FLT_MAX__;
+  }
 
   // the maximum's elements are counted, the others summed (only a wave that has it looks for them)
   float z = 0.0f, t = 0.0f;
@@ -168,35 +173,26 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
     s_t[wave] = t;
     s_ones[wave] = ones;
   }
-  unsigned long long *out = best + (long)blockIdx.x * n_top;
-  if (n_top > 0) {
-    const float thr = fmaxf(fmaxf(s_thr[0], s_thr[1]), fmaxf(s_thr[2], s_thr[3]));
-    // (a threshold of -inf: fewer than n_top lanes of every wave have anything else; every such element, up to
-    // the limit)
-    const bool mine = thr > kNegInf ? mt >= thr : mt > kNegInf;
-    if (__ballot(mine)) {
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) c += (v[i] >= thr) & (v[i] > kNegInf);
-      const int sum = kq4_scan_add(c);
-      int slot = 0;
-      if (lane == 63) slot = atomicAdd(&s_n, sum);
-      slot = __builtin_amdgcn_readlane(slot, 63) + sum - c;
-      if (mine) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if ((v[i] >= thr) & (v[i] > kNegInf)) {
-            if (slot < kCand) s_cand[slot] = ((unsigned long long)key_of(v[i]) << 32) | (uint32_t)~(base + at(i));
-            ++slot;
-          }
-      }
-    }
-  }
   __syncthreads();
   const bool has_nan = !(s_z[0] + s_z[1] + s_z[2] + s_z[3] >= 0.0f);
   if (n_top > 0) {
-    int nc = s_n;
-    if (nc > kCand || has_nan) {
+    unsigned long long *out = best + (long)blockIdx.x * n_top;
+    const float thr = s_thr;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool in = v[i] >= thr;
+      const unsigned long long all = __ballot(in);
+      if (all) {
+        const int slot = c + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+        if (in && slot < kCand) s_cand[wave][slot] = ((unsigned long long)key_of(v[i]) << 32) | (uint32_t)~(base + at(i));
+        c += (int)__popcll(all);
+      }
+    }
+    if (lane == 0) s_count[wave] = c;
+    __syncthreads();
+    int n0 = s_count[0], n1 = s_count[1], n2 = s_count[2], n3 = s_count[3];
+    if (n0 > kCand || n1 > kCand || n2 > kCand || n3 > kCand || has_nan) {
       // the n_top-th key by bisection, then how far into its equals
       auto count = [&](auto pred) {
         int c = 0;
@@ -224,19 +220,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
       if (tid == 0) s_n = 0;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < kPer; ++i) {       // (n_top elements, or fewer where there are no more than that)
         const uint32_t k = key_of(v[i]);
         if (k > lo || (k == lo && at(i) <= a))
-          s_cand[atomicAdd(&s_n, 1)] = ((unsigned long long)k << 32) | (uint32_t)~(base + at(i));
+          s_cand[0][atomicAdd(&s_n, 1)] = ((unsigned long long)k << 32) | (uint32_t)~(base + at(i));
       }
       __syncthreads();
-      nc = s_n;
+      n0 = s_n;
+      n1 = n2 = n3 = 0;
     }
-    for (int c = tid; c < nc; c += kThreads) {
-      const unsigned long long mine = s_cand[c];
+    const int nc = n0 + n1 + n2 + n3;
+    for (int i = tid; i < nc; i += kThreads) {
+      int w = 0, j = i;   // entry j of wave w's
+      if (j >= n0) { j -= n0; w = 1; }
+      if (w == 1 && j >= n1) { j -= n1; w = 2; }
+      if (w == 2 && j >= n2) { j -= n2; w = 3; }
+      const unsigned long long mine = s_cand[w][j];
       int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < nc; ++j) rank += s_cand[j] > mine;
+      for (int q = 0; q < n0; ++q) rank += s_cand[0][q] > mine;
+      for (int q = 0; q < n1; ++q) rank += s_cand[1][q] > mine;
+      for (int q = 0; q < n2; ++q) rank += s_cand[2][q] > mine;
+      for (int q = 0; q < n3; ++q) rank += s_cand[3][q] > mine;
       if (rank < n_top) out[rank] = mine;
     }
     for (int j = nc + tid; j < n_top; j += kThreads) out[j] = 0;
