@@ -48,6 +48,11 @@
  * Error convention: device-pointer calls return KQ4_OK (0) or a negative KQ4_E* code;
  * host-pointer drop-in calls return 1 (done on the GPU) or 0 (not done: the caller runs its
  * CPU path). kq4_last_error() describes the last failure of the calling thread.
+ *
+ * Between the linear layers: the paged int8 key/value cache (kq4_kv_append_dev), the attention
+ * that reads it (kq4_attn_dev) and the reading of the logits (kq4_logprobs_dev) take and leave
+ * fp32 rows on the device as the linear layers do, under the same rules for streams, graphs,
+ * workspace and errors.
  */
 #ifndef KQ4_H
 #define KQ4_H
@@ -130,7 +135,9 @@ const char *kq4_version(void);
  * -1 the planner's choice, the default), gemm_prio (the pipelined int8 GEMM's issue priority
  * falling with progress through K, so the workgroups sharing a CU end together: 0 off, 1 on,
  * -1 the planner's choice: token-major, on for 128x128 launches of whole rounds of two workgroups
- * per CU and for every 64x128 launch; on records, on; the same outputs). The initial value
+ * per CU and for every 64x128 launch; on records, on; the same outputs), attn_tile (the attention's
+ * form: 16, 128 or 256 rows a workgroup, 0 the planner's choice) and attn_split (ranges of a
+ * sequence's keys, 0 the planner's choice; both within the rounding of the sums). The initial value
  * of each comes from the environment variable KQ4_ + its upper-case name, else the built-in
  * default (for most, the planner's own choice); value < 0 restores that initial value. Takes
  * effect for launches planned after it returns. */
@@ -370,33 +377,36 @@ int kq4_moe_ffn_stages_dev(float *Y, const float *X, const int *sel, const float
 
 /* ---- the steps between the linear layers (device pointers, stream-ordered) ----------------- */
 
-/* A layer's paged int8 key/value cache and the batch that a call works on: `n_seq` sequences, whose
+/* A layer's paged int8 key/value cache and the batch that a call works on: n_seq sequences, whose
  * n_tok tokens lie one sequence after the other. All pointers are device memory.
  *
- * The cache is n_pages pages of page_tokens tokens (a power of two, 16..4096). 16 consecutive positions
- * of a sequence are a group; per kv head a group has 16 keys, 16 values, and one scale for each:
+ * The cache is n_pages pages of page_tokens tokens (a power of two, 16..4096). 16 consecutive
+ * positions of a sequence are a group; per kv head a group has 16 keys, 16 values, and one scale
+ * for each:
  *   codes   [n_pages][kv_heads][page_tokens / 16][2][16 * head_dim] bytes, first the keys as
- *           [head_dim / 16][16 tokens][16], then the values as [head_dim][16 tokens]; a byte is its
- *           code + 128, |code| <= 127 (16-byte aligned; kq4_kv_codes_bytes)
- *   scales  [n_pages][kv_heads][page_tokens / 16][2] floats (8-byte aligned; kq4_kv_scales_bytes)
- * and a code stands for code * scale. Memory of slots that hold no token is never used, so a new cache
- * needs no clearing.
+ *           [head_dim / 16][16 tokens][16], then the values as [head_dim][16 tokens]; a byte is
+ *           its code + 128, |code| <= 127 (16-byte aligned; kq4_kv_codes_bytes)
+ *   scales  [n_pages][kv_heads][page_tokens / 16][2] floats, key and value scale, at least 2^-100
+ *           (8-byte aligned; kq4_kv_scales_bytes)
+ * and a code stands for code * scale. Memory of slots that hold no token is never used, so a new
+ * cache needs no clearing.
  *
- * Position j of sequence i is on page block_table[i][j / page_tokens] (each row table_pages entries). Its
- * tokens are rows q_start[i] .. q_start[i + 1] - 1 of the call and its last positions before kv_len[i],
- * the length with them. Rows that belong to no sequence are neither read nor written. Entries that make no sense are
- * not followed: a page number outside the cache has no keys and takes none, positions past the table have
- * none either, tokens before position 0 (kv_len smaller than the sequence's tokens) have neither key nor
- * keys to see.
+ * Position j of sequence i is on page block_table[i][j / page_tokens] (rows of table_pages
+ * entries). Its tokens are rows q_start[i] .. q_start[i + 1] - 1 of the call and its last
+ * positions before kv_len[i], the length with them. Rows that belong to no sequence are neither
+ * read nor written. Entries that make no sense are not followed: a page number outside the cache
+ * has no keys and takes none, positions past the table have none either, and tokens before
+ * position 0 (kv_len smaller than the sequence's tokens) have neither a key nor keys to see.
  *
- * rope, when not NULL: rope_rows rows of rope_dim / 2 pairs (cos, sin), 8-byte aligned. Keys, as they are
- * appended, and queries, as they are read, have dimensions i and i + rope_dim / 2 rotated for i < rope_dim / 2
- * (rope_dim a multiple of 32, at most head_dim; 0 and NULL: no rotation) by the row of their position, or
- * by row rope_pos[token] where rope_pos is not NULL (an index per token of the call: sections of several
- * position axes, or another numbering). A token whose row the table does not have gets NaN for its key
- * (its group is NaN from then on) and for its attention.
+ * rope, when not NULL: rope_rows rows of rope_dim / 2 pairs (cos, sin), 8-byte aligned. Keys, as
+ * they are appended, and queries, as they are read, have dimensions i and i + rope_dim / 2 rotated
+ * for i < rope_dim / 2 (rope_dim a multiple of 32, at most head_dim; 0 and NULL: no rotation) by
+ * the row of their position, or by row rope_pos[token] where rope_pos is not NULL (an index per
+ * token of the call: sections of several position axes, or another numbering). A token whose row
+ * the table does not have gets NaN for its key (its group is NaN from then on) and its attention.
  *
- * No counterpart in the reference's GPU boundary: its KV cache and attention stay on the host. */
+ * No counterpart in the reference's accelerator boundary: its cache and attention stay on the
+ * host. */
 typedef struct kq4_kv {
   uint8_t *codes;
   float *scales;
@@ -415,44 +425,52 @@ typedef struct kq4_kv {
 size_t kq4_kv_codes_bytes(int n_pages, int page_tokens, int kv_heads, int head_dim);
 size_t kq4_kv_scales_bytes(int n_pages, int page_tokens, int kv_heads, int head_dim);
 
-/* Appends the call's keys and values (k, v: row t at t * ldk / t * ldv floats, [kv_heads][head_dim]; 16-byte
- * aligned, strides multiples of 4), the keys rotated. Over a group's new tokens the scale is
- * fl(amax / 127), at least 2^-100, and at least the group's present scale if it holds earlier tokens; codes are
- * rint(fl(x * fl(1 / scale))). Where the scale grows, the earlier tokens' codes are rewritten as
- * rint(fl(code * fl(old / new))); a group's scale starts anew with its first slot. Rotated keys are
- * x1 c - x2 s and x2 c + x1 s rounded to fp32 once. A NaN or infinity makes its group's scale NaN or
- * infinite. Tokens past a group's new ones are left as they were, and bytes of other groups. Pages that a
- * call appends to belong to one sequence each; any number of sequences may share the pages before. */
-int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v, long ldv, void *stream);
+/* Appends the call's keys and values (k, v: row t at t * ldk / t * ldv floats, [kv_heads]
+ * [head_dim]; 16-byte aligned, strides multiples of 4), the keys rotated. Over a group's new
+ * tokens the scale is fl(amax / 127), at least 2^-100, and at least the group's present scale if
+ * it holds earlier tokens; codes are rint(fl(x * fl(1 / scale))). Where the scale grows, the
+ * earlier tokens' codes are rewritten as rint(fl(code * fl(old / new))); a group's scale starts
+ * anew with its first slot. Rotated keys are x1 c - x2 s and x2 c + x1 s rounded to fp32 once. A
+ * NaN or infinity makes its group's scale NaN or infinite (codes 0). Slots of a group past its new
+ * tokens are left as they were. Every page that a call appends to belongs to one sequence; any
+ * number of sequences may share the pages before. Uses no workspace. */
+int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v, long ldv,
+                      void *stream);
 
 /* Attention of the call's queries over the cache (after kq4_kv_append_dev of the same batch):
- * out [n_tok][q_heads][head_dim] = softmax(scale * q . k) v over the keys at or before the query's position, with
- * window > 0 the last `window` of them (the query's own among them). q: row t at t * ldq floats, [q_heads]
- * [head_dim], 16-byte aligned, ldq a multiple of 4; query head j reads kv head j / (q_heads / kv_heads). A row that sees no key is
- * zeros. scale > 0. out must not overlap q. max_q and max_kv are the batch's largest number of tokens of a sequence and
- * largest kv_len, or bounds of them: they choose the launch's shape, and smaller or larger values
- * change no more than its speed (and the order of sums). The workspace holds the partial sums of a split
- * key axis: kq4_attn_workspace_bytes with the same numbers. */
-int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_heads, float scale, int window,
-                 int max_q, int max_kv, void *stream);
-size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim, int window,
-                                int max_q, int max_kv);
+ * out [n_tok][q_heads][head_dim] = softmax(scale * q . k) v over the keys at or before the query's
+ * position, with window > 0 the last `window` of them (the query's own among them). q: row t at
+ * t * ldq floats, [q_heads][head_dim], 16-byte aligned, ldq a multiple of 4; query head j reads
+ * kv head j / (q_heads / kv_heads). scale > 0. A row that sees no key is zeros. out must not
+ * overlap q. Results are within fp32's rounding of the definition; of values whose group scales
+ * lie more than 2^140 apart, the smaller ones may lose their share of a row's sum.
+ *
+ * max_q and max_kv are the batch's largest number of tokens of a sequence and largest kv_len, or
+ * bounds of them: they choose the launch's shape, and wrong values cost no more than speed (the
+ * order of sums goes with the shape). The workspace holds the partial sums of a split key axis:
+ * kq4_attn_workspace_bytes of the same numbers. */
+int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_heads, float scale,
+                 int window, int max_q, int max_kv, void *stream);
+size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim,
+                                int window, int max_q, int max_kv);
 
 /* Most alternatives and most logits of a row that kq4_logprobs_dev takes. */
 #define KQ4_LOGPROBS_MAX_TOP 32
 #define KQ4_LOGPROBS_MAX_VOCAB (1 << 20)
 
-/* What sampling and scoring read from n rows of logits (row t at t * ld floats, vocab of them; 4-byte aligned, faster where
- * 16-byte aligned with ld a multiple of 4), each output NULL where it is not wanted:
- *   logprob [n]               log softmax(logits)[token[t]] (NaN for a token outside the vocabulary: a row
- *                             that asks for none)
- *   entropy [n]               -sum p log p, in nats
- *   top_logprob, top_id [n][n_top]   the n_top (<= 32, <= vocab) largest, largest first, ties to the lowest id
- * A logit of -inf has probability 0 and comes last among the alternatives; a row of nothing else has log
- * probabilities -inf and entropy 0. A row with a NaN or +inf gets NaN (its top_id still order the logits, a NaN
- * before all). Workspace: kq4_logprobs_workspace_bytes. */
-int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *top_id, const float *logits, long ld,
-                     const int *token, int n, int vocab, int n_top, void *stream);
+/* What sampling and scoring read from n rows of logits (row t at t * ld floats, vocab of them;
+ * 4-byte aligned), each output NULL where it is not wanted:
+ *   logprob [n]                      log softmax(logits)[token[t]] (NaN for a token outside the
+ *                                    vocabulary: a row that asks for none)
+ *   entropy [n]                      -sum p log p, in nats
+ *   top_logprob, top_id [n][n_top]   the n_top (<= 32, <= vocab) largest, largest first, ties to
+ *                                    the lowest id
+ * A logit of -inf has probability 0 and comes last among the alternatives; a row of nothing else
+ * has log probabilities -inf and entropy 0. A row with a NaN or +inf gets NaN (its top_id still
+ * order the logits, a NaN before all). Workspace: kq4_logprobs_workspace_bytes. */
+int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *top_id,
+                     const float *logits, long ld, const int *token, int n, int vocab, int n_top,
+                     void *stream);
 size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top);
 
 #ifdef __cplusplus

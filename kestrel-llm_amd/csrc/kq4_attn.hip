@@ -868,6 +868,7 @@ void split_keys(long keys, long base, int want, int step, int min_chunk, int max
   long n = want / (base < 1 ? 1 : base);
   const long most = (keys + min_chunk - 1) / min_chunk, least = (keys + max_chunk - 1) / max_chunk;
   if (n > most) n = most;
+  if (keys <= 2L * min_chunk) n = 1;   // (a join costs as much as two turns save)
   if (n < least) n = least;
   if (force > 0) n = force;
   if (n > (keys + step - 1) / step) n = (keys + step - 1) / step;
@@ -884,7 +885,7 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   const int group = heads / kv_heads;
   const long rows = (long)max_q * group;
   // keys of a tile's queries, at most: the window's reach where that is less
-  long keys = max_kv < 1 ? 1 : max_kv;
+  long keys = max_kv < 1 ? 1 : max_kv > 1 << 30 ? 1 << 30 : max_kv;
   if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
   KQ4AttnPlan p{0, 0, 256, 0, 0, 64, 0};
   p.tile32 = force_tile == 16                                           ? 0

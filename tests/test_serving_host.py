@@ -95,6 +95,32 @@ result = [need, before, after]
     assert after == [[0, 2], [0, 2]]
 
 
+@pytest.mark.parametrize("batch,want", [
+    (dict(n_seq=1, n_tok=1, max_q=1, max_kv=800), ["rows16", "join_few"]),          # short: 4 waves, split
+    (dict(n_seq=1, n_tok=1, max_q=1, max_kv=200), ["rows16"]),
+    (dict(n_seq=64, n_tok=64, max_q=1, max_kv=4000), ["rows16"]),                    # a workgroup a CU without splits
+    (dict(n_seq=1, n_tok=1, max_q=1, max_kv=131072), ["rows16", "join"]),
+    (dict(n_seq=64, n_tok=64, max_q=1, max_kv=131072), ["rows16", "join_few"]),      # however long one may be
+    (dict(n_seq=1, n_tok=4, max_q=4, max_kv=800), ["rows16", "join_few"]),           # 16 rows per kv head
+    (dict(n_seq=1, n_tok=4096, max_q=4096, max_kv=4096), ["rows32"]),
+    (dict(n_seq=1, n_tok=128, max_q=128, max_kv=16000), ["rows32", "join_few"]),
+    (dict(n_seq=9, n_tok=200, max_q=150, max_kv=300), ["mixed"]),                    # decode steps and a prompt
+    (dict(n_seq=9, n_tok=9000, max_q=8000, max_kv=9000), ["rows32", "rows16", "join_few"]),
+    (dict(n_seq=4, n_tok=0, max_q=9, max_kv=9), []),
+])
+def test_attention_launches(standin, batch, want):  # noqa: F811
+    """Which kernels a batch takes (32 query heads, 8 kv heads of 128): the forms, and joins where keys are split."""
+    res = standin(SETUP + """
+hip.standin_clear()
+rc = attn(kv(n_seq=n_seq, n_tok=n_tok), out=at(20), max_q=max_q, max_kv=max_kv)
+result = [rc] + [s.split(" ")[0] for s in hip.standin_log().decode().split("\\n")[:-1]]
+""", **batch)
+    assert res[0] == 0
+    names = ["join_few" if "join_few" in s else "join" if "join" in s else "mixed" if "mixed" in s else
+             "rows16" if "rows16" in s else "rows32" if "rows32" in s else s for s in res[1:]]
+    assert names == want
+
+
 def test_sizes(kq4_cpu):
     assert kq4_cpu.kv_codes_shape(3, 32, 2, 64) == (3, 2, 2, 2, 1024)
     lib = kq4_cpu.lib()
