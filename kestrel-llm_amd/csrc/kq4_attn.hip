@@ -24,6 +24,7 @@
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
@@ -149,16 +150,28 @@ KQ4_DEV int row_shift(float amax) {
   return 13 - ilogbf(amax);
 }
 
+// Two weights as hi + lo (both rounded to nearest: an error without a sign of its own, which the row's sum, of the
+// unrounded weights, would not share).
+KQ4_DEV void split_pair(float p0, float p1, uint32_t &h, uint32_t &l) {
+  float minus = -1.0f;   // (not known to the compiler: p - hi as one fma that converts hi, not a conversion and a difference)
+  asm("" : "+s"(minus));
+  const half2v hi = __builtin_convertvector((float2v{p0, p1}), half2v);
+  const half2v lo = __builtin_convertvector((float2v{fmaf((float)hi[0], minus, p0), fmaf((float)hi[1], minus, p1)}),
+                                            half2v);
+  h = __builtin_bit_cast(uint32_t, hi);
+  l = __builtin_bit_cast(uint32_t, lo);
+}
+
 // Two of a lane's keys of a 32-key tile: their weights, summed and as the second product's operand.
 KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float &sum, Frag (&ph)[2],
                           Frag (&pl)[2]) {
   const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c, shift));
   const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c, shift));
   sum += p0 + p1;
-  const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-  const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
-  uint32_t h = __builtin_bit_cast(uint32_t, hi), l = __builtin_bit_cast(uint32_t, lo);
-  // (no instruction: keeps the above from being moved towards its use, behind the matrix instructions it stands between)
+  uint32_t h, l;
+  split_pair(p0, p1, h, l);
+  // (no instruction: keeps the above from being moved towards its use, behind the matrix instructions it stands
+  // between)
   asm volatile("" : "+v"(h), "+v"(l), "+v"(sum));
   ph[j >> 3].u[(j & 7) >> 1] = h;
   pl[j >> 3].u[(j & 7) >> 1] = l;
@@ -336,10 +349,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
             p1 = s[t4][j + 1] == kNegInf ? 0.0f : p1;
           }
           sum += p0 + p1;
-          const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-          const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
-          ph[t4 >> 1].u[2 * (t4 & 1) + (j >> 1)] = __builtin_bit_cast(uint32_t, hi);
-          pl[t4 >> 1].u[2 * (t4 & 1) + (j >> 1)] = __builtin_bit_cast(uint32_t, lo);
+          split_pair(p0, p1, ph[t4 >> 1].u[2 * (t4 & 1) + (j >> 1)], pl[t4 >> 1].u[2 * (t4 & 1) + (j >> 1)]);
         }
       l = fmaf(sum, rv, l);
 #pragma unroll
