@@ -502,11 +502,12 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
     const int slot = (((base + 32 * n) >> 4) + hh) >> a.log_pg;
     return table[slot < a.kv.table_pages ? slot : a.kv.table_pages - 1];
   };
-  auto group_of = [&](int n, int half, int page) -> long {
-    const int g = ((base + 32 * n) >> 4) + half;
-    return g < g_end && (g >> a.log_pg) < a.kv.table_pages && (unsigned)page < (unsigned)a.kv.n_pages
-               ? (((long)page * a.kv.kv_heads + h) << a.log_pg) | (g & ((1 << a.log_pg) - 1))
-               : -1;
+  // Index of a tile's group among the cache's, and whether it holds keys; without a branch, so that the loads stand
+  // among the matrix instructions (where there is none: a group of page 0, never used)
+  auto group_of = [&](int n, int half, int page, bool &ok) -> long {
+    const int g = ((base + 32 * n) >> 4) + half;   // (g < g_end: the table has an entry for it)
+    ok = (g < g_end) & ((unsigned)page < (unsigned)a.kv.n_pages);
+    return (((long)(page & -(int)ok) * a.kv.kv_heads + h) << a.log_pg) | (g & ((1 << a.log_pg) - 1));
   };
   uint4v raw[NL];
   float2v raw_sc = {1.0f, 0.0f};
@@ -525,27 +526,25 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
     }
   }
   auto load = [&](int n) {
-    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(ent, 0));
-    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(ent, 32));
+    bool ok0, ok1;
+    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(ent, 0), ok0);
+    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(ent, 32), ok1);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int j = i * NT + 64 * wave;
-      if (j < L) {
-        const long g = j / (2 * D) ? g1 : g0;
-        raw[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (g < 0 ? 0 : g) * (32 * D) +
+      if (L % NT == 0 || j < L)
+        raw[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (j / (2 * D) ? g1 : g0) * (32 * D) +
                                                    16 * (j % (2 * D)) + 16 * lane);
-      }
     }
-    const long g = hh ? g1 : g0;
-    raw_there = g >= 0;
-    raw_sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (g < 0 ? 0 : g));
+    raw_there = hh ? ok1 : ok0;
+    raw_sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (hh ? g1 : g0));
     ent = entry(n + 1);
   };
   auto store = [&](int n) {
     uint8_t *buf = s_kv[n & 3];
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      if (i * NT + 64 * wave < L) {
+      if (L % NT == 0 || i * NT + 64 * wave < L) {
         *reinterpret_cast<half8 *>(buf + put0[i]) = codes_f16(raw[i][0], raw[i][1]);
         *reinterpret_cast<half8 *>(buf + put1[i]) = codes_f16(raw[i][2], raw[i][3]);
       }
