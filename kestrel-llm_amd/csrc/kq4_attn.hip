@@ -252,9 +252,9 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 #pragma unroll
       for (int t4 = 0; t4 < 4; ++t4)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) kr[t4][t] = *reinterpret_cast<const uint4 *>(kp + 1024 * t + 64 * t4);
+        for (int t = 0; t < TT; ++t) kr[t4][t] = kq4_ld_nt(kp + 1024 * t + 64 * t4);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const uint4 *>(vp + 256 * d);
+      for (int d = 0; d < DT; ++d) vr[d] = kq4_ld_nt(vp + 256 * d);
     }
 
     half8 qh[TT][2], ql[TT][2];
@@ -294,7 +294,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
           const half8 k0 = codes_f16(kr[t4][t].x, kr[t4][t].y), k1 = codes_f16(kr[t4][t].z, kr[t4][t].w);
-          if constexpr (more.value) kr[t4][t] = *reinterpret_cast<const uint4 *>(kp + 1024 * t + 64 * t4);
+          if constexpr (more.value) kr[t4][t] = kq4_ld_nt(kp + 1024 * t + 64 * t4);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[t][0], s[t4], 0, 0, 0);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[t][0], s[t4], 0, 0, 0);
           s[t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[t][1], s[t4], 0, 0, 0);
@@ -355,7 +355,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const half8 v0 = codes_f16(vr[d].x, vr[d].y), v1 = codes_f16(vr[d].z, vr[d].w);
-        if constexpr (more.value) vr[d] = *reinterpret_cast<const uint4 *>(vp + 256 * d);
+        if constexpr (more.value) vr[d] = kq4_ld_nt(vp + 256 * d);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0].h, o[d], 0, 0, 0);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0].h, o[d], 0, 0, 0);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1].h, o[d], 0, 0, 0);

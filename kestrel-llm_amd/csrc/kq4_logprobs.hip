@@ -72,9 +72,7 @@ struct Piece {   // of one row: maximum, z and t relative to it, whether it has 
 // Element i of a thread is logit base + at(i).
 KQ4_DEV int at(int i) { return (i >> 2) * (4 * kThreads) + 4 * (int)threadIdx.x + (i & 3); }
 
-struct __attribute__((packed, aligned(4))) Four {   // 16 bytes at any 4-byte address
-  float v[4];
-};
+typedef float four __attribute__((ext_vector_type(4), aligned(4)));   // 16 bytes at any 4-byte address
 
 __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *__restrict__ logits, long ld,
                                                                   int vocab, int n_pieces, int n_top,
@@ -94,24 +92,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(const float *_
   if (n == kPiece) {
 #pragma unroll
     for (int i = 0; i < kPer; i += 4) {
-      const Four f = *reinterpret_cast<const Four *>(x + at(i));
+      const four f = __builtin_nontemporal_load(reinterpret_cast<const four *>(x + at(i)));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i + j] = f.v[j];
+      for (int j = 0; j < 4; ++j) v[i + j] = f[j];
     }
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; i += 4) {
       const int o = at(i);
-      Four f = {{kNegInf, kNegInf, kNegInf, kNegInf}};
+      four f = {kNegInf, kNegInf, kNegInf, kNegInf};
       if (o + 4 <= n) {
-        f = *reinterpret_cast<const Four *>(x + o);
+        f = *reinterpret_cast<const four *>(x + o);
       } else {
-        if (o < n) f.v[0] = x[o];
-        if (o + 1 < n) f.v[1] = x[o + 1];
-        if (o + 2 < n) f.v[2] = x[o + 2];
+        if (o < n) f[0] = x[o];
+        if (o + 1 < n) f[1] = x[o + 1];
+        if (o + 2 < n) f[2] = x[o + 2];
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i + j] = f.v[j];
+      for (int j = 0; j < 4; ++j) v[i + j] = f[j];
     }
   }
 
