@@ -467,26 +467,6 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   kq4_kv_sees(sp.p0 + (any ? w0 : last) / a.group, sp.len, a.window, &t_, &all_hi);
   if (see_hi > end) see_hi = end;
 
-  half8 qh[TT][2], ql[TT][2];
-  float descale;
-  {
-    const float *row = a.q + (sp.q0 + tq) * a.ldq + (long)head * D;
-    const QRope rope = q_rope(a.kv, sp.q0 + tq, sp.p0 + tq);
-    float x[TT][16], amax = 0.0f;
-#pragma unroll
-    for (int t = 0; t < TT; t += 2) load_q<2>(row, rope, 2 * t + hh, 2, x + t);
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
-    const int sh = row_shift(max_xor32(amax));
-    descale = ldexpf(a.scale2, -sh);
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) split_f16(&x[t][8 * u], sh, qh[t][u], ql[t][u]);
-  }
-
   float16v o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -525,39 +505,67 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
       put1[i] = put0[i] + 2 * D * 16;
     }
   }
-  auto load = [&](int n) {
+  auto fetch_tile = [&](int n, int entries, uint4v (&kv)[NL], float2v &sc, bool &there) {
     bool ok0, ok1;
-    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(ent, 0), ok0);
-    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(ent, 32), ok1);
+    const long g0 = group_of(n, 0, __builtin_amdgcn_readlane(entries, 0), ok0);
+    const long g1 = group_of(n, 1, __builtin_amdgcn_readlane(entries, 32), ok1);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int j = i * NT + 64 * wave;
       if (L % NT == 0 || j < L)
-        raw[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (j / (2 * D) ? g1 : g0) * (32 * D) +
-                                                   16 * (j % (2 * D)) + 16 * lane);
+        kv[i] = *reinterpret_cast<const uint4v *>(a.kv.codes + (j / (2 * D) ? g1 : g0) * (32 * D) +
+                                                  16 * (j % (2 * D)) + 16 * lane);
     }
-    raw_there = hh ? ok1 : ok0;
-    raw_sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (hh ? g1 : g0));
-    ent = entry(n + 1);
+    there = hh ? ok1 : ok0;
+    sc = *reinterpret_cast<const float2v *>(a.kv.scales + 2 * (hh ? g1 : g0));
   };
-  auto store = [&](int n) {
+  auto put_tile = [&](int n, const uint4v (&kv)[NL], float2v sc, bool there) {
     uint8_t *buf = s_kv[n & 3];
 #pragma unroll
     for (int i = 0; i < NL; ++i)
       if (L % NT == 0 || i * NT + 64 * wave < L) {
-        *reinterpret_cast<half8 *>(buf + put0[i]) = codes_f16(raw[i][0], raw[i][1]);
-        *reinterpret_cast<half8 *>(buf + put1[i]) = codes_f16(raw[i][2], raw[i][3]);
+        *reinterpret_cast<half8 *>(buf + put0[i]) = codes_f16(kv[i][0], kv[i][1]);
+        *reinterpret_cast<half8 *>(buf + put1[i]) = codes_f16(kv[i][2], kv[i][3]);
       }
     // (a group without a page: a value scale of 0, which no group has; every wave writes the same)
-    if (i32 == 0) s_sc[n & 3][hh] = raw_there ? raw_sc : float2v{1.0f, 0.0f};
+    if (i32 == 0) s_sc[n & 3][hh] = there ? sc : float2v{1.0f, 0.0f};
   };
+  auto load = [&](int n) {
+    fetch_tile(n, ent, raw, raw_sc, raw_there);
+    ent = entry(n + 1);
+  };
+  auto store = [&](int n) { put_tile(n, raw, raw_sc, raw_there); };
 
-  ent = entry(0);
-  load(0);
-  store(0);
-  load(1);
-  store(1);
-  load(2);
+  // the first three tiles and the query row, all on their way at once
+  half8 qh[TT][2], ql[TT][2];
+  float descale;
+  {
+    const int e0 = entry(0), e1 = entry(1), e2 = entry(2);
+    uint4v raw0[NL], raw1[NL];
+    float2v sc0, sc1;
+    bool there0, there1;
+    ent = entry(3);
+    fetch_tile(0, e0, raw0, sc0, there0);
+    fetch_tile(1, e1, raw1, sc1, there1);
+    fetch_tile(2, e2, raw, raw_sc, raw_there);
+    const float *row = a.q + (sp.q0 + tq) * a.ldq + (long)head * D;
+    const QRope rope = q_rope(a.kv, sp.q0 + tq, sp.p0 + tq);
+    float x[TT][16], amax = 0.0f;
+#pragma unroll
+    for (int t = 0; t < TT; t += 2) load_q<2>(row, rope, 2 * t + hh, 2, x + t);
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
+    const int sh = row_shift(max_xor32(amax));
+    descale = ldexpf(a.scale2, -sh);
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) split_f16(&x[t][8 * u], sh, qh[t][u], ql[t][u]);
+    put_tile(0, raw0, sc0, there0);
+    put_tile(1, raw1, sc1, there1);
+  }
   if (!any) {   // (a wave without rows keeps up the others' tiles and barriers)
     __syncthreads();
     for (int n = 0; n < tiles; ++n) {
