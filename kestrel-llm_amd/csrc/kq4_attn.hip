@@ -573,6 +573,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
       store(n + 2);
       load(n + 3);
     }
+    if constexpr (NW == 8) __syncthreads();
     return;
   }
 
@@ -580,12 +581,17 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   // of one operand fragment (F of each product, read AHEAD before use) and a share of the vector instructions
   // make a block; the compiler is kept to the order of blocks. (Tiles past the last are loaded as group 0, or what
   // follows it in the table, and never used.)
+  //
+  // Of 8 waves two share a SIMD. The upper 4 run half a step later, with the step's barrier between its two products
+  // where the lower 4 have it before both: one wave's scores stand beside the other's second product and the rest.
+  // Between barriers n and n + 1 the lower waves read tiles n + 1 and n, the upper ones n - 1 and n + 1, and both write
+  // n + 2: the four of the ring.
   constexpr int F = 2 * TT, AHEAD = 2;
   const int k_at = (hh * 2 * 32 + i32) * 16, v_at = KB + (hh * D + i32) * 16;
   float16v sa, sb;
   float c = 0.0f, lv = 0.0f, rv = 0.0f;   // of the tile whose scores are at hand: factor, log2 and 1 / value scale
-  auto step = [&](int n, float16v &s, float16v &s_n, auto has, auto more) {
-    __syncthreads();
+  auto step = [&](int n, float16v &s, float16v &s_n, auto has, auto more, auto late) {
+    if constexpr (!late.value || !has.value) __syncthreads();
     half8 f[2 * F];   // keys of tile n + 1, values of tile n
     auto fetch = [&](int i) {
       if (i < F)
@@ -612,6 +618,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
 #pragma unroll
     for (int i = first; i < stop; ++i) {
       __builtin_amdgcn_sched_barrier(0);
+      if (late.value && has.value && i == F) __syncthreads();
       if (i + AHEAD < stop) fetch(i + AHEAD);
       if (i < F) {
         s_n = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i], qh[i >> 1][i & 1], s_n, 0, 0, 0);
@@ -627,15 +634,17 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
           if (i == (p < 4 ? p : 2 * p - 4) * F / 8) softmax_pair(s, 2 * p, c, shift, sum, ph, pl);
       if constexpr (more.value) {
         if (i == F / 2 + 1) {
-          masked = (base + 32 * (n + 1) < all_lo) | (base + 32 * (n + 2) > all_hi) | (__ballot(scale[1] == 0.0f) != 0);
-          c_n = scale[0] * descale;
-          lv_n = __builtin_amdgcn_logf(scale[1]);
-          rv_n = __builtin_amdgcn_rcpf(scale[1]);
+          float sk = scale[0], sv = scale[1];
+          asm volatile("" : "+v"(sk), "+v"(sv));
+          masked = (base + 32 * (n + 1) < all_lo) | (base + 32 * (n + 2) > all_hi) | (__ballot(sv == 0.0f) != 0);
+          c_n = sk * descale;
+          lv_n = __builtin_amdgcn_logf(sv);
+          rv_n = __builtin_amdgcn_rcpf(sv);
           c_n = c_n == 0.0f ? 1e-37f : c_n;   // (a masked score, -inf, stays that)
           asm volatile("" : "+v"(c_n), "+v"(lv_n), "+v"(rv_n));
         }
-        if (has.value && i == F - 1) store(n + 2);
-        if (has.value && i == F) load(n + 3);
+        if (has.value && i == (late.value ? F : F - 1)) store(n + (late.value ? 3 : 2));
+        if (has.value && i == (late.value ? F + 1 : F)) load(n + (late.value ? 4 : 3));
         if (i >= F + F / 2) {
           constexpr int each = 32 / F;
 #pragma unroll
@@ -683,18 +692,28 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   };
   constexpr std::true_type yes;
   constexpr std::false_type no;
-  int n = 0;
-  step(-1, sb, sa, no, yes);
-  for (; n + 2 < tiles; n += 2) {
-    step(n, sa, sb, yes, yes);
-    step(n + 1, sb, sa, yes, yes);
-  }
-  if (n + 1 < tiles) {
-    step(n, sa, sb, yes, yes);
-    step(n + 1, sb, sa, yes, no);
-  } else if (n < tiles) {
-    step(n, sa, sb, yes, no);
-  }
+  auto run = [&](auto late) {
+    int n = 0;
+    step(-1, sb, sa, no, yes, late);
+    if constexpr (late.value) {
+      __syncthreads();
+      store(2);
+      load(3);
+    }
+    for (; n + 2 < tiles; n += 2) {
+      step(n, sa, sb, yes, yes, late);
+      step(n + 1, sb, sa, yes, yes, late);
+    }
+    if (n + 1 < tiles) {
+      step(n, sa, sb, yes, yes, late);
+      step(n + 1, sb, sa, yes, no, late);
+    } else if (n < tiles) {
+      step(n, sa, sb, yes, no, late);
+    }
+    if constexpr (NW == 8 && !late.value) __syncthreads();
+  };
+  if (NW == 8 && wave >= 4) run(yes);
+  else run(no);
 
   if (w0 + i32 > last) return;
   l = kq4_xor_add<32>(l);
