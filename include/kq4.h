@@ -398,7 +398,7 @@ int kq4_moe_ffn_stages_dev(float *Y, const float *X, const int *sel, const float
  * has no keys and takes none, positions past the table have none either, and tokens before
  * position 0 (kv_len smaller than the sequence's tokens) have neither a key nor keys to see.
  *
- * rope, when not NULL: rope_rows rows of rope_dim / 2 pairs (cos, sin), 8-byte aligned. Keys, as
+ * rope, when not NULL: rope_rows rows of rope_dim / 2 pairs (cos, sin), 16-byte aligned. Keys, as
  * they are appended, and queries, as they are read, have dimensions i and i + rope_dim / 2 rotated
  * for i < rope_dim / 2 (rope_dim a multiple of 32, at most head_dim; 0 and NULL: no rotation) by
  * the row of their position, or by row rope_pos[token] where rope_pos is not NULL (an index per

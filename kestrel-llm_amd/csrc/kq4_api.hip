@@ -1255,10 +1255,10 @@ int kv_check(const char *what, const kq4_kv *kv, int *log_pg) {
   if (kv->n_seq && kv->n_tok) {
     if (!kv->codes || !kv->scales || !kv->block_table || !kv->q_start || !kv->kv_len)
       return fail(KQ4_EINVAL, "%s: null cache or batch pointer", what);
-    if ((uintptr_t)kv->codes % 16 || (uintptr_t)kv->scales % 8 || (uintptr_t)kv->rope % 8 ||
+    if ((uintptr_t)kv->codes % 16 || (uintptr_t)kv->scales % 8 || (uintptr_t)kv->rope % 16 ||
         (uintptr_t)kv->block_table % 4 || (uintptr_t)kv->q_start % 4 || (uintptr_t)kv->kv_len % 4 ||
         (uintptr_t)kv->rope_pos % 4)
-      return fail(KQ4_EINVAL, "%s: codes must be 16-byte, scales and rope 8-byte, indexes 4-byte aligned", what);
+      return fail(KQ4_EINVAL, "%s: codes and rope must be 16-byte, scales 8-byte, indexes 4-byte aligned", what);
   }
   *log_pg = log2_of(kv->page_tokens) - 4;
   return KQ4_OK;

@@ -94,42 +94,50 @@ KQ4_DEV QRope q_rope(const kq4_kv &kv, int token, int pos) {
   return r;
 }
 
-// Chunks c0, c0 + step, .. (16 dimensions each) of a query row, rotated as the keys were (in fp32 here: q is not
-// rounded to a grid afterwards). All loads first.
+// Chunks c0, c0 + step, .. (16 dimensions each, N of them) of a query row, rotated as the keys were (in fp32 here: q
+// is not rounded to a grid afterwards). A row that the table does not have is left as it is: the caller makes its
+// scores NaN.
 template <int N>
 KQ4_DEV void load_q(const float *row, const QRope &r, int c0, int step, float (*x)[16]) {
-  float4v own[N][4], other[N][4], cs[N][8];
+  float4v own[N][4];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int c = c0 + k * step;
+  for (int k = 0; k < N; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) own[k][e] = reinterpret_cast<const float4v *>(row + 16 * c)[e];
-    if (r.rp) {   // (a chunk that is not rotated: itself and the table's first columns, not used)
-      const bool up = c >= r.rp, rot = c < 2 * r.rp;
-      const int o = !rot ? c : up ? c - r.rp : c + r.rp;
-      const float2v *t = reinterpret_cast<const float2v *>(r.cs) + (rot ? 16 * (up ? o : c) : 0);
+    for (int e = 0; e < 4; ++e) own[k][e] = reinterpret_cast<const float4v *>(row + 16 * (c0 + k * step))[e];
+  if (N % 2 == 0 && r.rp == step * N / 2) {
+    // a whole head's rotation: chunks k and k + N / 2 are pairs, both this lane's
+    constexpr int H = N > 1 ? N / 2 : 1;
+    float4v cs[H][8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) other[k][e] = reinterpret_cast<const float4v *>(row + 16 * o)[e];
+    for (int k = 0; k < H; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2v f = t[2 * e], g = t[2 * e + 1];
-        cs[k][e] = float4v{f[0], f[1], g[0], g[1]};
+      for (int e = 0; e < 8; ++e) cs[k][e] = reinterpret_cast<const float4v *>(r.cs)[8 * (c0 + k * step) + e];
+#pragma unroll
+    for (int k = 0; k < H; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float co = cs[k][e >> 1][2 * (e & 1)], si = cs[k][e >> 1][2 * (e & 1) + 1];
+        const float u = own[k][e >> 2][e & 3], v = own[(k + H) % N][e >> 2][e & 3];
+        x[k][e] = fmaf(u, co, -(v * si));
+        x[(k + H) % N][e] = fmaf(v, co, u * si);
       }
-    }
+    return;
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const int c = c0 + k * step;
-    const bool up = c >= r.rp, rot = c < 2 * r.rp;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[k][e] = own[k][e >> 2][e & 3];
-      if (r.rp) {
-        // the first of a pair: x1 c - x2 s, the second: x2 c + x1 s
-        const float co = cs[k][e >> 1][2 * (e & 1)], si = cs[k][e >> 1][2 * (e & 1) + 1];
-        const float y = fmaf(x[k][e], co, other[k][e >> 2][e & 3] * (up ? si : -si));
-        x[k][e] = !rot ? x[k][e] : r.bad ? __uint_as_float(0x7fc00000u) : y;
-      }
+    for (int e = 0; e < 16; ++e) x[k][e] = own[k][e >> 2][e & 3];
+    const int c = c0 + k * step;
+    if (c >= 2 * r.rp) continue;
+    const bool up = c >= r.rp;   // the second of a pair: x2 c + x1 s, else x1 c - x2 s
+    const int o = up ? c - r.rp : c + r.rp;
+    const float4v *t = reinterpret_cast<const float4v *>(r.cs) + 8 * (up ? o : c);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const float4v y = reinterpret_cast<const float4v *>(row + 16 * o)[e >> 2], f = t[e >> 1], g = t[(e >> 1) + 1];
+      const float co[4] = {f[0], f[2], g[0], g[2]}, si[4] = {f[1], f[3], g[1], g[3]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[k][e + i] = fmaf(x[k][e + i], co[i], up ? y[i] * si[i] : -(y[i] * si[i]));
     }
   }
 }
@@ -261,13 +269,14 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
     float descale;
     {
       float x[TT][16], amax = 0.0f;
-      load_q<TT>(a.q + (sp.q0 + tq) * a.ldq + (long)head * D, q_rope(a.kv, sp.q0 + tq, sp.p0 + tq), qd, 4, x);
+      const QRope rope = q_rope(a.kv, sp.q0 + tq, sp.p0 + tq);
+      load_q<TT>(a.q + (sp.q0 + tq) * a.ldq + (long)head * D, rope, qd, 4, x);
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
       const int sh = row_shift(max_xor32(max_xor16(amax)));
-      descale = ldexpf(a.scale2, -sh);
+      descale = rope.bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale2, -sh);
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
@@ -551,14 +560,13 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
     const float *row = a.q + (sp.q0 + tq) * a.ldq + (long)head * D;
     const QRope rope = q_rope(a.kv, sp.q0 + tq, sp.p0 + tq);
     float x[TT][16], amax = 0.0f;
-#pragma unroll
-    for (int t = 0; t < TT; t += 2) load_q<2>(row, rope, 2 * t + hh, 2, x + t);
+    load_q<TT>(row, rope, hh, 2, x);
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
     const int sh = row_shift(max_xor32(amax));
-    descale = ldexpf(a.scale2, -sh);
+    descale = rope.bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale2, -sh);
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll

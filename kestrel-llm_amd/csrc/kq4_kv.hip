@@ -133,10 +133,13 @@ KQ4_DEV void append_keys(const kq4_kv &kv, const float *__restrict__ k, long ldk
       }
       if (u < rp) {
         const int row = rope_row(kv, g.t0 + tok, g.pos0 + tok);
-        const float2 *cs = reinterpret_cast<const float2 *>(kv.rope) + (long)(row < 0 ? 0 : row) * (kv.rope_dim / 2) +
-                           16 * ca;
+        const float4 *cs = reinterpret_cast<const float4 *>(kv.rope + (long)(row < 0 ? 0 : row) * kv.rope_dim) + 8 * ca;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) rotate(ka[e], kb[e], cs[e]);
+        for (int e = 0; e < 16; e += 2) {
+          const float4 f = cs[e / 2];
+          rotate(ka[e], kb[e], make_float2(f.x, f.y));
+          rotate(ka[e + 1], kb[e + 1], make_float2(f.z, f.w));
+        }
         if (row < 0)
 #pragma unroll
           for (int e = 0; e < 16; ++e) ka[e] = kb[e] = nan;

@@ -37,7 +37,7 @@ CACHE = [dict(n_pages=0), dict(page_tokens=48), dict(page_tokens=8), dict(page_t
          dict(scales=None), dict(block_table=None), dict(q_start=None), dict(kv_len=None), dict(kv_len="at(5) + 2"),
          dict(n_seq=-1), dict(n_tok=-1), dict(table_pages=0), dict(table_pages=1 << 26), dict(rope_dim=0),
          dict(rope=None), dict(rope_dim=144), dict(rope_dim=160), dict(rope_dim=20), dict(rope_rows=0),
-         dict(rope="at(6) + 4"), dict(rope_pos="at(6) + 1")]
+         dict(rope="at(6) + 8"), dict(rope_pos="at(6) + 1")]
 
 
 def args(d):
