@@ -772,7 +772,7 @@ def _rows(t, name, n, width, device):
             t.dim() == 2:
         (rows, cols), (ld, step) = t.shape, t.stride()
         if rows >= n and cols == width and (step == 1 or width <= 1):
-            return ld if rows > 1 else max(ld, width)
+            return ld if rows > 1 else width   # (one row: any stride)
     _need_on(t, name, torch.float32, device)
     raise KQ4Error(f"{name}: expected [{n}, {width}] with unit column stride, got {tuple(t.shape)} "
                    f"strides {t.stride()}")

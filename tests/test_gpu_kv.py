@@ -383,3 +383,65 @@ def test_another_stream(kq4, torch_dev):
         kq4.attn_dev(outs[1], x, kv, 4, 0.125, max_q=9, max_kv=600, stream=s)
     s.synchronize()
     assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("lens,tile,split,hint", [
+    ([(1, 300), (1, 90)], 0, 0, 300),                # 16 rows of 4 waves, one range
+    ([(1, 300), (1, 90)], 0, 0, 60000),              # of 8 waves, by a bound of the lengths
+    ([(100, 200), (3, 700), (1, 64)], 0, 0, 700),    # short and long runs in one launch
+    ([(70, 500), (130, 130)], 128, 1, 500), ([(70, 500), (130, 130)], 256, 1, 500),
+    ([(70, 500), (130, 130)], 256, 3, 500), ([(9, 1500)], 16, 20, 1500),
+])
+def test_captured_forms(kq4, torch_dev, lens, tile, split, hint):
+    """Every form of the attention in a graph, replayed with other queries and lengths, each replay as the eager call
+    before it; other library calls that use the workspace in between."""
+    torch, rng = torch_dev, np.random.default_rng(17)
+    b = Batch(rng, lens, 2, 64, 16, 64)
+    b.fill(rng, upto="all", spread=1.0)
+    kv, most = b.device(torch, kq4), max(q for q, _ in lens)
+    q, out, want = (torch.zeros((b.n, 256), device="cuda") for _ in range(3))
+    logits = torch.randn((3, 9000), device="cuda")
+    ent = torch.empty(3, device="cuda")
+
+    def attn(o, stream=None):
+        kq4.attn_dev(o, q, kv, 4, 0.125, max_q=most, max_kv=hint, stream=stream)
+
+    kq4.set_option("attn_tile", tile)
+    kq4.set_option("attn_split", split)
+    try:
+        attn(want)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attn(out, torch.cuda.current_stream())
+        for i in range(4):
+            q.copy_(up(torch, rand(rng, b.n, 4, 64).reshape(b.n, -1)))
+            kv.tensors["kv_len"].copy_(torch.tensor([max(n, l - 7 * i) for n, l in lens], dtype=torch.int32))
+            attn(want)
+            kq4.logprobs_dev(logits, entropy=ent)
+            torch.cuda.synchronize()
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), i
+    finally:
+        kq4.set_option("attn_tile", -1)
+        kq4.set_option("attn_split", -1)
+
+
+@pytest.mark.parametrize("tile", [16, 128, 256])
+@pytest.mark.parametrize("dim,rope", [(64, 64), (64, 32), (128, 128), (128, 64), (128, 96), (128, 0)])
+def test_attention_rotations(kq4, torch_dev, tile, dim, rope):
+    """Whole and partial rotations in every form, a position off the table among the queries."""
+    rng = np.random.default_rng(18)
+    b = Batch(rng, [(40, 70), (1, 130)], 1, dim, 64, rope)
+    b.fill(rng, upto="all", spread=1.0)
+    if rope:
+        b.rope_pos = rng.integers(0, 130, b.n).astype(np.int32)
+        b.rope_pos[7], b.rope_pos[33] = -1, b.rope.shape[0]
+    kq4.set_option("attn_tile", tile)
+    try:
+        got = check_attn(kq4, torch_dev, b, rand(rng, b.n, 3, dim), 3)
+    finally:
+        kq4.set_option("attn_tile", -1)
+    assert np.isnan(got[7]).all() == np.isnan(got[33]).all() == bool(rope)
