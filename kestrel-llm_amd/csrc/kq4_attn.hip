@@ -18,6 +18,7 @@
 #include "kq4_internal.h"
 
 #include <limits.h>
+#include <math.h>
 
 #include <type_traits>
 
@@ -31,7 +32,8 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int kCus = 256;      // compute units of an MI355X
-constexpr int kMinChunk = 384; // keys that a split of the 32-row form has at least
+constexpr int kMinChunk = 128; // keys that a split of the 32-row form has at least
+constexpr int kRowKeys = 80;   // and the weight of its keys against its partial sums (kq4_attn_plan)
 constexpr int kJoinFew = 16;   // splits up to which a wave joins a row alone
 constexpr float kNegInf = -__builtin_inff();
 // P is held at 2^kTop for the running maximum, which is raised only where a key passes it by 2^kSlack:
@@ -791,29 +793,33 @@ KQ4_DEV float split_factor(float2 ml, float m) {
   return ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
 }
 
-// Joins the splits of a row, few of them: a wave a row.
+// Joins the splits of rows, few of them: a workgroup takes up to 1024 floats of a token, 4 a thread, so that one search
+// for the token's sequence serves several heads. Of a head's 16 or 32 lanes, lane s holds split s's factor.
 template <int D>
-__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long row = blockIdx.x * 4L + (threadIdx.x >> 6), n_rows = (long)a.kv.n_tok * a.heads;
-  if (row >= n_rows) return;
-  const int tok = __builtin_amdgcn_readfirstlane((int)(row / a.heads)), head = (int)(row - (long)tok * a.heads);
+__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int parts) {
+  static_assert(D / 4 >= kJoinFew, "a head's lanes hold a factor each");
+  const int lane = threadIdx.x & 63, tok = blockIdx.x / parts, part = blockIdx.x - tok * parts;
+  const int at = 1024 * part + 4 * (int)threadIdx.x, head = at / D;
   const int used = splits_used(a, tok, head, lane);
-  if (used <= 1) return;   // no sequence's row, or written by its only split
-  float m = kNegInf, sl = 0.0f, acc[E] = {};
-  for (int s = 0; s < used; ++s) m = fmaxf(m, a.part_ml[s * n_rows + row].x);
+  if (head >= a.heads || used <= 1) return;   // (no sequence's row, or written by its only split)
+  const long row = (long)tok * a.heads + head, n_rows = (long)a.kv.n_tok * a.heads;
+  const int s0 = lane & (kJoinFew - 1);
+  const float2 ml = s0 < used ? a.part_ml[s0 * n_rows + row] : make_float2(kNegInf, 0.0f);
+  float m = ml.x;
+#pragma unroll
+  for (int x = kJoinFew / 2; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+  const float f = split_factor(ml, m);
+  float sl = ml.y * f;
+#pragma unroll
+  for (int x = kJoinFew / 2; x; x >>= 1) sl += __shfl_xor(sl, x);
+  float4v acc = {0.f, 0.f, 0.f, 0.f};
+  const float *p = a.part_o + row * D + at % D;
 #pragma unroll 4
   for (int s = 0; s < used; ++s) {
-    const float2 ml = a.part_ml[s * n_rows + row];
-    const float f = split_factor(ml, m);
-    sl = fmaf(ml.y, f, sl);
-    const float *p = a.part_o + (s * n_rows + row) * D + E * lane;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(p[e], f, acc[e]);
+    const float fs = __shfl(f, (lane & -kJoinFew) + s);
+    acc += *reinterpret_cast<const float4v *>(p + s * n_rows * D) * fs;
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) a.out[row * D + E * lane + e] = sl == 0.0f ? 0.0f : acc[e] / sl;
+  *reinterpret_cast<float4v *>(a.out + row * D + at % D) = acc * (sl == 0.0f ? 0.0f : 1.0f / sl);
 }
 
 // Joins the splits of a row, many of them, 32 dimensions a workgroup: the factors of all splits into LDS, then 8
@@ -897,10 +903,12 @@ int launch(const AttnArgs &a, hipStream_t s) {
   const int ns = p.ns16 > p.ns32 ? p.ns16 : p.ns32;
   if (ns > 1) {
     const long n_rows = (long)a.kv.n_tok * a.heads;
-    if (ns <= kJoinFew)
-      attn_join_few_kernel<D><<<(unsigned)((n_rows + 3) / 4), 256, 0, s>>>(a);
-    else
+    if (ns <= kJoinFew) {
+      const int parts = (int)(((long)a.heads * D + 1023) / 1024);
+      attn_join_few_kernel<D><<<(unsigned)a.kv.n_tok * parts, 256, 0, s>>>(a, parts);
+    } else {
       attn_join_kernel<D><<<(unsigned)(n_rows * (D / 32)), 256, 0, s>>>(a);
+    }
   }
   return (int)hipGetLastError();
 }
@@ -912,7 +920,6 @@ void split_keys(long keys, long base, int want, int step, int min_chunk, int max
   long n = want / (base < 1 ? 1 : base);
   const long most = (keys + min_chunk - 1) / min_chunk, least = (keys + max_chunk - 1) / max_chunk;
   if (n > most) n = most;
-  if (keys <= 2L * min_chunk) n = 1;   // (a join costs as much as two turns save)
   if (n < least) n = least;
   if (force > 0) n = force;
   if (n > (keys + step - 1) / step) n = (keys + step - 1) / step;
@@ -944,11 +951,20 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // 1001 keys, 8 kv heads: 10.8 us in 4 splits of 4 waves, 11.9 in one of 8; one of 131072, 4 kv heads: 34.2 and 33.0)
     p.waves16 = !mixed && keys / 64 * n_seq * kv_heads > 4 * kCus ? 8 : 4;
     const int turn = 64 * p.waves16;
-    split_keys(keys, (long)n_seq * kv_heads, kCus, turn, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
+    // (two turns are not split: a join costs as much as it saves)
+    split_keys(keys, (long)n_seq * kv_heads, kCus, turn, keys <= 2L * turn ? 2 * turn : turn, mixed ? 1024 : 8192,
+               force_split, &p.chunk16, &p.ns16);
   }
-  if (p.tile32)
+  if (p.tile32) {
+    // A split more saves the longest workgroup tiles of keys (about 0.9 us each) and costs every row a partial sum
+    // written and read: keys / n + n rows / kRowKeys is least at n^2 = kRowKeys keys / rows. (kRowKeys 40 / 80 / 140:
+    // 64 tokens x 32 heads over 2000 keys 25.4 / 22.3 / 21.1 us, 3 x 200 x 8 over 400 32.1 / 27.7 / 27.8, 4 x 100 x 16
+    // over 900 33.1 / 29.3 / 32.3, 300 x 32 over 16000 86.7 / 78 / 78.)
+    const int best = (int)(sqrt((double)kRowKeys * keys / ((double)n_tok * heads)) + 0.5);
+    const long least = best < 2 ? keys : (keys + best - 1) / best;
     split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus, 64,
-               kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
+               least > kMinChunk ? (int)least : kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
+  }
   return p;
 }
 

@@ -104,7 +104,9 @@ result = [need, before, after]
     (dict(n_seq=1, n_tok=4, max_q=4, max_kv=800), ["rows16", "join_few"]),           # 16 rows per kv head
     (dict(n_seq=1, n_tok=4096, max_q=4096, max_kv=4096), ["rows32"]),
     (dict(n_seq=1, n_tok=128, max_q=128, max_kv=16000), ["rows32", "join_few"]),
-    (dict(n_seq=9, n_tok=200, max_q=150, max_kv=300), ["mixed"]),                    # decode steps and a prompt
+    (dict(n_seq=9, n_tok=200, max_q=150, max_kv=150), ["mixed"]),                    # decode steps and a prompt
+    (dict(n_seq=9, n_tok=200, max_q=150, max_kv=3000), ["mixed", "join_few"]),
+    (dict(n_seq=1, n_tok=1500, max_q=1500, max_kv=1500), ["rows32"]),                   # a split's sums would cost more
     (dict(n_seq=9, n_tok=9000, max_q=8000, max_kv=9000), ["rows32", "rows16", "join_few"]),
     (dict(n_seq=4, n_tok=0, max_q=9, max_kv=9), []),
 ])
