@@ -914,15 +914,18 @@ int launch(const AttnArgs &a, hipStream_t s) {
 }
 
 // Splits of `keys` keys so that `base` workgroups become about `want`, each of at least min_chunk keys and at most
-// max_chunk (a split's workgroup walks its keys alone, however long other sequences are).
-void split_keys(long keys, long base, int want, int step, int min_chunk, int max_chunk, int force, int *chunk,
+// max_chunk (a split's workgroup walks its keys alone, however long other sequences are); none that saves the longest
+// workgroup fewer than `save` steps of `step` keys.
+void split_keys(long keys, long base, int want, int step, int save, int min_chunk, int max_chunk, int force, int *chunk,
                 int *ns) {
   long n = want / (base < 1 ? 1 : base);
   const long most = (keys + min_chunk - 1) / min_chunk, least = (keys + max_chunk - 1) / max_chunk;
   if (n > most) n = most;
+  const long steps = (keys + step - 1) / step;
+  if (n > 1 && steps - (steps + n - 1) / n < save) n = 1;
   if (n < least) n = least;
   if (force > 0) n = force;
-  if (n > (keys + step - 1) / step) n = (keys + step - 1) / step;
+  if (n > steps) n = steps;
   if (n > KQ4_ATTN_MAX_SPLITS) n = KQ4_ATTN_MAX_SPLITS;
   if (n < 1) n = 1;
   *chunk = (int)(((keys + n - 1) / n + step - 1) / step * step);
@@ -947,13 +950,17 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   const bool mixed = p.tile32 && force_tile == 0 && n_seq > 1 && (long)n_tok != (long)n_seq * max_q;
   p.max16 = !p.tile32 ? INT_MAX : mixed ? 16 : 0;
   if (p.max16) {
-    // 8 waves a workgroup, 4 where 64 keys a wave leave SIMDs idle (the shortest path then counts: one sequence of
-    // 1001 keys, 8 kv heads: 10.8 us in 4 splits of 4 waves, 11.9 in one of 8; one of 131072, 4 kv heads: 34.2 and 33.0)
-    p.waves16 = !mixed && keys / 64 * n_seq * kv_heads > 4 * kCus ? 8 : 4;
+    // 4 waves a workgroup, two of which fit a CU, so that one's start stands beside the other's loads (64 sequences of
+    // 1000 keys, 8 kv heads: 25.3 us, 31.3 with 8 waves; 64 of up to 4000 65.0 and 70.5). 8 where splits make the
+    // workgroups, one a CU, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 29.6 us, 30.5
+    // with 4 waves; 8 of 8192, 8 kv heads: 29.4 and 30.1; but one of 16384 16.5 and 15.5).
+    const long base = (long)n_seq * kv_heads;
+    p.waves16 = !mixed && base < kCus && keys / 64 * base > 16 * kCus ? 8 : 4;
     const int turn = 64 * p.waves16;
-    // (two turns are not split: a join costs as much as it saves)
-    split_keys(keys, (long)n_seq * kv_heads, kCus, turn, keys <= 2L * turn ? 2 * turn : turn, mixed ? 1024 : 8192,
-               force_split, &p.chunk16, &p.ns16);
+    // A join costs as much as two turns: 16 sequences, 8 kv heads, 600 / 1000 / 8192 keys in one range 11.2 / 13.4 / 65.5
+    // us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences of up to
+    // 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
+    split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
   }
   if (p.tile32) {
     // A split more saves the longest workgroup tiles of keys (about 0.9 us each) and costs every row a partial sum
@@ -962,7 +969,7 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // over 900 33.1 / 29.3 / 32.3, 300 x 32 over 16000 86.7 / 78 / 78.)
     const int best = (int)(sqrt((double)kRowKeys * keys / ((double)n_tok * heads)) + 0.5);
     const long least = best < 2 ? keys : (keys + best - 1) / best;
-    split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus, 64,
+    split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus, 64, 0,
                least > kMinChunk ? (int)least : kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
   }
   return p;
