@@ -163,7 +163,8 @@ KQ4_DEV int row_shift(float amax) {
 // Two weights as hi + lo (both rounded to nearest: an error without a sign of its own, which the row's sum, of the
 // unrounded weights, would not share).
 KQ4_DEV void split_pair(float p0, float p1, uint32_t &h, uint32_t &l) {
-  float minus = -1.0f;   // (not known to the compiler: p - hi as one fma that converts hi, not a conversion and a difference)
+  // (not known to the compiler: p - hi as one fma that converts hi, not a conversion and a difference)
+  float minus = -1.0f;
   asm("" : "+s"(minus));
   const half2v hi = __builtin_convertvector((float2v{p0, p1}), half2v);
   const half2v lo = __builtin_convertvector((float2v{fmaf((float)hi[0], minus, p0), fmaf((float)hi[1], minus, p1)}),
@@ -187,10 +188,19 @@ KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float 
   pl[j >> 3].u[(j & 7) >> 1] = l;
 }
 
+// The factor of a split's, or wave's, sums in the joined row (one of which nothing was seen: 0; one whose scales were
+// all NaN keeps its NaN).
+KQ4_DEV float split_factor(float2 ml, float m) {
+  return ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
+}
+
 // ---- up to 16 rows (query tokens * heads per kv head) a tile: decode ---------------------------------
 // A workgroup is one sequence, kv head and split; its waves take 64 keys in turn straight from memory to
 // registers (nothing is shared between waves until they join), the next keys' loads in flight during the
-// softmax and the second product.
+// softmax and the second product. Each key is read once, without a place in the caches: 32 sequences of up to 8192
+// keys, 8 kv heads of 128 (321 MB) 68.5 us, 4.7 TB/s, the rate of a large copy (4.8), 1.01 times the bytes it owes; one
+// of 131072 keys, 4 kv heads (134 MB) 25.2 us and 4.5 us for the join. Bound by memory; a short call by its chain of
+// dependent loads (lengths, page, keys) and the join: one token over 1001 keys 6.8 us and 3.7 us.
 template <int D, int NW>
 constexpr int kLds16 = NW * 16 * ((D + 4) * 4 + 8);
 template <int D, int NW>
@@ -396,7 +406,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float2 ml = s_ml[w][rr];
-        const float f = ml.x == kNegInf && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x == kNegInf ? 0.0f : ml.x - m);
+        const float f = split_factor(ml, m);
         sl = fmaf(ml.y, f, sl);
         acc += *reinterpret_cast<const float4v *>(&s_o[w][rr][d]) * f;
       }
@@ -420,6 +430,11 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 // in flight meanwhile. LDS holds the operands in lane order, 16 bytes a lane without bank conflicts: keys as
 // [D/8][32 keys][8], values as [8-token half][group][D][8]. The scores of tile n + 1 are formed while tile n's go
 // through the softmax, so matrix instructions and vector instructions of a wave are independent of each other.
+// A prompt of 4096 tokens, 32 heads, 8 kv heads of 128: 246 us, 560 TFLOP/s of the definition's 137 GFLOP, twice that
+// of matrix instructions (hi + lo). Bound by issue: a tile and wave has 32 matrix instructions (1024 cycles of its
+// SIMD) and about 130 vector instructions (712, 16 of them exponentials), 1930 cycles are measured; the matrix unit
+// is busy 53 % of the cycles at 1.93 GHz. A call of one tile takes 6.8 us at 64 dimensions, 9.5 at 128 (dependent
+// loads, the rotation of the queries); a further tile of 4 waves 0.7 and 0.95 us.
 template <int D>
 constexpr int kLds32 = 4 * 64 * D * 2 + 64;
 template <int D, int NW>
@@ -750,7 +765,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_rows32_kernel(AttnArgs a) {
   attn_rows32<D, NW>(a, blockIdx.x, gridDim.x, blockIdx.y, dyn_lds);
 }
 // Both in one launch, for batches of short and long runs of tokens: the first blocks16 * ns16 workgroups are
-// attn_rows16's, each kind returning for the other's sequences.
+// attn_rows16's, each kind returning for the other's sequences. 7 sequences of 1 to 190 tokens in a window of 1024 of up
+// to 2901 keys, 12 heads, 4 kv heads of 64: 21.7 us and 4.7 us for the join, all of it the start and the tiles of the
+// longest workgroup (8.8 MB and 2.3 GFLOP would take 2 us).
 template <int D>
 __global__ __launch_bounds__(256, 2) void attn_mixed_kernel(AttnArgs a, int blocks16, int blocks32) {
   extern __shared__ __align__(16) uint8_t dyn_lds[];
@@ -787,14 +804,10 @@ KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
   return 0;
 }
 
-// The factor of a split's sums in the joined row (one of which nothing was seen: 0; one whose scales were all NaN
-// keeps its NaN).
-KQ4_DEV float split_factor(float2 ml, float m) {
-  return ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
-}
-
 // Joins the splits of rows, few of them: a workgroup takes up to 1024 floats of a token, 4 a thread, so that one search
-// for the token's sequence serves several heads. Of a head's 16 or 32 lanes, lane s holds split s's factor.
+// for the token's sequence serves several heads. Of a head's 16 or 32 lanes, lane s holds split s's factor. Bound by
+// latency (search, factors, sums: three dependent loads): 8400 rows of 64, 4 splits 4.7 us; a wave a row, the factors
+// one after the other, took 7.4.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int parts) {
   static_assert(D / 4 >= kJoinFew, "a head's lanes hold a factor each");
@@ -823,7 +836,7 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int part
 }
 
 // Joins the splits of a row, many of them, 32 dimensions a workgroup: the factors of all splits into LDS, then 8
-// threads a dimension take splits in turn.
+// threads a dimension take splits in turn (32 rows of 128, 64 splits 4.5 us, latency).
 template <int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   __shared__ float s_f[KQ4_ATTN_MAX_SPLITS];
@@ -942,6 +955,11 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   long keys = max_kv < 1 ? 1 : max_kv > 1 << 30 ? 1 << 30 : max_kv;
   if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
   KQ4AttnPlan p{0, 0, 256, 0, 0, 64, 0};
+  // 16 rows a tile up to 16 rows of a sequence and kv head (16 sequences of 4 tokens, 4 heads a kv head, 2000 keys:
+  // 21.6 us, 38.9 with 128 rows a workgroup; of 8 tokens, 32 rows, 37.4 and 43.4, but one of 16 tokens over 4000 keys
+  // 32.4 and 22.4). 256 where its workgroups fill the CUs (a prompt of 4096 tokens 247 us, 272 with 128; 4 of 500 tokens
+  // 37.0 and 41.2; one of 2000, whose longest workgroups end late, 95.7 and 87.9), else 128 (the mixed kernel's batch
+  // 26.3 us, 30.1 with 256; 500 tokens 26.1 and 32.8).
   p.tile32 = force_tile == 16                                           ? 0
              : force_tile == 128 || force_tile == 256                   ? force_tile
              : rows <= 16                                               ? 0
@@ -957,9 +975,9 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     const long base = (long)n_seq * kv_heads;
     p.waves16 = !mixed && base < kCus && keys / 64 * base > 16 * kCus ? 8 : 4;
     const int turn = 64 * p.waves16;
-    // A join costs as much as two turns: 16 sequences, 8 kv heads, 600 / 1000 / 8192 keys in one range 11.2 / 13.4 / 65.5
-    // us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences of up to
-    // 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
+    // A join costs as much as two turns: 16 sequences, 8 kv heads, 600 / 1000 / 8192 keys in one range 11.2 / 13.4 /
+    // 65.5 us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences
+    // of up to 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
     split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
   }
   if (p.tile32) {
