@@ -11,7 +11,7 @@
 // Keys lie as [D/16][16 tokens][16], values as [D][16 tokens], the orders in which the attention's lanes
 // read 16 bytes each. A group's only new token (a decode step) is written by the byte; more of them as whole
 // pieces of 16 bytes.
-// Bound by memory where there is enough of it: 4096 tokens, 8 heads of 128 (44 MB in and out) 12.0 us, 3.7 TB/s (a copy
+// Bound by memory where there is enough of it: 4096 tokens, 8 heads of 128 (44 MB in and out) 12.4 us, 3.5 TB/s (a copy
 // of many times that size 4.8; here the launch and the chain of dependent loads, lengths, page, rows, are 3 us of it).
 // A decode step is that chain alone: one token 2.6-3.1 us, 64 sequences 4.1. Keys and values to two waves: twice the
 // loads in flight for the same chain.
