@@ -38,7 +38,9 @@ KQ4_DEV float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// A wave's sum or maximum in every lane: DPP moves within rows of 16 lanes, then the swaps of rows and halves.
+// A wave's sum or maximum in every lane: DPP moves within rows of 16 lanes, then the swaps of rows and halves. (Rotations
+// add a row's quads in an order of each lane's own, so a sum of floats is lane 0's for all: results that lanes form with
+// it must not depend on which lane does.)
 template <int CTRL>
 KQ4_DEV uint32_t dpp(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
@@ -49,7 +51,7 @@ KQ4_DEV float wave_sum(float v) {
   v += __uint_as_float(dpp<kQuad2>(__float_as_uint(v)));
   v += __uint_as_float(dpp<kRow4>(__float_as_uint(v)));
   v += __uint_as_float(dpp<kRow8>(__float_as_uint(v)));
-  return kq4_xor_add<32>(kq4_xor_add<16>(v));
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(kq4_xor_add<32>(kq4_xor_add<16>(v)))));
 }
 KQ4_DEV int wave_sum(int n) {
   uint32_t v = (uint32_t)n;

@@ -145,3 +145,23 @@ def test_graph_replays(kq4, torch_dev):
         torch.cuda.synchronize()
         for a, b in zip(*outs):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("n,vocab,n_top", [(3, 40000, 6), (64, 151936, 20), (5, 1000, 32)])
+def test_same_bits_whatever_the_order(kq4, torch_dev, n, vocab, n_top):
+    """Which thread takes a candidate is not fixed, what it makes of it is: calls repeat to the bit, and an alternative
+    has the log probability that its token has when it is asked for."""
+    torch = torch_dev
+    x = torch.randn((n, vocab), generator=torch.Generator().manual_seed(1)).cuda()
+    first = None
+    for k in range(n_top):
+        lp, top, ids = (torch.empty(s, device="cuda", dtype=t) for s, t in
+                        (((n,), torch.float32), ((n, n_top), torch.float32), ((n, n_top), torch.int32)))
+        token = torch.zeros(n, dtype=torch.int32, device="cuda") if first is None else first[1][:, k].contiguous()
+        kq4.logprobs_dev(x, token, logprob=lp, top_logprob=top, top_id=ids)
+        torch.cuda.synchronize()
+        if first is None:
+            first = top, ids
+        else:
+            assert torch.equal(lp, first[0][:, k]), k
+        assert torch.equal(top, first[0]) and torch.equal(ids, first[1]), k
