@@ -445,3 +445,30 @@ def test_attention_rotations(kq4, torch_dev, tile, dim, rope):
     finally:
         kq4.set_option("attn_tile", -1)
     assert np.isnan(got[7]).all() == np.isnan(got[33]).all() == bool(rope)
+
+
+@pytest.mark.parametrize("tile,split", [(0, 0), (0, 3), (16, 3), (128, 1), (256, 20)])
+def test_attention_many_sequences(kq4, torch_dev, tile, split):
+    """More sequences than a wave has lanes, empty ones and a long one among them: the search for an item's and a row's
+    sequence goes round."""
+    rng = np.random.default_rng(19)
+    lens = [(int(rng.integers(0, 4)), int(rng.integers(4, 70))) for _ in range(150)]
+    lens[77], lens[131] = (30, 600), (20, 20)
+    b = Batch(rng, lens, 2, 64, 16, 64, pad=3)
+    b.fill(rng, upto="all", spread=1.0)
+    kq4.set_option("attn_tile", tile)
+    kq4.set_option("attn_split", split)
+    try:
+        check_attn(kq4, torch_dev, b, rand(rng, b.n, 4, 64), 4)
+    finally:
+        kq4.set_option("attn_tile", -1)
+        kq4.set_option("attn_split", -1)
+
+
+def test_large_pages(kq4, torch_dev):
+    """The largest page, appended to and attended over across its border."""
+    rng = np.random.default_rng(20)
+    b = Batch(rng, [(40, 4110), (1, 4096)], 1, 64, 4096, 64)
+    b.fill(rng, spread=1.0)
+    check_append(kq4, torch_dev, b, rand(rng, b.n, 1, 64), rand(rng, b.n, 1, 64))
+    check_attn(kq4, torch_dev, b, rand(rng, b.n, 2, 64), 2)

@@ -165,3 +165,8 @@ def test_same_bits_whatever_the_order(kq4, torch_dev, n, vocab, n_top):
         else:
             assert torch.equal(lp, first[0][:, k]), k
         assert torch.equal(top, first[0]) and torch.equal(ids, first[1]), k
+
+
+def test_many_rows_of_few_logits(kq4, torch_dev):
+    rng = np.random.default_rng(5)
+    check(kq4, torch_dev, (3 * rng.standard_normal((5000, 7))).astype(F32), rng.integers(0, 7, 5000), 7)
