@@ -197,10 +197,11 @@ KQ4_DEV float split_factor(float2 ml, float m) {
 // ---- up to 16 rows (query tokens * heads per kv head) a tile: decode ---------------------------------
 // A workgroup is one sequence, kv head and split; its waves take 64 keys in turn straight from memory to
 // registers (nothing is shared between waves until they join), the next keys' loads in flight during the
-// softmax and the second product. Each key is read once, without a place in the caches: 32 sequences of up to 8192
-// keys, 8 kv heads of 128 (321 MB) 68.5 us, 4.7 TB/s, the rate of a large copy (4.8), 1.01 times the bytes it owes; one
-// of 131072 keys, 4 kv heads (134 MB) 25.2 us and 4.5 us for the join. Bound by memory; a short call by its chain of
-// dependent loads (lengths, page, keys) and the join: one token over 1001 keys 6.8 us and 3.7 us.
+// softmax and the second product. Each key is read once, without a place in the caches: 32 sequences of 8192 keys, 8 kv
+// heads of 128 (537 MB) 84.7 us, 6.35 TB/s; of 1621 to 8192 keys (321 MB) 69 us, the longest ones' 2 us a turn of 4
+// waves (64 KB in flight); 1.01 times the bytes it owes. One of 131072 keys, 4 kv heads (134 MB) 25.2 us and 4.5 us for
+// the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and the join: one token
+// over 1001 keys 6.8 us and 3.7 us.
 template <int D, int NW>
 constexpr int kLds16 = NW * 16 * ((D + 4) * 4 + 8);
 template <int D, int NW>
