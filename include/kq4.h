@@ -34,8 +34,9 @@
  * whatever calls run after its capture. The workspace cannot grow while a stream is being
  * captured (that needs hipMalloc): such a call returns KQ4_EINVAL and launches nothing. Size it
  * before capturing with kq4_workspace_reserve (kq4_matmul_workspace_bytes,
- * kq4_moe_workspace_bytes, kq4_attn_workspace_bytes, kq4_logprobs_workspace_bytes), or by running the same calls once eagerly. kq4_workspace_trim frees
- * the outgrown workspaces once the graphs captured before the growth are destroyed. Only the
+ * kq4_moe_workspace_bytes, kq4_attn_workspace_bytes, kq4_logprobs_workspace_bytes), or by running
+ * the same calls once eagerly. kq4_workspace_trim frees the outgrown workspaces once the graphs
+ * captured before the growth are destroyed. Only the
  * call's own stream is asked whether it is capturing: a call that grows the workspace on
  * another stream while some stream captures in hipStreamCaptureModeGlobal fails in hipMalloc
  * (KQ4_ENOMEM) and invalidates that capture, so reserve first in that mode too.
