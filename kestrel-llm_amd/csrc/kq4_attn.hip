@@ -202,6 +202,36 @@ KQ4_DEV float split_factor(float2 ml, float m) {
 // waves (64 KB in flight); 1.01 times the bytes it owes. One of 131072 keys, 4 kv heads (134 MB) 25.2 us and 4.5 us for
 // the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and the join: one token
 // over 1001 keys 6.8 us and 3.7 us.
+// Which sequence a workgroup takes, longest first: of two that share a CU (it takes them in order, a round of kCus and
+// then another) one is long where the other is short. kHalves: the first range of the rank-th longest, the second one of
+// the rank-th shortest. kOrder: whole sequences, those of the second round shortest first, the others as slots free.
+enum { kPlain = 0, kOrder = 1, kHalves = 2 };
+KQ4_DEV int rank_at(const AttnArgs &a, int place, int split) {
+  if (a.plan.order16 == kHalves) return split ? a.kv.n_seq - 1 - place : place;
+  const int round = kCus / a.kv.kv_heads;
+  return place < round ? place : place < 2 * round ? a.kv.n_seq - 1 - (place - round) : place - round;
+}
+// The sequence with `rank` longer ones (ties by number); n_seq <= 64 NW.
+template <int NW>
+KQ4_DEV int ranked(const AttnArgs &a, int rank, uint8_t *lds) {
+  int *s_len = reinterpret_cast<int *>(lds), *s_seq = s_len + 64 * NW;
+  const int i = threadIdx.x, n = a.kv.n_seq;
+  const int len = i < n ? a.kv.kv_len[i] : INT_MIN;
+  s_len[i] = len;
+  __syncthreads();
+  int longer = 0;
+  for (int j = 0; j < n; j += 4) {   // (those past n are the shortest)
+    const int4 l = *reinterpret_cast<const int4 *>(s_len + j);
+    longer += (l.x > len || (l.x == len && j < i)) + (l.y > len || (l.y == len && j + 1 < i)) +
+              (l.z > len || (l.z == len && j + 2 < i)) + (l.w > len || (l.w == len && j + 3 < i));
+  }
+  if (i < n && longer == rank) *s_seq = i;
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(*s_seq);
+  __syncthreads();   // (the memory is used again)
+  return seq;
+}
+
 template <int D, int NW>
 constexpr int kLds16 = NW * 16 * ((D + 4) * 4 + 8);
 template <int D, int NW>
@@ -212,7 +242,8 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
   const int chunk = a.plan.chunk16, ns = a.plan.ns16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i16 = lane & 15, qd = lane >> 4;
-  const int seq = block / a.kv.kv_heads, h = block - seq * a.kv.kv_heads;
+  const int place = block / a.kv.kv_heads, h = block - place * a.kv.kv_heads;
+  const int seq = a.plan.order16 ? ranked<NW>(a, rank_at(a, place, split), lds) : place;
   const KQ4KvSpan sp = kq4_kv_span(a.kv.q_start[seq], a.kv.q_start[seq + 1], a.kv.kv_len[seq], a.kv.n_tok,
                                    a.kv.table_pages << (a.log_pg + 4));
   const int rows = sp.nq * a.group;
@@ -223,10 +254,14 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
   for (int r0 = 0; r0 < rows; r0 += 16) {
     const int last = r0 + 15 < rows ? r0 + 15 : rows - 1;
     int base, end;
-    const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, ns, &base, &end);
+    int part = chunk, used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, ns, &base, &end);
+    if (a.plan.order16 == kHalves) {
+      part = kq4_kv_half(base, end, 64 * NW);
+      used = end - base > part ? 2 : 1;
+    }
     if (split >= used) continue;
-    base += split * chunk;
-    if (split + 1 < used) end = base + chunk;
+    base += split * part;
+    if (split + 1 < used) end = base + part;
     const int g_end = (sp.len + 15) >> 4;      // groups that hold keys
 
     // this lane's query row, the keys it sees
@@ -798,8 +833,11 @@ KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
       const int r = (tok - sp.q0) * a.group + head % a.group, r0 = r - r % tile;
       const int last = r0 + tile - 1 < rows ? r0 + tile - 1 : rows - 1;
       int base, end;
-      return kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, small ? a.plan.chunk16 : a.plan.chunk32,
-                           small ? a.plan.ns16 : a.plan.ns32, &base, &end);
+      const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window,
+                                     small ? a.plan.chunk16 : a.plan.chunk32, small ? a.plan.ns16 : a.plan.ns32, &base,
+                                     &end);
+      if (a.plan.order16 == kHalves) return end - base > kq4_kv_half(base, end, 64 * a.plan.waves16) ? 2 : 1;
+      return used;
     }
   }
   return 0;
@@ -955,7 +993,7 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   // keys of a tile's queries, at most: the window's reach where that is less
   long keys = max_kv < 1 ? 1 : max_kv > 1 << 30 ? 1 << 30 : max_kv;
   if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
-  KQ4AttnPlan p{0, 0, 256, 0, 0, 64, 0};
+  KQ4AttnPlan p{0, 0, 256, 0, 0, 64, 0, kPlain};
   // 16 rows a tile up to 16 rows of a sequence and kv head (16 sequences of 4 tokens, 4 heads a kv head, 2000 keys:
   // 21.6 us, 38.9 with 128 rows a workgroup; of 8 tokens, 32 rows, 37.4 and 43.4, but one of 16 tokens over 4000 keys
   // 32.4 and 22.4). 256 where its workgroups fill the CUs (a prompt of 4096 tokens 247 us, 272 with 128; 4 of 500 tokens
@@ -980,6 +1018,18 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // 65.5 us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences
     // of up to 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
     split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
+    // Sequences dealt by length, where there are about as many workgroups as CUs or more and each is long. A CU draws
+    // about 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of
+    // 1621 to 8192 keys 69.0 -> 59.9 us in halves (the join among it; of 8192 each 85.5 -> 90.9), whole ones in order:
+    // 64 of up to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of
+    // 16 heads 115 -> 97. (From 129 to 255 workgroups halves neither gain nor lose.)
+    if (!mixed && force_split <= 0 && p.waves16 == 4 && n_seq <= 256 && keys >= 16 * turn && base > kCus / 2) {
+      if (base > kCus && p.ns16 == 1) p.order16 = kOrder;
+      if (base <= kCus && p.ns16 <= 2) {
+        p.order16 = kHalves;
+        p.ns16 = 2;
+      }
+    }
   }
   if (p.tile32) {
     // A split more saves the longest workgroup tiles of keys (about 0.9 us each) and costs every row a partial sum

@@ -68,3 +68,9 @@ KQ4_HD int kq4_kv_ranges(const KQ4KvSpan &s, int t0, int t1, int window, int chu
   const int n = *end > *base ? (*end - *base + chunk - 1) / chunk : 0;
   return n < 1 ? 1 : n > ns ? ns : n;
 }
+
+// Keys of the first of two about equal parts of [base, end), a multiple of `turn`.
+KQ4_HD int kq4_kv_half(int base, int end, int turn) {
+  const int n = end > base ? end - base : 0;
+  return ((n - n / 2) + turn - 1) / turn * turn;
+}

@@ -472,3 +472,16 @@ def test_large_pages(kq4, torch_dev):
     b.fill(rng, spread=1.0)
     check_append(kq4, torch_dev, b, rand(rng, b.n, 1, 64), rand(rng, b.n, 1, 64))
     check_attn(kq4, torch_dev, b, rand(rng, b.n, 2, 64), 2)
+
+
+@pytest.mark.parametrize("n_seq", [65, 70, 128, 150, 256])
+@pytest.mark.parametrize("heads,dim,window", [(4, 64, 0), (2, 128, 0), (4, 64, 40)])
+def test_attention_sequences_by_length(kq4, torch_dev, n_seq, heads, dim, window):
+    """Many sequences under a bound of the lengths that makes their order (whole or in halves) go by length: of all
+    lengths, equal ones and empty ones among them, one far longer than the others."""
+    rng = np.random.default_rng(n_seq)
+    lens = [(int(rng.integers(0, 3)), int(rng.choice([0, 1, 60, 255, 256, 257, 300]))) for _ in range(n_seq)]
+    lens[n_seq // 3] = (1, 1100)
+    b = Batch(rng, lens, 2, dim, 64, 64, pad=1)
+    b.fill(rng, upto="all", spread=1.0)
+    check_attn(kq4, torch_dev, b, rand(rng, b.n, heads, dim), heads, window=window, max_kv=5000, max_q=2)
