@@ -202,14 +202,56 @@ KQ4_DEV float split_factor(float2 ml, float m) {
 // waves (64 KB in flight); 1.01 times the bytes it owes. One of 131072 keys, 4 kv heads (134 MB) 25.2 us and 4.5 us for
 // the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and the join: one token
 // over 1001 keys 6.8 us and 3.7 us.
-// Which sequence a workgroup takes, longest first: of two that share a CU (it takes them in order, a round of kCus and
-// then another) one is long where the other is short. kHalves: the first range of the rank-th longest, the second one of
-// the rank-th shortest. kOrder: whole sequences, those of the second round shortest first, the others as slots free.
-enum { kPlain = 0, kOrder = 1, kHalves = 2 };
+// How sequences are dealt to the workgroups of the 16-row form (kq4_attn_plan). kOrder, kHalves: by length; of two
+// workgroups that share a CU (it takes them in order, a round of kCus and then another) one is long where the other is
+// short. kHalves: the first range of the rank-th longest, the second one of the rank-th shortest. kOrder: whole
+// sequences, those of the second round shortest first, the others as slots free. kShares: each sequence in as many
+// ranges as its part of all keys of the batch.
+enum { kPlain = 0, kOrder = 1, kHalves = 2, kShares = 3 };
+KQ4_HD int kq4_attn_shares(int kv_heads, int n_seq) { return kCus / kv_heads - n_seq / 2; }
 KQ4_DEV int rank_at(const AttnArgs &a, int place, int split) {
-  if (a.plan.order16 == kHalves) return split ? a.kv.n_seq - 1 - place : place;
+  if (a.plan.deal16 == kHalves) return split ? a.kv.n_seq - 1 - place : place;
   const int round = kCus / a.kv.kv_heads;
   return place < round ? place : place < 2 * round ? a.kv.n_seq - 1 - (place - round) : place - round;
+}
+// Turns that sequence i's whole range takes.
+KQ4_DEV int turns_of(const AttnArgs &a, int i) {
+  if (i >= a.kv.n_seq) return 0;
+  const KQ4KvSpan s = kq4_kv_span(a.kv.q_start[i], a.kv.q_start[i + 1], a.kv.kv_len[i], a.kv.n_tok,
+                                  a.kv.table_pages << (a.log_pg + 4));
+  int base, end;
+  kq4_kv_ranges(s, 0, s.nq - 1, a.window, 64, 1, &base, &end);
+  return s.nq ? kq4_kv_turns(base, end, 64 * a.plan.waves16) : 0;
+}
+// Turns of a share: all keys of the batch over the workgroups of a kv head that have a CU each, less the half ranges
+// that rounding up to whole ranges adds.
+KQ4_DEV int share_turns(const AttnArgs &a, int lane) {
+  int all = 0;
+  for (int b = 0; b < a.kv.n_seq; b += 64) all += __builtin_amdgcn_readlane(kq4_scan_add(turns_of(a, b + lane)), 63);
+  const int shares = kq4_attn_shares(a.kv.kv_heads, a.kv.n_seq);
+  return all > shares ? (all + shares - 1) / shares : 1;
+}
+// The sequence and range of item `item` of a kv head's; false where there is none. (A tile of a sequence has no more
+// ranges than its whole range.)
+KQ4_DEV bool shared_item(const AttnArgs &a, int item, int share, int lane, int *seq, int *split) {
+  for (int b = 0; b < a.kv.n_seq; b += 64) {
+    const int n = b + lane < a.kv.n_seq ? kq4_kv_parts(turns_of(a, b + lane), share, a.plan.ns16) : 0;
+    const int sum = kq4_scan_add(n);
+    const unsigned long long at = __ballot(sum > item);
+    if (at) {
+      const int l = __ffsll((long long)at) - 1;
+      *seq = b + l;
+      *split = item - __builtin_amdgcn_readlane(sum - n, l);
+      return true;
+    }
+    item -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+// Keys of a range of a dealt sequence's [base, end), and how many ranges it has.
+KQ4_DEV int dealt_part(const AttnArgs &a, int base, int end, int share, int *used) {
+  const int turn = 64 * a.plan.waves16, turns = kq4_kv_turns(base, end, turn);
+  return turn * kq4_kv_part(turns, a.plan.deal16 == kHalves ? 2 : kq4_kv_parts(turns, share, a.plan.ns16), used);
 }
 // The sequence with `rank` longer ones (ties by number); n_seq <= 64 NW.
 template <int NW>
@@ -243,7 +285,13 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i16 = lane & 15, qd = lane >> 4;
   const int place = block / a.kv.kv_heads, h = block - place * a.kv.kv_heads;
-  const int seq = a.plan.order16 ? ranked<NW>(a, rank_at(a, place, split), lds) : place;
+  int seq = place, share = 0;
+  if (a.plan.deal16 == kShares) {
+    share = share_turns(a, lane);
+    if (!shared_item(a, place, share, lane, &seq, &split)) return;
+  } else if (a.plan.deal16 != kPlain) {
+    seq = ranked<NW>(a, rank_at(a, place, split), lds);
+  }
   const KQ4KvSpan sp = kq4_kv_span(a.kv.q_start[seq], a.kv.q_start[seq + 1], a.kv.kv_len[seq], a.kv.n_tok,
                                    a.kv.table_pages << (a.log_pg + 4));
   const int rows = sp.nq * a.group;
@@ -255,10 +303,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
     const int last = r0 + 15 < rows ? r0 + 15 : rows - 1;
     int base, end;
     int part = chunk, used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, ns, &base, &end);
-    if (a.plan.order16 == kHalves) {
-      part = kq4_kv_half(base, end, 64 * NW);
-      used = end - base > part ? 2 : 1;
-    }
+    if (a.plan.deal16 >= kHalves) part = dealt_part(a, base, end, share, &used);
     if (split >= used) continue;
     base += split * part;
     if (split + 1 < used) end = base + part;
@@ -816,6 +861,7 @@ __global__ __launch_bounds__(256, 2) void attn_mixed_kernel(AttnArgs a, int bloc
 
 // The split plan of a row's sequence and the splits its tile used; 0 for a row of no sequence. Wave-uniform tok.
 KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
+  const int share = a.plan.deal16 == kShares ? share_turns(a, lane) : 0;
   for (int b = 0; b < a.kv.n_seq; b += 64) {
     const int i = b + lane;
     KQ4KvSpan t{0, 0, 0, 0};
@@ -833,10 +879,9 @@ KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
       const int r = (tok - sp.q0) * a.group + head % a.group, r0 = r - r % tile;
       const int last = r0 + tile - 1 < rows ? r0 + tile - 1 : rows - 1;
       int base, end;
-      const int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window,
-                                     small ? a.plan.chunk16 : a.plan.chunk32, small ? a.plan.ns16 : a.plan.ns32, &base,
-                                     &end);
-      if (a.plan.order16 == kHalves) return end - base > kq4_kv_half(base, end, 64 * a.plan.waves16) ? 2 : 1;
+      int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, small ? a.plan.chunk16 : a.plan.chunk32,
+                               small ? a.plan.ns16 : a.plan.ns32, &base, &end);
+      if (a.plan.deal16 >= kHalves) dealt_part(a, base, end, share, &used);
       return used;
     }
   }
@@ -922,7 +967,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 template <int D>
 int launch(const AttnArgs &a, hipStream_t s) {
   const KQ4AttnPlan &p = a.plan;
-  const int blocks16 = a.kv.n_seq * a.kv.kv_heads;
+  const int blocks16 =
+      (p.deal16 == kShares ? kq4_attn_shares(a.kv.kv_heads, a.kv.n_seq) + a.kv.n_seq : a.kv.n_seq) * a.kv.kv_heads;
+  const int ns16 = p.deal16 == kShares ? 1 : p.ns16;   // (a range is an item there)
   const int blocks32 = p.tile32 ? (int)(((long)a.kv.n_tok * a.group / p.tile32 + a.kv.n_seq) * a.kv.kv_heads) : 0;
   static std::atomic<unsigned long long> lds8{0}, lds4{0}, ldsm{0};
   constexpr int lds = kLds32<D>;
@@ -946,9 +993,9 @@ int launch(const AttnArgs &a, hipStream_t s) {
       static std::atomic<unsigned long long> lds16{0};
       const void *fn = reinterpret_cast<const void *>(&attn_rows16_kernel<D, 8>);
       if ((e = kq4_lds_limit_once(fn, kLds16<D, 8>, lds16)) != hipSuccess) return (int)e;
-      attn_rows16_kernel<D, 8><<<dim3(blocks16, p.ns16), 512, kLds16<D, 8>, s>>>(a);
+      attn_rows16_kernel<D, 8><<<dim3(blocks16, ns16), 512, kLds16<D, 8>, s>>>(a);
     } else if (p.max16) {
-      attn_rows16_kernel<D, 4><<<dim3(blocks16, p.ns16), 256, kLds16<D, 4>, s>>>(a);
+      attn_rows16_kernel<D, 4><<<dim3(blocks16, ns16), 256, kLds16<D, 4>, s>>>(a);
     }
   }
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
@@ -1018,15 +1065,24 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // 65.5 us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences
     // of up to 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
     split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
-    // Sequences dealt by length, where there are about as many workgroups as CUs or more and each is long. A CU draws
-    // about 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of
-    // 1621 to 8192 keys 69.0 -> 59.9 us in halves (the join among it; of 8192 each 85.5 -> 90.9), whole ones in order:
-    // 64 of up to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of
-    // 16 heads 115 -> 97. (From 129 to 255 workgroups halves neither gain nor lose.)
-    if (!mixed && force_split <= 0 && p.waves16 == 4 && n_seq <= 256 && keys >= 16 * turn && base > kCus / 2) {
-      if (base > kCus && p.ns16 == 1) p.order16 = kOrder;
+    // Sequences dealt by length, where there are more workgroups than half the CUs and each is long. A CU draws about
+    // 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of 1621 to
+    // 8192 keys 69.0 -> 59.9 us in halves (the join among it; of 8192 each 85.5 -> 90.9), whole ones in order: 64 of up
+    // to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of 16 heads
+    // 115 -> 97. (From 129 to 255 workgroups halves neither gain nor lose.)
+    // Fewer, where the bound makes ranges of 8 turns or more: by shares of all keys that the batch has, up to 4 times an
+    // even batch's ranges of a sequence. Finding them costs 2 us (8 sequences of 2000 keys bounded by 32768 21.7 -> 23.8),
+    // ranges of the bound far more where it is loose or lengths differ: 8 of up to 8000 bounded by 65536 59.5 -> 30.7 us,
+    // one of 16384 bounded by 131072 35.7 -> 19.2.
+    if (!mixed && force_split <= 0 && base <= kCus / 2 && p.ns16 > 1 && p.chunk16 >= 8 * turn) {
+      p.deal16 = kShares;
+      const long most = 4 * (kCus / base), have = (keys + turn - 1) / turn, places = kCus / kv_heads;
+      p.ns16 = (int)(most < have ? most : have);
+      if (p.ns16 > places) p.ns16 = (int)places;
+    } else if (!mixed && force_split <= 0 && p.waves16 == 4 && n_seq <= 256 && keys >= 16 * turn && base > kCus / 2) {
+      if (base > kCus && p.ns16 == 1) p.deal16 = kOrder;
       if (base <= kCus && p.ns16 <= 2) {
-        p.order16 = kHalves;
+        p.deal16 = kHalves;
         p.ns16 = 2;
       }
     }

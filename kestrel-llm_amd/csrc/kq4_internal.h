@@ -186,12 +186,12 @@ struct kq4_kv;
 int kq4_launch_kv_append(const kq4_kv &kv, int log_pg, const float *k, long ldk, const float *v, long ldv,
                          hipStream_t s);
 // The shape of an attention launch. Sequences of at most max16 rows (query tokens * query heads per kv head) take the
-// 16-row form (workgroups of waves16 waves; order16: how sequences are dealt to them), the others tiles of tile32 rows
+// 16-row form (workgroups of waves16 waves; deal16: how sequences are dealt to them), the others tiles of tile32 rows
 // (0: none; 128 or 256); each form splits a tile's keys into ranges of `chunk`, at most ns of them. part_o holds
 // max(ns16, ns32) * n_tok * heads * head_dim floats, part_ml two per row and split (none where that is at most 1).
 #define KQ4_ATTN_MAX_SPLITS 1024
 struct KQ4AttnPlan {
-  int max16, waves16, chunk16, ns16, tile32, chunk32, ns32, order16;
+  int max16, waves16, chunk16, ns16, tile32, chunk32, ns32, deal16;
 };
 KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int window,
                           int force_tile, int force_split);

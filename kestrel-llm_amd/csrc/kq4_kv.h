@@ -69,8 +69,20 @@ KQ4_HD int kq4_kv_ranges(const KQ4KvSpan &s, int t0, int t1, int window, int chu
   return n < 1 ? 1 : n > ns ? ns : n;
 }
 
-// Keys of the first of two about equal parts of [base, end), a multiple of `turn`.
-KQ4_HD int kq4_kv_half(int base, int end, int turn) {
-  const int n = end > base ? end - base : 0;
-  return ((n - n / 2) + turn - 1) / turn * turn;
+// Turns of `turn` keys that [base, end) takes.
+KQ4_HD int kq4_kv_turns(int base, int end, int turn) { return end > base ? (end - base + turn - 1) / turn : 0; }
+
+// Turns of each of about n equal parts (the last one takes fewer); *parts receives how many there are then.
+KQ4_HD int kq4_kv_part(int turns, int n, int *parts) {
+  const int part = n > 1 && turns > 1 ? (turns + n - 1) / n : turns < 1 ? 1 : turns;
+  *parts = turns < 1 ? 1 : (turns + part - 1) / part;
+  return part;
+}
+
+// Parts of a range of so many turns where a share is `share` turns: at most `most`, and none that saves the longest
+// part fewer than 3 turns.
+KQ4_HD int kq4_kv_parts(int turns, int share, int most) {
+  int n = (turns + share - 1) / share;
+  if (n > most) n = most;
+  return n > 1 && turns - (turns + n - 1) / n >= 3 ? n : 1;
 }

@@ -391,6 +391,9 @@ def test_another_stream(kq4, torch_dev):
     ([(100, 200), (3, 700), (1, 64)], 0, 0, 700),    # short and long runs in one launch
     ([(70, 500), (130, 130)], 128, 1, 500), ([(70, 500), (130, 130)], 256, 1, 500),
     ([(70, 500), (130, 130)], 256, 3, 500), ([(9, 1500)], 16, 20, 1500),
+    ([(1, 300)] * 40 + [(1, 90)] * 30, 0, 0, 5000),  # halves by length
+    ([(1, 90)] * 70 + [(1, 300)] * 70, 0, 0, 5000),  # whole by length
+    ([(1, 1900), (1, 90)], 0, 0, 1000000),           # shares of all keys
 ])
 def test_captured_forms(kq4, torch_dev, lens, tile, split, hint):
     """Every form of the attention in a graph, replayed with other queries and lengths, each replay as the eager call
@@ -485,3 +488,15 @@ def test_attention_sequences_by_length(kq4, torch_dev, n_seq, heads, dim, window
     b = Batch(rng, lens, 2, dim, 64, 64, pad=1)
     b.fill(rng, upto="all", spread=1.0)
     check_attn(kq4, torch_dev, b, rand(rng, b.n, heads, dim), heads, window=window, max_kv=5000, max_q=2)
+
+
+@pytest.mark.parametrize("lens", [[(1, 5000)], [(1, 2000), (1, 1), (0, 700), (1, 0), (2, 900)], [(1, 300)] * 60,
+                                  [(1, int(n)) for n in np.linspace(1, 900, 64)], [(9, 600), (1, 1500)]])
+@pytest.mark.parametrize("kv_heads,window", [(2, 0), (1, 0), (2, 333)])
+def test_attention_under_loose_bounds(kq4, torch_dev, lens, kv_heads, window):
+    """A bound far above the lengths: ranges by the keys that are there, also where a sequence has more rows than the
+    bound says."""
+    rng = np.random.default_rng(21)
+    b = Batch(rng, lens, kv_heads, 64, 64, 64, pad=1)
+    b.fill(rng, upto="all", spread=1.0)
+    check_attn(kq4, torch_dev, b, rand(rng, b.n, 4 * kv_heads, 64), 4 * kv_heads, window=window, max_q=1, max_kv=1000000)

@@ -103,6 +103,7 @@ result = [need, before, after]
     (dict(n_seq=64, n_tok=64, max_q=1, max_kv=131072), ["rows16", "join_few"]),      # however long one may be
     (dict(n_seq=32, n_tok=32, max_q=1, max_kv=8192), ["rows16", "join_few"]),        # in halves, by length
     (dict(n_seq=64, n_tok=64, max_q=1, max_kv=4100), ["rows16"]),                    # whole, by length
+    (dict(n_seq=8, n_tok=8, max_q=1, max_kv=65536), ["rows16", "join_few"]),         # shares of all keys
     (dict(n_seq=1, n_tok=4, max_q=4, max_kv=800), ["rows16", "join_few"]),           # 16 rows per kv head
     (dict(n_seq=1, n_tok=4096, max_q=4096, max_kv=4096), ["rows32"]),
     (dict(n_seq=1, n_tok=128, max_q=128, max_kv=16000), ["rows32", "join_few"]),
