@@ -198,10 +198,10 @@ KQ4_DEV float split_factor(float2 ml, float m) {
 // A workgroup is one sequence, kv head and split; its waves take 64 keys in turn straight from memory to
 // registers (nothing is shared between waves until they join), the next keys' loads in flight during the
 // softmax and the second product. Each key is read once, without a place in the caches: 32 sequences of 8192 keys, 8 kv
-// heads of 128 (537 MB) 84.7 us, 6.35 TB/s; of 1621 to 8192 keys (321 MB) 69 us, the longest ones' 2 us a turn of 4
-// waves (64 KB in flight); 1.01 times the bytes it owes. One of 131072 keys, 4 kv heads (134 MB) 25.2 us and 4.5 us for
-// the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and the join: one token
-// over 1001 keys 6.8 us and 3.7 us.
+// heads of 128 (537 MB) 84.7 us in whole sequences, 6.35 TB/s; of 1621 to 8192 keys (321 MB) 54.5 us, 5.9 TB/s, in
+// halves by length and 4.7 us for the join; 1.01 times the bytes it owes. One of 131072 keys, 4 kv heads (134 MB) 25.2
+// us and 4.5 us for the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and the
+// join: one token over 1001 keys 6.8 us and 3.7 us.
 // How sequences are dealt to the workgroups of the 16-row form (kq4_attn_plan). kOrder, kHalves: by length; of two
 // workgroups that share a CU (it takes them in order, a round of kCus and then another) one is long where the other is
 // short. kHalves: the first range of the rank-th longest, the second one of the rank-th shortest. kOrder: whole
@@ -1055,21 +1055,23 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   p.max16 = !p.tile32 ? INT_MAX : mixed ? 16 : 0;
   if (p.max16) {
     // 4 waves a workgroup, two of which fit a CU, so that one's start stands beside the other's loads (64 sequences of
-    // 1000 keys, 8 kv heads: 25.3 us, 31.3 with 8 waves; 64 of up to 4000 65.0 and 70.5). 8 where splits make the
-    // workgroups, one a CU, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 29.6 us, 30.5
-    // with 4 waves; 8 of 8192, 8 kv heads: 29.4 and 30.1; but one of 16384 16.5 and 15.5).
+    // 1000 keys, 8 kv heads: 25.3 us, 31.3 with 8 waves; 64 of up to 4000 65.0 and 70.5). 8 where there is at most one
+    // a CU, by splits or not, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 29.6 us,
+    // 30.5 with 4 waves; 8 of 8192, 8 kv heads: 29.4 and 30.1; but one of 16384 16.5 and 15.5).
     const long base = (long)n_seq * kv_heads;
-    p.waves16 = !mixed && base < kCus && keys / 64 * base > 16 * kCus ? 8 : 4;
+    const bool full = base >= kCus - kCus / 8;   // the CUs, without splits
+    p.waves16 = !mixed && !full && keys / 64 * base > 16 * kCus ? 8 : 4;
     const int turn = 64 * p.waves16;
     // A join costs as much as two turns: 16 sequences, 8 kv heads, 600 / 1000 / 8192 keys in one range 11.2 / 13.4 /
     // 65.5 us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences
     // of up to 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
     split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
-    // Sequences dealt by length, where there are more workgroups than half the CUs and each is long. A CU draws about
-    // 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of 1621 to
-    // 8192 keys 69.0 -> 59.9 us in halves (the join among it; of 8192 each 85.5 -> 90.9), whole ones in order: 64 of up
-    // to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of 16 heads
-    // 115 -> 97. (From 129 to 255 workgroups halves neither gain nor lose.)
+    // Sequences dealt by length, where there are about as many workgroups as CUs or more and each is long. A CU draws
+    // about 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of
+    // 1621 to 8192 keys 69.0 -> 59.5 us in halves (the join among it; of 8192 each 85.5 -> 90.9), 28 of up to 8192 66.9
+    // -> 58.7 (equal ones 78.5 -> 83.5; but 24 65.0 and 62.0, 73.1 and 79.4: whole, with 8 waves); whole ones in order:
+    // 64 of up to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of 16
+    // heads 115 -> 97.
     // Fewer, where the bound makes ranges of 8 turns or more: by shares of all keys that the batch has, up to 4 times an
     // even batch's ranges of a sequence. Finding them costs 2 us (8 sequences of 2000 keys bounded by 32768 21.7 -> 23.8),
     // ranges of the bound far more where it is loose or lengths differ: 8 of up to 8000 bounded by 65536 59.5 -> 30.7 us,
@@ -1079,7 +1081,7 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
       const long most = 4 * (kCus / base), have = (keys + turn - 1) / turn, places = kCus / kv_heads;
       p.ns16 = (int)(most < have ? most : have);
       if (p.ns16 > places) p.ns16 = (int)places;
-    } else if (!mixed && force_split <= 0 && p.waves16 == 4 && n_seq <= 256 && keys >= 16 * turn && base > kCus / 2) {
+    } else if (!mixed && force_split <= 0 && full && n_seq <= 64 * p.waves16 && keys >= 16 * turn) {
       if (base > kCus && p.ns16 == 1) p.deal16 = kOrder;
       if (base <= kCus && p.ns16 <= 2) {
         p.deal16 = kHalves;

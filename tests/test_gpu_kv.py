@@ -391,7 +391,7 @@ def test_another_stream(kq4, torch_dev):
     ([(100, 200), (3, 700), (1, 64)], 0, 0, 700),    # short and long runs in one launch
     ([(70, 500), (130, 130)], 128, 1, 500), ([(70, 500), (130, 130)], 256, 1, 500),
     ([(70, 500), (130, 130)], 256, 3, 500), ([(9, 1500)], 16, 20, 1500),
-    ([(1, 300)] * 40 + [(1, 90)] * 30, 0, 0, 5000),  # halves by length
+    ([(1, 300)] * 70 + [(1, 90)] * 50, 0, 0, 5000),  # halves by length
     ([(1, 90)] * 70 + [(1, 300)] * 70, 0, 0, 5000),  # whole by length
     ([(1, 1900), (1, 90)], 0, 0, 1000000),           # shares of all keys
 ])
@@ -477,7 +477,7 @@ def test_large_pages(kq4, torch_dev):
     check_attn(kq4, torch_dev, b, rand(rng, b.n, 2, 64), 2)
 
 
-@pytest.mark.parametrize("n_seq", [65, 70, 128, 150, 256])
+@pytest.mark.parametrize("n_seq", [65, 112, 128, 150, 256])
 @pytest.mark.parametrize("heads,dim,window", [(4, 64, 0), (2, 128, 0), (4, 64, 40)])
 def test_attention_sequences_by_length(kq4, torch_dev, n_seq, heads, dim, window):
     """Many sequences under a bound of the lengths that makes their order (whole or in halves) go by length: of all
