@@ -20,4 +20,8 @@ int t_ranges(int nq, int p0, int len, int t0, int t1, int window, int chunk, int
   return kq4_kv_ranges(s, t0, t1, window, chunk, ns, out, out + 1);
 }
 
+int t_parts(int turns, int share, int most) { return kq4_kv_parts(turns, share, most); }
+
+int t_part(int turns, int n, int *parts) { return kq4_kv_part(turns, n, parts); }
+
 }

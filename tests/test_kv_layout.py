@@ -90,3 +90,25 @@ def test_split_ranges_cover_the_keys(lib):
             got |= set(range(b, end if s + 1 == used else b + chunk))
             assert s == 0 or b < end                           # no split without a key beside the first
         assert seen <= got
+
+
+def test_parts_cover_a_range_and_fit_the_shares(lib):
+    """Ranges by shares: of any number of turns they cover it without an empty one, a shorter range of the sequence has
+    no more of them, and those of a batch fit the items that its launch has."""
+    used = ints(1)
+    for share in (1, 2, 3, 5, 7, 40):
+        for most in (1, 2, 4, 9, 64):
+            before = 1
+            for turns in range(200):
+                n = lib.t_parts(turns, share, most)
+                assert before <= n <= max(1, min(most, -(-turns // share)))
+                before = n
+                part = lib.t_part(turns, n, used)
+                assert 1 <= used[0] <= n and part >= 1
+                assert part * used[0] >= turns and (used[0] == 1 or part * (used[0] - 1) < turns)
+    rng = random.Random(3)
+    for _ in range(3000):
+        n_seq, shares = rng.randint(1, 64), rng.randint(1, 256)
+        turns = [rng.choice([0, 1, 2, rng.randint(0, 500)]) for _ in range(n_seq)]
+        share = max(1, -(-sum(turns) // shares))
+        assert sum(lib.t_parts(t, share, 1000) for t in turns) <= shares + n_seq
