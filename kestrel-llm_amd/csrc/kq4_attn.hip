@@ -200,8 +200,9 @@ KQ4_DEV float split_factor(float2 ml, float m) {
 // softmax and the second product. Each key is read once, without a place in the caches: 32 sequences of 8192 keys, 8 kv
 // heads of 128 (537 MB) 84.7 us in whole sequences, 6.35 TB/s; of 1621 to 8192 keys (321 MB) 54.5 us, 5.9 TB/s, in
 // halves by length and 4.7 us for the join; 1.01 times the bytes it owes. One of 131072 keys, 4 kv heads (134 MB) 25.2
-// us and 4.5 us for the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and the
-// join: one token over 1001 keys 6.8 us and 3.7 us.
+// us and 4.5 us for the join. Bound by memory; a short call by its chain of dependent loads (lengths, page, keys) and
+// the join: one token over 1001 keys 6.8 us and 3.7 us.
+
 // How sequences are dealt to the workgroups of the 16-row form (kq4_attn_plan). kOrder, kHalves: by length; of two
 // workgroups that share a CU (it takes them in order, a round of kCus and then another) one is long where the other is
 // short. kHalves: the first range of the rank-th longest, the second one of the rank-th shortest. kOrder: whole
@@ -1072,10 +1073,10 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // -> 58.7 (equal ones 78.5 -> 83.5; but 24 65.0 and 62.0, 73.1 and 79.4: whole, with 8 waves); whole ones in order:
     // 64 of up to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of 16
     // heads 115 -> 97.
-    // Fewer, where the bound makes ranges of 8 turns or more: by shares of all keys that the batch has, up to 4 times an
-    // even batch's ranges of a sequence. Finding them costs 2 us (8 sequences of 2000 keys bounded by 32768 21.7 -> 23.8),
-    // ranges of the bound far more where it is loose or lengths differ: 8 of up to 8000 bounded by 65536 59.5 -> 30.7 us,
-    // one of 16384 bounded by 131072 35.7 -> 19.2.
+    // Fewer, where the bound makes ranges of 8 turns or more: by shares of all keys that the batch has, up to 4 times
+    // an even batch's ranges of a sequence. Finding them costs 2 us (8 sequences of 2000 keys bounded by 32768 21.7 ->
+    // 23.8), ranges of the bound far more where it is loose or lengths differ: 8 of up to 8000 bounded by 65536 59.5 ->
+    // 30.7 us, one of 16384 bounded by 131072 35.7 -> 19.2.
     if (!mixed && force_split <= 0 && base <= kCus / 2 && p.ns16 > 1 && p.chunk16 >= 8 * turn) {
       p.deal16 = kShares;
       const long most = 4 * (kCus / base), have = (keys + turn - 1) / turn, places = kCus / kv_heads;
@@ -1096,8 +1097,8 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // over 900 33.1 / 29.3 / 32.3, 300 x 32 over 16000 86.7 / 78 / 78.)
     const int best = (int)(sqrt((double)kRowKeys * keys / ((double)n_tok * heads)) + 0.5);
     const long least = best < 2 ? keys : (keys + best - 1) / best;
-    split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus, 64, 0,
-               least > kMinChunk ? (int)least : kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
+    split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus,
+               64, 0, least > kMinChunk ? (int)least : kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
   }
   return p;
 }
