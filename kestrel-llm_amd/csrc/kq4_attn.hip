@@ -12,7 +12,9 @@
 //
 // With e_j = log2(p_j) + log2(vs_j) (vs_j the value scale of key j's group), O sums 2^(e_j - M) codes and l
 // sums 2^(e_j - M) / vs_j, M the running maximum of e_j: the value scale costs no instruction per key, and
-// the f16 range holds what O gets, whatever the scales are (they are at least 2^-100, so l stays finite).
+// the f16 range holds what O gets, whatever the scales are. A weight is at most 2^(kTop + kSlack) and a scale between
+// 2^-100 and 2^121, so l is held at kLow: 2^25 keys of the least scale fit below 2^128 (2^14 without the factor), and
+// a key of the largest scale at the maximum still counts 2^-126, the least normal number.
 #include "kq4_common.h"
 #include "kq4_kv.h"
 #include "kq4_internal.h"
@@ -39,6 +41,7 @@ constexpr float kNegInf = -__builtin_inff();
 // P is held at 2^kTop for the running maximum, which is raised only where a key passes it by 2^kSlack:
 // f16 holds 2^(kTop + kSlack), and lo's last bit at the maximum is 2^-31 of it.
 constexpr float kTop = 6.0f, kSlack = 8.0f;
+constexpr float kLow = 0x1p-11f;   // of a row's sum of weights, O is without it
 
 struct AttnArgs {
   kq4_kv kv;
@@ -51,7 +54,7 @@ struct AttnArgs {
   int window;
   KQ4AttnPlan plan;
   float *part_o;      // [splits][n_tok * heads][D], unnormalised
-  float2 *part_ml;    // [splits][n_tok * heads] maximum, sum
+  float2 *part_ml;    // [splits][n_tok * heads] maximum, sum (at kLow)
 };
 
 union Frag {
@@ -454,7 +457,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
           sum += p0 + p1;
           split_pair(p0, p1, ph[t4 >> 1].u[2 * (t4 & 1) + (j >> 1)], pl[t4 >> 1].u[2 * (t4 & 1) + (j >> 1)]);
         }
-      l = fmaf(sum, rv, l);
+      l = fmaf(sum * kLow, rv, l);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const half8 v0 = codes_f16(vr[d].x, vr[d].y), v1 = codes_f16(vr[d].z, vr[d].w);
@@ -496,7 +499,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
       const long row = (long)(sp.q0 + t) * a.heads + h * a.group + (r0 + rr - t * a.group);
       if (used == 1) {
         const float f = sl == 0.0f ? 0.0f : 1.0f / sl;
-        *reinterpret_cast<float4v *>(a.out + row * D + d) = acc * f;
+        *reinterpret_cast<float4v *>(a.out + row * D + d) = (acc * kLow) * f;
       } else {
         *reinterpret_cast<float4v *>(a.part_o + (split * n_rows + row) * D + d) = acc;
         if (d == 0) a.part_ml[split * n_rows + row] = make_float2(m, sl);
@@ -761,7 +764,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (has.value) l = fmaf(sum, rv, l);
+    if constexpr (has.value) l = fmaf(sum * kLow, rv, l);
     if constexpr (more.value) {
       if constexpr (!has.value)
 #pragma unroll
@@ -827,12 +830,13 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   const long row = (long)(sp.q0 + tq) * a.heads + head, n_rows = (long)a.kv.n_tok * a.heads;
   float *dst = used == 1 ? a.out + row * D : a.part_o + (split * n_rows + row) * D;
   const float f = used > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  const float low = used > 1 ? 1.0f : kLow;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int j = 0; j < 16; j += 4)
       *reinterpret_cast<float4 *>(dst + 32 * d + 2 * j + 4 * hh) =
-          make_float4(o[d][j] * f, o[d][j + 1] * f, o[d][j + 2] * f, o[d][j + 3] * f);
+          make_float4(o[d][j] * low * f, o[d][j + 1] * low * f, o[d][j + 2] * low * f, o[d][j + 3] * low * f);
   if (used > 1 && hh == 0) a.part_ml[split * n_rows + row] = make_float2(M, l);
 }
 
@@ -917,7 +921,7 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int part
     const float fs = __shfl(f, (lane & -kJoinFew) + s);
     acc += *reinterpret_cast<const float4v *>(p + s * n_rows * D) * fs;
   }
-  *reinterpret_cast<float4v *>(a.out + row * D + at % D) = acc * (sl == 0.0f ? 0.0f : 1.0f / sl);
+  *reinterpret_cast<float4v *>(a.out + row * D + at % D) = (acc * kLow) * (sl == 0.0f ? 0.0f : 1.0f / sl);
 }
 
 // Joins the splits of a row, many of them, 32 dimensions a workgroup: the factors of all splits into LDS, then 8
@@ -961,7 +965,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int w = 1; w < 8; ++w) acc += s_acc[w][tid];
     sl = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-    a.out[row * D + d] = sl == 0.0f ? 0.0f : acc / sl;
+    a.out[row * D + d] = sl == 0.0f ? 0.0f : acc * kLow / sl;
   }
 }
 
