@@ -100,8 +100,7 @@ KQ4_DEV QRope q_rope(const kq4_kv &kv, int token, int pos) {
 }
 
 // Chunks c0, c0 + step, .. (16 dimensions each, N of them) of a query row, rotated as the keys were (in fp32 here: q
-// is not rounded to a grid afterwards). A row that the table does not have is left as it is: the caller makes its
-// scores NaN.
+// is not rounded to a grid afterwards). A row that the table does not have is left as it is: the caller puts a NaN in.
 template <int N>
 KQ4_DEV void load_q(const float *row, const QRope &r, int c0, int step, float (*x)[16]) {
   float4v own[N][4];
@@ -363,7 +362,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
     }
 
     half8 qh[TT][2], ql[TT][2];
-    float descale;
+    int sh;
     {
       float x[TT][16], amax = 0.0f;
       const QRope rope = q_rope(a.kv, sp.q0 + tq, sp.p0 + tq);
@@ -372,8 +371,8 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
       for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
-      const int sh = row_shift(max_xor32(max_xor16(amax)));
-      descale = rope.bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale2, -sh);
+      sh = row_shift(max_xor32(max_xor16(amax)));
+      if (rope.bad) x[0][0] = __uint_as_float(0x7fc00000u);
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
@@ -409,7 +408,8 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
       }
 
       // this lane's 16 keys are tokens 4 t4 + j of group qd of the 64
-      float c = there ? scale.x * descale : 0.0f, lv = there ? __builtin_amdgcn_logf(scale.y) : 0.0f;
+      // (2^-sh last: alone with scale2 it is subnormal for queries below 2^-110)
+      float c = there ? ldexpf(scale.x * a.scale2, -sh) : 0.0f, lv = there ? __builtin_amdgcn_logf(scale.y) : 0.0f;
       float rv = there ? __builtin_amdgcn_rcpf(scale.y) : 0.0f;
       const bool masked = key < all_lo || key + 64 > all_hi || __ballot(!there) != 0;
       if (masked) {
@@ -649,7 +649,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
 
   // the first three tiles and the query row, all on their way at once
   half8 qh[TT][2], ql[TT][2];
-  float descale;
+  int sh;
   {
     const int e0 = entry(0), e1 = entry(1), e2 = entry(2);
     uint4v raw0[NL], raw1[NL];
@@ -667,8 +667,8 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[t][e]));
-    const int sh = row_shift(max_xor32(amax));
-    descale = rope.bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale2, -sh);
+    sh = row_shift(max_xor32(amax));
+    if (rope.bad) x[0][0] = __uint_as_float(0x7fc00000u);
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
@@ -747,7 +747,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
           float sk = scale[0], sv = scale[1];
           asm volatile("" : "+v"(sk), "+v"(sv));
           masked = (base + 32 * (n + 1) < all_lo) | (base + 32 * (n + 2) > all_hi) | (__ballot(sv == 0.0f) != 0);
-          c_n = sk * descale;
+          c_n = ldexpf(sk * a.scale2, -sh);   // (as in the 16-row form)
           lv_n = __builtin_amdgcn_logf(sv);
           rv_n = __builtin_amdgcn_rcpf(sv);
           c_n = c_n == 0.0f ? 1e-37f : c_n;   // (a masked score, -inf, stays that)
