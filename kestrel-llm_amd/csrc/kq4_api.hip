@@ -1276,15 +1276,6 @@ KQ4AttnPlan attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, 
   return kq4_attn_plan(n_tok, n_seq, heads, kv_heads, max_q, max_kv, window, opt(kAttnTile), opt(kAttnSplit));
 }
 
-size_t attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int heads, int head_dim, size_t *o_bytes) {
-  *o_bytes = 0;
-  const int ns = p.ns16 > p.ns32 ? p.ns16 : p.ns32;
-  if (ns <= 1) return 0;
-  const size_t rows = (size_t)ns * n_tok * heads;
-  *o_bytes = al256(rows * head_dim * sizeof(float));
-  return *o_bytes + al256(rows * 2 * sizeof(float));
-}
-
 size_t logprobs_bytes(int n, int vocab, int n_top, size_t *piece_bytes) {
   const size_t np = (size_t)n * kq4_logprobs_pieces(vocab);
   *piece_bytes = al256(np * kq4_logprobs_piece_bytes());
@@ -1349,15 +1340,14 @@ int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_h
                                            kv->n_seq) * kv->kv_heads * plan.ns32 : 0);
   if (blocks > 0x7fffffffLL)
     return fail(KQ4_EINVAL, "attn: n_seq=%d n_tok=%d q_heads=%d", kv->n_seq, kv->n_tok, q_heads);
-  size_t o_bytes = 0;
-  const size_t bytes = attn_part_bytes(plan, kv->n_tok, q_heads, kv->head_dim, &o_bytes);
+  size_t bytes16 = 0;
+  const size_t bytes = kq4_attn_part_bytes(plan, kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, kv->head_dim, &bytes16);
   char *ws = nullptr;
   if (bytes) {
     if ((rc = ensure_ws(Ws{&ds->ws, ds}, bytes, s))) return rc;
     ws = static_cast<char *>(ds->ws.p);
   }
-  KQ4_HIP((hipError_t)kq4_launch_attn(out, *kv, log_pg, q, ldq, q_heads, scale, window, plan,
-                                      reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + o_bytes), s));
+  KQ4_HIP((hipError_t)kq4_launch_attn(out, *kv, log_pg, q, ldq, q_heads, scale, window, plan, ws, s));
   return KQ4_OK;
 }
 
@@ -1366,9 +1356,9 @@ size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads,
   if (n_tok < 1 || n_seq < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads ||
       (head_dim != 64 && head_dim != 128) || window < 0 || max_q < 0 || max_kv < 0)
     return 0;
-  size_t o_bytes = 0;
-  return attn_part_bytes(attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv, window), n_tok, q_heads, head_dim,
-                         &o_bytes);
+  size_t bytes16 = 0;
+  return kq4_attn_part_bytes(attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv, window), n_tok, n_seq, q_heads,
+                             kv_heads, head_dim, &bytes16);
 }
 
 int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *top_id, const float *logits, long ld,

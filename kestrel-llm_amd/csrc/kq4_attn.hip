@@ -36,6 +36,7 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 constexpr int kCus = 256;      // compute units of an MI355X
 constexpr int kMinChunk = 128; // keys that a split of the 32-row form has at least
 constexpr int kRowKeys = 80;   // and the weight of its keys against its partial sums (kq4_attn_plan)
+constexpr long kPartRows = 1 << 18;   // rows of partial sums of the 16-row form, at most (136 MB of 128 dimensions)
 constexpr int kJoinFew = 16;   // splits up to which a wave joins a row alone
 constexpr float kNegInf = -__builtin_inff();
 // P is held at 2^kTop for the running maximum, which is raised only where a key passes it by 2^kSlack:
@@ -45,17 +46,25 @@ constexpr float kLow = 0x1p-11f;   // of a row's sum of weights, O is without it
 
 struct AttnArgs {
   kq4_kv kv;
-  int log_pg;
   const float *q;
   long ldq;
   float *out;
+  int log_pg;
   int heads, group;   // query heads, and those per kv head
   float scale2;       // softmax scale * log2(e)
   int window;
   KQ4AttnPlan plan;
-  float *part_o;      // [splits][n_tok * heads][D], unnormalised
-  float2 *part_ml;    // [splits][n_tok * heads] maximum, sum (at kLow)
+  // partial sums [splits][rows][D], unnormalised, then [splits][rows] maximum and sum (at kLow). Rows of the 16-row
+  // form: [n_seq][kv_heads][plan.cap16]; of the 32-row form: [n_tok][heads].
+  float *part16, *part32;
 };
+static_assert(sizeof(AttnArgs) <= 192, "a fourth line of arguments costs a short launch 0.25 us");
+
+// A split's sums of a row, of n splits of so many rows.
+KQ4_DEV float *part_o(float *part, long rows, long row, int split, int dim) { return part + (split * rows + row) * dim; }
+KQ4_DEV float2 *part_ml(float *part, int n, long rows, long row, int split, int dim) {
+  return reinterpret_cast<float2 *>(part + n * rows * dim) + split * rows + row;
+}
 
 union Frag {
   uint32_t u[4];
@@ -190,6 +199,9 @@ KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float 
   pl[j >> 3].u[(j & 7) >> 1] = l;
 }
 
+// Rows that have partial sums in the 16-row form.
+KQ4_HD long slots_of(const AttnArgs &a) { return (long)a.kv.n_seq * a.kv.kv_heads * a.plan.cap16; }
+
 // The factor of a split's, or wave's, sums in the joined row (one of which nothing was seen: 0; one whose scales were
 // all NaN keeps its NaN).
 KQ4_DEV float split_factor(float2 ml, float m) {
@@ -217,14 +229,14 @@ KQ4_DEV int rank_at(const AttnArgs &a, int place, int split) {
   const int round = kCus / a.kv.kv_heads;
   return place < round ? place : place < 2 * round ? a.kv.n_seq - 1 - (place - round) : place - round;
 }
-// Turns that sequence i's whole range takes.
+// Turns that sequence i's whole range takes, 0 where it is not split (no rows, or more than its partial sums' room).
 KQ4_DEV int turns_of(const AttnArgs &a, int i) {
   if (i >= a.kv.n_seq) return 0;
   const KQ4KvSpan s = kq4_kv_span(a.kv.q_start[i], a.kv.q_start[i + 1], a.kv.kv_len[i], a.kv.n_tok,
                                   a.kv.table_pages << (a.log_pg + 4));
   int base, end;
   kq4_kv_ranges(s, 0, s.nq - 1, a.window, 64, 1, &base, &end);
-  return s.nq ? kq4_kv_turns(base, end, 64 * a.plan.waves16) : 0;
+  return s.nq && s.nq * a.group <= a.plan.cap16 ? kq4_kv_turns(base, end, 64 * a.plan.waves16) : 0;
 }
 // Turns of a share: all keys of the batch over the workgroups of a kv head that have a CU each, less the half ranges
 // that rounding up to whole ranges adds.
@@ -284,7 +296,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
   constexpr int TT = D / 64, DT = D / 16, LD = D + 4;
   float(*s_o)[16][LD] = reinterpret_cast<float(*)[16][LD]>(lds);
   float2(*s_ml)[16] = reinterpret_cast<float2(*)[16]>(lds + NW * 16 * LD * 4);
-  const int chunk = a.plan.chunk16, ns = a.plan.ns16;
+  const int chunk = a.plan.chunk16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i16 = lane & 15, qd = lane >> 4;
   const int place = block / a.kv.kv_heads, h = block - place * a.kv.kv_heads;
@@ -299,14 +311,15 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
                                    a.kv.table_pages << (a.log_pg + 4));
   const int rows = sp.nq * a.group;
   if (rows > a.plan.max16) return;
+  const bool whole = rows > a.plan.cap16;
   const int *table = a.kv.block_table + (long)seq * a.kv.table_pages;
-  const long n_rows = (long)a.kv.n_tok * a.heads;
 
   for (int r0 = 0; r0 < rows; r0 += 16) {
     const int last = r0 + 15 < rows ? r0 + 15 : rows - 1;
     int base, end;
-    int part = chunk, used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, ns, &base, &end);
-    if (a.plan.deal16 >= kHalves) part = dealt_part(a, base, end, share, &used);
+    int part = chunk, used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, chunk, whole ? 1 : a.plan.ns16,
+                                           &base, &end);
+    if (a.plan.deal16 >= kHalves && !whole) part = dealt_part(a, base, end, share, &used);
     if (split >= used) continue;
     base += split * part;
     if (split + 1 < used) end = base + part;
@@ -495,14 +508,15 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
         sl = fmaf(ml.y, f, sl);
         acc += *reinterpret_cast<const float4v *>(&s_o[w][rr][d]) * f;
       }
-      const int t = (r0 + rr) / a.group;
-      const long row = (long)(sp.q0 + t) * a.heads + h * a.group + (r0 + rr - t * a.group);
       if (used == 1) {
+        const int t = (r0 + rr) / a.group;
+        const long row = (long)(sp.q0 + t) * a.heads + h * a.group + (r0 + rr - t * a.group);
         const float f = sl == 0.0f ? 0.0f : 1.0f / sl;
         *reinterpret_cast<float4v *>(a.out + row * D + d) = (acc * kLow) * f;
       } else {
-        *reinterpret_cast<float4v *>(a.part_o + (split * n_rows + row) * D + d) = acc;
-        if (d == 0) a.part_ml[split * n_rows + row] = make_float2(m, sl);
+        const int slot = (seq * a.kv.kv_heads + h) * a.plan.cap16 + rr;   // (r0 is 0)
+        *reinterpret_cast<float4v *>(part_o(a.part16, slots_of(a), slot, split, D) + d) = acc;
+        if (d == 0) *part_ml(a.part16, a.plan.ns16, slots_of(a), slot, split, D) = make_float2(m, sl);
       }
     }
     __syncthreads();
@@ -828,7 +842,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
   if (w0 + i32 > last) return;
   l = kq4_xor_add<32>(l);
   const long row = (long)(sp.q0 + tq) * a.heads + head, n_rows = (long)a.kv.n_tok * a.heads;
-  float *dst = used == 1 ? a.out + row * D : a.part_o + (split * n_rows + row) * D;
+  float *dst = used == 1 ? a.out + row * D : part_o(a.part32, n_rows, row, split, D);
   const float f = used > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
   const float low = used > 1 ? 1.0f : kLow;
 #pragma unroll
@@ -837,7 +851,7 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
     for (int j = 0; j < 16; j += 4)
       *reinterpret_cast<float4 *>(dst + 32 * d + 2 * j + 4 * hh) =
           make_float4(o[d][j] * low * f, o[d][j + 1] * low * f, o[d][j + 2] * low * f, o[d][j + 3] * low * f);
-  if (used > 1 && hh == 0) a.part_ml[split * n_rows + row] = make_float2(M, l);
+  if (used > 1 && hh == 0) *part_ml(a.part32, a.plan.ns32, n_rows, row, split, D) = make_float2(M, l);
 }
 
 template <int D, int NW>
@@ -864,9 +878,36 @@ __global__ __launch_bounds__(256, 2) void attn_mixed_kernel(AttnArgs a, int bloc
     attn_rows32<D, 4>(a, (b - n16) % blocks32, blocks32, (b - n16) / blocks32, dyn_lds);
 }
 
-// The split plan of a row's sequence and the splits its tile used; 0 for a row of no sequence. Wave-uniform tok.
-KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
+// A row that a thread joins: where its partial sums and its output stand, and how many ranges it has (0: none to join).
+struct JoinRow {
+  float *part;
+  long rows, row, out;
+  int n, used;
+};
+
+// Row `slot` of the 16-row form's (fewer than 2^18 and a workgroup's); every lane takes part, slots may differ.
+KQ4_DEV JoinRow join_row16(const AttnArgs &a, int slot, int lane) {
   const int share = a.plan.deal16 == kShares ? share_turns(a, lane) : 0;
+  JoinRow j{a.part16, slots_of(a), slot, 0, a.plan.ns16, 0};
+  const int sh = slot / a.plan.cap16, r = slot - sh * a.plan.cap16;
+  const int seq = sh / a.kv.kv_heads, h = sh - seq * a.kv.kv_heads;
+  if (seq >= a.kv.n_seq) return j;
+  const KQ4KvSpan sp = kq4_kv_span(a.kv.q_start[seq], a.kv.q_start[seq + 1], a.kv.kv_len[seq], a.kv.n_tok,
+                                   a.kv.table_pages << (a.log_pg + 4));
+  const int rows = sp.nq * a.group;
+  if (r >= rows || rows > a.plan.cap16 || rows > a.plan.max16) return j;
+  int base, end;
+  j.used = kq4_kv_ranges(sp, 0, sp.nq - 1, a.window, a.plan.chunk16, a.plan.ns16, &base, &end);
+  if (a.plan.deal16 >= kHalves) dealt_part(a, base, end, share, &j.used);
+  const int t = r / a.group;
+  j.out = (long)(sp.q0 + t) * a.heads + h * a.group + (r - t * a.group);
+  return j;
+}
+
+// Token tok's row of a head in the 32-row form; tok is the same for the wave, whose lanes all take part.
+KQ4_DEV JoinRow join_row32(const AttnArgs &a, int tok, int head, int lane) {
+  const long row = (long)tok * a.heads + head;
+  JoinRow j{a.part32, (long)a.kv.n_tok * a.heads, row, row, a.plan.ns32, 0};
   for (int b = 0; b < a.kv.n_seq; b += 64) {
     const int i = b + lane;
     KQ4KvSpan t{0, 0, 0, 0};
@@ -879,34 +920,36 @@ KQ4_DEV int splits_used(const AttnArgs &a, int tok, int head, int lane) {
       const KQ4KvSpan sp{__builtin_amdgcn_readlane(t.q0, l), __builtin_amdgcn_readlane(t.nq, l),
                          __builtin_amdgcn_readlane(t.p0, l), __builtin_amdgcn_readlane(t.len, l)};
       const int rows = sp.nq * a.group;
-      const bool small = rows <= a.plan.max16;
-      const int tile = small ? 16 : a.plan.tile32;
-      const int r = (tok - sp.q0) * a.group + head % a.group, r0 = r - r % tile;
-      const int last = r0 + tile - 1 < rows ? r0 + tile - 1 : rows - 1;
+      if (rows <= a.plan.max16 || head >= a.heads) return j;
+      const int r = (tok - sp.q0) * a.group + head % a.group, r0 = r - r % a.plan.tile32;
+      const int last = r0 + a.plan.tile32 - 1 < rows ? r0 + a.plan.tile32 - 1 : rows - 1;
       int base, end;
-      int used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, small ? a.plan.chunk16 : a.plan.chunk32,
-                               small ? a.plan.ns16 : a.plan.ns32, &base, &end);
-      if (a.plan.deal16 >= kHalves) dealt_part(a, base, end, share, &used);
-      return used;
+      j.used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, a.plan.chunk32, a.plan.ns32, &base, &end);
+      return j;
     }
   }
-  return 0;
+  return j;
 }
 
-// Joins the splits of rows, few of them: a workgroup takes up to 1024 floats of a token, 4 a thread, so that one search
-// for the token's sequence serves several heads. Of a head's 16 or 32 lanes, lane s holds split s's factor. Bound by
-// latency (search, factors, sums: three dependent loads): 8400 rows of 64, 4 splits 4.7 us; a wave a row, the factors
-// one after the other, took 7.4.
+// Joins the splits of rows, few of them: a workgroup takes up to 1024 floats, 4 a thread, of neighbouring rows: blocks16
+// workgroups those of the 16-row form, the others `parts` each of a token of the 32-row form. Of a row's 16 or 32 lanes,
+// lane s holds split s's factor. Bound by latency (lengths, factors, sums: three dependent loads): 8400 rows of 64, 4
+// splits 4.7 us; a wave a row, the factors one after the other, took 7.4.
 template <int D>
-__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int parts) {
-  static_assert(D / 4 >= kJoinFew, "a head's lanes hold a factor each");
-  const int lane = threadIdx.x & 63, tok = blockIdx.x / parts, part = blockIdx.x - tok * parts;
-  const int at = 1024 * part + 4 * (int)threadIdx.x, head = at / D;
-  const int used = splits_used(a, tok, head, lane);
-  if (head >= a.heads || used <= 1) return;   // (no sequence's row, or written by its only split)
-  const long row = (long)tok * a.heads + head, n_rows = (long)a.kv.n_tok * a.heads;
+__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int blocks16, int parts) {
+  static_assert(D / 4 >= kJoinFew, "a row's lanes hold a factor each");
+  const int lane = threadIdx.x & 63, b = blockIdx.x - blocks16;
+  JoinRow j;
+  if (b < 0) {
+    j = join_row16(a, (int)blockIdx.x * (1024 / D) + 4 * (int)threadIdx.x / D, lane);
+  } else {
+    const int tok = b / parts;
+    j = join_row32(a, tok, (1024 * (b - tok * parts) + 4 * (int)threadIdx.x) / D, lane);
+  }
+  const int used = j.used, d = 4 * (int)threadIdx.x % D;
+  if (used <= 1) return;   // (no row, or written by its only split)
   const int s0 = lane & (kJoinFew - 1);
-  const float2 ml = s0 < used ? a.part_ml[s0 * n_rows + row] : make_float2(kNegInf, 0.0f);
+  const float2 ml = s0 < used ? *part_ml(j.part, j.n, j.rows, j.row, s0, D) : make_float2(kNegInf, 0.0f);
   float m = ml.x;
 #pragma unroll
   for (int x = kJoinFew / 2; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
@@ -915,30 +958,40 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int part
 #pragma unroll
   for (int x = kJoinFew / 2; x; x >>= 1) sl += __shfl_xor(sl, x);
   float4v acc = {0.f, 0.f, 0.f, 0.f};
-  const float *p = a.part_o + row * D + at % D;
+  const float *p = part_o(j.part, j.rows, j.row, 0, D) + d;
 #pragma unroll 4
   for (int s = 0; s < used; ++s) {
     const float fs = __shfl(f, (lane & -kJoinFew) + s);
-    acc += *reinterpret_cast<const float4v *>(p + s * n_rows * D) * fs;
+    acc += *reinterpret_cast<const float4v *>(p + s * j.rows * D) * fs;
   }
-  *reinterpret_cast<float4v *>(a.out + row * D + at % D) = (acc * kLow) * (sl == 0.0f ? 0.0f : 1.0f / sl);
+  *reinterpret_cast<float4v *>(a.out + j.out * D + d) = (acc * kLow) * (sl == 0.0f ? 0.0f : 1.0f / sl);
 }
 
-// Joins the splits of a row, many of them, 32 dimensions a workgroup: the factors of all splits into LDS, then 8
-// threads a dimension take splits in turn (32 rows of 128, 64 splits 4.5 us, latency).
+// Joins the splits of a row, many of them, 32 dimensions a workgroup (blocks16 of the 16-row form's rows, then the
+// 32-row form's): the factors of all splits into LDS, then 8 threads a dimension take splits in turn (32 rows of 128, 64
+// splits 4.5 us, latency).
 template <int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks16) {
   __shared__ float s_f[KQ4_ATTN_MAX_SPLITS];
   __shared__ float s_acc[8][32], s_m[4], s_l[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long row = blockIdx.x / (D / 32), n_rows = (long)a.kv.n_tok * a.heads;
-  const int d = 32 * (int)(blockIdx.x % (D / 32)) + (tid & 31);
-  const int tok = (int)(row / a.heads), head = (int)(row - (long)tok * a.heads);
-  const int used = splits_used(a, tok, head, lane);
+  const bool few_rows = (int)blockIdx.x < blocks16;
+  const int b = few_rows ? blockIdx.x : blockIdx.x - blocks16;
+  const long row = b / (D / 32);
+  const int d = 32 * (b % (D / 32)) + (tid & 31);
+  JoinRow j;
+  if (few_rows) {
+    j = join_row16(a, (int)row, lane);
+  } else {
+    const int tok = (int)(row / a.heads);
+    j = join_row32(a, tok, (int)(row - (long)tok * a.heads), lane);
+  }
+  const int used = j.used;
   if (used <= 1) return;
+  const float2 *ml0 = part_ml(j.part, j.n, j.rows, j.row, 0, D);
 
   float m = kNegInf;
-  for (int s = tid; s < used; s += 256) m = fmaxf(m, a.part_ml[s * n_rows + row].x);
+  for (int s = tid; s < used; s += 256) m = fmaxf(m, ml0[s * j.rows].x);
 #pragma unroll
   for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
   if (lane == 0) s_m[wave] = m;
@@ -946,7 +999,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
   float sl = 0.0f;
   for (int s = tid; s < used; s += 256) {
-    const float2 ml = a.part_ml[s * n_rows + row];
+    const float2 ml = ml0[s * j.rows];
     const float f = split_factor(ml, m);
     s_f[s] = f;
     sl = fmaf(ml.y, f, sl);
@@ -956,16 +1009,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (lane == 0) s_l[wave] = sl;
   __syncthreads();
   float acc = 0.0f;
-  const float *p = a.part_o + row * D + d;
+  const float *p = part_o(j.part, j.rows, j.row, 0, D) + d;
 #pragma unroll 8
-  for (int s = tid >> 5; s < used; s += 8) acc = fmaf(p[s * n_rows * D], s_f[s], acc);
+  for (int s = tid >> 5; s < used; s += 8) acc = fmaf(p[s * j.rows * D], s_f[s], acc);
   s_acc[tid >> 5][tid & 31] = acc;
   __syncthreads();
   if (tid < 32) {
 #pragma unroll
     for (int w = 1; w < 8; ++w) acc += s_acc[w][tid];
     sl = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-    a.out[row * D + d] = sl == 0.0f ? 0.0f : acc * kLow / sl;
+    a.out[j.out * D + d] = sl == 0.0f ? 0.0f : acc * kLow / sl;
   }
 }
 
@@ -1004,24 +1057,27 @@ int launch(const AttnArgs &a, hipStream_t s) {
     }
   }
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-  const int ns = p.ns16 > p.ns32 ? p.ns16 : p.ns32;
-  if (ns > 1) {
-    const long n_rows = (long)a.kv.n_tok * a.heads;
-    if (ns <= kJoinFew) {
-      const int parts = (int)(((long)a.heads * D + 1023) / 1024);
-      attn_join_few_kernel<D><<<(unsigned)a.kv.n_tok * parts, 256, 0, s>>>(a, parts);
-    } else {
-      attn_join_kernel<D><<<(unsigned)(n_rows * (D / 32)), 256, 0, s>>>(a);
-    }
+  const long slots = slots_of(a), n_rows = (long)a.kv.n_tok * a.heads;
+  const auto few = [](int ns) { return ns > 1 && ns <= kJoinFew; };
+  if (few(p.ns16) || few(p.ns32)) {
+    const long b16 = few(p.ns16) ? (slots * D + 1023) / 1024 : 0;
+    const int parts = (int)(((long)a.heads * D + 1023) / 1024);
+    attn_join_few_kernel<D><<<(unsigned)(b16 + (few(p.ns32) ? (long)a.kv.n_tok * parts : 0)), 256, 0, s>>>(a, (int)b16,
+                                                                                                        parts);
+    if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  }
+  if (p.ns16 > kJoinFew || p.ns32 > kJoinFew) {
+    const long b16 = p.ns16 > kJoinFew ? slots * (D / 32) : 0;
+    attn_join_kernel<D><<<(unsigned)(b16 + (p.ns32 > kJoinFew ? n_rows * (D / 32) : 0)), 256, 0, s>>>(a, (int)b16);
   }
   return (int)hipGetLastError();
 }
 
 // Splits of `keys` keys so that `base` workgroups become about `want`, each of at least min_chunk keys and at most
 // max_chunk (a split's workgroup walks its keys alone, however long other sequences are); none that saves the longest
-// workgroup fewer than `save` steps of `step` keys.
-void split_keys(long keys, long base, int want, int step, int save, int min_chunk, int max_chunk, int force, int *chunk,
-                int *ns) {
+// workgroup fewer than `save` steps of `step` keys, and never more than `top`.
+void split_keys(long keys, long base, int want, int step, int save, int min_chunk, int max_chunk, int force, long top,
+                int *chunk, int *ns) {
   long n = want / (base < 1 ? 1 : base);
   const long most = (keys + min_chunk - 1) / min_chunk, least = (keys + max_chunk - 1) / max_chunk;
   if (n > most) n = most;
@@ -1030,6 +1086,7 @@ void split_keys(long keys, long base, int want, int step, int save, int min_chun
   if (n < least) n = least;
   if (force > 0) n = force;
   if (n > steps) n = steps;
+  if (n > top) n = top;
   if (n > KQ4_ATTN_MAX_SPLITS) n = KQ4_ATTN_MAX_SPLITS;
   if (n < 1) n = 1;
   *chunk = (int)(((keys + n - 1) / n + step - 1) / step * step);
@@ -1045,7 +1102,7 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   // keys of a tile's queries, at most: the window's reach where that is less
   long keys = max_kv < 1 ? 1 : max_kv > 1 << 30 ? 1 << 30 : max_kv;
   if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
-  KQ4AttnPlan p{0, 0, 256, 0, 0, 64, 0, kPlain};
+  KQ4AttnPlan p{0, 0, 0, 256, 0, 0, 64, 0, kPlain};
   // 16 rows a tile up to 16 rows of a sequence and kv head (16 sequences of 4 tokens, 4 heads a kv head, 2000 keys:
   // 21.6 us, 38.9 with 128 rows a workgroup; of 8 tokens, 32 rows, 37.4 and 43.4, but one of 16 tokens over 4000 keys
   // 32.4 and 22.4). 256 where its workgroups fill the CUs (a prompt of 4096 tokens 247 us, 272 with 128; 4 of 500 tokens
@@ -1064,13 +1121,19 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // a CU, by splits or not, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 29.6 us,
     // 30.5 with 4 waves; 8 of 8192, 8 kv heads: 29.4 and 30.1; but one of 16384 16.5 and 15.5).
     const long base = (long)n_seq * kv_heads;
+    // Room for partial sums: of as many rows as the bounds say a sequence has, none past a tile; longer ones, where a
+    // bound is wrong, are not split. (A prompt among decode steps has none here, however many keys they have: one step
+    // over 131072 keys beside a chunk of 2048 tokens takes 17 MB.)
+    const long most = mixed && group <= 16 ? 16 / group * group : rows < 1 ? group : rows;
+    p.cap16 = (int)(most < 16 ? most : 16);
+    const long top = kPartRows / (base * p.cap16);
     const bool full = base >= kCus - kCus / 8;   // the CUs, without splits
     p.waves16 = !mixed && !full && keys / 64 * base > 16 * kCus ? 8 : 4;
     const int turn = 64 * p.waves16;
     // A join costs as much as two turns: 16 sequences, 8 kv heads, 600 / 1000 / 8192 keys in one range 11.2 / 13.4 /
     // 65.5 us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences
     // of up to 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
-    split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, &p.chunk16, &p.ns16);
+    split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, top, &p.chunk16, &p.ns16);
     // Sequences dealt by length, where there are about as many workgroups as CUs or more and each is long. A CU draws
     // about 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of
     // 1621 to 8192 keys 69.0 -> 59.5 us in halves (the join among it; of 8192 each 85.5 -> 90.9), 28 of up to 8192 66.9
@@ -1102,14 +1165,30 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     const int best = (int)(sqrt((double)kRowKeys * keys / ((double)n_tok * heads)) + 0.5);
     const long least = best < 2 ? keys : (keys + best - 1) / best;
     split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus,
-               64, 0, least > kMinChunk ? (int)least : kMinChunk, INT_MAX, force_split, &p.chunk32, &p.ns32);
+               64, 0, least > kMinChunk ? (int)least : kMinChunk, INT_MAX, force_split, LONG_MAX, &p.chunk32, &p.ns32);
   }
   return p;
 }
 
+namespace {
+
+size_t part_bytes(long rows, int head_dim) {   // (a multiple of 256)
+  return ((size_t)rows * (head_dim * sizeof(float) + sizeof(float2)) + 255) & ~(size_t)255;
+}
+
+}  // namespace
+
+size_t kq4_attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads, int kv_heads, int head_dim,
+                           size_t *bytes16) {
+  *bytes16 = p.ns16 > 1 ? part_bytes((long)p.ns16 * n_seq * kv_heads * p.cap16, head_dim) : 0;
+  return *bytes16 + (p.ns32 > 1 ? part_bytes((long)p.ns32 * n_tok * heads, head_dim) : 0);
+}
+
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
-                    int window, const KQ4AttnPlan &plan, float *part_o, float *part_ml, hipStream_t s) {
-  AttnArgs a{kv, log_pg, q, ldq, out, heads, heads / kv.kv_heads, scale * 1.44269504088896340736f, window,
-             plan, part_o, reinterpret_cast<float2 *>(part_ml)};
+                    int window, const KQ4AttnPlan &plan, char *ws, hipStream_t s) {
+  size_t at;
+  const bool split = kq4_attn_part_bytes(plan, kv.n_tok, kv.n_seq, heads, kv.kv_heads, kv.head_dim, &at) > 0;
+  AttnArgs a{kv, q, ldq, out, log_pg, heads, heads / kv.kv_heads, scale * 1.44269504088896340736f, window, plan,
+             reinterpret_cast<float *>(ws), reinterpret_cast<float *>(split ? ws + at : ws)};
   return kv.head_dim == 128 ? launch<128>(a, s) : launch<64>(a, s);
 }

@@ -187,16 +187,19 @@ int kq4_launch_kv_append(const kq4_kv &kv, int log_pg, const float *k, long ldk,
                          hipStream_t s);
 // The shape of an attention launch. Sequences of at most max16 rows (query tokens * query heads per kv head) take the
 // 16-row form (workgroups of waves16 waves; deal16: how sequences are dealt to them), the others tiles of tile32 rows
-// (0: none; 128 or 256); each form splits a tile's keys into ranges of `chunk`, at most ns of them. part_o holds
-// max(ns16, ns32) * n_tok * heads * head_dim floats, part_ml two per row and split (none where that is at most 1).
+// (0: none; 128 or 256); each form splits a tile's keys into ranges of `chunk`, at most ns of them, the 16-row form those
+// of sequences of at most cap16 rows (<= 16).
 #define KQ4_ATTN_MAX_SPLITS 1024
 struct KQ4AttnPlan {
-  int max16, waves16, chunk16, ns16, tile32, chunk32, ns32, deal16;
+  int max16, cap16, waves16, chunk16, ns16, tile32, chunk32, ns32, deal16;
 };
 KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int window,
                           int force_tile, int force_split);
+// Bytes of a plan's partial sums, 0 where nothing is split; *bytes16: the 16-row form's part, which comes first.
+size_t kq4_attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads, int kv_heads, int head_dim,
+                           size_t *bytes16);
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
-                    int window, const KQ4AttnPlan &plan, float *part_o, float *part_ml, hipStream_t s);
+                    int window, const KQ4AttnPlan &plan, char *ws, hipStream_t s);
 // Pieces of a row, and a piece's bytes; best holds n * pieces * n_top keys.
 int kq4_logprobs_pieces(int vocab);
 size_t kq4_logprobs_piece_bytes();
