@@ -450,8 +450,11 @@ int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v
  *
  * max_q and max_kv are the batch's largest number of tokens of a sequence and largest kv_len, or
  * bounds of them: they choose the launch's shape, and wrong values cost no more than speed (the
- * order of sums goes with the shape). The workspace holds the partial sums of a split key axis:
- * kq4_attn_workspace_bytes of the same numbers. */
+ * order of sums goes with the shape). The workspace holds the partial sums of a split key axis.
+ * kq4_attn_workspace_bytes is what the calls with up to so many tokens, sequences, max_q and max_kv
+ * need at most (the same heads, dimensions and window, under the present planner options): a
+ * smaller batch may need more than a larger one, whose keys need no split, but never more than
+ * this. */
 int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_heads, float scale,
                  int window, int max_q, int max_kv, void *stream);
 size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads, int head_dim,

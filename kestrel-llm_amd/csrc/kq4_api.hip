@@ -1356,9 +1356,8 @@ size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads,
   if (n_tok < 1 || n_seq < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads ||
       (head_dim != 64 && head_dim != 128) || window < 0 || max_q < 0 || max_kv < 0)
     return 0;
-  size_t bytes16 = 0;
-  return kq4_attn_part_bytes(attn_plan(n_tok, n_seq, q_heads, kv_heads, max_q, max_kv, window), n_tok, n_seq, q_heads,
-                             kv_heads, head_dim, &bytes16);
+  return kq4_attn_most_part_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv, window, opt(kAttnTile),
+                                  opt(kAttnSplit));
 }
 
 int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *top_id, const float *logits, long ld,

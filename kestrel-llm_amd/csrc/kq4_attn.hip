@@ -1093,15 +1093,18 @@ void split_keys(long keys, long base, int want, int step, int save, int min_chun
   *ns = (int)((keys + *chunk - 1) / *chunk);
 }
 
+// Keys of a tile's queries, at most: the window's reach where that is less.
+long most_keys(int max_q, int max_kv, int window) {
+  const long keys = max_kv < 1 ? 1 : max_kv > 1 << 30 ? 1 << 30 : max_kv, reach = (long)window + max_q + 64;
+  return window > 0 && reach < keys ? reach : keys;
+}
+
 }  // namespace
 
 KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max_q, int max_kv, int window,
                           int force_tile, int force_split) {
   const int group = heads / kv_heads;
-  const long rows = (long)max_q * group;
-  // keys of a tile's queries, at most: the window's reach where that is less
-  long keys = max_kv < 1 ? 1 : max_kv > 1 << 30 ? 1 << 30 : max_kv;
-  if (window > 0 && (long)window + max_q + 64 < keys) keys = (long)window + max_q + 64;
+  const long rows = (long)max_q * group, keys = most_keys(max_q, max_kv, window);
   KQ4AttnPlan p{0, 0, 0, 256, 0, 0, 64, 0, kPlain};
   // 16 rows a tile up to 16 rows of a sequence and kv head (16 sequences of 4 tokens, 4 heads a kv head, 2000 keys:
   // 21.6 us, 38.9 with 128 rows a workgroup; of 8 tokens, 32 rows, 37.4 and 43.4, but one of 16 tokens over 4000 keys
@@ -1182,6 +1185,33 @@ size_t kq4_attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads
                            size_t *bytes16) {
   *bytes16 = p.ns16 > 1 ? part_bytes((long)p.ns16 * n_seq * kv_heads * p.cap16, head_dim) : 0;
   return *bytes16 + (p.ns32 > 1 ? part_bytes((long)p.ns32 * n_tok * heads, head_dim) : 0);
+}
+
+// No batch of at most these numbers has more: the 16-row form makes of `base` workgroups at most kCus by its splits,
+// 4 kCus by shares, or as many as its longest range allows, of at least 4 turns of 256 keys; the 32-row form 2 kCus of
+// 128 rows or kCus of 256.
+size_t kq4_attn_most_part_bytes(int n_tok, int n_seq, int heads, int kv_heads, int head_dim, int max_q, int max_kv,
+                                int window, int force_tile, int force_split) {
+  const long group = heads / kv_heads, rows = max_q * group, keys = most_keys(max_q, max_kv, window);
+  const long base = (long)n_seq * kv_heads, turns = (keys + 255) / 256;
+  long rows16 = 0, rows32 = 0;
+  if (force_tile != 128 && force_tile != 256) {
+    const long cap = rows < 1 ? group : rows, longest = rows > 16 ? 1024 : 8192, least = (keys + longest - 1) / longest;
+    long ranges = base * least > 4 * kCus ? base * least : 4 * kCus;
+    if (base * turns < ranges) ranges = base * turns;
+    if (force_split > 0) ranges = base * (force_split < turns ? force_split : turns);
+    else if (turns < 4) ranges = 0;
+    rows16 = ranges * (cap < 16 ? cap : 16);
+    if (rows16 > kPartRows) rows16 = kPartRows;
+  }
+  if (force_tile == 128 || force_tile == 256 || (force_tile != 16 && rows > 16)) {
+    const long all = (long)n_tok * heads, steps = (keys + 63) / 64;
+    long n = force_split < steps ? force_split : steps;
+    if (n > KQ4_ATTN_MAX_SPLITS) n = KQ4_ATTN_MAX_SPLITS;
+    rows32 = force_split > 0 ? all * n : keys > kMinChunk ? all * ((keys + kMinChunk - 1) / kMinChunk) : 0;
+    if (force_split <= 0 && rows32 > kCus * 256) rows32 = kCus * 256;
+  }
+  return part_bytes(rows16, head_dim) + part_bytes(rows32, head_dim);
 }
 
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,

@@ -198,6 +198,9 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
 // Bytes of a plan's partial sums, 0 where nothing is split; *bytes16: the 16-row form's part, which comes first.
 size_t kq4_attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads, int kv_heads, int head_dim,
                            size_t *bytes16);
+// Bytes that hold those of every plan for at most so many tokens and sequences and bounds up to these.
+size_t kq4_attn_most_part_bytes(int n_tok, int n_seq, int heads, int kv_heads, int head_dim, int max_q, int max_kv,
+                                int window, int force_tile, int force_split);
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
                     int window, const KQ4AttnPlan &plan, char *ws, hipStream_t s);
 // Pieces of a row, and a piece's bytes; best holds n * pieces * n_top keys.

@@ -848,6 +848,7 @@ def kv_append_dev(kv, k, v, stream=None):
 
 
 def attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, max_q, max_kv, window=0):
+    """What attn_dev calls of up to so many tokens and sequences, max_q and max_kv need at most."""
     return lib().kq4_attn_workspace_bytes(n_tok, n_seq, q_heads, kv_heads, head_dim, window, max_q, max_kv)
 
 

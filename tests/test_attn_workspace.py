@@ -33,3 +33,35 @@ result = [rc] + [s for s in hip.standin_log().decode().split("\\n")[:-1] if "joi
     assert res[0] == 0 and len(res) == 2, res
     grid = int(res[1].split(" ")[-2])
     assert grid == 2 * KV * 16 * (DIM // 32)
+
+
+@pytest.mark.parametrize("tile,split", [(-1, -1), (-1, 3), (16, -1), (16, 40), (128, -1), (256, 5)])
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (8, 1), (20, 1), (12, 4), (64, 64)])
+def test_a_reservation_holds_every_smaller_batch(standin, heads, kv_heads, tile, split):  # noqa: F811
+    """The size for a largest batch is enough for any of fewer tokens, sequences and lower bounds: captured calls, which
+    cannot grow the workspace, all run."""
+    res = standin(SETUP + """
+import random
+rng = random.Random(heads * 100 + tile + split)
+assert k.kq4_set_option(b"attn_tile", tile) == 0 and k.kq4_set_option(b"attn_split", split) == 0
+log = lambda n: max(0, int(round((n + 1) ** rng.random())) - rng.randint(0, 1))
+result = []
+for n_seq, max_q, max_kv, window in [(1, 1, 1000, 0), (64, 1, 8192, 0), (33, 1, 200000, 0), (300, 2, 5000, 0), (8, 4, 70000, 0),
+                                     (4, 2048, 16384, 0), (70, 600, 131072, 0), (9, 300, 100000, 1500), (1, 1, 700, 0),
+                                     (1, 8192, 8192, 0)]:
+    n_tok = max(n_seq, min(n_seq * max_q, 9000))
+    need = k.kq4_attn_workspace_bytes(n_tok, n_seq, heads, kv_heads, 128, window, max_q, max_kv)
+    hip.standin_capture(0)
+    assert k.kq4_shutdown() is None and k.kq4_init(0) == 0
+    reserve_exactly(need)
+    hip.standin_capture(1)
+    for i in range(400):
+        s = n_seq if i % 3 == 0 else max(1, min(n_seq, log(n_seq)))
+        q, m = min(max_q, log(max_q)), min(max_kv, log(max_kv) if i % 2 else rng.randint(max_kv // 2, max_kv))
+        t = max(1, min(n_tok, rng.choice([s, s * q, log(n_tok), n_tok])))
+        c = kv(n_seq=s, n_tok=t, kv_heads=kv_heads)
+        rc = attn(c, out=at(30), q=at(20), ldq=heads * 128, heads=heads, window=window, max_q=q, max_kv=m)
+        if rc:
+            result.append((n_seq, max_q, max_kv, window, s, q, m, t, rc, kq4.last_error()))
+""", heads=heads, kv_heads=kv_heads, tile=tile, split=split)
+    assert res == []
