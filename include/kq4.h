@@ -465,7 +465,7 @@ size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads,
 #define KQ4_LOGPROBS_MAX_VOCAB (1 << 20)
 
 /* What sampling and scoring read from n rows of logits (row t at t * ld floats, vocab of them;
- * 4-byte aligned), each output NULL where it is not wanted:
+ * 4-byte aligned; n * ceil(vocab / 8192) below 2^24), each output NULL where it is not wanted:
  *   logprob [n]                      log softmax(logits)[token[t]] (NaN for a token outside the
  *                                    vocabulary: a row that asks for none)
  *   entropy [n]                      -sum p log p, in nats

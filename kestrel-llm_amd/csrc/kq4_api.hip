@@ -1284,7 +1284,7 @@ size_t logprobs_bytes(int n, int vocab, int n_top, size_t *piece_bytes) {
 
 bool logprobs_shape_ok(int n, int vocab, int n_top) {
   return n >= 0 && vocab >= 1 && vocab <= KQ4_LOGPROBS_MAX_VOCAB && n_top >= 0 && n_top <= KQ4_LOGPROBS_MAX_TOP &&
-         n_top <= vocab && (long long)n * kq4_logprobs_pieces(vocab) <= 0x7fffffffLL;
+         n_top <= vocab && (long long)n * kq4_logprobs_pieces(vocab) < 1 << 24;   // (2^32 threads)
 }
 
 }  // namespace
@@ -1335,10 +1335,7 @@ int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_h
   if ((rc = cur_dev(&ds))) return rc;
   hipStream_t s = (hipStream_t)stream;
   const KQ4AttnPlan plan = attn_plan(kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, max_q, max_kv, window);
-  const long long blocks = (long long)kv->n_seq * kv->kv_heads * plan.ns16 +
-                           (plan.tile32 ? ((long long)kv->n_tok * (q_heads / kv->kv_heads) / plan.tile32 +
-                                           kv->n_seq) * kv->kv_heads * plan.ns32 : 0);
-  if (blocks > 0x7fffffffLL)
+  if (!kq4_attn_fits(plan, kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, kv->head_dim))
     return fail(KQ4_EINVAL, "attn: n_seq=%d n_tok=%d q_heads=%d", kv->n_seq, kv->n_tok, q_heads);
   size_t bytes16 = 0;
   const size_t bytes = kq4_attn_part_bytes(plan, kv->n_tok, kv->n_seq, q_heads, kv->kv_heads, kv->head_dim, &bytes16);
@@ -1363,7 +1360,8 @@ size_t kq4_attn_workspace_bytes(int n_tok, int n_seq, int q_heads, int kv_heads,
 int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *top_id, const float *logits, long ld,
                      const int *token, int n, int vocab, int n_top, void *stream) {
   if (!logprobs_shape_ok(n, vocab, n_top) || ld < vocab)
-    return fail(KQ4_EINVAL, "logprobs: n=%d vocab=%d (at most %d) ld=%ld n_top=%d (at most %d and vocab)", n, vocab,
+    return fail(KQ4_EINVAL, "logprobs: n=%d (times pieces of 8192 logits below 2^24) vocab=%d (at most %d) "
+                "ld=%ld n_top=%d (at most %d and vocab)", n, vocab,
                 KQ4_LOGPROBS_MAX_VOCAB, ld, n_top, KQ4_LOGPROBS_MAX_TOP);
   if (n == 0) return KQ4_OK;
   if (!logits || (logprob && !token) || (n_top != 0) != (top_logprob != nullptr) ||

@@ -1022,13 +1022,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks16
   }
 }
 
+// Workgroups of a plan's launches: of each form (times its ranges), and of the joins.
+struct Grids {
+  long blocks16, blocks32, few16, few32, many16, many32;
+};
+Grids grids(const KQ4AttnPlan &p, long n_tok, long n_seq, long heads, long kv_heads, long head_dim) {
+  const auto few = [](int ns) { return ns > 1 && ns <= kJoinFew; };
+  const long floats16 = n_seq * kv_heads * p.cap16 * head_dim, parts = (heads * head_dim + 1023) / 1024;
+  return Grids{p.max16 ? (p.deal16 == kShares ? kq4_attn_shares((int)kv_heads, (int)n_seq) + n_seq : n_seq) * kv_heads : 0,
+               p.tile32 ? (n_tok * (heads / kv_heads) / p.tile32 + n_seq) * kv_heads : 0,
+               few(p.ns16) ? (floats16 + 1023) / 1024 : 0,
+               few(p.ns32) ? n_tok * parts : 0,
+               p.ns16 > kJoinFew ? floats16 / 32 : 0,
+               p.ns32 > kJoinFew ? n_tok * heads * (head_dim / 32) : 0};
+}
+
 template <int D>
 int launch(const AttnArgs &a, hipStream_t s) {
   const KQ4AttnPlan &p = a.plan;
-  const int blocks16 =
-      (p.deal16 == kShares ? kq4_attn_shares(a.kv.kv_heads, a.kv.n_seq) + a.kv.n_seq : a.kv.n_seq) * a.kv.kv_heads;
+  const Grids g = grids(p, a.kv.n_tok, a.kv.n_seq, a.heads, a.kv.kv_heads, D);
+  const int blocks16 = (int)g.blocks16, blocks32 = (int)g.blocks32;
   const int ns16 = p.deal16 == kShares ? 1 : p.ns16;   // (a range is an item there)
-  const int blocks32 = p.tile32 ? (int)(((long)a.kv.n_tok * a.group / p.tile32 + a.kv.n_seq) * a.kv.kv_heads) : 0;
   static std::atomic<unsigned long long> lds8{0}, lds4{0}, ldsm{0};
   constexpr int lds = kLds32<D>;
   hipError_t e = hipSuccess;
@@ -1057,19 +1071,12 @@ int launch(const AttnArgs &a, hipStream_t s) {
     }
   }
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-  const long slots = slots_of(a), n_rows = (long)a.kv.n_tok * a.heads;
-  const auto few = [](int ns) { return ns > 1 && ns <= kJoinFew; };
-  if (few(p.ns16) || few(p.ns32)) {
-    const long b16 = few(p.ns16) ? (slots * D + 1023) / 1024 : 0;
-    const int parts = (int)(((long)a.heads * D + 1023) / 1024);
-    attn_join_few_kernel<D><<<(unsigned)(b16 + (few(p.ns32) ? (long)a.kv.n_tok * parts : 0)), 256, 0, s>>>(a, (int)b16,
-                                                                                                        parts);
+  if (g.few16 + g.few32) {
+    attn_join_few_kernel<D><<<(unsigned)(g.few16 + g.few32), 256, 0, s>>>(a, (int)g.few16,
+                                                                          (int)(((long)a.heads * D + 1023) / 1024));
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
   }
-  if (p.ns16 > kJoinFew || p.ns32 > kJoinFew) {
-    const long b16 = p.ns16 > kJoinFew ? slots * (D / 32) : 0;
-    attn_join_kernel<D><<<(unsigned)(b16 + (p.ns32 > kJoinFew ? n_rows * (D / 32) : 0)), 256, 0, s>>>(a, (int)b16);
-  }
+  if (g.many16 + g.many32) attn_join_kernel<D><<<(unsigned)(g.many16 + g.many32), 256, 0, s>>>(a, (int)g.many16);
   return (int)hipGetLastError();
 }
 
@@ -1212,6 +1219,13 @@ size_t kq4_attn_most_part_bytes(int n_tok, int n_seq, int heads, int kv_heads, i
     if (force_split <= 0 && rows32 > kCus * 256) rows32 = kCus * 256;
   }
   return part_bytes(rows16, head_dim) + part_bytes(rows32, head_dim);
+}
+
+bool kq4_attn_fits(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads, int kv_heads, int head_dim) {
+  const Grids g = grids(p, n_tok, n_seq, heads, kv_heads, head_dim);
+  const long forms = p.tile32 == 256 || p.waves16 == 8 ? 512 : 256, most = 0xffffffffL;
+  return (g.blocks16 * p.ns16 + g.blocks32 * p.ns32) * forms <= most && (g.few16 + g.few32) * 256 <= most &&
+         (g.many16 + g.many32) * 256 <= most;
 }
 
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,

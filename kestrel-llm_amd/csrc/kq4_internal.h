@@ -201,6 +201,8 @@ size_t kq4_attn_part_bytes(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads
 // Bytes that hold those of every plan for at most so many tokens and sequences and bounds up to these.
 size_t kq4_attn_most_part_bytes(int n_tok, int n_seq, int heads, int kv_heads, int head_dim, int max_q, int max_kv,
                                 int window, int force_tile, int force_split);
+// Whether its launches have fewer than 2^32 threads each, which is what a launch takes.
+bool kq4_attn_fits(const KQ4AttnPlan &p, int n_tok, int n_seq, int heads, int kv_heads, int head_dim);
 int kq4_launch_attn(float *out, const kq4_kv &kv, int log_pg, const float *q, long ldq, int heads, float scale,
                     int window, const KQ4AttnPlan &plan, char *ws, hipStream_t s);
 // Pieces of a row, and a piece's bytes; best holds n * pieces * n_top keys.
