@@ -442,7 +442,7 @@ int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v
  * out [n_tok][q_heads][head_dim] = softmax(scale * q . k) v over the keys at or before the query's
  * position, with window > 0 the last `window` of them (the query's own among them). q: row t at
  * t * ldq floats, [q_heads][head_dim], 16-byte aligned, ldq a multiple of 4; query head j reads
- * kv head j / (q_heads / kv_heads). scale > 0. A row that sees no key is zeros. out must not
+ * kv head j / (q_heads / kv_heads). 0 < scale <= 2e38. A row that sees no key is zeros. out must not
  * overlap q. Results are within fp32's rounding of the definition while scale * q . k is within
  * fp32's range, of a row's values whose group scales lie no more than 2^100 apart (of others, the
  * smaller ones may lose their share of the row's sum; an appended group of zeros has 2^-100), and

@@ -1319,8 +1319,8 @@ int kq4_attn_dev(float *out, const kq4_kv *kv, const float *q, long ldq, int q_h
   int log_pg = 0, rc = kv_check("attn", kv, &log_pg);
   if (rc) return rc;
   if (q_heads < 1 || q_heads % kv->kv_heads || window < 0 || max_q < 0 || max_kv < 0 || !(scale > 0.0f) ||
-      scale > 3.0e38f)
-    return fail(KQ4_EINVAL, "attn: q_heads=%d (a multiple of kv_heads=%d) scale=%g (> 0) window=%d max_q=%d "
+      scale > 2.0e38f)   // (times log2(e) it is a number)
+    return fail(KQ4_EINVAL, "attn: q_heads=%d (a multiple of kv_heads=%d) scale=%g (> 0, at most 2e38) window=%d max_q=%d "
                 "max_kv=%d", q_heads, kv->kv_heads, scale, window, max_q, max_kv);
   if (!kv->n_seq || !kv->n_tok) return KQ4_OK;
   const long width = (long)q_heads * kv->head_dim;

@@ -20,3 +20,9 @@ def test_launches_that_fit(standin, call, want):  # noqa: F811
 
 def test_sizes_of_refused_rows(kq4_cpu):
     assert kq4_cpu.logprobs_workspace_bytes((1 << 24) - 1, 5, 1) > 0 == kq4_cpu.logprobs_workspace_bytes(1 << 24, 5, 1)
+
+
+def test_scales_past_the_exponent(standin):  # noqa: F811
+    """The scale times log2(e) has to be a number."""
+    assert standin(SETUP + "result = [launched(lambda: attn(kv(), max_kv=100, scale=s)) for s in (1.9e38, 2.5e38)]") == \
+        [[0, 1], [-1, 0]]
