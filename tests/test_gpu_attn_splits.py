@@ -36,3 +36,18 @@ def test_given_numbers_of_ranges(kq4, torch_dev, lens, tile, split):
     with kq4.options(attn_tile=tile, attn_split=split):
         check_attn(kq4, torch_dev, b, x, 8)
         check_attn(kq4, torch_dev, b, x, 8, window=900)
+
+
+@pytest.mark.parametrize("kv_heads,lens", [
+    (2, [(1, 5000)]), (1, [(1, 2000), (1, 1), (0, 700), (1, 0), (2, 900)]),     # more than 16 ranges: the join of many
+    (2, [(1, 300 + 31 * i) for i in range(40)]), (8, [(1, 2000), (1, 5), (1, 700)] * 4),   # up to 16: that of few
+    (2, [(9, 600), (1, 1500), (5, 40)]),                       # more rows than the bound says: those stay whole
+])
+@pytest.mark.parametrize("window", [0, 333])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_shares_of_all_keys(kq4, torch_dev, lens, kv_heads, window, dim):
+    """A bound far above the lengths, so that ranges go by the keys that are there, of both head sizes."""
+    rng = np.random.default_rng(dim + len(lens))
+    b = Batch(rng, lens, kv_heads, dim, 64, dim, pad=1)
+    b.fill(rng, upto="all", spread=1.0)
+    check_attn(kq4, torch_dev, b, rand(rng, b.n, 4 * kv_heads, dim), 4 * kv_heads, window=window, max_q=1, max_kv=1000000)
