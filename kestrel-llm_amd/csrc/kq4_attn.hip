@@ -514,7 +514,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
         const float f = sl == 0.0f ? 0.0f : 1.0f / sl;
         *reinterpret_cast<float4v *>(a.out + row * D + d) = (acc * kLow) * f;
       } else {
-        const int slot = (seq * a.kv.kv_heads + h) * a.plan.cap16 + rr;   // (r0 is 0)
+        const int slot = (seq * a.kv.kv_heads + h) * a.plan.cap16 + r0 + rr;
         *reinterpret_cast<float4v *>(part_o(a.part16, slots_of(a), slot, split, D) + d) = acc;
         if (d == 0) *part_ml(a.part16, a.plan.ns16, slots_of(a), slot, split, D) = make_float2(m, sl);
       }
@@ -897,7 +897,8 @@ KQ4_DEV JoinRow join_row16(const AttnArgs &a, int slot, int lane) {
   const int rows = sp.nq * a.group;
   if (r >= rows || rows > a.plan.cap16 || rows > a.plan.max16) return j;
   int base, end;
-  j.used = kq4_kv_ranges(sp, 0, sp.nq - 1, a.window, a.plan.chunk16, a.plan.ns16, &base, &end);
+  const int r0 = r - r % 16, last = r0 + 15 < rows ? r0 + 15 : rows - 1;
+  j.used = kq4_kv_ranges(sp, r0 / a.group, last / a.group, a.window, a.plan.chunk16, a.plan.ns16, &base, &end);
   if (a.plan.deal16 >= kHalves) dealt_part(a, base, end, share, &j.used);
   const int t = r / a.group;
   j.out = (long)(sp.q0 + t) * a.heads + h * a.group + (r - t * a.group);
@@ -1131,11 +1132,11 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     // a CU, by splits or not, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 29.6 us,
     // 30.5 with 4 waves; 8 of 8192, 8 kv heads: 29.4 and 30.1; but one of 16384 16.5 and 15.5).
     const long base = (long)n_seq * kv_heads;
-    // Room for partial sums: of as many rows as the bounds say a sequence has, none past a tile; longer ones, where a
-    // bound is wrong, are not split. (A prompt among decode steps has none here, however many keys they have: one step
-    // over 131072 keys beside a chunk of 2048 tokens takes 17 MB.)
-    const long most = mixed && group <= 16 ? 16 / group * group : rows < 1 ? group : rows;
-    p.cap16 = (int)(most < 16 ? most : 16);
+    // Room for partial sums: of as many rows as the bounds say a sequence of this form has; longer ones, where a bound
+    // is wrong, are not split. (A prompt among decode steps has none here, however many keys they have: one step over
+    // 131072 keys beside a chunk of 2048 tokens takes 17 MB.)
+    const long room = !mixed ? rows < 1 ? group : rows : group <= 16 ? 16 / group * group : 16;
+    p.cap16 = (int)(room < kPartRows ? room : kPartRows);
     const long top = kPartRows / (base * p.cap16);
     const bool full = base >= kCus - kCus / 8;   // the CUs, without splits
     p.waves16 = !mixed && !full && keys / 64 * base > 16 * kCus ? 8 : 4;
@@ -1159,9 +1160,10 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
       const long most = 4 * (kCus / base), have = (keys + turn - 1) / turn, places = kCus / kv_heads;
       p.ns16 = (int)(most < have ? most : have);
       if (p.ns16 > places) p.ns16 = (int)places;
+      if (p.ns16 > top) p.ns16 = (int)top;
     } else if (!mixed && force_split <= 0 && full && n_seq <= 64 * p.waves16 && keys >= 16 * turn) {
       if (base > kCus && p.ns16 == 1) p.deal16 = kOrder;
-      if (base <= kCus && p.ns16 <= 2) {
+      if (base <= kCus && p.ns16 <= 2 && top > 1) {
         p.deal16 = kHalves;
         p.ns16 = 2;
       }
@@ -1203,13 +1205,13 @@ size_t kq4_attn_most_part_bytes(int n_tok, int n_seq, int heads, int kv_heads, i
   const long base = (long)n_seq * kv_heads, turns = (keys + 255) / 256;
   long rows16 = 0, rows32 = 0;
   if (force_tile != 128 && force_tile != 256) {
-    const long cap = rows < 1 ? group : rows, longest = rows > 16 ? 1024 : 8192, least = (keys + longest - 1) / longest;
+    const long tile = group > 16 ? group : 16, cap = rows < 1 ? group : force_tile == 16 || rows < tile ? rows : tile;
+    const long longest = rows > 16 ? 1024 : 8192, least = (keys + longest - 1) / longest;
     long ranges = base * least > 4 * kCus ? base * least : 4 * kCus;
     if (base * turns < ranges) ranges = base * turns;
     if (force_split > 0) ranges = base * (force_split < turns ? force_split : turns);
     else if (turns < 4) ranges = 0;
-    rows16 = ranges * (cap < 16 ? cap : 16);
-    if (rows16 > kPartRows) rows16 = kPartRows;
+    rows16 = ranges * cap < kPartRows ? ranges * cap : kPartRows;
   }
   if (force_tile == 128 || force_tile == 256 || (force_tile != 16 && rows > 16)) {
     const long all = (long)n_tok * heads, steps = (keys + 63) / 64;

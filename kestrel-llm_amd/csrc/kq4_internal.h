@@ -188,7 +188,7 @@ int kq4_launch_kv_append(const kq4_kv &kv, int log_pg, const float *k, long ldk,
 // The shape of an attention launch. Sequences of at most max16 rows (query tokens * query heads per kv head) take the
 // 16-row form (workgroups of waves16 waves; deal16: how sequences are dealt to them), the others tiles of tile32 rows
 // (0: none; 128 or 256); each form splits a tile's keys into ranges of `chunk`, at most ns of them, the 16-row form those
-// of sequences of at most cap16 rows (<= 16).
+// of sequences of at most cap16 rows.
 #define KQ4_ATTN_MAX_SPLITS 1024
 struct KQ4AttnPlan {
   int max16, cap16, waves16, chunk16, ns16, tile32, chunk32, ns32, deal16;

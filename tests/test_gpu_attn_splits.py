@@ -28,7 +28,7 @@ def test_decode_steps_beside_prompts(kq4, torch_dev, lens, group, dim):
     ([(1, 3000), (4, 2000), (3, 2500)], 16, 20), ([(1, 3000), (9, 2000), (4, 2500)], 16, 3),
 ])
 def test_given_numbers_of_ranges(kq4, torch_dev, lens, tile, split):
-    """Also of sequences with more rows than a tile, which the 16-row form leaves whole."""
+    """Also of sequences with more rows than a tile of the 16-row form."""
     rng = np.random.default_rng(split)
     b = Batch(rng, lens, 2, 128, 32, 128, pad=1)
     b.fill(rng, upto="all", spread=1.0)
