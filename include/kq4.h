@@ -433,8 +433,8 @@ size_t kq4_kv_scales_bytes(int n_pages, int page_tokens, int kv_heads, int head_
  * earlier tokens' codes are rewritten as rint(fl(code * fl(old / new))); a group's scale starts
  * anew with its first slot. Rotated keys are x1 c - x2 s and x2 c + x1 s rounded to fp32 once. A
  * NaN or infinity makes its group's scale NaN or infinite (codes 0). Slots of a group past its new
- * tokens are left as they were. Every page that a call appends to belongs to one sequence; any
- * number of sequences may share the pages before. Uses no workspace. */
+ * tokens are left as they were. Every page that a call appends to belongs to one sequence and stands
+ * once in its row of the table; any number of sequences may share the pages before. Uses no workspace. */
 int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v, long ldv,
                       void *stream);
 
@@ -449,8 +449,10 @@ int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v
  * of no more than 2^25 keys whose value scale is the least.
  *
  * max_q and max_kv are the batch's largest number of tokens of a sequence and largest kv_len, or
- * bounds of them: they choose the launch's shape, and wrong values cost no more than speed (the
- * order of sums goes with the shape). The workspace holds the partial sums of a split key axis.
+ * bounds of them: they choose the launch's shape, and wrong values cost no more than speed. The
+ * order of a row's sums goes with the shape, and where few sequences are split by the keys that are
+ * there also with the other sequences' lengths: the same row in another batch is equal within
+ * rounding, the same batch to the bit. The workspace holds the partial sums of a split key axis.
  * kq4_attn_workspace_bytes is what the calls with up to so many tokens, sequences, max_q and max_kv
  * need at most (the same heads, dimensions and window, under the present planner options): a
  * smaller batch may need more than a larger one, whose keys need no split, but never more than
