@@ -202,10 +202,16 @@ KQ4_DEV void softmax_pair(const float16v &s, int j, float c, float shift, float 
 // Rows that have partial sums in the 16-row form.
 KQ4_HD long slots_of(const AttnArgs &a) { return (long)a.kv.n_seq * a.kv.kv_heads * a.plan.cap16; }
 
-// The factor of a split's, or wave's, sums in the joined row (one of which nothing was seen: 0; one whose scales were
-// all NaN keeps its NaN).
-KQ4_DEV float split_factor(float2 ml, float m) {
-  return ml.x == kNegInf ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - m);
+// 2^d, d <= 0, as two factors: a row's sum over small value scales is large, and something of it is left where 2^d
+// alone is 0.
+KQ4_DEV float2 two_factors(float d) {
+  const float a = fmaxf(d, -120.0f);
+  return make_float2(__builtin_amdgcn_exp2f(a), __builtin_amdgcn_exp2f(d - a));
+}
+
+// The factors of a split's, or wave's, sums in the joined row (one without a maximum has zeros, or NaN: it keeps them).
+KQ4_DEV float2 split_factors(float2 ml, float m) {
+  return ml.x == kNegInf ? make_float2(1.0f, 1.0f) : two_factors(ml.x - m);
 }
 
 // ---- up to 16 rows (query tokens * heads per kv head) a tile: decode ---------------------------------
@@ -448,8 +454,9 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
       em = max_xor32(max_xor16(em));
       if (__ballot(em > M + kSlack)) {
         const float m = em > M + kSlack ? em : M;
-        const float f = M == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(M - m);
-        l *= f;
+        const float2 by = two_factors(M == kNegInf ? kNegInf : M - m);
+        const float f = by.x * by.y;
+        l = l * by.y * by.x;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
         M = m;
@@ -504,9 +511,9 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float2 ml = s_ml[w][rr];
-        const float f = split_factor(ml, m);
-        sl = fmaf(ml.y, f, sl);
-        acc += *reinterpret_cast<const float4v *>(&s_o[w][rr][d]) * f;
+        const float2 f = split_factors(ml, m);
+        sl = fmaf(ml.y * f.y, f.x, sl);
+        acc += *reinterpret_cast<const float4v *>(&s_o[w][rr][d]) * (f.x * f.y);
       }
       if (used == 1) {
         const int t = (r0 + rr) / a.group;
@@ -806,8 +813,9 @@ KQ4_DEV void attn_rows32(const AttnArgs &a, int block, int blocks, int split, ui
       const float em = max_xor32(fmaf(mx, c, lv));
       if (__ballot(em > M + kSlack)) {
         const float m = em > M + kSlack ? em : M;
-        const float x = M == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(M - m);
-        l *= x;
+        const float2 by = two_factors(M == kNegInf ? kNegInf : M - m);
+        const float x = by.x * by.y;
+        l = l * by.y * by.x;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= x;
         M = m;
@@ -954,8 +962,9 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int bloc
   float m = ml.x;
 #pragma unroll
   for (int x = kJoinFew / 2; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  const float f = split_factor(ml, m);
-  float sl = ml.y * f;
+  const float2 by = split_factors(ml, m);
+  const float f = by.x * by.y;
+  float sl = ml.y * by.y * by.x;
 #pragma unroll
   for (int x = kJoinFew / 2; x; x >>= 1) sl += __shfl_xor(sl, x);
   float4v acc = {0.f, 0.f, 0.f, 0.f};
@@ -1001,9 +1010,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks16
   float sl = 0.0f;
   for (int s = tid; s < used; s += 256) {
     const float2 ml = ml0[s * j.rows];
-    const float f = split_factor(ml, m);
-    s_f[s] = f;
-    sl = fmaf(ml.y, f, sl);
+    const float2 f = split_factors(ml, m);
+    s_f[s] = f.x * f.y;
+    sl = fmaf(ml.y * f.y, f.x, sl);
   }
 #pragma unroll
   for (int x = 32; x; x >>= 1) sl += __shfl_xor(sl, x);
