@@ -431,10 +431,11 @@ size_t kq4_kv_scales_bytes(int n_pages, int page_tokens, int kv_heads, int head_
  * tokens the scale is fl(amax / 127), at least 2^-100, and at least the group's present scale if
  * it holds earlier tokens; codes are rint(fl(x * fl(1 / scale))). Where the scale grows, the
  * earlier tokens' codes are rewritten as rint(fl(code * fl(old / new))); a group's scale starts
- * anew with its first slot. Rotated keys are x1 c - x2 s and x2 c + x1 s rounded to fp32 once. A
- * NaN or infinity makes its group's scale NaN or infinite (codes 0). Slots of a group past its new
- * tokens are left as they were. Every page that a call appends to belongs to one sequence and stands
- * once in its row of the table; any number of sequences may share the pages before. Uses no workspace. */
+ * anew with its first slot. Rotated keys are x1 c - x2 s and x2 c + x1 s formed in 64 bits, then
+ * rounded to fp32. A NaN or infinity makes its group's scale NaN or infinite (codes 0). Slots of a
+ * group past its new tokens are left as they were. Every page that a call appends to belongs to one
+ * sequence and stands once in its row of the table; any number of sequences may share the pages
+ * before. Uses no workspace. */
 int kq4_kv_append_dev(const kq4_kv *kv, const float *k, long ldk, const float *v, long ldv,
                       void *stream);
 

@@ -536,7 +536,7 @@ KQ4_DEV void attn_rows16(const AttnArgs &a, int block, int split, uint8_t *lds) 
 // in flight meanwhile. LDS holds the operands in lane order, 16 bytes a lane without bank conflicts: keys as
 // [D/8][32 keys][8], values as [8-token half][group][D][8]. The scores of tile n + 1 are formed while tile n's go
 // through the softmax, so matrix instructions and vector instructions of a wave are independent of each other.
-// A prompt of 4096 tokens, 32 heads, 8 kv heads of 128: 246 us, 560 TFLOP/s of the definition's 137 GFLOP, twice that
+// A prompt of 4096 tokens, 32 heads, 8 kv heads of 128: 250 us, 550 TFLOP/s of the definition's 137 GFLOP, twice that
 // of matrix instructions (hi + lo). Bound by issue: a tile and wave has 32 matrix instructions (1024 cycles of its
 // SIMD) and about 130 vector instructions (712, 16 of them exponentials), 1930 cycles are measured; the matrix unit
 // is busy 53 % of the cycles at 1.93 GHz. A call of one tile takes 6.8 us at 64 dimensions, 9.5 at 128 (dependent
@@ -1124,10 +1124,10 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   const long rows = (long)max_q * group, keys = most_keys(max_q, max_kv, window);
   KQ4AttnPlan p{0, 0, 0, 256, 0, 0, 64, 0, kPlain};
   // 16 rows a tile up to 16 rows of a sequence and kv head (16 sequences of 4 tokens, 4 heads a kv head, 2000 keys:
-  // 21.6 us, 38.9 with 128 rows a workgroup; of 8 tokens, 32 rows, 37.4 and 43.4, but one of 16 tokens over 4000 keys
-  // 32.4 and 22.4). 256 where its workgroups fill the CUs (a prompt of 4096 tokens 247 us, 272 with 128; 4 of 500 tokens
-  // 37.0 and 41.2; one of 2000, whose longest workgroups end late, 95.7 and 87.9), else 128 (the mixed kernel's batch
-  // 26.3 us, 30.1 with 256; 500 tokens 26.1 and 32.8).
+  // 20.9 us, 39.4 with 128 rows a workgroup; of 8 tokens, 32 rows, 35.7 and 42.6, but one of 16 tokens over 4000 keys
+  // 32.8 and 22.8). 256 where its workgroups fill the CUs (a prompt of 4096 tokens 251 us, 277 with 128; 4 of 500 tokens
+  // 36.6 and 38.6; one of 2000, whose longest workgroups end late, 95.7 and 85.8), else 128 (the mixed kernel's batch
+  // 26.3 us, 30.1 with 256; 500 tokens 26.5 and 32.6).
   p.tile32 = force_tile == 16                                           ? 0
              : force_tile == 128 || force_tile == 256                   ? force_tile
              : rows <= 16                                               ? 0
@@ -1137,9 +1137,9 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   p.max16 = !p.tile32 ? INT_MAX : mixed ? 16 : 0;
   if (p.max16) {
     // 4 waves a workgroup, two of which fit a CU, so that one's start stands beside the other's loads (64 sequences of
-    // 1000 keys, 8 kv heads: 25.3 us, 31.3 with 8 waves; 64 of up to 4000 65.0 and 70.5). 8 where there is at most one
-    // a CU, by splits or not, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 29.6 us,
-    // 30.5 with 4 waves; 8 of 8192, 8 kv heads: 29.4 and 30.1; but one of 16384 16.5 and 15.5).
+    // 1000 keys, 8 kv heads: 25.1 us, 30.9 with 8 waves; 64 of up to 4000 64.8 and 71.0). 8 where there is at most one
+    // a CU, by splits or not, and each of its waves has two turns or more (one of 131072 keys, 4 kv heads: 30.0 us,
+    // 32.4 with 4 waves; 8 of 8192, 8 kv heads: 29.5 and 32.1; but one of 16384 16.3 and 15.2).
     const long base = (long)n_seq * kv_heads;
     // Room for partial sums: of as many rows as the bounds say a sequence of this form has; longer ones, where a bound
     // is wrong, are not split. (A prompt among decode steps has none here, however many keys they have: one step over
@@ -1152,18 +1152,19 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
     const int turn = 64 * p.waves16;
     // A join costs as much as two turns: 16 sequences, 8 kv heads, 600 / 1000 / 8192 keys in one range 11.2 / 13.4 /
     // 65.5 us, in two 13.4 / 14.6 / 49.2. (At most 1024 keys where the other form's workgroups run beside: 8 sequences
-    // of up to 600 tokens and 8000 keys 364.7 us, 393.7 at 512 and 395.5 at 4096.)
+    // of up to 600 tokens and 8000 keys, 16 heads, 355 us, 389 at 512 and at 4096; with 32 heads 533, 535 and 533.)
     split_keys(keys, base, kCus, turn, 3, turn, mixed ? 1024 : 8192, force_split, top, &p.chunk16, &p.ns16);
     // Sequences dealt by length, where there are about as many workgroups as CUs or more and each is long. A CU draws
     // about 30 GB/s whatever is on it, so the time is that of the CU with the most keys: 32 sequences, 8 kv heads, of
     // 1621 to 8192 keys 69.0 -> 59.5 us in halves (the join among it; of 8192 each 85.5 -> 90.9), 28 of up to 8192 66.9
-    // -> 58.7 (equal ones 78.5 -> 83.5; but 24 65.0 and 62.0, 73.1 and 79.4: whole, with 8 waves); whole ones in order:
-    // 64 of up to 4100 65.9 -> 53.9 (of 4100 each 88.3 -> 90.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of 16
+    // -> 59.0 (equal ones 77.6 -> 83.9; but 24 65.0 and 62.0, 73.1 and 79.4: whole, with 8 waves); whole ones in order:
+    // 64 of up to 4100 66.8 -> 54.4 (of 4100 each 86.6 -> 89.5), 48 of up to 5000 74.1 -> 55.2, 100 of up to 4500 of 16
     // heads 115 -> 97.
     // Fewer, where the bound makes ranges of 8 turns or more: by shares of all keys that the batch has, up to 4 times
     // an even batch's ranges of a sequence. Finding them costs 2 us (8 sequences of 2000 keys bounded by 32768 21.7 ->
     // 23.8), ranges of the bound far more where it is loose or lengths differ: 8 of up to 8000 bounded by 65536 59.5 ->
-    // 30.7 us, one of 16384 bounded by 131072 35.7 -> 19.2.
+    // 30.7 us, one of 16384 bounded by 131072 35.7 -> 19.2. Between half and 7/8 of the CUs neither rule applies and each
+    // sequence is one range: 17 of up to 8192 keys take 62 us, 46.7 in 4 ranges each; 17 equal ones 67.0 and 69.1.
     if (!mixed && force_split <= 0 && base <= kCus / 2 && p.ns16 > 1 && p.chunk16 >= 8 * turn) {
       p.deal16 = kShares;
       const long most = 4 * (kCus / base), have = (keys + turn - 1) / turn, places = kCus / kv_heads;
@@ -1181,8 +1182,8 @@ KQ4AttnPlan kq4_attn_plan(int n_tok, int n_seq, int heads, int kv_heads, int max
   if (p.tile32) {
     // A split more saves the longest workgroup tiles of keys (about 0.9 us each) and costs every row a partial sum
     // written and read: keys / n + n rows / kRowKeys is least at n^2 = kRowKeys keys / rows. (kRowKeys 40 / 80 / 140:
-    // 64 tokens x 32 heads over 2000 keys 25.4 / 22.3 / 21.1 us, 3 x 200 x 8 over 400 32.1 / 27.7 / 27.8, 4 x 100 x 16
-    // over 900 33.1 / 29.3 / 32.3, 300 x 32 over 16000 86.7 / 78 / 78.)
+    // 64 tokens x 32 heads over 2000 keys 27.9 / 25.8 / 26.5 us, 3 x 200 x 8 over 400 24.7 / 23.6 / 23.5, 4 x 100 x 16
+    // over 900 32.9 / 29.4 / 32.0.)
     const int best = (int)(sqrt((double)kRowKeys * keys / ((double)n_tok * heads)) + 0.5);
     const long least = best < 2 ? keys : (keys + best - 1) / best;
     split_keys(keys, ((long)n_tok * group + p.tile32 - 1) / p.tile32 * kv_heads, p.tile32 == 128 ? 2 * kCus : kCus,
