@@ -65,7 +65,8 @@ KQ4_HD int kq4_kv_ranges(const KQ4KvSpan &s, int t0, int t1, int window, int chu
   kq4_kv_sees(s.p0 + t1, s.len, window, &lo, end);
   kq4_kv_sees(s.p0 + t0, s.len, window, &lo, &hi);
   *base = lo & ~63;
-  const int n = *end > *base ? (*end - *base + chunk - 1) / chunk : 0;
+  // (unsigned: keys and chunk together may pass 2^31)
+  const int n = *end > *base ? (int)(((unsigned)(*end - *base) + chunk - 1u) / (unsigned)chunk) : 0;
   return n < 1 ? 1 : n > ns ? ns : n;
 }
 
