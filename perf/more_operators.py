@@ -1,0 +1,334 @@
+"""Performance cases of kq4's microscaled operators: quantisation to 4- and 8-bit floating point with a
+power-of-two scale per block of 32 columns, the product of such activations with 4-bit weights, and the gated
+feed-forward projections over them.
+
+A case is one of four kinds of call:
+
+  quantize  fp32 rows into a microscaled matrix, as the products read it
+  matmul    out = [residual +] x . W^T: fp32 rows quantized to `act` bits on the way, W of 4 bits
+  qkv       one quantization of the rows, three products with it
+  gated     silu(x . G^T) * (x . U^T), G and U of 4 bits
+
+An element of 4 bits is e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), of 8 bits e4m3 (up to 448). A block
+has the scale 2^e, e the least from -127 on for which its largest magnitude over 2^e, rounded to the element's
+precision, is not above the largest element; it is held as the byte e + 127. An element is the nearest one to x / 2^e, ties to even. All of that is exact, so a quantized
+matrix is whole numbers, returned as it lies in memory: pieces of 16 bytes of a row (32 columns of 4 bits, 16 of 8)
+in tiles of 16 rows x 128 columns, [piece][row][16], the tiles [group of 128 rows][128 columns][tile of the group];
+then the scales in tiles of 16 rows x 512 columns, [block of 128 columns][row][which 128 columns], in the same order.
+What lies beyond the rows and columns is zero.
+
+Sizes are those of Qwen3-VL-2B (2048 wide, 6144 in the feed-forward block, 151936 tokens), of Qwen3-8B (4096 and
+12288, 32 query and 8 key heads of 128), or generic.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+DEV = "cuda"
+FP4 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def listed():
+    return [
+        # the hidden state of one decode token: the smallest call, all latency
+        dict(name="quantize_1", kind="quantize", n=1, cols=4096, act=8),
+        # a prompt's feed-forward activations before the down projection
+        dict(name="quantize_prompt", kind="quantize", n=2048, cols=12288, act=4),
+        # one token through an attention output projection, added to the residual stream
+        dict(name="matmul_1", kind="matmul", n=1, rows=4096, cols=4096, act=8, residual=True, pad=0),
+        # one token's logits (Qwen3-VL-2B): the largest matrix a decode step reads
+        dict(name="matmul_logits", kind="matmul", n=1, rows=151936, cols=2048, act=8, residual=False, pad=0),
+        # a decode step of 64 sequences through the down projection (Qwen3-8B)
+        dict(name="matmul_64", kind="matmul", n=64, rows=4096, cols=12288, act=8, residual=True, pad=0),
+        # an odd chunk, odd rows, a width that ends inside a tile, rows that are columns of a wider tensor
+        dict(name="matmul_odd", kind="matmul", n=301, rows=1999, cols=2016, act=4, residual=False, pad=96),
+        # a whole prompt through the down projection at both widths of the activations, the largest calls
+        dict(name="matmul_prompt_8", kind="matmul", n=4096, rows=4096, cols=12288, act=8, residual=True, pad=0),
+        dict(name="matmul_prompt_4", kind="matmul", n=4096, rows=4096, cols=12288, act=4, residual=True, pad=0),
+        # queries, keys and values of 8 sequences' tokens (Qwen3-8B)
+        dict(name="qkv_8", kind="qkv", n=8, heads=32, kv_heads=8, cols=4096, act=8),
+        # the feed-forward block's first half: one token (Qwen3-8B), an odd decode batch (Qwen3-VL-2B), a prompt
+        dict(name="gated_1", kind="gated", n=1, rows=12288, cols=4096, act=8),
+        dict(name="gated_29", kind="gated", n=29, rows=6144, cols=2048, act=4),
+        dict(name="gated_prompt", kind="gated", n=2048, rows=12288, cols=4096, act=4),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """One more case: sizes log-uniform over the listed range, odd ones among them."""
+    kind = rng.choice(["quantize", "matmul", "matmul", "qkv", "gated", "gated"])
+    n = 1 if rng.random() < 0.2 else _log_int(rng, 1, 4096)
+    c = dict(kind=kind, n=n, cols=32 * _log_int(rng, 1, 384), act=rng.choice([4, 8]))
+    if kind == "quantize":
+        c["n"] = min(n, 2048 * 12288 // c["cols"])
+        return c
+    if kind == "qkv":
+        c["kv_heads"] = rng.choice([1, 2, 4, 8])
+        c["heads"] = c["kv_heads"] * rng.choice([1, 2, 3, 4, 7])
+        return c
+    c["rows"] = _log_int(rng, 16, 151936 if kind == "matmul" and n < 16 else 12288)
+    matrices = 2 if kind == "gated" else 1
+    while matrices * c["rows"] * c["cols"] > 151936 * 2048 or \
+            matrices * c["rows"] * c["cols"] * c["n"] > 4096 * 4096 * 12288:
+        c["rows"] = max(1, c["rows"] // 2)
+    if kind == "matmul":
+        c.update(residual=rng.random() < 0.5, pad=rng.choice([0, 0, 4, 96, 1000]))
+    return c
+
+
+# ---- inputs --------------------------------------------------------------------------------------
+
+def _gen(seed, salt):
+    g = torch.Generator(device=DEV)
+    g.manual_seed((seed * 1000003 + salt * 7919 + 17) & 0x7FFFFFFF)
+    return g
+
+
+def _acts(n, cols, seed, salt):
+    """N(0, 1), a few channels many times as large, as hidden states have."""
+    g = _gen(seed, salt)
+    gain = 1.0 + 15.0 * (torch.rand(cols, device=DEV, generator=g) < 0.005).float()
+    return torch.randn(n, cols, device=DEV, generator=g) * gain
+
+
+def _weights(rows, cols, seed, salt):
+    """Normal weights as a checkpoint of this format holds them: codes [rows][cols / 2], the even column in the low
+    four bits, and scales [rows][cols / 32]."""
+    w = 0.02 * torch.randn(rows, cols, device=DEV, generator=_gen(seed, salt))
+    codes, scales = _quantized(w, 4)
+    return codes[:, 0::2] | (codes[:, 1::2] << 4), scales
+
+
+def _matrices(c):
+    if c["kind"] == "qkv":
+        return [128 * c["heads"], 128 * c["kv_heads"], 128 * c["kv_heads"]]
+    return {"quantize": [], "matmul": [c.get("rows")], "gated": [c.get("rows")] * 2}[c["kind"]]
+
+
+def prepare(case, seed):
+    c = case
+    n, cols = c["n"], c["cols"]
+    rows = _matrices(c)
+    s = dict(case=c, x=_acts(n, cols + c.get("pad", 0), seed, 1)[:, :cols],
+             w=[_weights(r, cols, seed, 10 + i) for i, r in enumerate(rows)],
+             out=[torch.empty(n, r, device=DEV) for r in (rows[:1] if c["kind"] == "gated" else rows)])
+    s["residual"] = torch.randn(n, rows[0], device=DEV, generator=_gen(seed, 3)) if c.get("residual") else None
+    if own:   # what a program makes once, as it loads a model: the weights in the products' order, a place for the rows
+        kq4 = _kq4()
+        s["m"] = []
+        for (codes, scales), r in zip(s["w"], rows):
+            s["m"].append(kq4.MX(r, cols, 4))
+            kq4.mx_pack_dev(s["m"][-1], codes, scales)
+        if c["kind"] in ("quantize", "qkv"):
+            s["xq"] = kq4.MX(n, cols, c["act"])
+    return s
+
+
+# ---- the framework's calls -------------------------------------------------------------------------
+
+def _kq4():
+    """The binding, initialised once: a program keeps the module."""
+    global _binding
+    if _binding is None:
+        sys.path.insert(0, os.path.abspath("kestrel-llm_amd"))
+        import kq4
+        kq4.init(0)
+        _binding = kq4
+    return _binding
+
+
+_binding = None
+
+
+def _run_own(s):
+    c, kq4 = s["case"], _kq4()
+    if c["kind"] == "quantize":
+        kq4.mx_quantize_dev(s["xq"], s["x"])
+        return s["xq"].data
+    if c["kind"] == "matmul":
+        kq4.mx_matmul_dev(s["out"][0], s["x"], s["m"][0], act=c["act"], residual=s["residual"])
+    elif c["kind"] == "qkv":
+        kq4.mx_quantize_dev(s["xq"], s["x"])
+        for out, m in zip(s["out"], s["m"]):
+            kq4.mx_matmul_q_dev(out, s["xq"], m)
+    else:
+        kq4.mx_gated_dev(s["out"][0], s["x"], s["m"][0], s["m"][1], act=c["act"])
+    return s["out"]
+
+
+# ---- the plain forms ---------------------------------------------------------------------------------
+
+def _scales_of(x, bits):
+    """Scale bytes [n][cols / 32] of fp32 x."""
+    amax = x.reshape(x.shape[0], -1, 32).abs().amax(2)
+    m, e = torch.frexp(amax)                                  # amax = m 2^e, m in [1/2, 1)
+    up = (m >= 0.875) if bits == 4 else (m > 0.90625)         # 7 / 8 rounds to 8, 464 / 512 to 448
+    e = e - 1 - (2 if bits == 4 else 8) + up.int()
+    return torch.where(amax > 0, e.clamp(min=-127), torch.full_like(e, -127)) + 127
+
+
+def _rounded(x, bits):
+    """(x / 2^e as the nearest element, its scale's byte), x / 2^e exact in 32 bits but for what rounds to 0 anyway."""
+    b = _scales_of(x, bits)
+    inverse = torch.exp2(127.0 - b.double()).float()
+    y = x.reshape(x.shape[0], -1, 32) * inverse[:, :, None]
+    lead = torch.frexp(y)[1] - 1
+    step = torch.exp2((lead.clamp(min=0) - 1 if bits == 4 else lead.clamp(min=-6) - 3).float())
+    top = 6.0 if bits == 4 else 448.0
+    return ((y / step).round() * step).clamp(-top, top), b
+
+
+def _quantized(x, bits):
+    """(codes [n][cols], scale bytes [n][cols / 32]), uint8."""
+    v, b = _rounded(x, bits)
+    a = v.abs()
+    if bits == 4:
+        code = torch.where(a < 2, 2 * a, torch.where(a < 4, a + 2, a / 2 + 4))
+    else:
+        e = (torch.frexp(a)[1] - 1).clamp(min=-6)
+        code = torch.where(a < 2.0 ** -6, a * 512, a * torch.exp2(3.0 - e) + 8 * (e + 6).float())
+    code = code.to(torch.uint8) | (torch.signbit(v).to(torch.uint8) << (3 if bits == 4 else 7))
+    return code.view(x.shape), b.to(torch.uint8)
+
+
+def _zero_padded(x, rows, cols):
+    return torch.nn.functional.pad(x, (0, cols - x.shape[1], 0, rows - x.shape[0]))
+
+
+def _in_groups(t):
+    """Tiles [row tile][column tile][bytes] as they lie in memory: the whole groups of 8 row tiles, then the rest."""
+    whole = t.shape[0] // 8 * 8
+    first = t[:whole].view(-1, 8, t.shape[1], t.shape[2]).transpose(1, 2).reshape(-1)
+    return torch.cat([first, t[whole:].transpose(0, 1).reshape(-1)])
+
+
+def _matrix(codes, scales, bits):
+    """The bytes of a microscaled matrix."""
+    n, cols = codes.shape
+    nt, kt, kq = -(-n // 16), -(-cols // 128), -(-cols // 512)
+    codes = _zero_padded(codes, 16 * nt, 128 * kt)
+    if bits == 4:
+        codes = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    tiles = codes.view(nt, 16, kt, bits, 16).permute(0, 2, 3, 1, 4).reshape(nt, kt, -1)
+    scales = _zero_padded(scales, 16 * nt, 16 * kq)
+    stiles = scales.view(nt, 16, kq, 4, 4).permute(0, 2, 4, 1, 3).reshape(nt, kq, -1)
+    return torch.cat([_in_groups(tiles), _in_groups(stiles)])
+
+
+def _values(w):
+    """fp32 [rows][cols] of a checkpoint's codes and scales."""
+    codes, scales = w
+    table = torch.tensor(FP4 + tuple(-v for v in FP4), device=DEV)
+    v = torch.stack([table[(codes & 15).int()], table[(codes >> 4).int()]], 2)
+    s = torch.exp2(scales.double() - 127).float()
+    return (v.view(codes.shape[0], -1, 32) * s[:, :, None]).view(codes.shape[0], -1)
+
+
+def _run_plain(s):
+    c, x = s["case"], s["x"]
+    if c["kind"] == "quantize":
+        return _matrix(*_quantized(x, c["act"]), c["act"])
+    v, b = _rounded(x, c["act"])
+    x = (v * torch.exp2(b.double() - 127).float()[:, :, None]).view(x.shape)
+    got = [x @ _values(w).t() for w in s["w"]]
+    if c["kind"] == "gated":
+        g, u = got
+        return [g / (1 + torch.exp(-g)) * u]
+    return [got[0] + s["residual"]] if s["residual"] is not None else got
+
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+# ---- 64 bits, from the definitions ---------------------------------------------------------------------
+
+def _elements(bits):
+    """The non-negative elements by their codes."""
+    if bits == 4:
+        return [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+    return [m / 512 if e == 0 else (8 + m) * 2.0 ** (e - 10) for e in range(16) for m in range(8)][:127]
+
+
+def _exact_quantized(x, bits):
+    """(codes, exponents, values) by search: in each block the least exponent that fits, then among the elements'
+    midpoints, a midpoint belonging to the even code."""
+    el = _elements(bits)
+    x = x.double().reshape(x.shape[0], -1, 32)
+    top, past = el[-1], el[-1] + (2.0 if bits == 4 else 32.0)     # the next element, were there one
+    mid = (top + past) / 2
+    amax = x.abs().amax(2)
+    e = torch.full(amax.shape, -127, dtype=torch.int64, device=DEV)
+    for step in (128, 64, 32, 16, 8, 4, 2, 1):                    # the largest exponent that does not fit, plus one
+        trial = e + step - 1
+        over = amax * torch.exp2(-trial.double())
+        fits = (over < mid) if bits == 4 else (over <= mid)       # 7 goes to 8, 464 to 448: ties to even
+        e = torch.where(fits, e, e + step)
+    y = x * torch.exp2(-e.double())[:, :, None]
+    bounds = [(a + b) / 2 for a, b in zip(el, el[1:])]
+    bounds = [math.nextafter(m, math.inf) if i % 2 == 0 else m for i, m in enumerate(bounds)]
+    code = torch.bucketize(y.abs(), torch.tensor(bounds, dtype=torch.float64, device=DEV), right=True)
+    value = torch.tensor(el, dtype=torch.float64, device=DEV)[code] * torch.sign(x) * torch.exp2(e.double())[:, :, None]
+    code = code + torch.signbit(x).long() * (8 if bits == 4 else 128)
+    shape = (x.shape[0], -1)
+    return code.reshape(shape), e + 127, value.reshape(shape)
+
+
+def _exact_matrix(code, scale, bits):
+    """A microscaled matrix, byte by byte from where each element lies."""
+    n, cols = code.shape
+    nt, kt, kq = -(-n // 16), -(-cols // 128), -(-cols // 512)
+    first, tile = nt * kt * 256 * bits, 256 * bits
+    m = torch.zeros(first + nt * kq * 256, dtype=torch.int64, device=DEV)
+    r = torch.arange(n, device=DEV)[:, None]
+    group, t = r // 128, r // 16 % 8
+    held = torch.minimum(torch.tensor(8, device=DEV), nt - 8 * group)
+    k = torch.arange(cols, device=DEV)[None]
+    per = 16 * 8 // bits                                          # elements of a piece
+    at = ((8 * group * kt + k // 128 * held + t) * tile + k % 128 // per * 256 + r % 16 * 16 + k % per * bits // 8)
+    m.index_add_(0, at.reshape(-1), (code << ((k % 2) * 4 if bits == 4 else k * 0)).reshape(-1))
+    b = torch.arange(cols // 32, device=DEV)[None]
+    at = first + (8 * group * kq + b // 16 * held + t) * 256 + b % 4 * 64 + r % 16 * 4 + b // 4 % 4
+    m.index_add_(0, at.reshape(-1), scale.reshape(-1))
+    return m.to(torch.uint8)
+
+
+def _exact_weights(w):
+    codes, scales = w
+    el = torch.tensor(_elements(4), dtype=torch.float64, device=DEV)
+    out = torch.empty(codes.shape[0], 2 * codes.shape[1], dtype=torch.float64, device=DEV)
+    for half in range(2):
+        n = (codes.int() >> (4 * half)) & 15
+        out[:, half::2] = el[n & 7] * (1 - 2 * (n >> 3))
+    return out * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    code, scale, x = _exact_quantized(s["x"], case["act"])
+    if case["kind"] == "quantize":
+        return _exact_matrix(code, scale, case["act"])
+    got = [torch.matmul(x, _exact_weights(w).t().contiguous()) for w in s["w"]]
+    if case["kind"] == "gated":
+        return [got[0] * torch.sigmoid(got[0]) * got[1]]
+    return [got[0] + s["residual"].double()] if s["residual"] is not None else got
+
+
+# ---- what a pass cannot do without ---------------------------------------------------------------------
+
+def work(case):
+    c = case
+    n, cols = c["n"], c["cols"]
+    if c["kind"] == "quantize":
+        return {"bytes": n * cols * (4 + c["act"] / 8 + 1 / 32), "flops": 2.0 * n * cols}
+    rows = _matrices(c)
+    weights = sum(rows) * cols * (0.5 + 1 / 32)
+    out = n * (rows[0] if c["kind"] == "gated" else sum(rows)) * 4.0 * (2 if c.get("residual") else 1)
+    return {"bytes": weights + 4.0 * n * cols + out, "flops": 2.0 * n * sum(rows) * cols}
