@@ -1,4 +1,4 @@
-"""Performance cases of kq4's microscaled operators: quantisation to 4- and 8-bit floating point with a
+"""Performance cases of kq4's microscaled operators: quantisation to 4- and 6-bit floating point with a
 power-of-two scale per block of 32 columns, the product of such activations with 4-bit weights, and the gated
 feed-forward projections over them.
 
@@ -9,12 +9,13 @@ A case is one of four kinds of call:
   qkv       one quantization of the rows, three products with it
   gated     silu(x . G^T) * (x . U^T), G and U of 4 bits
 
-An element of 4 bits is e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), of 8 bits e4m3 (up to 448). A block
+An element of 4 bits is e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), of 6 bits e2m3 (multiples of 1/8 up
+to 2, of 1/4 up to 4, of 1/2 up to 7.5). A block
 has the scale 2^e, e the least from -127 on for which its largest magnitude over 2^e, rounded to the element's
 precision, is not above the largest element; it is held as the byte e + 127. An element is the nearest one to x / 2^e, ties to even. All of that is exact, so a quantized
-matrix is whole numbers, returned as it lies in memory: pieces of 16 bytes of a row (32 columns of 4 bits, 16 of 8)
-in tiles of 16 rows x 128 columns, [piece][row][16], the tiles [group of 128 rows][128 columns][tile of the group];
-then the scales in tiles of 16 rows x 512 columns, [block of 128 columns][row][which 128 columns], in the same order.
+matrix is whole numbers, returned as it lies in memory: a block's elements one after the other in its 16 or 24 bytes, in
+tiles of 16 rows x 128 columns, [block][row][first 16 bytes], then [block][row][last 8] where there are 24; the tiles
+[group of 128 rows][128 columns][tile of the group]; then the scales in tiles of 16 rows x 512 columns, [block of 128 columns][row][which 128 columns], in the same order.
 What lies beyond the rows and columns is zero.
 
 Sizes are those of Qwen3-VL-2B (2048 wide, 6144 in the feed-forward block, 151936 tokens), of Qwen3-8B (4096 and
@@ -34,24 +35,24 @@ FP4 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 def listed():
     return [
         # the hidden state of one decode token: the smallest call, all latency
-        dict(name="quantize_1", kind="quantize", n=1, cols=4096, act=8),
+        dict(name="quantize_1", kind="quantize", n=1, cols=4096, act=6),
         # a prompt's feed-forward activations before the down projection
         dict(name="quantize_prompt", kind="quantize", n=2048, cols=12288, act=4),
         # one token through an attention output projection, added to the residual stream
-        dict(name="matmul_1", kind="matmul", n=1, rows=4096, cols=4096, act=8, residual=True, pad=0),
+        dict(name="matmul_1", kind="matmul", n=1, rows=4096, cols=4096, act=6, residual=True, pad=0),
         # one token's logits (Qwen3-VL-2B): the largest matrix a decode step reads
-        dict(name="matmul_logits", kind="matmul", n=1, rows=151936, cols=2048, act=8, residual=False, pad=0),
+        dict(name="matmul_logits", kind="matmul", n=1, rows=151936, cols=2048, act=6, residual=False, pad=0),
         # a decode step of 64 sequences through the down projection (Qwen3-8B)
-        dict(name="matmul_64", kind="matmul", n=64, rows=4096, cols=12288, act=8, residual=True, pad=0),
+        dict(name="matmul_64", kind="matmul", n=64, rows=4096, cols=12288, act=6, residual=True, pad=0),
         # an odd chunk, odd rows, a width that ends inside a tile, rows that are columns of a wider tensor
         dict(name="matmul_odd", kind="matmul", n=301, rows=1999, cols=2016, act=4, residual=False, pad=96),
         # a whole prompt through the down projection at both widths of the activations, the largest calls
-        dict(name="matmul_prompt_8", kind="matmul", n=4096, rows=4096, cols=12288, act=8, residual=True, pad=0),
+        dict(name="matmul_prompt_6", kind="matmul", n=4096, rows=4096, cols=12288, act=6, residual=True, pad=0),
         dict(name="matmul_prompt_4", kind="matmul", n=4096, rows=4096, cols=12288, act=4, residual=True, pad=0),
         # queries, keys and values of 8 sequences' tokens (Qwen3-8B)
-        dict(name="qkv_8", kind="qkv", n=8, heads=32, kv_heads=8, cols=4096, act=8),
+        dict(name="qkv_8", kind="qkv", n=8, heads=32, kv_heads=8, cols=4096, act=6),
         # the feed-forward block's first half: one token (Qwen3-8B), an odd decode batch (Qwen3-VL-2B), a prompt
-        dict(name="gated_1", kind="gated", n=1, rows=12288, cols=4096, act=8),
+        dict(name="gated_1", kind="gated", n=1, rows=12288, cols=4096, act=6),
         dict(name="gated_29", kind="gated", n=29, rows=6144, cols=2048, act=4),
         dict(name="gated_prompt", kind="gated", n=2048, rows=12288, cols=4096, act=4),
     ]
@@ -65,7 +66,7 @@ def draw(rng):
     """One more case: sizes log-uniform over the listed range, odd ones among them."""
     kind = rng.choice(["quantize", "matmul", "matmul", "qkv", "gated", "gated"])
     n = 1 if rng.random() < 0.2 else _log_int(rng, 1, 4096)
-    c = dict(kind=kind, n=n, cols=32 * _log_int(rng, 1, 384), act=rng.choice([4, 8]))
+    c = dict(kind=kind, n=n, cols=32 * _log_int(rng, 1, 384), act=rng.choice([4, 6]))
     if kind == "quantize":
         c["n"] = min(n, 2048 * 12288 // c["cols"])
         return c
@@ -169,8 +170,8 @@ def _scales_of(x, bits):
     """Scale bytes [n][cols / 32] of fp32 x."""
     amax = x.reshape(x.shape[0], -1, 32).abs().amax(2)
     m, e = torch.frexp(amax)                                  # amax = m 2^e, m in [1/2, 1)
-    up = (m >= 0.875) if bits == 4 else (m > 0.90625)         # 7 / 8 rounds to 8, 464 / 512 to 448
-    e = e - 1 - (2 if bits == 4 else 8) + up.int()
+    up = m >= (0.875 if bits == 4 else 0.96875)               # 7 / 8 and 7.75 / 8 are ties that go to 1
+    e = e - 3 + up.int()
     return torch.where(amax > 0, e.clamp(min=-127), torch.full_like(e, -127)) + 127
 
 
@@ -180,8 +181,8 @@ def _rounded(x, bits):
     inverse = torch.exp2(127.0 - b.double()).float()
     y = x.reshape(x.shape[0], -1, 32) * inverse[:, :, None]
     lead = torch.frexp(y)[1] - 1
-    step = torch.exp2((lead.clamp(min=0) - 1 if bits == 4 else lead.clamp(min=-6) - 3).float())
-    top = 6.0 if bits == 4 else 448.0
+    step = torch.exp2((lead.clamp(min=0) - (1 if bits == 4 else 3)).float())
+    top = 6.0 if bits == 4 else 7.5
     return ((y / step).round() * step).clamp(-top, top), b
 
 
@@ -189,12 +190,9 @@ def _quantized(x, bits):
     """(codes [n][cols], scale bytes [n][cols / 32]), uint8."""
     v, b = _rounded(x, bits)
     a = v.abs()
-    if bits == 4:
-        code = torch.where(a < 2, 2 * a, torch.where(a < 4, a + 2, a / 2 + 4))
-    else:
-        e = (torch.frexp(a)[1] - 1).clamp(min=-6)
-        code = torch.where(a < 2.0 ** -6, a * 512, a * torch.exp2(3.0 - e) + 8 * (e + 6).float())
-    code = code.to(torch.uint8) | (torch.signbit(v).to(torch.uint8) << (3 if bits == 4 else 7))
+    unit = 2 if bits == 4 else 8                               # elements per 1 below 2, half and a quarter of it beyond
+    code = unit * torch.where(a < 2, a, torch.where(a < 4, a / 2 + 1, a / 4 + 2))
+    code = code.to(torch.uint8) | (torch.signbit(v).to(torch.uint8) << (bits - 1))
     return code.view(x.shape), b.to(torch.uint8)
 
 
@@ -215,8 +213,12 @@ def _matrix(codes, scales, bits):
     nt, kt, kq = -(-n // 16), -(-cols // 128), -(-cols // 512)
     codes = _zero_padded(codes, 16 * nt, 128 * kt)
     if bits == 4:
-        codes = codes[:, 0::2] | (codes[:, 1::2] << 4)
-    tiles = codes.view(nt, 16, kt, bits, 16).permute(0, 2, 3, 1, 4).reshape(nt, kt, -1)
+        held = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    else:                                                       # four codes in three bytes
+        a, b, c, d = (codes[:, i::4] for i in range(4))
+        held = torch.stack([a | (b << 6), (b >> 2) | (c << 4), (c >> 4) | (d << 2)], 2)
+    held = held.reshape(nt, 16, kt, 4, 4 * bits).permute(0, 2, 3, 1, 4)
+    tiles = torch.cat([held[..., :16].reshape(nt, kt, -1), held[..., 16:].reshape(nt, kt, -1)], 2)
     scales = _zero_padded(scales, 16 * nt, 16 * kq)
     stiles = scales.view(nt, 16, kq, 4, 4).permute(0, 2, 4, 1, 3).reshape(nt, kq, -1)
     return torch.cat([_in_groups(tiles), _in_groups(stiles)])
@@ -254,7 +256,7 @@ def _elements(bits):
     """The non-negative elements by their codes."""
     if bits == 4:
         return [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
-    return [m / 512 if e == 0 else (8 + m) * 2.0 ** (e - 10) for e in range(16) for m in range(8)][:127]
+    return [m / 8 if e == 0 else (8 + m) * 2.0 ** (e - 4) for e in range(4) for m in range(8)]
 
 
 def _exact_quantized(x, bits):
@@ -262,21 +264,19 @@ def _exact_quantized(x, bits):
     midpoints, a midpoint belonging to the even code."""
     el = _elements(bits)
     x = x.double().reshape(x.shape[0], -1, 32)
-    top, past = el[-1], el[-1] + (2.0 if bits == 4 else 32.0)     # the next element, were there one
-    mid = (top + past) / 2
+    mid = (el[-1] + 8.0) / 2                                      # halfway to the next element, were there one
     amax = x.abs().amax(2)
     e = torch.full(amax.shape, -127, dtype=torch.int64, device=DEV)
     for step in (128, 64, 32, 16, 8, 4, 2, 1):                    # the largest exponent that does not fit, plus one
         trial = e + step - 1
         over = amax * torch.exp2(-trial.double())
-        fits = (over < mid) if bits == 4 else (over <= mid)       # 7 goes to 8, 464 to 448: ties to even
-        e = torch.where(fits, e, e + step)
+        e = torch.where(over < mid, e, e + step)                  # the tie goes to 8: the code after the last is even
     y = x * torch.exp2(-e.double())[:, :, None]
     bounds = [(a + b) / 2 for a, b in zip(el, el[1:])]
     bounds = [math.nextafter(m, math.inf) if i % 2 == 0 else m for i, m in enumerate(bounds)]
     code = torch.bucketize(y.abs(), torch.tensor(bounds, dtype=torch.float64, device=DEV), right=True)
     value = torch.tensor(el, dtype=torch.float64, device=DEV)[code] * torch.sign(x) * torch.exp2(e.double())[:, :, None]
-    code = code + torch.signbit(x).long() * (8 if bits == 4 else 128)
+    code = code + torch.signbit(x).long() * 2 ** (bits - 1)
     shape = (x.shape[0], -1)
     return code.reshape(shape), e + 127, value.reshape(shape)
 
@@ -291,9 +291,13 @@ def _exact_matrix(code, scale, bits):
     group, t = r // 128, r // 16 % 8
     held = torch.minimum(torch.tensor(8, device=DEV), nt - 8 * group)
     k = torch.arange(cols, device=DEV)[None]
-    per = 16 * 8 // bits                                          # elements of a piece
-    at = ((8 * group * kt + k // 128 * held + t) * tile + k % 128 // per * 256 + r % 16 * 16 + k % per * bits // 8)
-    m.index_add_(0, at.reshape(-1), (code << ((k % 2) * 4 if bits == 4 else k * 0)).reshape(-1))
+    code = code << (k % 32 * bits % 8)
+    for part in range(2):                                         # an element lies in one byte or across two
+        y = k % 32 * bits // 8 + part
+        y = torch.minimum(y, torch.tensor(4 * bits - 1, device=DEV))   # (past the block's last byte: adds nothing)
+        place = torch.where(y < 16, k % 128 // 32 * 256 + r % 16 * 16 + y, 1024 + k % 128 // 32 * 128 + r % 16 * 8 + y - 16)
+        at = (8 * group * kt + k // 128 * held + t) * tile + place
+        m.index_add_(0, at.reshape(-1), ((code >> (8 * part)) & 255).reshape(-1))
     b = torch.arange(cols // 32, device=DEV)[None]
     at = first + (8 * group * kq + b // 16 * held + t) * 256 + b % 4 * 64 + r % 16 * 4 + b // 4 % 4
     m.index_add_(0, at.reshape(-1), scale.reshape(-1))
