@@ -34,7 +34,8 @@
  * whatever calls run after its capture. The workspace cannot grow while a stream is being
  * captured (that needs hipMalloc): such a call returns KQ4_EINVAL and launches nothing. Size it
  * before capturing with kq4_workspace_reserve (kq4_matmul_workspace_bytes,
- * kq4_moe_workspace_bytes, kq4_attn_workspace_bytes, kq4_logprobs_workspace_bytes), or by running
+ * kq4_moe_workspace_bytes, kq4_attn_workspace_bytes, kq4_logprobs_workspace_bytes,
+ * kq4_mx_workspace_bytes, kq4_mx_ffn_workspace_bytes), or by running
  * the same calls once eagerly. kq4_workspace_trim frees the outgrown workspaces once the graphs
  * captured before the growth are destroyed. Only the
  * call's own stream is asked whether it is capturing: a call that grows the workspace on
@@ -53,7 +54,8 @@
  * Between the linear layers: the paged int8 key/value cache (kq4_kv_append_dev), the attention
  * that reads it (kq4_attn_dev) and the reading of the logits (kq4_logprobs_dev) take and leave
  * fp32 rows on the device as the linear layers do, under the same rules for streams, graphs,
- * workspace and errors.
+ * workspace and errors. So do the linear layers and the gated feed-forward block over microscaled
+ * 4-bit floating point weights (kq4_mx_*).
  */
 #ifndef KQ4_H
 #define KQ4_H
@@ -481,6 +483,80 @@ int kq4_logprobs_dev(float *logprob, float *entropy, float *top_logprob, int *to
                      const float *logits, long ld, const int *token, int n, int vocab, int n_top,
                      void *stream);
 size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top);
+
+/* ---- microscaled matrices: 4-bit weights, 4- or 6-bit activations (device pointers) ---------- */
+
+/* Bits of an element of a microscaled matrix (the OCP formats): FP4 is e2m1 (0, .5, 1, 1.5, 2, 3,
+ * 4, 6 and their negatives), FP6 is e2m3 (multiples of 1/8 up to 2, of 1/4 up to 4, of 1/2 up to
+ * 7.5). 32 consecutive columns of a row are a block with one scale, a byte b that stands for
+ * 2^(b - 127); 255 makes the block NaN.
+ * gfx950's matrix unit multiplies by the scales itself, so these products have no arithmetic per
+ * block beside it, which is what bounds the q4 x int8 GEMM. It takes both types at one rate and sums
+ * their products as fp32 does; 8-bit elements would halve the rate, and their products lose up to 2^-13 of a
+ * sum's largest term (measured), so they are not offered. No counterpart in the reference, whose
+ * weights are Q4_0 or Q8_0. */
+#define KQ4_MX_FP4 4
+#define KQ4_MX_FP6 6
+
+/* A microscaled matrix of rows x cols (cols % 32 == 0; fewer than 2^24 tiles of 16 rows x 512
+ * columns, rows <= 2^24) is kq4_mx_bytes bytes, 16-byte aligned; 0 for a bad shape. First the codes
+ * in tiles of 16 rows x 128 columns: a block's elements lie one after the other, the first in the
+ * lowest bits, in 16 (FP4) or 24 (FP6) bytes, and a tile is [4 blocks][16 rows][the first 16 bytes],
+ * then for FP6 [4 blocks][16 rows][the last 8]. Groups of 8 row tiles (the last one of
+ * what is left) one after the other, in each [column tile][row tile]. Then the scales in tiles of
+ * 16 rows x 512 columns, each [4][16 rows][4]: byte [i][r][j] is the scale of block 4 j + i of the
+ * tile's 16 in row r; the tiles in the same order. What lies past the rows and columns is zero
+ * (written by every call that writes a matrix). */
+size_t kq4_mx_bytes(int rows, int cols, int type);
+
+/* fp32 rows (row t at x + t * ldx floats; 16-byte aligned, ldx a multiple of 4) into a microscaled
+ * matrix of `type` bits. A block's scale is the least 2^e, e >= -127, for which its largest
+ * magnitude over 2^e, rounded to the element's precision, is not above the largest element (so no
+ * element is off by more than half a step of its format); an element is the nearest one to x / 2^e,
+ * ties to even, signs of zeros kept. A block that holds a NaN or infinity gets scale 255, codes 0.
+ * This is the activations' way into the products, and the way of fp32 weights into the format. */
+int kq4_mx_quantize_dev(uint8_t *m, const float *x, long ldx, int rows, int cols, int type,
+                        void *stream);
+
+/* A checkpoint's row-major codes ([rows][cols * type / 8] bytes, a 4-bit element's even column in
+ * the low half, 6-bit ones one after the other from the lowest bits; 16-byte aligned) and scales ([rows][cols / 32] bytes) into a microscaled matrix,
+ * once per weight matrix, and back. Matrices of whole groups of 128 rows may be stacked by packing
+ * them as one of their summed rows. */
+int kq4_mx_pack_dev(uint8_t *m, const uint8_t *codes, const uint8_t *scales, int rows, int cols,
+                    int type, void *stream);
+int kq4_mx_unpack_dev(uint8_t *codes, uint8_t *scales, const uint8_t *m, int rows, int cols,
+                      int type, void *stream);
+
+/* out = [residual +] W . x for n_batch tokens: W a 4-bit matrix of rows x cols, x [n_batch][cols]
+ * fp32 rows (as for kq4_mx_quantize_dev) quantized to `act` bits (KQ4_MX_FP6: a quarter of FP4's
+ * steps), sums in fp32 (an output's sum below 2^-126 is zero). Token t's outputs are at out + t * ldo floats,
+ * its residual at residual + t * ldo (4-byte aligned; residual may be NULL or out, and must not
+ * overlap out otherwise; out must not overlap x). A NaN block of a row of x makes that token's
+ * outputs NaN, one of W that row's. The order of a token's sums goes with the shape of the call:
+ * the same token in a batch of another size is equal within rounding, the same call to the bit. */
+int kq4_mx_matmul_dev(float *out, long ldo, const float *x, long ldx, const float *residual,
+                      const uint8_t *w, int rows, int cols, int n_batch, int act, void *stream);
+/* The same from rows that are quantized already (xq: a matrix of n_batch x cols of `act` bits), for
+ * several products of one activation (Q, K and V). Uses no workspace for xq. */
+int kq4_mx_matmul_q_dev(float *out, long ldo, const uint8_t *xq, const float *residual,
+                        const uint8_t *w, int rows, int cols, int n_batch, int act, void *stream);
+
+/* The gated half of a feed-forward block: out = silu(gate . x) * (up . x), silu(g) = g / (1 + e^-g),
+ * both projections (4-bit matrices of rows x cols) and the product in one kernel. x, out, act as
+ * for kq4_mx_matmul_dev. */
+int kq4_mx_gated_dev(float *out, long ldo, const float *x, long ldx, const uint8_t *gate,
+                     const uint8_t *up, int rows, int cols, int n_batch, int act, void *stream);
+
+/* The whole block: out = [residual +] down . h, h = silu(gate . x) * (up . x) quantized to `act`
+ * bits; gate and up of ffn x dim (ffn % 32 == 0), down of dim x ffn. */
+int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *residual,
+                   const uint8_t *gate, const uint8_t *up, const uint8_t *down, int dim, int ffn,
+                   int n_batch, int act, void *stream);
+
+/* Workspace bytes that hold every product and gated call of up to n_batch tokens and cols columns
+ * (whatever its rows and act), and every whole block of up to these sizes; 0 for a bad shape. */
+size_t kq4_mx_workspace_bytes(int n_batch, int cols);
+size_t kq4_mx_ffn_workspace_bytes(int n_batch, int dim, int ffn);
 
 #ifdef __cplusplus
 }

@@ -1391,6 +1391,192 @@ size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top) {
 
 }  // extern "C"
 
+// ---- microscaled matrices ----------------------------------------------------------------------
+
+namespace {
+
+bool mx_shape_ok(int rows, int cols, int type) {
+  if (rows < 1 || rows > 1 << 24 || cols < 32 || cols % 32 || (type != KQ4_MX_FP4 && type != KQ4_MX_FP6)) return false;
+  const KQ4MxDims d = kq4_mx_dims(rows, cols);
+  return (long long)d.nt * d.kq < 1 << 24;   // (2^32 threads)
+}
+
+int mx_matrix_check(const char *what, const char *name, const void *m, int rows, int cols, int type) {
+  if (!mx_shape_ok(rows, cols, type))
+    return fail(KQ4_EINVAL, "%s: %s of rows=%d (1..2^24) cols=%d (%%32) type=%d (4 or 6), fewer than 2^24 tiles of "
+                "16 x 512", what, name, rows, cols, type);
+  if (!m || (uintptr_t)m % 16) return fail(KQ4_EINVAL, "%s: %s must be 16-byte aligned", what, name);
+  return KQ4_OK;
+}
+
+// Whether n rows of w floats at p and m rows of v floats at q share memory. Rows of the same stride may lie side by
+// side in one wider tensor.
+bool rows_overlap(const float *p, long ldp, long w, long n, const float *q, long ldq, long v, long m) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  const uintptr_t ae = a + ((n - 1) * (size_t)ldp + w) * sizeof(float), be = b + ((m - 1) * (size_t)ldq + v) * sizeof(float);
+  if (ae <= b || be <= a) return false;
+  if (ldp != ldq) return true;
+  const size_t ld = (size_t)ldp * sizeof(float);
+  const size_t off = b >= a ? (b - a) % ld : (ld - (a - b) % ld) % ld;   // q's columns from p's, modulo a row
+  return off < w * sizeof(float) || off + v * sizeof(float) > ld;
+}
+
+// The checks that the products share. x: fp32 rows, or nullptr where xq is the activations.
+int mx_product_check(const char *what, const float *out, long ldo, const float *x, long ldx, const uint8_t *xq,
+                     const float *residual, int rows, int cols, int n, int act) {
+  int rc;
+  if (n < 0) return fail(KQ4_EINVAL, "%s: n_batch=%d", what, n);
+  if (act != KQ4_MX_FP4 && act != KQ4_MX_FP6) return fail(KQ4_EINVAL, "%s: act=%d (4 or 6)", what, act);
+  if (n == 0) return KQ4_OK;
+  if (x || !xq) {
+    if (!mx_shape_ok(n, cols, act)) return fail(KQ4_EINVAL, "%s: n_batch=%d cols=%d", what, n, cols);
+    if ((rc = rows_check(what, "x", x, ldx, cols))) return rc;
+  } else if ((rc = mx_matrix_check(what, "xq", xq, n, cols, act))) {
+    return rc;
+  }
+  if (!out || (uintptr_t)out % 4 || (uintptr_t)residual % 4 || ldo < rows)
+    return fail(KQ4_EINVAL, "%s: out and residual must be 4-byte aligned, their stride (%ld) at least %d", what, ldo, rows);
+  if (x && rows_overlap(out, ldo, rows, n, x, ldx, cols, n)) return fail(KQ4_EINVAL, "%s: out overlaps x", what);
+  if (residual && residual != out && rows_overlap(out, ldo, rows, n, residual, ldo, rows, n))
+    return fail(KQ4_EINVAL, "%s: out overlaps the residual and is not it", what);
+  return KQ4_OK;
+}
+
+size_t mx_bytes(int rows, int cols, int type) { return al256(kq4_mx_size(kq4_mx_dims(rows, cols), type)); }
+
+KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, const uint8_t *w1, const uint8_t *xq,
+                  int rows, int cols, int n) {
+  KQ4MxArgs a;
+  a.w[0] = w0;
+  a.w[1] = w1;
+  a.x = xq;
+  a.out = out;
+  a.res = res;
+  a.ldo = ldo;
+  a.rows = rows;
+  a.n = n;
+  a.dw = kq4_mx_dims(rows, cols);
+  a.dx = kq4_mx_dims(n, cols);
+  return a;
+}
+
+// x (or xq) through W (w0; with w1 the gated pair), everything checked.
+int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq, const float *residual,
+               const uint8_t *w0, const uint8_t *w1, int rows, int cols, int n, int act, hipStream_t s) {
+  DevState *ds = nullptr;
+  int rc = cur_dev(&ds);
+  if (rc) return rc;
+  if (!xq) {
+    if ((rc = ensure_ws(Ws{&ds->ws, ds}, mx_bytes(n, cols, act), s))) return rc;
+    uint8_t *q = static_cast<uint8_t *>(ds->ws.p);
+    KQ4_HIP((hipError_t)kq4_launch_mx_quantize(q, x, ldx, n, cols, act, s));
+    xq = q;
+  }
+  KQ4_HIP((hipError_t)kq4_launch_mx_rows(mx_args(out, ldo, residual, w0, w1, xq, rows, cols, n), act, s));
+  return KQ4_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kq4_mx_bytes(int rows, int cols, int type) {
+  return mx_shape_ok(rows, cols, type) ? kq4_mx_size(kq4_mx_dims(rows, cols), type) : 0;
+}
+
+int kq4_mx_quantize_dev(uint8_t *m, const float *x, long ldx, int rows, int cols, int type, void *stream) {
+  if (rows == 0 && mx_shape_ok(1, cols, type)) return KQ4_OK;
+  int rc = mx_matrix_check("mx_quantize", "m", m, rows, cols, type);
+  if (rc || (rc = rows_check("mx_quantize", "x", x, ldx, cols))) return rc;
+  DevState *ds = nullptr;
+  if ((rc = cur_dev(&ds))) return rc;
+  KQ4_HIP((hipError_t)kq4_launch_mx_quantize(m, x, ldx, rows, cols, type, (hipStream_t)stream));
+  return KQ4_OK;
+}
+
+int kq4_mx_pack_dev(uint8_t *m, const uint8_t *codes, const uint8_t *scales, int rows, int cols, int type,
+                    void *stream) {
+  int rc = mx_matrix_check("mx_pack", "m", m, rows, cols, type);
+  if (rc) return rc;
+  if (!codes || !scales || (uintptr_t)codes % 16) return fail(KQ4_EINVAL, "mx_pack: codes must be 16-byte aligned");
+  DevState *ds = nullptr;
+  if ((rc = cur_dev(&ds))) return rc;
+  KQ4_HIP((hipError_t)kq4_launch_mx_pack(m, const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales), rows, cols,
+                                         type, true, (hipStream_t)stream));
+  return KQ4_OK;
+}
+
+int kq4_mx_unpack_dev(uint8_t *codes, uint8_t *scales, const uint8_t *m, int rows, int cols, int type,
+                      void *stream) {
+  int rc = mx_matrix_check("mx_unpack", "m", m, rows, cols, type);
+  if (rc) return rc;
+  if (!codes || !scales || (uintptr_t)codes % 16) return fail(KQ4_EINVAL, "mx_unpack: codes must be 16-byte aligned");
+  DevState *ds = nullptr;
+  if ((rc = cur_dev(&ds))) return rc;
+  KQ4_HIP((hipError_t)kq4_launch_mx_pack(const_cast<uint8_t *>(m), codes, scales, rows, cols, type, false,
+                                         (hipStream_t)stream));
+  return KQ4_OK;
+}
+
+int kq4_mx_matmul_dev(float *out, long ldo, const float *x, long ldx, const float *residual, const uint8_t *w,
+                      int rows, int cols, int n_batch, int act, void *stream) {
+  int rc = mx_matrix_check("mx_matmul", "w", w, rows, cols, KQ4_MX_FP4);
+  if (rc || (rc = mx_product_check("mx_matmul", out, ldo, x, ldx, nullptr, residual, rows, cols, n_batch, act)) || !n_batch)
+    return rc;
+  return mx_product(out, ldo, x, ldx, nullptr, residual, w, nullptr, rows, cols, n_batch, act, (hipStream_t)stream);
+}
+
+int kq4_mx_matmul_q_dev(float *out, long ldo, const uint8_t *xq, const float *residual, const uint8_t *w, int rows,
+                        int cols, int n_batch, int act, void *stream) {
+  int rc = mx_matrix_check("mx_matmul_q", "w", w, rows, cols, KQ4_MX_FP4);
+  if (!rc && n_batch > 0 && !xq) return fail(KQ4_EINVAL, "mx_matmul_q: xq must be 16-byte aligned");
+  if (rc || (rc = mx_product_check("mx_matmul_q", out, ldo, nullptr, 0, xq, residual, rows, cols, n_batch, act)) || !n_batch)
+    return rc;
+  return mx_product(out, ldo, nullptr, 0, xq, residual, w, nullptr, rows, cols, n_batch, act, (hipStream_t)stream);
+}
+
+int kq4_mx_gated_dev(float *out, long ldo, const float *x, long ldx, const uint8_t *gate, const uint8_t *up, int rows,
+                     int cols, int n_batch, int act, void *stream) {
+  int rc = mx_matrix_check("mx_gated", "gate", gate, rows, cols, KQ4_MX_FP4);
+  if (rc || (rc = mx_matrix_check("mx_gated", "up", up, rows, cols, KQ4_MX_FP4)) ||
+      (rc = mx_product_check("mx_gated", out, ldo, x, ldx, nullptr, nullptr, rows, cols, n_batch, act)) || !n_batch)
+    return rc;
+  return mx_product(out, ldo, x, ldx, nullptr, nullptr, gate, up, rows, cols, n_batch, act, (hipStream_t)stream);
+}
+
+int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *residual, const uint8_t *gate,
+                   const uint8_t *up, const uint8_t *down, int dim, int ffn, int n_batch, int act, void *stream) {
+  int rc = mx_matrix_check("mx_ffn", "gate", gate, ffn, dim, KQ4_MX_FP4);
+  if (rc || (rc = mx_matrix_check("mx_ffn", "up", up, ffn, dim, KQ4_MX_FP4)) ||
+      (rc = mx_matrix_check("mx_ffn", "down", down, dim, ffn, KQ4_MX_FP4)) ||
+      (rc = mx_product_check("mx_ffn", out, ldo, x, ldx, nullptr, residual, dim, dim, n_batch, act)) || !n_batch)
+    return rc;
+  if (!mx_shape_ok(n_batch, ffn, act)) return fail(KQ4_EINVAL, "mx_ffn: n_batch=%d ffn=%d", n_batch, ffn);
+  DevState *ds = nullptr;
+  if ((rc = cur_dev(&ds))) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  if ((rc = ensure_ws(Ws{&ds->ws, ds}, kq4_mx_ffn_workspace_bytes(n_batch, dim, ffn), s))) return rc;
+  Carve c{static_cast<char *>(ds->ws.p)};
+  uint8_t *xq = c.take<uint8_t>(mx_bytes(n_batch, dim, act)), *hq = c.take<uint8_t>(mx_bytes(n_batch, ffn, act));
+  float *h = c.take<float>((size_t)n_batch * ffn);
+  KQ4_HIP((hipError_t)kq4_launch_mx_quantize(xq, x, ldx, n_batch, dim, act, s));
+  KQ4_HIP((hipError_t)kq4_launch_mx_rows(mx_args(h, ffn, nullptr, gate, up, xq, ffn, dim, n_batch), act, s));
+  KQ4_HIP((hipError_t)kq4_launch_mx_quantize(hq, h, ffn, n_batch, ffn, act, s));
+  KQ4_HIP((hipError_t)kq4_launch_mx_rows(mx_args(out, ldo, residual, down, nullptr, hq, dim, ffn, n_batch), act, s));
+  return KQ4_OK;
+}
+
+size_t kq4_mx_workspace_bytes(int n_batch, int cols) {
+  return mx_shape_ok(n_batch, cols, KQ4_MX_FP6) ? mx_bytes(n_batch, cols, KQ4_MX_FP6) : 0;
+}
+
+size_t kq4_mx_ffn_workspace_bytes(int n_batch, int dim, int ffn) {
+  if (!mx_shape_ok(n_batch, dim, KQ4_MX_FP6) || !mx_shape_ok(n_batch, ffn, KQ4_MX_FP6)) return 0;
+  return mx_bytes(n_batch, dim, KQ4_MX_FP6) + mx_bytes(n_batch, ffn, KQ4_MX_FP6) + al256((size_t)n_batch * ffn * sizeof(float));
+}
+
+}  // extern "C"
+
 // ---- host-pointer drop-in API ----------------------------------------------------------------
 
 extern "C" {

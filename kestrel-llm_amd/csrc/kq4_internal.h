@@ -6,6 +6,8 @@
 
 #include <atomic>
 
+#include "kq4_mx.h"
+
 // Raises kernel fn's dynamic LDS limit to `bytes` on the current device once per (kernel,
 // device): `done`, one per kernel, holds a bit per device id below 64 (devices beyond make the
 // call every time). Thread-safe: threads that race both make the idempotent call.
@@ -211,3 +213,19 @@ size_t kq4_logprobs_piece_bytes();
 int kq4_launch_logprobs(const float *logits, long ld, int n, int vocab, int n_top, const int *token, float *logprob,
                         float *entropy, float *top_logprob, int *top_id, void *pieces, unsigned long long *best,
                         hipStream_t s);
+
+// Microscaled matrices (kq4_mx.h has their layout): quantisation, the way from and to row-major codes and scales, and
+// products of a quantized activation matrix (n tokens, `type` bits) with 4-bit weights.
+int kq4_launch_mx_quantize(uint8_t *m, const float *x, long ldx, int rows, int cols, int type, hipStream_t s);
+int kq4_launch_mx_pack(uint8_t *m, uint8_t *codes, uint8_t *scales, int rows, int cols, int type, bool pack,
+                       hipStream_t s);
+struct KQ4MxArgs {
+  const uint8_t *w[2];   // weights; the second one, where there is one, is the gated block's up projection
+  const uint8_t *x;
+  float *out;            // token t's outputs at t * ldo
+  const float *res;      // at the same stride, or nullptr
+  long ldo;
+  int rows, n;
+  KQ4MxDims dw, dx;
+};
+int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, hipStream_t s);

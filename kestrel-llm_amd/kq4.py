@@ -74,6 +74,17 @@ SIGNATURES = [
     ("kq4_attn_workspace_bytes", ctypes.c_size_t, [_I] * 8),
     ("kq4_logprobs_dev", _I, [_P, _P, _P, _P, _P, ctypes.c_long, _P, _I, _I, _I, _P]),
     ("kq4_logprobs_workspace_bytes", ctypes.c_size_t, [_I, _I, _I]),
+    ("kq4_mx_bytes", ctypes.c_size_t, [_I, _I, _I]),
+    ("kq4_mx_quantize_dev", _I, [_P, _P, ctypes.c_long, _I, _I, _I, _P]),
+    ("kq4_mx_pack_dev", _I, [_P, _P, _P, _I, _I, _I, _P]),
+    ("kq4_mx_unpack_dev", _I, [_P, _P, _P, _I, _I, _I, _P]),
+    ("kq4_mx_matmul_dev", _I, [_P, ctypes.c_long, _P, ctypes.c_long, _P, _P, _I, _I, _I, _I, _P]),
+    ("kq4_mx_matmul_q_dev", _I, [_P, ctypes.c_long, _P, _P, _P, _I, _I, _I, _I, _P]),
+    ("kq4_mx_gated_dev", _I, [_P, ctypes.c_long, _P, ctypes.c_long, _P, _P, _I, _I, _I, _I, _P]),
+    ("kq4_mx_ffn_dev", _I,
+     [_P, ctypes.c_long, _P, ctypes.c_long, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    ("kq4_mx_workspace_bytes", ctypes.c_size_t, [_I, _I]),
+    ("kq4_mx_ffn_workspace_bytes", ctypes.c_size_t, [_I, _I, _I]),
     # C11 op wrappers (include/kq4_ops.h)
     ("kq4_dyn_matvec_q4_q8", _I, [_P, _P, _P, _I, _I]),
     ("kq4_dyn_matvec_q4_q8_fused_gate_up", _I, [_P, _P, _P, _P, _P, _I, _I]),
@@ -895,3 +906,132 @@ def logprobs_dev(logits, token=None, logprob=None, entropy=None, top_logprob=Non
     check(lib().kq4_logprobs_dev(_tp(logprob), _tp(entropy), _tp(top_logprob), _tp(top_id),
                                  logits.data_ptr(), ld, _tp(token), n, vocab, n_top,
                                  _stream_ptr(stream)), "kq4_logprobs_dev")
+
+
+# ---- microscaled matrices ------------------------------------------------------------------------
+
+MX_FP4, MX_FP6 = 4, 6
+
+
+class MX:
+    """A microscaled matrix of rows x cols of 4 or 6 bits (include/kq4.h kq4_mx_bytes): `data`, its uint8 tensor, new
+    or given, checked once. Weights are packed into one as a model is loaded (mx_pack_dev), activations quantized
+    into one that the program keeps (mx_quantize_dev)."""
+
+    def __init__(self, rows, cols, type, data=None, device="cuda"):
+        import torch
+        n = lib().kq4_mx_bytes(rows, cols, type)
+        if n == 0:
+            raise KQ4Error(f"bad microscaled matrix: {rows} x {cols} of {type} bits")
+        if data is None:
+            data = torch.empty(n, dtype=torch.uint8, device=device)
+        _need(data, "data", torch.uint8, n)
+        self.data, self.rows, self.cols, self.type = data, rows, cols, type
+        self.device, self.p = data.get_device(), data.data_ptr()
+
+
+def mx_workspace_bytes(n, cols):
+    return lib().kq4_mx_workspace_bytes(n, cols)
+
+
+def mx_ffn_workspace_bytes(n, dim, ffn):
+    return lib().kq4_mx_ffn_workspace_bytes(n, dim, ffn)
+
+
+def mx_quantize_dev(m, x, stream=None):
+    """fp32 x [rows][cols] (unit column stride) into the microscaled matrix m."""
+    ldx = _rows(x, "x", m.rows, m.cols, m.device)
+    _check_here(m.device, "m")
+    check(lib().kq4_mx_quantize_dev(m.p, x.data_ptr(), ldx, m.rows, m.cols, m.type, _stream_ptr(stream)),
+          "kq4_mx_quantize_dev")
+
+
+def _mx_row_major(m, codes, scales):
+    import torch
+    _need_on(codes, "codes", torch.uint8, m.device, m.rows * m.cols * m.type // 8)
+    _need_on(scales, "scales", torch.uint8, m.device, m.rows * m.cols // 32)
+    _check_here(m.device, "m")
+
+
+def mx_pack_dev(m, codes, scales, stream=None):
+    """A checkpoint's row-major codes and scales (uint8) into the microscaled matrix m."""
+    _mx_row_major(m, codes, scales)
+    check(lib().kq4_mx_pack_dev(m.p, codes.data_ptr(), scales.data_ptr(), m.rows, m.cols, m.type,
+                                _stream_ptr(stream)), "kq4_mx_pack_dev")
+
+
+def mx_unpack_dev(codes, scales, m, stream=None):
+    """The microscaled matrix m into row-major codes and scales (uint8)."""
+    _mx_row_major(m, codes, scales)
+    check(lib().kq4_mx_unpack_dev(codes.data_ptr(), scales.data_ptr(), m.p, m.rows, m.cols, m.type,
+                                  _stream_ptr(stream)), "kq4_mx_unpack_dev")
+
+
+def _mx_w(w, name, rows, cols, device):
+    """Raises unless w is a 4-bit matrix of rows x cols (None: any) on `device`."""
+    if not isinstance(w, MX) or w.type != MX_FP4 or (rows is not None and w.rows != rows) or w.cols != cols:
+        raise KQ4Error(f"{name}: expected a 4-bit MX of {rows} x {cols}, got "
+                       + (f"{w.rows} x {w.cols} of {w.type} bits" if isinstance(w, MX) else repr(type(w))))
+    if w.device != device:
+        raise KQ4Error(f"{name}: on device {w.device}, expected {device}")
+
+
+def _mx_out(out, residual, n, rows, device):
+    """The row stride that out and residual share."""
+    ldo = _rows(out, "out", n, rows, device)
+    if residual is not None:
+        ldr = _rows(residual, "residual", n, rows, device)
+        if n > 1 and ldr != ldo:
+            raise KQ4Error(f"residual: row stride {ldr}, out has {ldo}")
+    return ldo
+
+
+def _mx_x(x, cols, device):
+    if getattr(x, "ndim", 0) != 2:
+        raise KQ4Error(f"x: expected a [n, {cols}] device tensor")
+    n = x.shape[0]
+    return n, _rows(x, "x", n, cols, device)
+
+
+def mx_matmul_dev(out, x, w, act=MX_FP6, residual=None, stream=None):
+    """out [n][w.rows] = [residual +] W . x for fp32 x [n][w.cols], quantized to `act` bits on the way."""
+    _mx_w(w, "w", None, w.cols if isinstance(w, MX) else 0, w.device if isinstance(w, MX) else None)
+    n, ldx = _mx_x(x, w.cols, w.device)
+    ldo = _mx_out(out, residual, n, w.rows, w.device)
+    _check_here(w.device, "w")
+    check(lib().kq4_mx_matmul_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), w.p, w.rows, w.cols, n, act,
+                                  _stream_ptr(stream)), "kq4_mx_matmul_dev")
+
+
+def mx_matmul_q_dev(out, xq, w, residual=None, stream=None):
+    """The same from activations that are quantized already (an MX of n x w.cols)."""
+    if not isinstance(xq, MX):
+        raise KQ4Error("xq: expected an MX")
+    _mx_w(w, "w", None, xq.cols, xq.device)
+    ldo = _mx_out(out, residual, xq.rows, w.rows, w.device)
+    _check_here(w.device, "w")
+    check(lib().kq4_mx_matmul_q_dev(out.data_ptr(), ldo, xq.p, _tp(residual), w.p, w.rows, w.cols, xq.rows, xq.type,
+                                    _stream_ptr(stream)), "kq4_mx_matmul_q_dev")
+
+
+def mx_gated_dev(out, x, gate, up, act=MX_FP6, stream=None):
+    """out [n][gate.rows] = silu(gate . x) * (up . x) for fp32 x [n][gate.cols]."""
+    _mx_w(gate, "gate", None, gate.cols if isinstance(gate, MX) else 0, gate.device if isinstance(gate, MX) else None)
+    _mx_w(up, "up", gate.rows, gate.cols, gate.device)
+    n, ldx = _mx_x(x, gate.cols, gate.device)
+    ldo = _mx_out(out, None, n, gate.rows, gate.device)
+    _check_here(gate.device, "gate")
+    check(lib().kq4_mx_gated_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, gate.p, up.p, gate.rows, gate.cols, n, act,
+                                 _stream_ptr(stream)), "kq4_mx_gated_dev")
+
+
+def mx_ffn_dev(out, x, gate, up, down, act=MX_FP6, residual=None, stream=None):
+    """out [n][dim] = [residual +] down . (silu(gate . x) * (up . x)), gate and up [ffn][dim], down [dim][ffn]."""
+    _mx_w(gate, "gate", None, gate.cols if isinstance(gate, MX) else 0, gate.device if isinstance(gate, MX) else None)
+    _mx_w(up, "up", gate.rows, gate.cols, gate.device)
+    _mx_w(down, "down", gate.cols, gate.rows, gate.device)
+    n, ldx = _mx_x(x, gate.cols, gate.device)
+    ldo = _mx_out(out, residual, n, gate.cols, gate.device)
+    _check_here(gate.device, "gate")
+    check(lib().kq4_mx_ffn_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), gate.p, up.p, down.p, gate.cols,
+                               gate.rows, n, act, _stream_ptr(stream)), "kq4_mx_ffn_dev")
