@@ -498,8 +498,8 @@ size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top);
 #define KQ4_MX_FP4 4
 #define KQ4_MX_FP6 6
 
-/* A microscaled matrix of rows x cols (cols % 32 == 0; fewer than 2^24 tiles of 16 rows x 512
- * columns, rows <= 2^24) is kq4_mx_bytes bytes, 16-byte aligned; 0 for a bad shape. First the codes
+/* A microscaled matrix of rows x cols (cols % 32 == 0, cols <= 2^20, rows <= 2^24; fewer than
+ * 2^24 tiles of 16 rows x 512 columns) is kq4_mx_bytes bytes, 16-byte aligned; 0 for a bad shape. First the codes
  * in tiles of 16 rows x 128 columns: a block's elements lie one after the other, the first in the
  * lowest bits, in 16 (FP4) or 24 (FP6) bytes, and a tile is [4 blocks][16 rows][the first 16 bytes],
  * then for FP6 [4 blocks][16 rows][the last 8]. Groups of 8 row tiles (the last one of

@@ -1396,14 +1396,14 @@ size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top) {
 namespace {
 
 bool mx_shape_ok(int rows, int cols, int type) {
-  if (rows < 1 || rows > 1 << 24 || cols < 32 || cols % 32 || (type != KQ4_MX_FP4 && type != KQ4_MX_FP6)) return false;
+  if (rows < 1 || rows > 1 << 24 || cols < 32 || cols > 1 << 20 || cols % 32 || (type != KQ4_MX_FP4 && type != KQ4_MX_FP6)) return false;
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   return (long long)d.nt * d.kq < 1 << 24;   // (2^32 threads)
 }
 
 int mx_matrix_check(const char *what, const char *name, const void *m, int rows, int cols, int type) {
   if (!mx_shape_ok(rows, cols, type))
-    return fail(KQ4_EINVAL, "%s: %s of rows=%d (1..2^24) cols=%d (%%32) type=%d (4 or 6), fewer than 2^24 tiles of "
+    return fail(KQ4_EINVAL, "%s: %s of rows=%d (1..2^24) cols=%d (%%32, at most 2^20) type=%d (4 or 6), fewer than 2^24 tiles of "
                 "16 x 512", what, name, rows, cols, type);
   if (!m || (uintptr_t)m % 16) return fail(KQ4_EINVAL, "%s: %s must be 16-byte aligned", what, name);
   return KQ4_OK;
@@ -1434,6 +1434,8 @@ int mx_product_check(const char *what, const float *out, long ldo, const float *
   } else if ((rc = mx_matrix_check(what, "xq", xq, n, cols, act))) {
     return rc;
   }
+  if ((long long)((rows + 127) / 128) * ((n + 63) / 64) >= 1 << 24)   // (2^32 threads)
+    return fail(KQ4_EINVAL, "%s: n_batch=%d rows=%d", what, n, rows);
   if (!out || (uintptr_t)out % 4 || (uintptr_t)residual % 4 || ldo < rows)
     return fail(KQ4_EINVAL, "%s: out and residual must be 4-byte aligned, their stride (%ld) at least %d", what, ldo, rows);
   if (x && rows_overlap(out, ldo, rows, n, x, ldx, cols, n)) return fail(KQ4_EINVAL, "%s: out overlaps x", what);
@@ -1460,6 +1462,10 @@ KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, con
   return a;
 }
 
+int mx_launch(const KQ4MxArgs &a, int type, hipStream_t s) {
+  return a.n > 64 ? kq4_launch_mx_gemm(a, type, s) : kq4_launch_mx_rows(a, type, s);
+}
+
 // x (or xq) through W (w0; with w1 the gated pair), everything checked.
 int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq, const float *residual,
                const uint8_t *w0, const uint8_t *w1, int rows, int cols, int n, int act, hipStream_t s) {
@@ -1472,7 +1478,7 @@ int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq
     KQ4_HIP((hipError_t)kq4_launch_mx_quantize(q, x, ldx, n, cols, act, s));
     xq = q;
   }
-  KQ4_HIP((hipError_t)kq4_launch_mx_rows(mx_args(out, ldo, residual, w0, w1, xq, rows, cols, n), act, s));
+  KQ4_HIP((hipError_t)mx_launch(mx_args(out, ldo, residual, w0, w1, xq, rows, cols, n), act, s));
   return KQ4_OK;
 }
 
@@ -1560,9 +1566,9 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
   uint8_t *xq = c.take<uint8_t>(mx_bytes(n_batch, dim, act)), *hq = c.take<uint8_t>(mx_bytes(n_batch, ffn, act));
   float *h = c.take<float>((size_t)n_batch * ffn);
   KQ4_HIP((hipError_t)kq4_launch_mx_quantize(xq, x, ldx, n_batch, dim, act, s));
-  KQ4_HIP((hipError_t)kq4_launch_mx_rows(mx_args(h, ffn, nullptr, gate, up, xq, ffn, dim, n_batch), act, s));
+  KQ4_HIP((hipError_t)mx_launch(mx_args(h, ffn, nullptr, gate, up, xq, ffn, dim, n_batch), act, s));
   KQ4_HIP((hipError_t)kq4_launch_mx_quantize(hq, h, ffn, n_batch, ffn, act, s));
-  KQ4_HIP((hipError_t)kq4_launch_mx_rows(mx_args(out, ldo, residual, down, nullptr, hq, dim, ffn, n_batch), act, s));
+  KQ4_HIP((hipError_t)mx_launch(mx_args(out, ldo, residual, down, nullptr, hq, dim, ffn, n_batch), act, s));
   return KQ4_OK;
 }
 

@@ -229,3 +229,4 @@ struct KQ4MxArgs {
   KQ4MxDims dw, dx;
 };
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, hipStream_t s);
+int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, hipStream_t s);

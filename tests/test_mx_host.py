@@ -45,7 +45,7 @@ def launched(f):
     "matmul(w=at(4) + 8)", "matmul(rows=0, ldo=0)", "matmul(rows=-4)", "matmul(cols=33, ldx=36)", "matmul(n=-1)",
     "matmul(n=(1 << 24) + 1)", "matmul(act=5)", "matmul(act=0)", "matmul(act=16)", "matmul(out=at(2))", "matmul(out=at(2) + 16)",
     "matmul(out=at(2) + 4 * 300, ldo=512)", "matmul(res=at(1) + 4)", "matmul(res=at(1) + 4 * 300)",
-    "matmul_q(xq=None)", "matmul_q(xq=at(2) + 8)", "matmul_q(out=None)", "matmul_q(act=3)", "matmul_q(w=None)", "matmul_q(n=-5)",
+    "matmul(n=1 << 20, rows=1 << 24, ldo=1 << 24, cols=32, ldx=32, res=None)", "matmul_q(xq=None)", "matmul_q(xq=at(2) + 8)", "matmul_q(out=None)", "matmul_q(act=3)", "matmul_q(w=None)", "matmul_q(n=-5)",
     "matmul_q(ldo=10)", "matmul_q(res=at(1) + 4)",
     "gated(gate=None)", "gated(up=None)", "gated(gate=at(3) + 4)", "gated(up=at(4) + 4)", "gated(out=None)", "gated(x=None)",
     "gated(ldo=200)", "gated(out=at(2) + 64)", "gated(n=-1)", "gated(act=9)", "gated(rows=0)", "gated(cols=0)",

@@ -85,7 +85,7 @@ def test_kq4_mx_bytes(kq4_cpu):
         for bits in (4, 6):
             assert f(rows, cols, bits) == nt * kt * 256 * bits + nt * kq * 256
     for bad in ((0, 32, 4), (-1, 32, 4), (1, 0, 4), (1, 31, 4), (1, 48, 6), (1, 32, 8), (1, -32, 4), (1 << 25, 32, 4),
-                (1 << 24, 16384, 4), ((1 << 31) - 1, 1 << 30, 6)):
+                (1 << 24, 16384, 4), (16, (1 << 20) + 32, 4), ((1 << 31) - 1, 1 << 30, 6)):
         assert f(*bad) == 0
         with pytest.raises(kq4_cpu.KQ4Error):
             kq4_cpu.MX(*bad, device="cpu")
