@@ -201,26 +201,43 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
 #undef KQ4_MX_PRODUCTS
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the loads past the last stage: LDS is not given back before
 
+  // The residual's loads of 32 tokens are all on their way before the first of them is waited for (it may be out: an
+  // element is read and written by one lane). Past the edges they read the last row's or column's, which is not stored.
+  const bool inside = m0 + T::BM <= a.n && n0 + RG <= a.rows;
+  const int c0 = n0 + 32 * (TJ / G) * wn + l32;
 #pragma unroll
-  for (int i = 0; i < TI; ++i)
+  for (int i = 0; i < TI; ++i) {
+    const int t0 = m0 + 32 * (TI * wm + i) + 4 * half;
+    float y[16][TJ / G];
+    if (a.res) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int tok = m0 + 32 * (TI * wm + i) + 8 * (e >> 2) + 4 * half + (e & 3);
-      if (tok < a.n) {
-        float *o = a.out + (size_t)tok * a.ldo;
-        const float *res = a.res ? a.res + (size_t)tok * a.ldo : nullptr;
+      for (int e = 0; e < 16; ++e) {
+        const float *r = a.res + (size_t)min(t0 + 8 * (e >> 2) + (e & 3), a.n - 1) * a.ldo;
 #pragma unroll
-        for (int j = 0; j < TJ / G; ++j) {
-          const int row = n0 + 32 * (TJ / G * wn + j) + l32;
-          if (row < a.rows) {
-            float y = acc[i][j][e];
-            if constexpr (G == 2) y = kq4_mx_gate(y, acc[i][TJ / 2 + j][e]);
-            if (res) y += res[row];
-            o[row] = y;
-          }
-        }
+        for (int j = 0; j < TJ / G; ++j) y[e][j] = r[min(c0 + 32 * j, a.rows - 1)];
       }
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+      for (int j = 0; j < TJ / G; ++j) {
+        const float p = G == 2 ? kq4_mx_gate(acc[i][j][e], acc[i][G == 2 ? TJ / 2 + j : j][e]) : acc[i][j][e];
+        y[e][j] = a.res ? p + y[e][j] : p;
+      }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int tok = t0 + 8 * (e >> 2) + (e & 3);
+      float *o = a.out + (size_t)tok * a.ldo + c0;
+      if (inside) {
+#pragma unroll
+        for (int j = 0; j < TJ / G; ++j) o[32 * j] = y[e][j];
+      } else if (tok < a.n) {
+#pragma unroll
+        for (int j = 0; j < TJ / G; ++j)
+          if (c0 + 32 * j < a.rows) o[32 * j] = y[e][j];
+      }
+    }
+  }
 }
 
 template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC>
