@@ -1452,18 +1452,26 @@ KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, con
   a.w[0] = w0;
   a.w[1] = w1;
   a.x = xq;
+  a.xf = nullptr;
+  a.ldx = 0;
   a.out = out;
   a.res = res;
   a.ldo = ldo;
   a.rows = rows;
+  a.cols = cols;
   a.n = n;
   a.dw = kq4_mx_dims(rows, cols);
   a.dx = kq4_mx_dims(n, cols);
   return a;
 }
 
-int mx_launch(const KQ4MxArgs &a, int type, hipStream_t s) {
-  return a.n > 64 ? kq4_launch_mx_gemm(a, type, s) : kq4_launch_mx_rows(a, type, s);
+int mx_launch(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
+  return a.n > 64 ? kq4_launch_mx_gemm(a, type, s) : kq4_launch_mx_rows(a, type, ncu, s);
+}
+
+// Whether the rows kernel quantizes the activations itself.
+bool mx_fused(int n, int cols, int type) {
+  return n <= 16 && n * (long)cols <= 16384 && kq4_mx_rows_lds(n, kq4_mx_dims(n, cols), type) <= 64 * 1024;
 }
 
 // x (or xq) through W (w0; with w1 the gated pair), everything checked.
@@ -1472,13 +1480,17 @@ int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq
   DevState *ds = nullptr;
   int rc = cur_dev(&ds);
   if (rc) return rc;
-  if (!xq) {
+  KQ4MxArgs a = mx_args(out, ldo, residual, w0, w1, xq, rows, cols, n);
+  if (!xq && mx_fused(n, cols, act)) {
+    a.xf = x;
+    a.ldx = ldx;
+  } else if (!xq) {
     if ((rc = ensure_ws(Ws{&ds->ws, ds}, mx_bytes(n, cols, act), s))) return rc;
     uint8_t *q = static_cast<uint8_t *>(ds->ws.p);
     KQ4_HIP((hipError_t)kq4_launch_mx_quantize(q, x, ldx, n, cols, act, s));
-    xq = q;
+    a.x = q;
   }
-  KQ4_HIP((hipError_t)mx_launch(mx_args(out, ldo, residual, w0, w1, xq, rows, cols, n), act, s));
+  KQ4_HIP((hipError_t)mx_launch(a, act, ds->ncu, s));
   return KQ4_OK;
 }
 
@@ -1566,9 +1578,9 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
   uint8_t *xq = c.take<uint8_t>(mx_bytes(n_batch, dim, act)), *hq = c.take<uint8_t>(mx_bytes(n_batch, ffn, act));
   float *h = c.take<float>((size_t)n_batch * ffn);
   KQ4_HIP((hipError_t)kq4_launch_mx_quantize(xq, x, ldx, n_batch, dim, act, s));
-  KQ4_HIP((hipError_t)mx_launch(mx_args(h, ffn, nullptr, gate, up, xq, ffn, dim, n_batch), act, s));
+  KQ4_HIP((hipError_t)mx_launch(mx_args(h, ffn, nullptr, gate, up, xq, ffn, dim, n_batch), act, ds->ncu, s));
   KQ4_HIP((hipError_t)kq4_launch_mx_quantize(hq, h, ffn, n_batch, ffn, act, s));
-  KQ4_HIP((hipError_t)mx_launch(mx_args(out, ldo, residual, down, nullptr, hq, dim, ffn, n_batch), act, s));
+  KQ4_HIP((hipError_t)mx_launch(mx_args(out, ldo, residual, down, nullptr, hq, dim, ffn, n_batch), act, ds->ncu, s));
   return KQ4_OK;
 }
 

@@ -221,12 +221,15 @@ int kq4_launch_mx_pack(uint8_t *m, uint8_t *codes, uint8_t *scales, int rows, in
                        hipStream_t s);
 struct KQ4MxArgs {
   const uint8_t *w[2];   // weights; the second one, where there is one, is the gated block's up projection
-  const uint8_t *x;
+  const uint8_t *x;      // a quantized matrix, or with xf (rows kernel) nullptr
+  const float *xf;       // fp32 rows that the kernel quantizes itself, row t at t * ldx
+  long ldx;
   float *out;            // token t's outputs at t * ldo
   const float *res;      // at the same stride, or nullptr
   long ldo;
-  int rows, n;
+  int rows, cols, n;
   KQ4MxDims dw, dx;
 };
-int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, hipStream_t s);
+size_t kq4_mx_rows_lds(int n, const KQ4MxDims &d, int type);   // of the rows kernel with xf
+int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s);
 int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, hipStream_t s);

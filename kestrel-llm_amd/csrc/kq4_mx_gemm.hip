@@ -162,6 +162,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
   _Pragma("unroll") for (int i = 0; i < TI; ++i) _Pragma("unroll") for (int j = 0; j < TJ; ++j) acc[i][j] =      \
       __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[H][i], fb[H][j], acc[i][j], kq4_mx_fmt<TYPE>, 4, J,      \
                                                       (int)sa[H][i], J, (int)sb[H][j]);
+// products and LDS reads in turn: reads issued in a row hold the matrix unit up
+#define KQ4_MX_INTERLEAVE                                                                                         \
+  _Pragma("unroll") for (int z = 0; z < TI + TJ; ++z) {                                                           \
+    __builtin_amdgcn_sched_group_barrier(0x8, TI * TJ / (TI + TJ), 0);                                            \
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                                            \
+  }
 
   load_scales(0);
 #pragma unroll
@@ -178,6 +184,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
     const int next = slot + 1 == S ? 0 : slot + 1;
     read(1, slot);
     KQ4_MX_PRODUCTS(0, J)
+    KQ4_MX_INTERLEAVE
     __builtin_amdgcn_sched_barrier(0);
     // this wave's part of the next stage has come, and its reads of this one are done
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * T::LPW) : "memory");
@@ -188,6 +195,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
     read(0, next);
     if constexpr (J == 3) read_scales();
     KQ4_MX_PRODUCTS(1, J)
+    KQ4_MX_INTERLEAVE
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (J == 3) take_scales();
     slot = next;
@@ -199,6 +207,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
     if (k + 3 < nk) stage(k + 3, std::integral_constant<int, 3>{});
   }
 #undef KQ4_MX_PRODUCTS
+#undef KQ4_MX_INTERLEAVE
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the loads past the last stage: LDS is not given back before
 
   // The residual's loads of 32 tokens are all on their way before the first of them is waited for (it may be out: an
