@@ -139,8 +139,10 @@ const char *kq4_version(void);
  * falling with progress through K, so the workgroups sharing a CU end together: 0 off, 1 on,
  * -1 the planner's choice: token-major, on for 128x128 launches of whole rounds of two workgroups
  * per CU and for every 64x128 launch; on records, on; the same outputs), attn_tile (the attention's
- * form: 16, 128 or 256 rows a workgroup, 0 the planner's choice) and attn_split (ranges of a
- * sequence's keys, 0 the planner's choice; both within the rounding of the sums). The initial value
+ * form: 16, 128 or 256 rows a workgroup, 0 the planner's choice), attn_split (ranges of a
+ * sequence's keys, 0 the planner's choice), mx_form (microscaled products: 1 the rows kernel, 2 the
+ * GEMM, 0 the planner's choice) and mx_split (K slices of that GEMM, 0 the planner's choice; all of these
+ * within the rounding of the sums). The initial value
  * of each comes from the environment variable KQ4_ + its upper-case name, else the built-in
  * default (for most, the planner's own choice); value < 0 restores that initial value. Takes
  * effect for launches planned after it returns. */
@@ -554,7 +556,9 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
                    int n_batch, int act, void *stream);
 
 /* Workspace bytes that hold every product and gated call of up to n_batch tokens and cols columns
- * (whatever its rows and act), and every whole block of up to these sizes; 0 for a bad shape. */
+ * (whatever its rows and act), and every whole block of up to these sizes; 0 for a bad shape. From
+ * 17 tokens on they include 32 MiB for the sums of a split K (the planner's splits never need more;
+ * one forced through mx_split may). */
 size_t kq4_mx_workspace_bytes(int n_batch, int cols);
 size_t kq4_mx_ffn_workspace_bytes(int n_batch, int dim, int ffn);
 

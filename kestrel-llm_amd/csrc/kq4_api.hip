@@ -10,6 +10,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <unordered_map>
@@ -214,7 +215,7 @@ int env_int(const char *name, int dflt) {
 enum OptId {
   kGemvKind, kGemvMfmaFrom, kGemvHs, kGemvRps, kGemvWaves, kGemvWpcu, kGemvMaxw,
   kGemvFq, kGemvFqWork, kGemvSiluFqWork, kGemvChunkMax, kGemmKind, kGemmTile, kGemmSplit,
-  kGemmPrio, kAttnTile, kAttnSplit, kOptCount
+  kGemmPrio, kAttnTile, kAttnSplit, kMxForm, kMxSplit, kOptCount
 };
 struct OptDef {
   const char *name, *env;
@@ -231,6 +232,7 @@ const OptDef kOpts[kOptCount] = {
     {"gemm_kind", "KQ4_GEMM_KIND", -1},          {"gemm_tile", "KQ4_GEMM_TILE", 0},
     {"gemm_split", "KQ4_GEMM_SPLIT", -1},        {"gemm_prio", "KQ4_GEMM_PRIO", -1},
     {"attn_tile", "KQ4_ATTN_TILE", 0},           {"attn_split", "KQ4_ATTN_SPLIT", 0},
+    {"mx_form", "KQ4_MX_FORM", 0},               {"mx_split", "KQ4_MX_SPLIT", 0},
 };
 std::atomic<int> g_opt[kOptCount];
 int g_opt_init[kOptCount];   // each option's value at load: its environment variable or default
@@ -1457,6 +1459,8 @@ KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, con
   a.out = out;
   a.res = res;
   a.ldo = ldo;
+  a.part = nullptr;
+  a.q = nullptr;
   a.rows = rows;
   a.cols = cols;
   a.n = n;
@@ -1465,13 +1469,35 @@ KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, con
   return a;
 }
 
-int mx_launch(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
-  return a.n > 64 ? kq4_launch_mx_gemm(a, type, s) : kq4_launch_mx_rows(a, type, ncu, s);
-}
-
-// Whether the rows kernel quantizes the activations itself.
+// Whether the rows kernel quantizes the activations itself, every workgroup all of them: 16384 elements take it less than
+// a launch of the quantizer (3.2 us and its gap).
 bool mx_fused(int n, int cols, int type) {
   return n <= 16 && n * (long)cols <= 16384 && kq4_mx_rows_lds(n, kq4_mx_dims(n, cols), type) <= 64 * 1024;
+}
+
+KQ4MxPlan mx_plan(DevState *ds, int n, int rows, int cols, int matrices, int act) {
+  return kq4_mx_plan(n, rows, cols, matrices, act, ds->ncu, opt(kMxForm), opt(kMxSplit));
+}
+
+// Bytes of a product's activations in the workspace, 0 where the rows kernel quantizes them.
+size_t mx_x_bytes(const KQ4MxPlan &p, int n, int cols, int act) {
+  return !p.gemm && mx_fused(n, cols, act) ? 0 : mx_bytes(n, cols, act);
+}
+
+// A product as planned, from fp32 rows x (quantized into xq where the kernel does not do that) or, without, from xq; its
+// partial sums in part.
+int mx_run(DevState *ds, const KQ4MxPlan &p, KQ4MxArgs a, const float *x, long ldx, uint8_t *xq, float *part, int act,
+           hipStream_t s) {
+  if (x && !mx_x_bytes(p, a.n, a.cols, act)) {
+    a.xf = x;
+    a.ldx = ldx;
+  } else {
+    if (x) KQ4_HIP((hipError_t)kq4_launch_mx_quantize(xq, x, ldx, a.n, a.cols, act, s));
+    a.x = xq;
+  }
+  a.part = part;
+  KQ4_HIP((hipError_t)(p.gemm ? kq4_launch_mx_gemm(a, act, p.ksplit, ds->ncu, s) : kq4_launch_mx_rows(a, act, ds->ncu, s)));
+  return KQ4_OK;
 }
 
 // x (or xq) through W (w0; with w1 the gated pair), everything checked.
@@ -1480,18 +1506,13 @@ int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq
   DevState *ds = nullptr;
   int rc = cur_dev(&ds);
   if (rc) return rc;
-  KQ4MxArgs a = mx_args(out, ldo, residual, w0, w1, xq, rows, cols, n);
-  if (!xq && mx_fused(n, cols, act)) {
-    a.xf = x;
-    a.ldx = ldx;
-  } else if (!xq) {
-    if ((rc = ensure_ws(Ws{&ds->ws, ds}, mx_bytes(n, cols, act), s))) return rc;
-    uint8_t *q = static_cast<uint8_t *>(ds->ws.p);
-    KQ4_HIP((hipError_t)kq4_launch_mx_quantize(q, x, ldx, n, cols, act, s));
-    a.x = q;
-  }
-  KQ4_HIP((hipError_t)mx_launch(a, act, ds->ncu, s));
-  return KQ4_OK;
+  const int matrices = w1 ? 2 : 1;
+  const KQ4MxPlan p = mx_plan(ds, n, rows, cols, matrices, act);
+  const size_t xb = x ? mx_x_bytes(p, n, cols, act) : 0, pb = kq4_mx_part_bytes(n, rows, matrices, p.ksplit);
+  if (xb + pb && (rc = ensure_ws(Ws{&ds->ws, ds}, xb + pb, s))) return rc;
+  uint8_t *ws = static_cast<uint8_t *>(ds->ws.p);
+  return mx_run(ds, p, mx_args(out, ldo, residual, w0, w1, nullptr, rows, cols, n), x, ldx,
+                x ? ws : const_cast<uint8_t *>(xq), reinterpret_cast<float *>(ws + xb), act, s);
 }
 
 }  // namespace
@@ -1573,24 +1594,30 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;
   hipStream_t s = (hipStream_t)stream;
-  if ((rc = ensure_ws(Ws{&ds->ws, ds}, kq4_mx_ffn_workspace_bytes(n_batch, dim, ffn), s))) return rc;
-  Carve c{static_cast<char *>(ds->ws.p)};
-  uint8_t *xq = c.take<uint8_t>(mx_bytes(n_batch, dim, act)), *hq = c.take<uint8_t>(mx_bytes(n_batch, ffn, act));
-  float *h = c.take<float>((size_t)n_batch * ffn);
-  KQ4_HIP((hipError_t)kq4_launch_mx_quantize(xq, x, ldx, n_batch, dim, act, s));
-  KQ4_HIP((hipError_t)mx_launch(mx_args(h, ffn, nullptr, gate, up, xq, ffn, dim, n_batch), act, ds->ncu, s));
-  KQ4_HIP((hipError_t)kq4_launch_mx_quantize(hq, h, ffn, n_batch, ffn, act, s));
-  KQ4_HIP((hipError_t)mx_launch(mx_args(out, ldo, residual, down, nullptr, hq, dim, ffn, n_batch), act, ds->ncu, s));
-  return KQ4_OK;
+  const KQ4MxPlan pg = mx_plan(ds, n_batch, ffn, dim, 2, act), pd = mx_plan(ds, n_batch, dim, ffn, 1, act);
+  const bool direct = pg.gemm && pg.ksplit == 1;   // h leaves the gated kernel quantized
+  const size_t xb = mx_x_bytes(pg, n_batch, dim, act), hb = direct ? mx_bytes(n_batch, ffn, act) : mx_x_bytes(pd, n_batch, ffn, act);
+  const size_t fb = direct ? 0 : al256((size_t)n_batch * ffn * sizeof(float));
+  const size_t pb = std::max(kq4_mx_part_bytes(n_batch, ffn, 2, pg.ksplit), kq4_mx_part_bytes(n_batch, dim, 1, pd.ksplit));
+  if ((rc = ensure_ws(Ws{&ds->ws, ds}, xb + hb + fb + pb, s))) return rc;
+  uint8_t *xq = static_cast<uint8_t *>(ds->ws.p), *hq = xq + xb;
+  float *h = reinterpret_cast<float *>(hq + hb), *part = reinterpret_cast<float *>(hq + hb + fb);
+  KQ4MxArgs g = mx_args(h, ffn, nullptr, gate, up, nullptr, ffn, dim, n_batch);
+  if (direct) g.q = hq;
+  if ((rc = mx_run(ds, pg, g, x, ldx, xq, part, act, s))) return rc;
+  return mx_run(ds, pd, mx_args(out, ldo, residual, down, nullptr, nullptr, dim, ffn, n_batch), direct ? nullptr : h, ffn,
+                hq, part, act, s);
 }
 
 size_t kq4_mx_workspace_bytes(int n_batch, int cols) {
-  return mx_shape_ok(n_batch, cols, KQ4_MX_FP6) ? mx_bytes(n_batch, cols, KQ4_MX_FP6) : 0;
+  if (!mx_shape_ok(n_batch, cols, KQ4_MX_FP6)) return 0;
+  return mx_bytes(n_batch, cols, KQ4_MX_FP6) + (n_batch > 16 ? (size_t)KQ4_MX_PART_MAX : 0);
 }
 
 size_t kq4_mx_ffn_workspace_bytes(int n_batch, int dim, int ffn) {
   if (!mx_shape_ok(n_batch, dim, KQ4_MX_FP6) || !mx_shape_ok(n_batch, ffn, KQ4_MX_FP6)) return 0;
-  return mx_bytes(n_batch, dim, KQ4_MX_FP6) + mx_bytes(n_batch, ffn, KQ4_MX_FP6) + al256((size_t)n_batch * ffn * sizeof(float));
+  return mx_bytes(n_batch, dim, KQ4_MX_FP6) + mx_bytes(n_batch, ffn, KQ4_MX_FP6) + al256((size_t)n_batch * ffn * sizeof(float)) +
+         (n_batch > 16 ? (size_t)KQ4_MX_PART_MAX : 0);
 }
 
 }  // extern "C"

@@ -227,9 +227,23 @@ struct KQ4MxArgs {
   float *out;            // token t's outputs at t * ldo
   const float *res;      // at the same stride, or nullptr
   long ldo;
+  float *part;           // the GEMM's sums by K slice
+  uint8_t *q;            // the GEMM of two matrices in one slice: where not nullptr, the outputs as a matrix of n x rows of the
+                         // activations' type, in place of out (tokens past n are not written)
   int rows, cols, n;
   KQ4MxDims dw, dx;
 };
 size_t kq4_mx_rows_lds(int n, const KQ4MxDims &d, int type);   // of the rows kernel with xf
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s);
-int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, hipStream_t s);
+// ksplit > 1 (as kq4_mx_split gives it): K in that many slices, each its own sums in part (kq4_mx_part_bytes), added in
+// slice order by a second launch.
+int kq4_mx_split(int kq, int want);
+size_t kq4_mx_part_bytes(int n, int rows, int matrices, int ksplit);
+int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, int ksplit, int ncu, hipStream_t s);
+// The form of a product (1: the GEMM, 0: the rows kernel) and the GEMM's K slices. force_form 1 / 2: the rows kernel / the
+// GEMM; force_split > 0: that many slices where K has them.
+#define KQ4_MX_PART_MAX (32u << 20)   // bytes of the planner's partial sums, at most
+struct KQ4MxPlan {
+  int gemm, ksplit;
+};
+KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu, int force_form, int force_split);

@@ -17,12 +17,14 @@ struct KQ4MxTile {
   static constexpr int TA = 256 * TYPE;                       // bytes of an activation tile (16 x 128)
   static constexpr int A = BM / 16 * TA, B = BN / 16 * 1024;  // a stage's operands
   static constexpr int STAGE = A + B;
-  static constexpr int LA = A / 1024 / NW, LB = B / 1024 / NW, LPW = LA + LB;   // a wave's loads
+  static constexpr int LA = (A / 1024 + NW - 1) / NW, LB = B / 1024 / NW, LPW = LA + LB;   // a wave's loads
   static constexpr int SCALES = (BM + BN) / 16 * KQ4_MX_STILE, SLOADS = SCALES / 1024;
   static constexpr int SPW = (SLOADS + NW - 1) / NW;
   static constexpr int LDS = S * STAGE + SCALES;
   // a wave's runs lie in one group of 8 row tiles, and (gated) in one matrix
-  static_assert(A % (1024 * NW) == 0 && B % (1024 * NW) == 0 && SLOADS % SPW == 0, "kq4_mx_gemm: runs per wave");
+  static_assert(B % (1024 * NW) == 0 && SLOADS % SPW == 0, "kq4_mx_gemm: runs per wave");
+  // the first run of a wave's activations (where there are not as many for each, the last waves bring the last ones)
+  static __device__ int first_a(int wave) { return wave * LA < A / 1024 - LA ? wave * LA : A / 1024 - LA; }
   static_assert(8 * TA % (LA * 1024) == 0 && 8 % LB == 0 && BM % 128 == 0 && BN % 256 == 0, "kq4_mx_gemm: groups");
   static_assert(LDS <= 160 * 1024, "kq4_mx_gemm: LDS");
 };
@@ -49,7 +51,7 @@ KQ4_DEV void kq4_mx_load(const kq4_rsrc4 &r, uint32_t v16, uint32_t soff, uint32
 }
 
 template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArgs a, int mtiles, int ntiles) {
+__global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArgs a, int mtiles, int ntiles, int ksplit, int per) {
   using T = KQ4MxTile<TYPE, TI, TJ, WM, WN, S>;
   constexpr int RG = T::BN / G;                 // output rows of the workgroup
   extern __shared__ __align__(16) uint8_t lds[];
@@ -57,8 +59,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
   const int wm = wave % WM, wn = wave / WM, l32 = lane & 31, half = lane >> 5;
 
   // XCD x works on a run of tiles, in bands of 8 tiles of tokens, so that what it reads at a time is shared
-  const int ntile = mtiles * ntiles, xcd = blockIdx.x & 7, q8 = ntile >> 3, r8 = ntile & 7;
-  const int v = xcd * q8 + (xcd < r8 ? xcd : r8) + (int)(blockIdx.x >> 3);
+  const int all = mtiles * ntiles * ksplit, xcd = blockIdx.x & 7, q8 = all >> 3, r8 = all & 7;
+  const int vs = xcd * q8 + (xcd < r8 ? xcd : r8) + (int)(blockIdx.x >> 3);
+  const int slice = vs / (mtiles * ntiles), v = vs - slice * (mtiles * ntiles);
   const int band = v / (8 * ntiles), bm = min(8, mtiles - 8 * band), u = v - band * 8 * ntiles;
   const int m0 = (8 * band + u % bm) * T::BM, n0 = (u / bm) * RG;
 
@@ -79,7 +82,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
     return r;
   };
   uint32_t step_a, step_b, step_s[T::SPW];
-  const kq4_rsrc4 ra = runs(a.x, dx, TYPE, false, m0 >> 4, wave * T::LA * 1024, step_a);
+  const kq4_rsrc4 ra = runs(a.x, dx, TYPE, false, m0 >> 4, T::first_a(wave) * 1024, step_a);
   constexpr int PER = T::B / G;                 // a stage's bytes of one weight matrix
   const int ob = wave * T::LB * 1024;
   const kq4_rsrc4 rb = runs(a.w[ob / PER], dw, 4, false, n0 >> 4, ob % PER, step_b);
@@ -93,14 +96,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)&lds[0];
   const uint32_t v16 = 16u * lane;
-  const int nk = dw.kt, nq = dw.kq;
+  // the slice's stages and groups of four
+  const int q0 = slice * per, nq = min(per, dw.kq - q0), nk = min(4 * per, dw.kt - 4 * q0);
   auto load_stage = [&](int k, int slot) {      // (past the last stage: that one again, not used)
-    const uint32_t kk = (uint32_t)min(k, nk - 1), to = lds0 + slot * T::STAGE;
-    kq4_mx_load<T::LA>(ra, v16, kk * step_a, to + wave * T::LA * 1024);
+    const uint32_t kk = (uint32_t)(4 * q0 + min(k, nk - 1)), to = lds0 + slot * T::STAGE;
+    kq4_mx_load<T::LA>(ra, v16, kk * step_a, to + T::first_a(wave) * 1024);
     kq4_mx_load<T::LB>(rb, v16, kk * step_b, to + T::A + wave * T::LB * 1024);
   };
   auto load_scales = [&](int q) {
-    const uint32_t qq = (uint32_t)min(q, nq - 1);
+    const uint32_t qq = (uint32_t)(q0 + min(q, nq - 1));
 #pragma unroll
     for (int l = 0; l < T::SPW; ++l)
       kq4_mx_load<1>(rs[l], v16, qq * step_s[l],
@@ -210,10 +214,72 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
 #undef KQ4_MX_INTERLEAVE
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the loads past the last stage: LDS is not given back before
 
+  const int c0 = n0 + 32 * (TJ / G) * wn + l32;
+  if (ksplit > 1) {   // the sums of a slice, [slice][matrix][token][row]
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int tok = m0 + 32 * (TI * wm + i) + 8 * (e >> 2) + 4 * half + (e & 3);
+        float *o = a.part + ((size_t)slice * G * a.n + tok) * a.rows + c0;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+          const int c = 32 * (j % (TJ / G));
+          if (tok < a.n && c0 + c < a.rows) o[(size_t)(j / (TJ / G)) * a.n * a.rows + c] = acc[i][j][e];
+        }
+      }
+    return;
+  }
+  if constexpr (G == 2)
+    if (a.q) {
+      // The gated product as the activations of the next one: 32 tokens of each wave at a time go through LDS, where a thread
+      // then finds a block of 32 columns. The workgroup's 128 columns are one column tile of the matrix.
+      constexpr int LD = 128 + 4;
+      static_assert(RG == 128 && 32 * WM * LD * 4 <= T::LDS, "kq4_mx_gemm: quantized outputs");
+      float *buf = reinterpret_cast<float *>(lds);
+      const KQ4MxDims dq = kq4_mx_dims(a.n, a.rows);
+      const int kt = n0 >> 7;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+          for (int j = 0; j < TJ / 2; ++j)
+            buf[(32 * wm + 8 * (e >> 2) + 4 * half + (e & 3)) * LD + 32 * (TJ / 2 * wn + j) + l32] =
+                kq4_mx_gate(acc[i][j][e], acc[i][TJ / 2 + j][e]);
+        __syncthreads();
+        for (int u = threadIdx.x; u < 32 * WM * 4; u += 64 * T::NW) {
+          const int row = u >> 2, b = u & 3, tok = m0 + 32 * (TI * (row >> 5) + i) + (row & 31);
+          if (tok >= a.n) continue;
+          float f[32];
+          uint32_t m = 0, o[TYPE] = {}, sc = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 x = *reinterpret_cast<const float4 *>(&buf[row * LD + 32 * b + 4 * k]);
+            f[4 * k] = x.x; f[4 * k + 1] = x.y; f[4 * k + 2] = x.z; f[4 * k + 3] = x.w;
+          }
+          if (n0 + 32 * b < a.rows) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) m = max(m, kq4_absbits(f[k]));
+            sc = kq4_mx_scale_byte(m, TYPE);
+            kq4_mx_encode<TYPE>(f, sc, o);
+          }
+          const int tile = tok >> 4;
+          const long at = kq4_mx_first(tile, dq.kt) + (long)kt * kq4_mx_step(tile, dq.nt);
+          kq4_mx_put<TYPE>(a.q + at * T::TA, b, tok & 15, o);
+          uint8_t *ps = a.q + kq4_mx_codes_size(dq, TYPE) +
+                        (kq4_mx_first(tile, dq.kq) + (long)(kt >> 2) * kq4_mx_step(tile, dq.nt)) * KQ4_MX_STILE;
+          ps[kq4_mx_scale_at(4 * (kt & 3) + b, tok & 15)] = (uint8_t)sc;
+          if (kt == dq.kt - 1)   // the column tiles that the scales' last tile has and the codes do not
+            for (int k = (kt & 3) + 1; k < 4; ++k) ps[kq4_mx_scale_at(4 * k + b, tok & 15)] = 0;
+        }
+      }
+      return;
+    }
   // The residual's loads of 32 tokens are all on their way before the first of them is waited for (it may be out: an
   // element is read and written by one lane). Past the edges they read the last row's or column's, which is not stored.
   const bool inside = m0 + T::BM <= a.n && n0 + RG <= a.rows;
-  const int c0 = n0 + 32 * (TJ / G) * wn + l32;
 #pragma unroll
   for (int i = 0; i < TI; ++i) {
     const int t0 = m0 + 32 * (TI * wm + i) + 4 * half;
@@ -249,19 +315,114 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
   }
 }
 
+// out = [res +] the slices' sums in slice order (gated: of both matrices). A thread four outputs of a token, 256 apart,
+// with the loads of four slices on their way at a time.
+template <int G>
+__global__ __launch_bounds__(256) void kq4_mx_join_kernel(KQ4MxArgs a, int ksplit, int chunks) {
+  const int t = (int)(blockIdx.x / (unsigned)chunks), c0 = ((int)blockIdx.x - t * chunks) * 1024 + (int)threadIdx.x;
+  const size_t m = (size_t)a.n * a.rows;
+  const float *p = a.part + (size_t)t * a.rows;
+  float y[4][G] = {}, res[4];
+  if (a.res)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) res[i] = a.res[(size_t)t * a.ldo + min(c0 + 256 * i, a.rows - 1)];
+  for (int s = 0; s < ksplit; s += 4) {
+    float v[4][G][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i][g][u] = p[((size_t)min(s + u, ksplit - 1) * G + g) * m + min(c0 + 256 * i, a.rows - 1)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i][g] += s + u < ksplit ? v[i][g][u] : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (c0 + 256 * i >= a.rows) continue;
+    const float o = G == 2 ? kq4_mx_gate(y[i][0], y[i][G - 1]) : y[i][0];
+    a.out[(size_t)t * a.ldo + c0 + 256 * i] = a.res ? o + res[i] : o;
+  }
+}
+
 template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC>
-static int launch(const KQ4MxArgs &a, hipStream_t s) {
+static int launch(const KQ4MxArgs &a, int ksplit, hipStream_t s) {
   using T = KQ4MxTile<TYPE, TI, TJ, WM, WN, S>;
   auto *k = kq4_mx_gemm_kernel<TYPE, G, TI, TJ, WM, WN, S, OCC>;
   static std::atomic<unsigned long long> done{0};
-  const hipError_t e = kq4_lds_limit_once(reinterpret_cast<const void *>(k), T::LDS, done);
+  hipError_t e = kq4_lds_limit_once(reinterpret_cast<const void *>(k), T::LDS, done);
   if (e != hipSuccess) return (int)e;
   const int mt = (a.n + T::BM - 1) / T::BM, nt = (a.rows + T::BN / G - 1) / (T::BN / G);
-  hipLaunchKernelGGL(k, dim3((unsigned)mt * nt), dim3(64 * T::NW), T::LDS, s, a, mt, nt);
+  const int per = (a.dw.kq + ksplit - 1) / ksplit;   // (every slice has some: kq4_mx_split)
+  hipLaunchKernelGGL(k, dim3((unsigned)mt * nt * ksplit), dim3(64 * T::NW), T::LDS, s, a, mt, nt, ksplit, per);
+  e = hipGetLastError();
+  if (e != hipSuccess || ksplit == 1) return (int)e;
+  const int chunks = (a.rows + 1023) / 1024;
+  hipLaunchKernelGGL(kq4_mx_join_kernel<G>, dim3((unsigned)chunks * a.n), dim3(256), 0, s, a, ksplit, chunks);
   return (int)hipGetLastError();
 }
 
-int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, hipStream_t s) {
-  if (a.w[1]) return type == 4 ? launch<4, 2, 2, 4, 2, 2, 3, 2>(a, s) : launch<6, 2, 2, 4, 2, 2, 2, 2>(a, s);
-  return type == 4 ? launch<4, 1, 2, 4, 2, 2, 3, 2>(a, s) : launch<6, 1, 2, 4, 2, 2, 2, 2>(a, s);
+// As many slices of whole groups as there are with `want` asked for.
+int kq4_mx_split(int kq, int want) {
+  if (want > kq) want = kq;
+  if (want < 1) want = 1;
+  const int per = (kq + want - 1) / want;
+  return (kq + per - 1) / per;
+}
+
+// Launches that leave a workgroup alone on its CU run it in 8 waves of 64 x 64 with a stage more in its ring, two waves per
+// SIMD as elsewhere two workgroups have (512 x 4096 x 4096: 17.3 us instead of 19.4, of 6 bits 20.0 instead of 23.8).
+template <int TYPE, int G>
+static int launch_form(const KQ4MxArgs &a, int ksplit, int ncu, hipStream_t s) {
+  const long wgs = (long)((a.n + 127) / 128) * ((a.rows + 256 / G - 1) / (256 / G)) * ksplit;
+  if (wgs <= ncu) return launch<TYPE, G, 2, 2, 2, 4, 3, 1>(a, ksplit, s);
+  return launch<TYPE, G, 2, 4, 2, 2, TYPE == 4 ? 3 : 2, 2>(a, ksplit, s);
+}
+
+int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, int ksplit, int ncu, hipStream_t s) {
+  if (a.w[1]) return type == 4 ? launch_form<4, 2>(a, ksplit, ncu, s) : launch_form<6, 2>(a, ksplit, ncu, s);
+  return type == 4 ? launch_form<4, 1>(a, ksplit, ncu, s) : launch_form<6, 1>(a, ksplit, ncu, s);
+}
+
+size_t kq4_mx_part_bytes(int n, int rows, int matrices, int ksplit) {
+  return ksplit > 1 ? (size_t)ksplit * matrices * n * rows * sizeof(float) : 0;
+}
+
+// The form by estimated microseconds, from measured times (profiles of both sides of each choice in
+// profiles/mx_planner_sweeps.md):
+//   rows kernel   3 + 1.8 per million outputs + products at 0.75e9 a microsecond (6 bits 0.6e9; gated 0.85e9, 0.66e9)
+//   GEMM          6.5 + its stages: 0.38 (6 bits 0.48) for a workgroup alone on its CU, 1.05 a round for two
+//   K in slices   2.5 for the second launch + the sums written and read at 4.5e6 bytes a microsecond
+// e.g. 4096 x 4096, 6 bits: 256 tokens 13.3 us in the rows kernel against 16.6 (two slices) and 18.7 in the GEMM, 768 28.5 against
+// 20.8; 4096 x 12288, 512 tokens: 33.8 in four slices, 50.9 in one, 50.4 in the rows kernel.
+KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu, int force_form, int force_split) {
+  const KQ4MxDims d = kq4_mx_dims(rows, cols);
+  const double outputs = (double)n * rows, products = outputs * cols * matrices;
+  const double rate = matrices == 2 ? (type == 4 ? 0.85e9 : 0.66e9) : (type == 4 ? 0.75e9 : 0.6e9);
+  KQ4MxPlan best = {0, 1};
+  double least = 3.0 + 1.8e-6 * outputs + products / rate;
+  const double tiles = (double)((n + 127) / 128) * ((rows + 256 / matrices - 1) / (256 / matrices));
+  // what is forced is done where its launches have fewer than 2^32 threads
+  if (n <= 16 || (force_form == 1 && (double)d.nt * ((n + 15) >> 4) < 1 << 23)) least = 0.0;   // (a token tile: no GEMM)
+  if (force_form == 2) least = 1e30;
+  if (tiles * force_split >= 1 << 23 || (double)((rows + 1023) / 1024) * n >= 1 << 24) force_split = 1;
+  for (int want = 1; want <= 16; want *= 2) {
+    if (force_split > 0 && want > 1) break;
+    const int ks = kq4_mx_split(d.kq, force_split > 0 ? force_split : want);
+    const double wgs = tiles * ks;
+    if (want > 1 && (ks <= best.ksplit || wgs > 2.0 * ncu || kq4_mx_part_bytes(n, rows, matrices, ks) > KQ4_MX_PART_MAX)) break;
+    const int stages = 4 * ((d.kq + ks - 1) / ks);
+    double us = 6.5 + stages * (wgs <= ncu ? (type == 4 ? 0.38 : 0.48) : 1.05 * (double)(long)((wgs + 2 * ncu - 1) / (2 * ncu)));
+    if (ks > 1) us += 2.5 + (ks + 1.5) * matrices * outputs * 4.0 / 4.5e6;
+    if (us < least) {
+      least = us;
+      best = {1, ks};
+    }
+  }
+  return best;
 }

@@ -141,6 +141,16 @@ def test_matmul_of_odd_sizes_and_strides(kq4, torch_dev, n, rows, cols, act, qua
                  pad_out=n % 3, quantized=quantized)
 
 
+@pytest.mark.parametrize("act", [4, 6])
+@pytest.mark.parametrize("n,rows,cols", [(1, 130, 544), (16, 300, 2080), (33, 515, 1120), (129, 257, 4096), (300, 600, 1536), (1100, 2100, 544)])
+@pytest.mark.parametrize("form,split", [(1, 0), (2, 1), (2, 2), (2, 3), (2, 50)])
+def test_every_form(kq4, torch_dev, n, rows, cols, act, form, split):
+    """The rows kernel and the GEMM, whole and with K in slices, at sizes of either, with and without a residual."""
+    with kq4.options(mx_form=form, mx_split=split):
+        check_matmul(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act, split % 2, pad_x=4, pad_out=1)
+        check_gated(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act)
+
+
 @pytest.mark.parametrize("n", [1, 20, 200])
 @pytest.mark.parametrize("act", [4, 6])
 def test_nan_stays_in_its_token_and_row(kq4, torch_dev, n, act):
@@ -184,11 +194,7 @@ def test_scales_at_their_ends(kq4, torch_dev, n):
     assert (np.abs(out.cpu().numpy() - want) <= tol).all()
 
 
-@pytest.mark.parametrize("act", [4, 6])
-@pytest.mark.parametrize("n,rows,cols", [(1, 16, 32), (1, 333, 1024), (3, 100, 544), (16, 64, 512), (29, 260, 2048), (66, 129, 96),
-                                         (130, 520, 640), (300, 288, 1056)])
-def test_gated(kq4, torch_dev, n, rows, cols, act):
-    torch, rng = torch_dev, np.random.default_rng(rows)
+def check_gated(kq4, torch, rng, n, rows, cols, act):
     g, u = R.random_weights(rng, rows, cols), R.random_weights(rng, rows, cols)
     x = R.acts(rng, n, cols) * F32(0.5 / np.sqrt(cols))
     want, tol = R.gated(R.values(*R.quantize(x, act), act), R.values(*g, 4), R.values(*u, 4))
@@ -197,6 +203,13 @@ def test_gated(kq4, torch_dev, n, rows, cols, act):
     got = wide.cpu().numpy()
     assert (np.abs(got[:, :rows] - want) <= tol).all(), (np.abs(got[:, :rows] - want) / tol).max()
     assert (got[:, rows:] == 7.0).all()
+
+
+@pytest.mark.parametrize("act", [4, 6])
+@pytest.mark.parametrize("n,rows,cols", [(1, 16, 32), (1, 333, 1024), (3, 100, 544), (16, 64, 512), (29, 260, 2048), (66, 129, 96),
+                                         (130, 520, 640), (300, 288, 1056)])
+def test_gated(kq4, torch_dev, n, rows, cols, act):
+    check_gated(kq4, torch_dev, np.random.default_rng(rows), n, rows, cols, act)
 
 
 def test_gate_far_from_zero(kq4, torch_dev):
@@ -237,8 +250,15 @@ def hull(h, tol, bits):
 
 @pytest.mark.parametrize("act", [4, 6])
 @pytest.mark.parametrize("n,dim,ffn", [(1, 96, 160), (1, 512, 1056), (5, 128, 544), (40, 256, 640), (140, 192, 288)])
-def test_ffn(kq4, torch_dev, n, dim, ffn, act):
-    """The block as one call: within the product's bound of some h that the fp32 sums of gate and up allow."""
+@pytest.mark.parametrize("form,split", [(0, 0), (1, 0), (2, 1), (2, 2)])
+def test_ffn(kq4, torch_dev, n, dim, ffn, act, form, split):
+    """The block as one call: within the product's bound of some h that the fp32 sums of gate and up allow. The GEMM in one
+    slice hands h over quantized."""
+    with kq4.options(mx_form=form, mx_split=split):
+        check_ffn(kq4, torch_dev, n, dim, ffn, act)
+
+
+def check_ffn(kq4, torch_dev, n, dim, ffn, act):
     torch, rng = torch_dev, np.random.default_rng(n + ffn)
     g, u, d = R.random_weights(rng, ffn, dim), R.random_weights(rng, ffn, dim), R.random_weights(rng, dim, ffn)
     x = R.acts(rng, n, dim) * F32(0.5 / np.sqrt(dim))

@@ -100,6 +100,47 @@ result = [before, after, smaller]
     assert smaller == [0] * len(smaller)
 
 
+@pytest.mark.parametrize("shape,want", [
+    ((1, 4096, 4096, "matmul"), ["rows"]), ((4, 4096, 4096, "matmul"), ["rows"]), ((5, 4096, 4096, "matmul"), ["quantize", "rows"]),
+    ((16, 151936, 2048, "matmul"), ["quantize", "rows"]), ((64, 4096, 12288, "matmul"), ["quantize", "rows"]),
+    ((256, 4096, 4096, "matmul"), ["quantize", "rows"]), ((768, 4096, 4096, "matmul"), ["quantize", "gemm"]),
+    ((512, 4096, 12288, "matmul"), ["quantize", "gemm", "join"]), ((4096, 4096, 12288, "matmul"), ["quantize", "gemm"]),
+    ((1, 12288, 4096, "gated"), ["rows"]), ((29, 6144, 2048, "gated"), ["quantize", "rows"]),
+    ((2048, 12288, 4096, "gated"), ["quantize", "gemm"]), ((300, 1024, 512, "gated"), ["quantize", "rows"]),
+    ((1, 4096, 12288, "ffn"), ["rows", "rows"]), ((8, 4096, 12288, "ffn"), ["quantize", "rows", "quantize", "rows"]),
+    ((2048, 4096, 12288, "ffn"), ["quantize", "gemm", "gemm"]),
+])
+def test_launches(standin, shape, want):  # noqa: F811
+    """Which kernels a call takes on 256 CUs (6-bit activations): one launch for few tokens, h quantized in the GEMM."""
+    res = standin(SETUP + """
+n, rows, cols, kind = shape
+hip.standin_clear()
+far = dict(out=at(200), x=at(300))
+rc = matmul(n=n, rows=rows, ldo=rows, cols=cols, ldx=cols, res=None, w=at(4), **far) if kind == "matmul" else \\
+    gated(n=n, rows=rows, ldo=rows, cols=cols, ldx=cols, **far) if kind == "gated" else \\
+    ffn(n=n, dim=rows, ffn=cols, ldo=rows, ldx=rows, res=None, **far)
+result = [rc] + [s.split(" ")[0] for s in hip.standin_log().decode().split("\\n")[:-1]]
+""", shape=shape)
+    assert res[0] == 0
+    assert [next(k for k in ("quantize", "rows", "gemm", "join") if "kq4_mx_" + k in s) for s in res[1:]] == want
+
+
+def test_planner_options(standin):  # noqa: F811
+    """mx_form and mx_split choose the form and the slices; a split that K does not have is the most that it has."""
+    res = standin(SETUP + """
+def names(**o):
+    for k_, v in o.items():
+        assert k.kq4_set_option(k_.encode(), v) == 0
+    hip.standin_clear()
+    rc = matmul(n=300, rows=600, ldo=600, cols=1536, ldx=1536, res=None, out=at(20))
+    return [rc] + [s.split(" ")[0].split("kq4_mx_")[1][:4] + " " + s.split(" ")[1] for s in hip.standin_log().decode().split("\\n")[1:-1]]
+result = [names(mx_form=1), names(mx_form=2, mx_split=1), names(mx_split=2), names(mx_split=99), names(mx_form=-1, mx_split=-1)]
+""")
+    assert [r[0] for r in res] == [0] * 5
+    assert res[1][1:] == ["gemm 9"] and res[2][1:] == ["gemm 18", "join 300"] and res[3][1:] == ["gemm 27", "join 300"]
+    assert len(res[0]) == 2 and res[0][1].startswith("rows") and res[4] == res[0]
+
+
 def test_binding_refuses_host_tensors_and_shapes(kq4_cpu):
     import torch
     with pytest.raises(kq4_cpu.KQ4Error, match="device tensor"):
