@@ -151,17 +151,19 @@ class MoeLayer(ctypes.Structure):
 
 
 _lib = None
+_torch = None   # the torch module, once libkq4 is loaded beside it
 
 
 def lib():
     """Loads libkq4.so (built in-tree by `make -C kestrel-llm_amd`); raises if absent."""
-    global _lib
+    global _lib, _torch
     if _lib is None:
         # torch's wheel ships its own libamdhip64.so.7 (same soname as /opt/rocm's). Whichever
         # loads first serves the whole process, and torch cannot use the system one; so when
         # torch is installed, let it load first and libkq4 binds to the same runtime.
         try:
-            import torch  # noqa: F401
+            import torch
+            _torch = torch
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -771,20 +773,21 @@ def rope_table(rows, dim, theta, device="cuda"):
 
 def _check_here(device, name):
     """Raises unless `device` (an index) is the current one, which the call's launches go to."""
-    import torch
-    if device != torch.cuda.current_device():
-        raise KQ4Error(f"{name}: on device {device}, the current device is {torch.cuda.current_device()}")
+    if device != _torch.cuda.current_device():
+        raise KQ4Error(f"{name}: on device {device}, the current device is {_torch.cuda.current_device()}")
 
 
 def _rows(t, name, n, width, device):
     """Row stride of a [>= n][width] fp32 tensor on `device` with unit column stride, checked."""
-    import torch
-    if isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is torch.float32 and \
-            t.dim() == 2:
-        (rows, cols), (ld, step) = t.shape, t.stride()
-        if rows >= n and cols == width and (step == 1 or width <= 1):
-            return ld if rows > 1 else width   # (one row: any stride)
-    _need_on(t, name, torch.float32, device)
+    if isinstance(t, _torch.Tensor) and t.dtype is _torch.float32 and t.get_device() == device:
+        shape = t.shape
+        if len(shape) == 2 and shape[0] >= n and shape[1] == width:
+            if t.is_contiguous():
+                return width
+            ld, step = t.stride()
+            if step == 1 or width <= 1:
+                return ld if shape[0] > 1 else width   # (one row: any stride)
+    _need_on(t, name, _torch.float32, device)
     raise KQ4Error(f"{name}: expected [{n}, {width}] with unit column stride, got {tuple(t.shape)} "
                    f"strides {t.stride()}")
 
@@ -940,9 +943,10 @@ def mx_ffn_workspace_bytes(n, dim, ffn):
 
 def mx_quantize_dev(m, x, stream=None):
     """fp32 x [rows][cols] (unit column stride) into the microscaled matrix m."""
-    ldx = _rows(x, "x", m.rows, m.cols, m.device)
-    _check_here(m.device, "m")
-    check(lib().kq4_mx_quantize_dev(m.p, x.data_ptr(), ldx, m.rows, m.cols, m.type, _stream_ptr(stream)),
+    rows, cols, dev = m.rows, m.cols, m.device
+    ldx = _rows(x, "x", rows, cols, dev)
+    _check_here(dev, "m")
+    check(_lib.kq4_mx_quantize_dev(m.p, x.data_ptr(), ldx, rows, cols, m.type, _stream_ptr(stream)),
           "kq4_mx_quantize_dev")
 
 
@@ -967,13 +971,14 @@ def mx_unpack_dev(codes, scales, m, stream=None):
                                   _stream_ptr(stream)), "kq4_mx_unpack_dev")
 
 
-def _mx_w(w, name, rows, cols, device):
-    """Raises unless w is a 4-bit matrix of rows x cols (None: any) on `device`."""
-    if not isinstance(w, MX) or w.type != MX_FP4 or (rows is not None and w.rows != rows) or w.cols != cols:
-        raise KQ4Error(f"{name}: expected a 4-bit MX of {rows} x {cols}, got "
-                       + (f"{w.rows} x {w.cols} of {w.type} bits" if isinstance(w, MX) else repr(type(w))))
-    if w.device != device:
-        raise KQ4Error(f"{name}: on device {w.device}, expected {device}")
+def _mx_w(w, name, rows=None, cols=None, device=None):
+    """Raises unless w is a 4-bit matrix of rows x cols on `device` (each where it is given)."""
+    if isinstance(w, MX) and w.type == MX_FP4 and (rows is None or rows == w.rows) and (cols is None or cols == w.cols):
+        if device is not None and w.device != device:
+            raise KQ4Error(f"{name}: on device {w.device}, expected {device}")
+        return
+    raise KQ4Error(f"{name}: expected a 4-bit MX of {rows or 'n'} x {cols or 'n'}, got "
+                   + (f"{w.rows} x {w.cols} of {w.type} bits" if isinstance(w, MX) else repr(type(w))))
 
 
 def _mx_out(out, residual, n, rows, device):
@@ -986,52 +991,56 @@ def _mx_out(out, residual, n, rows, device):
     return ldo
 
 
-def _mx_x(x, cols, device):
-    if getattr(x, "ndim", 0) != 2:
+def _mx_n(x, cols):
+    """The rows of x."""
+    if not isinstance(x, _torch.Tensor) or x.dim() != 2:
         raise KQ4Error(f"x: expected a [n, {cols}] device tensor")
-    n = x.shape[0]
-    return n, _rows(x, "x", n, cols, device)
+    return x.shape[0]
 
 
 def mx_matmul_dev(out, x, w, act=MX_FP6, residual=None, stream=None):
     """out [n][w.rows] = [residual +] W . x for fp32 x [n][w.cols], quantized to `act` bits on the way."""
-    _mx_w(w, "w", None, w.cols if isinstance(w, MX) else 0, w.device if isinstance(w, MX) else None)
-    n, ldx = _mx_x(x, w.cols, w.device)
-    ldo = _mx_out(out, residual, n, w.rows, w.device)
-    _check_here(w.device, "w")
-    check(lib().kq4_mx_matmul_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), w.p, w.rows, w.cols, n, act,
-                                  _stream_ptr(stream)), "kq4_mx_matmul_dev")
+    _mx_w(w, "w")
+    rows, cols, dev = w.rows, w.cols, w.device
+    n = _mx_n(x, cols)
+    ldx, ldo = _rows(x, "x", n, cols, dev), _mx_out(out, residual, n, rows, dev)
+    _check_here(dev, "w")
+    check(_lib.kq4_mx_matmul_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), w.p, rows, cols, n, act,
+                                 _stream_ptr(stream)), "kq4_mx_matmul_dev")
 
 
 def mx_matmul_q_dev(out, xq, w, residual=None, stream=None):
     """The same from activations that are quantized already (an MX of n x w.cols)."""
     if not isinstance(xq, MX):
         raise KQ4Error("xq: expected an MX")
-    _mx_w(w, "w", None, xq.cols, xq.device)
-    ldo = _mx_out(out, residual, xq.rows, w.rows, w.device)
-    _check_here(w.device, "w")
-    check(lib().kq4_mx_matmul_q_dev(out.data_ptr(), ldo, xq.p, _tp(residual), w.p, w.rows, w.cols, xq.rows, xq.type,
-                                    _stream_ptr(stream)), "kq4_mx_matmul_q_dev")
+    n, cols, dev = xq.rows, xq.cols, xq.device
+    _mx_w(w, "w", None, cols, dev)
+    ldo = _mx_out(out, residual, n, w.rows, dev)
+    _check_here(dev, "w")
+    check(_lib.kq4_mx_matmul_q_dev(out.data_ptr(), ldo, xq.p, _tp(residual), w.p, w.rows, cols, n, xq.type,
+                                   _stream_ptr(stream)), "kq4_mx_matmul_q_dev")
 
 
 def mx_gated_dev(out, x, gate, up, act=MX_FP6, stream=None):
     """out [n][gate.rows] = silu(gate . x) * (up . x) for fp32 x [n][gate.cols]."""
-    _mx_w(gate, "gate", None, gate.cols if isinstance(gate, MX) else 0, gate.device if isinstance(gate, MX) else None)
-    _mx_w(up, "up", gate.rows, gate.cols, gate.device)
-    n, ldx = _mx_x(x, gate.cols, gate.device)
-    ldo = _mx_out(out, None, n, gate.rows, gate.device)
-    _check_here(gate.device, "gate")
-    check(lib().kq4_mx_gated_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, gate.p, up.p, gate.rows, gate.cols, n, act,
-                                 _stream_ptr(stream)), "kq4_mx_gated_dev")
+    _mx_w(gate, "gate")
+    rows, cols, dev = gate.rows, gate.cols, gate.device
+    _mx_w(up, "up", rows, cols, dev)
+    n = _mx_n(x, cols)
+    ldx, ldo = _rows(x, "x", n, cols, dev), _rows(out, "out", n, rows, dev)
+    _check_here(dev, "gate")
+    check(_lib.kq4_mx_gated_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, gate.p, up.p, rows, cols, n, act,
+                                _stream_ptr(stream)), "kq4_mx_gated_dev")
 
 
 def mx_ffn_dev(out, x, gate, up, down, act=MX_FP6, residual=None, stream=None):
     """out [n][dim] = [residual +] down . (silu(gate . x) * (up . x)), gate and up [ffn][dim], down [dim][ffn]."""
-    _mx_w(gate, "gate", None, gate.cols if isinstance(gate, MX) else 0, gate.device if isinstance(gate, MX) else None)
-    _mx_w(up, "up", gate.rows, gate.cols, gate.device)
-    _mx_w(down, "down", gate.cols, gate.rows, gate.device)
-    n, ldx = _mx_x(x, gate.cols, gate.device)
-    ldo = _mx_out(out, residual, n, gate.cols, gate.device)
-    _check_here(gate.device, "gate")
-    check(lib().kq4_mx_ffn_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), gate.p, up.p, down.p, gate.cols,
-                               gate.rows, n, act, _stream_ptr(stream)), "kq4_mx_ffn_dev")
+    _mx_w(gate, "gate")
+    ffn, dim, dev = gate.rows, gate.cols, gate.device
+    _mx_w(up, "up", ffn, dim, dev)
+    _mx_w(down, "down", dim, ffn, dev)
+    n = _mx_n(x, dim)
+    ldx, ldo = _rows(x, "x", n, dim, dev), _mx_out(out, residual, n, dim, dev)
+    _check_here(dev, "gate")
+    check(_lib.kq4_mx_ffn_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), gate.p, up.p, down.p, dim, ffn, n,
+                              act, _stream_ptr(stream)), "kq4_mx_ffn_dev")
