@@ -1469,26 +1469,20 @@ KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, con
   return a;
 }
 
-// Whether the rows kernel quantizes the activations itself, every workgroup all of them: 16384 elements take it less than
-// a launch of the quantizer (3.2 us and its gap).
-bool mx_fused(int n, int cols, int type) {
-  return n <= 16 && n * (long)cols <= 16384 && kq4_mx_rows_lds(n, kq4_mx_dims(n, cols), type) <= 64 * 1024;
-}
-
 KQ4MxPlan mx_plan(DevState *ds, int n, int rows, int cols, int matrices, int act) {
   return kq4_mx_plan(n, rows, cols, matrices, act, ds->ncu, opt(kMxForm), opt(kMxSplit));
 }
 
 // Bytes of a product's activations in the workspace, 0 where the rows kernel quantizes them.
-size_t mx_x_bytes(const KQ4MxPlan &p, int n, int cols, int act) {
-  return !p.gemm && mx_fused(n, cols, act) ? 0 : mx_bytes(n, cols, act);
+size_t mx_x_bytes(DevState *ds, const KQ4MxPlan &p, int n, int rows, int cols, int matrices, int act) {
+  return !p.gemm && kq4_mx_rows_fused(n, rows, cols, matrices, act, ds->ncu) ? 0 : mx_bytes(n, cols, act);
 }
 
 // A product as planned, from fp32 rows x (quantized into xq where the kernel does not do that) or, without, from xq; its
 // partial sums in part.
 int mx_run(DevState *ds, const KQ4MxPlan &p, KQ4MxArgs a, const float *x, long ldx, uint8_t *xq, float *part, int act,
            hipStream_t s) {
-  if (x && !mx_x_bytes(p, a.n, a.cols, act)) {
+  if (x && !mx_x_bytes(ds, p, a.n, a.rows, a.cols, a.w[1] ? 2 : 1, act)) {
     a.xf = x;
     a.ldx = ldx;
   } else {
@@ -1508,7 +1502,7 @@ int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq
   if (rc) return rc;
   const int matrices = w1 ? 2 : 1;
   const KQ4MxPlan p = mx_plan(ds, n, rows, cols, matrices, act);
-  const size_t xb = x ? mx_x_bytes(p, n, cols, act) : 0, pb = kq4_mx_part_bytes(n, rows, matrices, p.ksplit);
+  const size_t xb = x ? mx_x_bytes(ds, p, n, rows, cols, matrices, act) : 0, pb = kq4_mx_part_bytes(n, rows, matrices, p.ksplit);
   if (xb + pb && (rc = ensure_ws(Ws{&ds->ws, ds}, xb + pb, s))) return rc;
   uint8_t *ws = static_cast<uint8_t *>(ds->ws.p);
   return mx_run(ds, p, mx_args(out, ldo, residual, w0, w1, nullptr, rows, cols, n), x, ldx,
@@ -1596,7 +1590,8 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
   hipStream_t s = (hipStream_t)stream;
   const KQ4MxPlan pg = mx_plan(ds, n_batch, ffn, dim, 2, act), pd = mx_plan(ds, n_batch, dim, ffn, 1, act);
   const bool direct = pg.gemm && pg.ksplit == 1;   // h leaves the gated kernel quantized
-  const size_t xb = mx_x_bytes(pg, n_batch, dim, act), hb = direct ? mx_bytes(n_batch, ffn, act) : mx_x_bytes(pd, n_batch, ffn, act);
+  const size_t xb = mx_x_bytes(ds, pg, n_batch, ffn, dim, 2, act);
+  const size_t hb = direct ? mx_bytes(n_batch, ffn, act) : mx_x_bytes(ds, pd, n_batch, dim, ffn, 1, act);
   const size_t fb = direct ? 0 : al256((size_t)n_batch * ffn * sizeof(float));
   const size_t pb = std::max(kq4_mx_part_bytes(n_batch, ffn, 2, pg.ksplit), kq4_mx_part_bytes(n_batch, dim, 1, pd.ksplit));
   if ((rc = ensure_ws(Ws{&ds->ws, ds}, xb + hb + fb + pb, s))) return rc;

@@ -233,7 +233,7 @@ struct KQ4MxArgs {
   int rows, cols, n;
   KQ4MxDims dw, dx;
 };
-size_t kq4_mx_rows_lds(int n, const KQ4MxDims &d, int type);   // of the rows kernel with xf
+bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu);   // whether xf is the faster way
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s);
 // ksplit > 1 (as kq4_mx_split gives it): K in that many slices, each its own sums in part (kq4_mx_part_bytes), added in
 // slice order by a second launch.

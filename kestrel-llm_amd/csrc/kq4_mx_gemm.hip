@@ -277,42 +277,46 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
       }
       return;
     }
-  // The residual's loads of 32 tokens are all on their way before the first of them is waited for (it may be out: an
-  // element is read and written by one lane). Past the edges they read the last row's or column's, which is not stored.
+  // The residual's loads of 32 tokens are all on their way before the first of them is waited for (it may be out: an element
+  // is read and written by one lane). Past the edges they read the last row's or column's, which is not stored.
   const bool inside = m0 + T::BM <= a.n && n0 + RG <= a.rows;
+  auto store = [&](auto with_res) {
+    constexpr bool RES = decltype(with_res)::value;
 #pragma unroll
-  for (int i = 0; i < TI; ++i) {
-    const int t0 = m0 + 32 * (TI * wm + i) + 4 * half;
-    float y[16][TJ / G];
-    if (a.res) {
+    for (int i = 0; i < TI; ++i) {
+      const int t0 = m0 + 32 * (TI * wm + i) + 4 * half;
+      float y[16][TJ / G];
+      if constexpr (RES)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float *r = a.res + (size_t)min(t0 + 8 * (e >> 2) + (e & 3), a.n - 1) * a.ldo;
+#pragma unroll
+          for (int j = 0; j < TJ / G; ++j) y[e][j] = r[min(c0 + 32 * j, a.rows - 1)];
+        }
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int j = 0; j < TJ / G; ++j) {
+          const float p = G == 2 ? kq4_mx_gate(acc[i][j][e], acc[i][G == 2 ? TJ / 2 + j : j][e]) : acc[i][j][e];
+          y[e][j] = RES ? p + y[e][j] : p;
+        }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float *r = a.res + (size_t)min(t0 + 8 * (e >> 2) + (e & 3), a.n - 1) * a.ldo;
+        const int tok = t0 + 8 * (e >> 2) + (e & 3);
+        float *o = a.out + (size_t)tok * a.ldo + c0;
+        if (inside) {
 #pragma unroll
-        for (int j = 0; j < TJ / G; ++j) y[e][j] = r[min(c0 + 32 * j, a.rows - 1)];
+          for (int j = 0; j < TJ / G; ++j) o[32 * j] = y[e][j];
+        } else if (tok < a.n) {
+#pragma unroll
+          for (int j = 0; j < TJ / G; ++j)
+            if (c0 + 32 * j < a.rows) o[32 * j] = y[e][j];
+        }
       }
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-#pragma unroll
-      for (int j = 0; j < TJ / G; ++j) {
-        const float p = G == 2 ? kq4_mx_gate(acc[i][j][e], acc[i][G == 2 ? TJ / 2 + j : j][e]) : acc[i][j][e];
-        y[e][j] = a.res ? p + y[e][j] : p;
-      }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int tok = t0 + 8 * (e >> 2) + (e & 3);
-      float *o = a.out + (size_t)tok * a.ldo + c0;
-      if (inside) {
-#pragma unroll
-        for (int j = 0; j < TJ / G; ++j) o[32 * j] = y[e][j];
-      } else if (tok < a.n) {
-#pragma unroll
-        for (int j = 0; j < TJ / G; ++j)
-          if (c0 + 32 * j < a.rows) o[32 * j] = y[e][j];
-      }
-    }
-  }
+  };
+  if (a.res) store(std::true_type{});
+  else store(std::false_type{});
 }
 
 // out = [res +] the slices' sums in slice order (gated: of both matrices). A thread four outputs of a token, 256 apart,

@@ -199,7 +199,8 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
   }
 }
 
-size_t kq4_mx_rows_lds(int n, const KQ4MxDims &d, int type) { return (size_t)n * (4 * d.kt * 4 * type + 16 * d.kq); }
+// LDS of the activations that a workgroup quantizes itself.
+static size_t kq4_mx_rows_lds(int n, const KQ4MxDims &d, int type) { return (size_t)n * (4 * d.kt * 4 * type + 16 * d.kq); }
 
 template <int TYPE, int G, int RT, int TT, int NW, bool FQ>
 static int launch(const KQ4MxArgs &a, int ks, hipStream_t s) {
@@ -210,13 +211,20 @@ static int launch(const KQ4MxArgs &a, int ks, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+// The waves that share a row tile: 8 (a workgroup) where K has that many pieces and the launch then is at most 16 waves a
+// CU, else 4 or as many as there are pieces, in workgroups of 4 waves. One token: 4096 x 4096 4.4 us with 8 and 4.9 with 4,
+// 12288 x 4096 8.2 and 7.0, 151936 x 2048 51 and 26.
+static int slices(const KQ4MxDims &dw, long tiles, int ncu) {
+  if (dw.kq >= 8 && tiles * 8 <= 16L * ncu) return 8;
+  int ks = 4;
+  while (ks > dw.kq) ks /= 2;
+  return ks;
+}
+
 template <int TYPE, int G, int RT, int TT, bool FQ>
 static int launch_k(const KQ4MxArgs &a, int ncu, hipStream_t s) {
-  const long tiles = (long)((a.dw.nt + RT - 1) / RT) * ((a.dx.nt + TT - 1) / TT);
-  if (a.dw.kq >= 8 && tiles * 8 <= 16L * ncu) return launch<TYPE, G, RT, TT, 8, FQ>(a, 8, s);
-  int ks = 4;
-  while (ks > a.dw.kq) ks /= 2;
-  return launch<TYPE, G, RT, TT, 4, FQ>(a, ks, s);
+  const int ks = slices(a.dw, (long)((a.dw.nt + RT - 1) / RT) * ((a.dx.nt + TT - 1) / TT), ncu);
+  return ks == 8 ? launch<TYPE, G, RT, TT, 8, FQ>(a, ks, s) : launch<TYPE, G, RT, TT, 4, FQ>(a, ks, s);
 }
 
 template <int TYPE, int G>
@@ -231,4 +239,16 @@ static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
   if (a.w[1]) return type == 4 ? launch_t<4, 2>(a, ncu, s) : launch_t<6, 2>(a, ncu, s);
   return type == 4 ? launch_t<4, 1>(a, ncu, s) : launch_t<6, 1>(a, ncu, s);
+}
+
+// Every workgroup quantizes all the activations, 0.12 us for 1000 elements of each workgroup that its CU runs, against a
+// launch of the quantizer (2.5 to 3.4 us, and as much of the host's time). Worth it up to 32768 elements a CU (4096 x 4096:
+// four tokens 6.4 us against 7.4, eight 8.3 against 7.8 and a launch less, sixteen 12.3 against 7.8), and where the weights
+// take the memory longer than that anyway (151936 x 2048: one token 26 against 38 us, eight 80 against 38).
+bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu) {
+  const KQ4MxDims d = kq4_mx_dims(rows, cols);
+  if (n > 16 || kq4_mx_rows_lds(n, d, type) > 64 * 1024) return false;
+  const int ks = slices(d, d.nt, ncu), tpw = (ks == 8 ? 8 : 4) / ks;
+  const double wgs = (d.nt + tpw - 1) / tpw, each = (double)((long)((wgs + ncu - 1) / ncu)) * n * cols;
+  return each <= 32768.0 || each * 0.12e-3 <= 0.4 * matrices * rows * (double)cols * 0.53 / 6.0e6;
 }
