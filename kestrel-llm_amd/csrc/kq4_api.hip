@@ -1448,24 +1448,16 @@ int mx_product_check(const char *what, const float *out, long ldo, const float *
 
 size_t mx_bytes(int rows, int cols, int type) { return al256(kq4_mx_size(kq4_mx_dims(rows, cols), type)); }
 
-KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, const uint8_t *w1, const uint8_t *xq,
-                  int rows, int cols, int n) {
-  KQ4MxArgs a;
+KQ4MxArgs mx_args(float *out, long ldo, const float *res, const uint8_t *w0, const uint8_t *w1, int rows, int cols, int n) {
+  KQ4MxArgs a = {};
   a.w[0] = w0;
   a.w[1] = w1;
-  a.x = xq;
-  a.xf = nullptr;
-  a.ldx = 0;
   a.out = out;
   a.res = res;
   a.ldo = ldo;
-  a.part = nullptr;
-  a.q = nullptr;
   a.rows = rows;
   a.cols = cols;
   a.n = n;
-  a.dw = kq4_mx_dims(rows, cols);
-  a.dx = kq4_mx_dims(n, cols);
   return a;
 }
 
@@ -1483,7 +1475,7 @@ size_t mx_x_bytes(DevState *ds, const KQ4MxPlan &p, int n, int rows, int cols, i
 int mx_run(DevState *ds, const KQ4MxPlan &p, KQ4MxArgs a, const float *x, long ldx, uint8_t *xq, float *part, int act,
            hipStream_t s) {
   if (x && !mx_x_bytes(ds, p, a.n, a.rows, a.cols, a.w[1] ? 2 : 1, act)) {
-    a.xf = x;
+    a.x = x;
     a.ldx = ldx;
   } else {
     if (x) KQ4_HIP((hipError_t)kq4_launch_mx_quantize(xq, x, ldx, a.n, a.cols, act, s));
@@ -1505,7 +1497,7 @@ int mx_product(float *out, long ldo, const float *x, long ldx, const uint8_t *xq
   const size_t xb = x ? mx_x_bytes(ds, p, n, rows, cols, matrices, act) : 0, pb = kq4_mx_part_bytes(n, rows, matrices, p.ksplit);
   if (xb + pb && (rc = ensure_ws(Ws{&ds->ws, ds}, xb + pb, s))) return rc;
   uint8_t *ws = static_cast<uint8_t *>(ds->ws.p);
-  return mx_run(ds, p, mx_args(out, ldo, residual, w0, w1, nullptr, rows, cols, n), x, ldx,
+  return mx_run(ds, p, mx_args(out, ldo, residual, w0, w1, rows, cols, n), x, ldx,
                 x ? ws : const_cast<uint8_t *>(xq), reinterpret_cast<float *>(ws + xb), act, s);
 }
 
@@ -1597,10 +1589,10 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
   if ((rc = ensure_ws(Ws{&ds->ws, ds}, xb + hb + fb + pb, s))) return rc;
   uint8_t *xq = static_cast<uint8_t *>(ds->ws.p), *hq = xq + xb;
   float *h = reinterpret_cast<float *>(hq + hb), *part = reinterpret_cast<float *>(hq + hb + fb);
-  KQ4MxArgs g = mx_args(h, ffn, nullptr, gate, up, nullptr, ffn, dim, n_batch);
+  KQ4MxArgs g = mx_args(h, ffn, nullptr, gate, up, ffn, dim, n_batch);
   if (direct) g.q = hq;
   if ((rc = mx_run(ds, pg, g, x, ldx, xq, part, act, s))) return rc;
-  return mx_run(ds, pd, mx_args(out, ldo, residual, down, nullptr, nullptr, dim, ffn, n_batch), direct ? nullptr : h, ffn,
+  return mx_run(ds, pd, mx_args(out, ldo, residual, down, nullptr, dim, ffn, n_batch), direct ? nullptr : h, ffn,
                 hq, part, act, s);
 }
 

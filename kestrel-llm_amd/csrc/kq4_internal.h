@@ -219,19 +219,18 @@ int kq4_launch_logprobs(const float *logits, long ld, int n, int vocab, int n_to
 int kq4_launch_mx_quantize(uint8_t *m, const float *x, long ldx, int rows, int cols, int type, hipStream_t s);
 int kq4_launch_mx_pack(uint8_t *m, uint8_t *codes, uint8_t *scales, int rows, int cols, int type, bool pack,
                        hipStream_t s);
+// (With a kernel's own integers at most 112 bytes: in about every other process a launch with 128 bytes of arguments or
+// more costs the host 0.8 us more, 3.4 against 2.6. So the dimensions in tiles are not among them.)
 struct KQ4MxArgs {
   const uint8_t *w[2];   // weights; the second one, where there is one, is the gated block's up projection
-  const uint8_t *x;      // a quantized matrix, or with xf (rows kernel) nullptr
-  const float *xf;       // fp32 rows that the kernel quantizes itself, row t at t * ldx
-  long ldx;
+  const void *x;         // a quantized matrix, or (rows kernel) fp32 rows that it quantizes itself, row t at t * ldx floats
   float *out;            // token t's outputs at t * ldo
   const float *res;      // at the same stride, or nullptr
-  long ldo;
   float *part;           // the GEMM's sums by K slice
   uint8_t *q;            // the GEMM of two matrices in one slice: where not nullptr, the outputs as a matrix of n x rows of the
                          // activations' type, in place of out (tokens past n are not written)
+  long ldx, ldo;         // ldx 0: x is quantized
   int rows, cols, n;
-  KQ4MxDims dw, dx;
 };
 bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu);   // whether xf is the faster way
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s);

@@ -67,7 +67,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
 
   // A matrix' runs from byte `off` of the stage (or of the scales) of the workgroup's rows, which start with row tile t0 (a
   // group's first): where they lie and how far the next stage's do. Loads past the matrix read zeros.
-  const KQ4MxDims dw = a.dw, dx = a.dx;
+  const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
+  const uint8_t *xq = static_cast<const uint8_t *>(a.x);
   auto runs = [](const uint8_t *m, const KQ4MxDims &d, int type, bool scales, int t0, int off, uint32_t &step) {
     const int tb = scales ? KQ4_MX_STILE : kq4_mx_tile_bytes(type), t = t0 + off / (8 * tb) * 8;
     const long all = (long)kq4_mx_size(d, type);
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
     return r;
   };
   uint32_t step_a, step_b, step_s[T::SPW];
-  const kq4_rsrc4 ra = runs(a.x, dx, TYPE, false, m0 >> 4, T::first_a(wave) * 1024, step_a);
+  const kq4_rsrc4 ra = runs(xq, dx, TYPE, false, m0 >> 4, T::first_a(wave) * 1024, step_a);
   constexpr int PER = T::B / G;                 // a stage's bytes of one weight matrix
   const int ob = wave * T::LB * 1024;
   const kq4_rsrc4 rb = runs(a.w[ob / PER], dw, 4, false, n0 >> 4, ob % PER, step_b);
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
 #pragma unroll
   for (int l = 0; l < T::SPW; ++l) {
     const int o = (min(wave * T::SPW, T::SLOADS - T::SPW) + l) * 1024;
-    if (o < SA) rs[l] = runs(a.x, dx, TYPE, true, m0 >> 4, o, step_s[l]);
+    if (o < SA) rs[l] = runs(xq, dx, TYPE, true, m0 >> 4, o, step_s[l]);
     else rs[l] = runs(a.w[(o - SA) / SB], dw, 4, true, n0 >> 4, (o - SA) % SB, step_s[l]);
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)&lds[0];
@@ -362,7 +363,7 @@ static int launch(const KQ4MxArgs &a, int ksplit, hipStream_t s) {
   hipError_t e = kq4_lds_limit_once(reinterpret_cast<const void *>(k), T::LDS, done);
   if (e != hipSuccess) return (int)e;
   const int mt = (a.n + T::BM - 1) / T::BM, nt = (a.rows + T::BN / G - 1) / (T::BN / G);
-  const int per = (a.dw.kq + ksplit - 1) / ksplit;   // (every slice has some: kq4_mx_split)
+  const int kq = kq4_mx_dims(a.rows, a.cols).kq, per = (kq + ksplit - 1) / ksplit;   // (every slice has some: kq4_mx_split)
   hipLaunchKernelGGL(k, dim3((unsigned)mt * nt * ksplit), dim3(64 * T::NW), T::LDS, s, a, mt, nt, ksplit, per);
   e = hipGetLastError();
   if (e != hipSuccess || ksplit == 1) return (int)e;

@@ -10,24 +10,26 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 as they lie, a tile one 16-byte load per lane.
 // The activations come the same way from a quantized matrix (FQ = 0), or the workgroup quantizes the fp32 rows into LDS
 // while its first weights are on their way (FQ = 1): one launch instead of two. Loads return in order, so what is needed
-// first is asked for first: the activations before the weights.
-template <int TYPE, int G, int RT, int TT, int NW, bool FQ>
-__global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int ks, int mtiles) {
+// first is asked for first: the activations before the weights. AHEAD: all loads of a piece are on their way before its
+// first product; left alone they alternate with the products in fewer registers. It pays with fewer than 8
+// waves a CU (64 x 4096 x 12288: 12.1 us with, 15.8 without) and costs above (256 x 4096 x 4096: 11.3 with, 10.4 without).
+template <int TYPE, int G, int RT, int TT, int NW, bool FQ, bool AHEAD>
+__global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int ks, int mtiles, int all) {
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
   constexpr int W = G * RT;                              // weight tiles of a wave: [matrix][row tile]
   // XCD x works on a run of row tiles, each against all tokens before the next: its cache reads the weights once
-  const int all = gridDim.x, xcd = blockIdx.x & 7, q8 = all >> 3, r8 = all & 7;
+  const int xcd = blockIdx.x & 7, q8 = all >> 3, r8 = all & 7;
   const int v = xcd * q8 + (xcd < r8 ? xcd : r8) + (int)(blockIdx.x >> 3);
   const int t = (v / mtiles * (NW / ks) + wave / ks) * RT, slice = wave % ks, m0 = v % mtiles * TT;
-  const KQ4MxDims dw = a.dw, dx = a.dx;
-  long wstep[W];
+  const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
+  uint32_t wstep[W];   // from a tile to the next, in tiles (a row tile's offsets stay below 2^32: cols <= 2^20)
   const uint8_t *w[W], *ws[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) {
     const int tc = min(t + i % RT, dw.nt - 1);           // past the last tile: that one again, not stored
-    wstep[i] = kq4_mx_step(tc, dw.nt);
+    wstep[i] = (uint32_t)kq4_mx_step(tc, dw.nt);
     w[i] = a.w[i / RT] + kq4_mx_first(tc, dw.kt) * 1024;
     ws[i] = a.w[i / RT] + kq4_mx_codes_size(dw, 4) + kq4_mx_first(tc, dw.kq) * KQ4_MX_STILE;
   }
@@ -35,11 +37,13 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
 
   // FQ: [token][block] codes (their first 16 bytes, then the rest of all), then [token][512 columns][4] scale dwords
   const int nb = 4 * dw.kt, nbs = 16 * nq, real = a.cols >> 5;   // blocks of a token: with codes, with scales, with values
-  uint8_t *xc = lds, *xr = lds + (size_t)a.n * nb * 16, *xsc = xr + (TYPE == 6 ? (size_t)a.n * nb * 8 : 0);
+  const int nt = min(16 * TT, a.n - 16 * m0);                    // the workgroup's tokens
+  uint8_t *xc = lds, *xr = lds + (size_t)nt * nb * 16, *xsc = xr + (TYPE == 6 ? (size_t)nt * nb * 8 : 0);
   float4 fx[8];
   auto fetch = [&](int e) {
     const int t = e / nbs, b = min(e - t * nbs, real - 1);       // (a block past the columns: the last one, not used)
-    const float4 *p = reinterpret_cast<const float4 *>(a.xf + (size_t)min(t, a.n - 1) * a.ldx + 32 * b);
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.x) +
+                                                       (size_t)(16 * m0 + min(t, nt - 1)) * a.ldx + 32 * b);
 #pragma unroll
     for (int i = 0; i < 8; ++i) fx[i] = p[i];
   };
@@ -64,16 +68,15 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
     }
     xsc[((size_t)t * nq + (b >> 4)) * 16 + 4 * (b & 3) + ((b >> 2) & 3)] = (uint8_t)s;
   };
-  const int tok = min(r16, a.n - 1);                     // FQ: lanes past the tokens repeat the last one
   const uint8_t *x[TT], *xs[TT];
-  long xstep[TT];
+  uint32_t xstep[TT];
   if constexpr (!FQ) {
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
       const int u = min(m0 + i, dx.nt - 1);
-      xstep[i] = kq4_mx_step(u, dx.nt);
-      x[i] = a.x + kq4_mx_first(u, dx.kt) * (256 * TYPE);
-      xs[i] = a.x + kq4_mx_codes_size(dx, TYPE) + kq4_mx_first(u, dx.kq) * KQ4_MX_STILE;
+      xstep[i] = (uint32_t)kq4_mx_step(u, dx.nt);
+      x[i] = static_cast<const uint8_t *>(a.x) + kq4_mx_first(u, dx.kt) * (256 * TYPE);
+      xs[i] = static_cast<const uint8_t *>(a.x) + kq4_mx_codes_size(dx, TYPE) + kq4_mx_first(u, dx.kq) * KQ4_MX_STILE;
     }
   }
 
@@ -86,8 +89,9 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
   auto load_x = [&](Acts &p, int q) {
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
+      const int tok = min(16 * j + r16, nt - 1);         // FQ: lanes past the tokens repeat the last one
       if constexpr (FQ) p.s[j] = *reinterpret_cast<const uint32_t *>(xsc + ((size_t)tok * nq + q) * 16 + 4 * g4);
-      else p.s[j] = reinterpret_cast<const uint32_t *>(xs[j] + q * xstep[j] * KQ4_MX_STILE)[lane];
+      else p.s[j] = reinterpret_cast<const uint32_t *>(xs[j] + (uint32_t)q * (xstep[j] * KQ4_MX_STILE))[lane];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int k = min(4 * q + s, last);
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
           p.c[s][j] = *reinterpret_cast<const uint4 *>(xc + b * 16);
           if constexpr (TYPE == 6) p.r[s][j] = *reinterpret_cast<const uint2 *>(xr + b * 8);
         } else {
-          const uint8_t *c = x[j] + k * xstep[j] * (256 * TYPE);
+          const uint8_t *c = x[j] + (uint32_t)k * (xstep[j] * (256 * TYPE));
           p.c[s][j] = reinterpret_cast<const uint4 *>(c)[lane];
           if constexpr (TYPE == 6) p.r[s][j] = reinterpret_cast<const uint2 *>(c + 1024)[lane];
         }
@@ -111,11 +115,12 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
   auto load_w = [&](Weights &p, int q) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const uint32_t *sp = reinterpret_cast<const uint32_t *>(ws[i] + q * wstep[i] * KQ4_MX_STILE) + lane;
+      const uint32_t *sp = reinterpret_cast<const uint32_t *>(ws[i] + (uint32_t)q * (wstep[i] * KQ4_MX_STILE)) + lane;
       p.s[i] = TT == 1 ? __builtin_nontemporal_load(sp) : *sp;   // (several workgroups read them for more tokens)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const kq4_v4u *cp = reinterpret_cast<const kq4_v4u *>(w[i] + min(4 * q + j, last) * wstep[i] * 1024) + lane;
+        const kq4_v4u *cp =
+            reinterpret_cast<const kq4_v4u *>(w[i] + (uint32_t)min(4 * q + j, last) * (wstep[i] * 1024)) + lane;
         p.c[i][j] = TT == 1 ? __builtin_nontemporal_load(cp) : *cp;
       }
     }
@@ -149,8 +154,8 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
   if constexpr (FQ) {
     fetch(threadIdx.x);
     load_w(pw, min(slice, nq - 1));
-    for (int e = threadIdx.x; e < a.n * nbs; e += blockDim.x) {
-      if (e >= (int)blockDim.x) fetch(e);
+    for (int e = threadIdx.x; e < nt * nbs; e += 64 * NW) {
+      if (e >= 64 * NW) fetch(e);
       quantize(e);
     }
     __syncthreads();
@@ -159,6 +164,7 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
     Acts px;
     load_x(px, q);
     if (!FQ || q != slice) load_w(pw, q);
+    if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
     products(pw, px);
   }
 
@@ -202,20 +208,21 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
 // LDS of the activations that a workgroup quantizes itself.
 static size_t kq4_mx_rows_lds(int n, const KQ4MxDims &d, int type) { return (size_t)n * (4 * d.kt * 4 * type + 16 * d.kq); }
 
-template <int TYPE, int G, int RT, int TT, int NW, bool FQ>
+template <int TYPE, int G, int RT, int TT, int NW, bool FQ, bool AHEAD>
 static int launch(const KQ4MxArgs &a, int ks, hipStream_t s) {
-  const int tpw = NW / ks * RT, mtiles = FQ ? 1 : (a.dx.nt + TT - 1) / TT;
-  const dim3 grid((unsigned)((a.dw.nt + tpw - 1) / tpw) * mtiles);
-  const size_t red = ks > 1 ? (size_t)NW * G * RT * TT * 1024 : 0, x = FQ ? kq4_mx_rows_lds(a.n, a.dw, TYPE) : 0;
-  hipLaunchKernelGGL((kq4_mx_rows_kernel<TYPE, G, RT, TT, NW, FQ>), grid, dim3(64 * NW), red > x ? red : x, s, a, ks, mtiles);
+  const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
+  const int tpw = NW / ks * RT, mtiles = (dx.nt + TT - 1) / TT, all = (dw.nt + tpw - 1) / tpw * mtiles;
+  const size_t red = ks > 1 ? (size_t)NW * G * RT * TT * 1024 : 0, x = FQ ? kq4_mx_rows_lds(min(a.n, 16 * TT), dw, TYPE) : 0;
+  hipLaunchKernelGGL((kq4_mx_rows_kernel<TYPE, G, RT, TT, NW, FQ, AHEAD>), dim3((unsigned)all), dim3(64 * NW), red > x ? red : x, s,
+                     a, ks, mtiles, all);
   return (int)hipGetLastError();
 }
 
-// The waves that share a row tile: 8 (a workgroup) where K has that many pieces and the launch then is at most 16 waves a
+// The waves that share a row tile: 8 (a workgroup) where K has that many pieces and the launch then is at most 8 waves a
 // CU, else 4 or as many as there are pieces, in workgroups of 4 waves. One token: 4096 x 4096 4.4 us with 8 and 4.9 with 4,
 // 12288 x 4096 8.2 and 7.0, 151936 x 2048 51 and 26.
 static int slices(const KQ4MxDims &dw, long tiles, int ncu) {
-  if (dw.kq >= 8 && tiles * 8 <= 16L * ncu) return 8;
+  if (dw.kq >= 8 && tiles <= ncu) return 8;
   int ks = 4;
   while (ks > dw.kq) ks /= 2;
   return ks;
@@ -223,13 +230,16 @@ static int slices(const KQ4MxDims &dw, long tiles, int ncu) {
 
 template <int TYPE, int G, int RT, int TT, bool FQ>
 static int launch_k(const KQ4MxArgs &a, int ncu, hipStream_t s) {
-  const int ks = slices(a.dw, (long)((a.dw.nt + RT - 1) / RT) * ((a.dx.nt + TT - 1) / TT), ncu);
-  return ks == 8 ? launch<TYPE, G, RT, TT, 8, FQ>(a, ks, s) : launch<TYPE, G, RT, TT, 4, FQ>(a, ks, s);
+  const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
+  const long tiles = (long)((dw.nt + RT - 1) / RT) * ((dx.nt + TT - 1) / TT);
+  const int ks = slices(dw, tiles, ncu);
+  if (ks == 8) return launch<TYPE, G, RT, TT, 8, FQ, true>(a, ks, s);
+  return tiles * ks < 8L * ncu ? launch<TYPE, G, RT, TT, 4, FQ, true>(a, ks, s) : launch<TYPE, G, RT, TT, 4, FQ, false>(a, ks, s);
 }
 
 template <int TYPE, int G>
 static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
-  if (a.xf) return launch_k<TYPE, G, 1, 1, true>(a, ncu, s);
+  if (a.ldx) return a.n <= 16 ? launch_k<TYPE, G, 1, 1, true>(a, ncu, s) : launch_k<TYPE, G, 1, 2, true>(a, ncu, s);
   if (a.n <= 16) return launch_k<TYPE, G, 1, 1, false>(a, ncu, s);
   if (a.n <= 32) return launch_k<TYPE, G, 1, 2, false>(a, ncu, s);
   if constexpr (G == 2) return launch_k<TYPE, G, 1, 4, false>(a, ncu, s);
@@ -241,14 +251,15 @@ int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
   return type == 4 ? launch_t<4, 1>(a, ncu, s) : launch_t<6, 1>(a, ncu, s);
 }
 
-// Every workgroup quantizes all the activations, 0.12 us for 1000 elements of each workgroup that its CU runs, against a
+// Every workgroup quantizes its tokens' activations, 0.12 us for 1000 elements of each workgroup that its CU runs, against a
 // launch of the quantizer (2.5 to 3.4 us, and as much of the host's time). Worth it up to 32768 elements a CU (4096 x 4096:
 // four tokens 6.4 us against 7.4, eight 8.3 against 7.8 and a launch less, sixteen 12.3 against 7.8), and where the weights
 // take the memory longer than that anyway (151936 x 2048: one token 26 against 38 us, eight 80 against 38).
 bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
-  if (n > 16 || kq4_mx_rows_lds(n, d, type) > 64 * 1024) return false;
-  const int ks = slices(d, d.nt, ncu), tpw = (ks == 8 ? 8 : 4) / ks;
-  const double wgs = (d.nt + tpw - 1) / tpw, each = (double)((long)((wgs + ncu - 1) / ncu)) * n * cols;
-  return each <= 32768.0 || each * 0.12e-3 <= 0.4 * matrices * rows * (double)cols * 0.53 / 6.0e6;
+  const int tiles = n <= 16 ? 1 : 2, tokens = min(n, 16 * tiles), mtiles = (n + 16 * tiles - 1) / (16 * tiles);
+  if (kq4_mx_rows_lds(tokens, d, type) > 64 * 1024) return false;
+  const int ks = slices(d, (long)d.nt * mtiles, ncu), tpw = (ks == 8 ? 8 : 4) / ks;
+  const double wgs = (double)((d.nt + tpw - 1) / tpw) * mtiles, each = (double)((long)((wgs + ncu - 1) / ncu)) * tokens * cols;
+  return each <= 32768.0 || (n <= 16 && each * 0.12e-3 <= 0.4 * matrices * rows * (double)cols * 0.53 / 6.0e6);
 }
