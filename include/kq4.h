@@ -512,7 +512,7 @@ size_t kq4_logprobs_workspace_bytes(int n, int vocab, int n_top);
 size_t kq4_mx_bytes(int rows, int cols, int type);
 
 /* fp32 rows (row t at x + t * ldx floats; 16-byte aligned, ldx a multiple of 4) into a microscaled
- * matrix of `type` bits. A block's scale is the least 2^e, e >= -127, for which its largest
+ * matrix of `type` bits that does not overlap them. A block's scale is the least 2^e, e >= -127, for which its largest
  * magnitude over 2^e, rounded to the element's precision, is not above the largest element (so no
  * element is off by more than half a step of its format); an element is the nearest one to x / 2^e,
  * ties to even, signs of zeros kept. A block that holds a NaN or infinity gets scale 255, codes 0.
@@ -521,8 +521,9 @@ int kq4_mx_quantize_dev(uint8_t *m, const float *x, long ldx, int rows, int cols
                         void *stream);
 
 /* A checkpoint's row-major codes ([rows][cols * type / 8] bytes, a 4-bit element's even column in
- * the low half, 6-bit ones one after the other from the lowest bits; 16-byte aligned) and scales ([rows][cols / 32] bytes) into a microscaled matrix,
- * once per weight matrix, and back. Matrices of whole groups of 128 rows may be stacked by packing
+ * the low half, 6-bit ones one after the other from the lowest bits; 16-byte aligned) and scales
+ * ([rows][cols / 32] bytes) into a microscaled matrix, once per weight matrix, and back; the three do
+ * not overlap. Matrices of whole groups of 128 rows may be stacked by packing
  * them as one of their summed rows. */
 int kq4_mx_pack_dev(uint8_t *m, const uint8_t *codes, const uint8_t *scales, int rows, int cols,
                     int type, void *stream);
@@ -533,13 +534,13 @@ int kq4_mx_unpack_dev(uint8_t *codes, uint8_t *scales, const uint8_t *m, int row
  * fp32 rows (as for kq4_mx_quantize_dev) quantized to `act` bits (KQ4_MX_FP6: a quarter of FP4's
  * steps), sums in fp32 (an output's sum below 2^-126 is zero). Token t's outputs are at out + t * ldo floats,
  * its residual at residual + t * ldo (4-byte aligned; residual may be NULL or out, and must not
- * overlap out otherwise; out must not overlap x). A NaN block of a row of x makes that token's
+ * overlap out otherwise; out must not overlap x or W). A NaN block of a row of x makes that token's
  * outputs NaN, one of W that row's. The order of a token's sums goes with the shape of the call:
  * the same token in a batch of another size is equal within rounding, the same call to the bit. */
 int kq4_mx_matmul_dev(float *out, long ldo, const float *x, long ldx, const float *residual,
                       const uint8_t *w, int rows, int cols, int n_batch, int act, void *stream);
 /* The same from rows that are quantized already (xq: a matrix of n_batch x cols of `act` bits), for
- * several products of one activation (Q, K and V). Uses no workspace for xq. */
+ * several products of one activation (Q, K and V); out must not overlap xq. Uses no workspace for xq. */
 int kq4_mx_matmul_q_dev(float *out, long ldo, const uint8_t *xq, const float *residual,
                         const uint8_t *w, int rows, int cols, int n_batch, int act, void *stream);
 
@@ -558,7 +559,7 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
 /* Workspace bytes that hold every product and gated call of up to n_batch tokens and cols columns
  * (whatever its rows and act), and every whole block of up to these sizes; 0 for a bad shape. From
  * 17 tokens on they include 32 MiB for the sums of a split K (the planner's splits never need more;
- * one forced through mx_split may). */
+ * a GEMM forced through mx_form at fewer tokens does, a split forced through mx_split may). */
 size_t kq4_mx_workspace_bytes(int n_batch, int cols);
 size_t kq4_mx_ffn_workspace_bytes(int n_batch, int dim, int ffn);
 

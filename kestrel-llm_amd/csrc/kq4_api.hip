@@ -1423,9 +1423,22 @@ bool rows_overlap(const float *p, long ldp, long w, long n, const float *q, long
   return off < w * sizeof(float) || off + v * sizeof(float) > ld;
 }
 
-// The checks that the products share. x: fp32 rows, or nullptr where xq is the activations.
+// Whether np bytes at p and nq bytes at q share any.
+bool bytes_overlap(const void *p, size_t np, const void *q, size_t nq) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return a < b + nq && b < a + np;
+}
+
+size_t rows_bytes(long ld, long width, long n) { return ((n - 1) * (size_t)ld + width) * sizeof(float); }
+
+// Whether the n rows of out share memory with a microscaled matrix (nullptr: none).
+bool mx_out_overlap(const float *out, long ldo, long width, long n, const uint8_t *m, int rows, int cols, int type) {
+  return m && bytes_overlap(out, rows_bytes(ldo, width, n), m, kq4_mx_size(kq4_mx_dims(rows, cols), type));
+}
+
+// The checks that the products share. x: fp32 rows, or nullptr where xq is the activations. w0, w1: weights of rows x cols.
 int mx_product_check(const char *what, const float *out, long ldo, const float *x, long ldx, const uint8_t *xq,
-                     const float *residual, int rows, int cols, int n, int act) {
+                     const float *residual, const uint8_t *w0, const uint8_t *w1, int rows, int cols, int n, int act) {
   int rc;
   if (n < 0) return fail(KQ4_EINVAL, "%s: n_batch=%d", what, n);
   if (act != KQ4_MX_FP4 && act != KQ4_MX_FP6) return fail(KQ4_EINVAL, "%s: act=%d (4 or 6)", what, act);
@@ -1443,6 +1456,19 @@ int mx_product_check(const char *what, const float *out, long ldo, const float *
   if (x && rows_overlap(out, ldo, rows, n, x, ldx, cols, n)) return fail(KQ4_EINVAL, "%s: out overlaps x", what);
   if (residual && residual != out && rows_overlap(out, ldo, rows, n, residual, ldo, rows, n))
     return fail(KQ4_EINVAL, "%s: out overlaps the residual and is not it", what);
+  if (mx_out_overlap(out, ldo, rows, n, xq, n, cols, act) || mx_out_overlap(out, ldo, rows, n, w0, rows, cols, KQ4_MX_FP4) ||
+      mx_out_overlap(out, ldo, rows, n, w1, rows, cols, KQ4_MX_FP4))
+    return fail(KQ4_EINVAL, "%s: out overlaps the quantized activations or the weights", what);
+  return KQ4_OK;
+}
+
+// A matrix' row-major codes and scales.
+int mx_row_major_check(const char *what, const uint8_t *m, const uint8_t *codes, const uint8_t *scales, int rows, int cols,
+                       int type) {
+  if (!codes || !scales || (uintptr_t)codes % 16) return fail(KQ4_EINVAL, "%s: codes must be 16-byte aligned", what);
+  const size_t nm = kq4_mx_size(kq4_mx_dims(rows, cols), type), nc = (size_t)rows * (cols / 8) * type, ns = (size_t)rows * (cols / 32);
+  if (bytes_overlap(m, nm, codes, nc) || bytes_overlap(m, nm, scales, ns) || bytes_overlap(codes, nc, scales, ns))
+    return fail(KQ4_EINVAL, "%s: the matrix, its codes and its scales overlap", what);
   return KQ4_OK;
 }
 
@@ -1513,6 +1539,8 @@ int kq4_mx_quantize_dev(uint8_t *m, const float *x, long ldx, int rows, int cols
   if (rows == 0 && mx_shape_ok(1, cols, type)) return KQ4_OK;
   int rc = mx_matrix_check("mx_quantize", "m", m, rows, cols, type);
   if (rc || (rc = rows_check("mx_quantize", "x", x, ldx, cols))) return rc;
+  if (bytes_overlap(m, kq4_mx_bytes(rows, cols, type), x, rows_bytes(ldx, cols, rows)))
+    return fail(KQ4_EINVAL, "mx_quantize: m overlaps x");
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;
   KQ4_HIP((hipError_t)kq4_launch_mx_quantize(m, x, ldx, rows, cols, type, (hipStream_t)stream));
@@ -1523,7 +1551,7 @@ int kq4_mx_pack_dev(uint8_t *m, const uint8_t *codes, const uint8_t *scales, int
                     void *stream) {
   int rc = mx_matrix_check("mx_pack", "m", m, rows, cols, type);
   if (rc) return rc;
-  if (!codes || !scales || (uintptr_t)codes % 16) return fail(KQ4_EINVAL, "mx_pack: codes must be 16-byte aligned");
+  if ((rc = mx_row_major_check("mx_pack", m, codes, scales, rows, cols, type))) return rc;
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;
   KQ4_HIP((hipError_t)kq4_launch_mx_pack(m, const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales), rows, cols,
@@ -1535,7 +1563,7 @@ int kq4_mx_unpack_dev(uint8_t *codes, uint8_t *scales, const uint8_t *m, int row
                       void *stream) {
   int rc = mx_matrix_check("mx_unpack", "m", m, rows, cols, type);
   if (rc) return rc;
-  if (!codes || !scales || (uintptr_t)codes % 16) return fail(KQ4_EINVAL, "mx_unpack: codes must be 16-byte aligned");
+  if ((rc = mx_row_major_check("mx_unpack", m, codes, scales, rows, cols, type))) return rc;
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;
   KQ4_HIP((hipError_t)kq4_launch_mx_pack(const_cast<uint8_t *>(m), codes, scales, rows, cols, type, false,
@@ -1546,7 +1574,7 @@ int kq4_mx_unpack_dev(uint8_t *codes, uint8_t *scales, const uint8_t *m, int row
 int kq4_mx_matmul_dev(float *out, long ldo, const float *x, long ldx, const float *residual, const uint8_t *w,
                       int rows, int cols, int n_batch, int act, void *stream) {
   int rc = mx_matrix_check("mx_matmul", "w", w, rows, cols, KQ4_MX_FP4);
-  if (rc || (rc = mx_product_check("mx_matmul", out, ldo, x, ldx, nullptr, residual, rows, cols, n_batch, act)) || !n_batch)
+  if (rc || (rc = mx_product_check("mx_matmul", out, ldo, x, ldx, nullptr, residual, w, nullptr, rows, cols, n_batch, act)) || !n_batch)
     return rc;
   return mx_product(out, ldo, x, ldx, nullptr, residual, w, nullptr, rows, cols, n_batch, act, (hipStream_t)stream);
 }
@@ -1555,7 +1583,7 @@ int kq4_mx_matmul_q_dev(float *out, long ldo, const uint8_t *xq, const float *re
                         int cols, int n_batch, int act, void *stream) {
   int rc = mx_matrix_check("mx_matmul_q", "w", w, rows, cols, KQ4_MX_FP4);
   if (!rc && n_batch > 0 && !xq) return fail(KQ4_EINVAL, "mx_matmul_q: xq must be 16-byte aligned");
-  if (rc || (rc = mx_product_check("mx_matmul_q", out, ldo, nullptr, 0, xq, residual, rows, cols, n_batch, act)) || !n_batch)
+  if (rc || (rc = mx_product_check("mx_matmul_q", out, ldo, nullptr, 0, xq, residual, w, nullptr, rows, cols, n_batch, act)) || !n_batch)
     return rc;
   return mx_product(out, ldo, nullptr, 0, xq, residual, w, nullptr, rows, cols, n_batch, act, (hipStream_t)stream);
 }
@@ -1564,7 +1592,7 @@ int kq4_mx_gated_dev(float *out, long ldo, const float *x, long ldx, const uint8
                      int cols, int n_batch, int act, void *stream) {
   int rc = mx_matrix_check("mx_gated", "gate", gate, rows, cols, KQ4_MX_FP4);
   if (rc || (rc = mx_matrix_check("mx_gated", "up", up, rows, cols, KQ4_MX_FP4)) ||
-      (rc = mx_product_check("mx_gated", out, ldo, x, ldx, nullptr, nullptr, rows, cols, n_batch, act)) || !n_batch)
+      (rc = mx_product_check("mx_gated", out, ldo, x, ldx, nullptr, nullptr, gate, up, rows, cols, n_batch, act)) || !n_batch)
     return rc;
   return mx_product(out, ldo, x, ldx, nullptr, nullptr, gate, up, rows, cols, n_batch, act, (hipStream_t)stream);
 }
@@ -1574,8 +1602,11 @@ int kq4_mx_ffn_dev(float *out, long ldo, const float *x, long ldx, const float *
   int rc = mx_matrix_check("mx_ffn", "gate", gate, ffn, dim, KQ4_MX_FP4);
   if (rc || (rc = mx_matrix_check("mx_ffn", "up", up, ffn, dim, KQ4_MX_FP4)) ||
       (rc = mx_matrix_check("mx_ffn", "down", down, dim, ffn, KQ4_MX_FP4)) ||
-      (rc = mx_product_check("mx_ffn", out, ldo, x, ldx, nullptr, residual, dim, dim, n_batch, act)) || !n_batch)
+      (rc = mx_product_check("mx_ffn", out, ldo, x, ldx, nullptr, residual, nullptr, nullptr, dim, dim, n_batch, act)) || !n_batch)
     return rc;
+  for (const uint8_t *w : {gate, up, down})
+    if (mx_out_overlap(out, ldo, dim, n_batch, w, w == down ? dim : ffn, w == down ? ffn : dim, KQ4_MX_FP4))
+      return fail(KQ4_EINVAL, "mx_ffn: out overlaps the weights");
   if (!mx_shape_ok(n_batch, ffn, act)) return fail(KQ4_EINVAL, "mx_ffn: n_batch=%d ffn=%d", n_batch, ffn);
   DevState *ds = nullptr;
   if ((rc = cur_dev(&ds))) return rc;

@@ -36,7 +36,8 @@ KQ4_DEV void kq4_mx_load(const kq4_rsrc4 &r, uint32_t v16, uint32_t soff, uint32
   if constexpr (N >= 4)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
                  "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds\n\tbuffer_load_dwordx4 %1, %2, %3 offen offset:2048 lds\n\t"
-                 "buffer_load_dwordx4 %1, %2, %3 offen offset:3072 lds" ::"s"(to), "v"(v16), "s"(r), "s"(soff) : "memory", "m0");
+                 "buffer_load_dwordx4 %1, %2, %3 offen offset:%4 lds" ::"s"(to), "v"(v16), "s"(r), "s"(soff), "n"(3 * 1024)
+                 : "memory", "m0");
   else if constexpr (N == 3)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
                  "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds\n\tbuffer_load_dwordx4 %1, %2, %3 offen offset:2048 lds"

@@ -773,12 +773,16 @@ def rope_table(rows, dim, theta, device="cuda"):
 
 def _check_here(device, name):
     """Raises unless `device` (an index) is the current one, which the call's launches go to."""
+    if _torch is None:
+        lib()
     if device != _torch.cuda.current_device():
         raise KQ4Error(f"{name}: on device {device}, the current device is {_torch.cuda.current_device()}")
 
 
 def _rows(t, name, n, width, device):
     """Row stride of a [>= n][width] fp32 tensor on `device` with unit column stride, checked."""
+    if _torch is None:
+        lib()
     if isinstance(t, _torch.Tensor) and t.dtype is _torch.float32 and t.get_device() == device:
         shape = t.shape
         if len(shape) == 2 and shape[0] >= n and shape[1] == width:
@@ -943,6 +947,8 @@ def mx_ffn_workspace_bytes(n, dim, ffn):
 
 def mx_quantize_dev(m, x, stream=None):
     """fp32 x [rows][cols] (unit column stride) into the microscaled matrix m."""
+    if not isinstance(m, MX):
+        raise KQ4Error("m: expected an MX")
     rows, cols, dev = m.rows, m.cols, m.device
     ldx = _rows(x, "x", rows, cols, dev)
     _check_here(dev, "m")
@@ -952,6 +958,8 @@ def mx_quantize_dev(m, x, stream=None):
 
 def _mx_row_major(m, codes, scales):
     import torch
+    if not isinstance(m, MX):
+        raise KQ4Error("m: expected an MX")
     _need_on(codes, "codes", torch.uint8, m.device, m.rows * m.cols * m.type // 8)
     _need_on(scales, "scales", torch.uint8, m.device, m.rows * m.cols // 32)
     _check_here(m.device, "m")

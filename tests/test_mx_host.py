@@ -1,7 +1,12 @@
 """The host side of the microscaled calls without a GPU, on the stand-in for the HIP runtime (tests/c/hip_standin.c):
 what they refuse, launch and ask of the workspace; and the binding's refusals."""
+import os
+import subprocess
+import sys
+
 import pytest
 
+import kq4
 from test_workspace_routes import standin  # noqa: F401
 
 SETUP = """
@@ -52,6 +57,11 @@ def launched(f):
     "ffn(gate=None)", "ffn(up=None)", "ffn(down=None)", "ffn(down=at(6) + 8)", "ffn(ffn=300)", "ffn(ffn=0)", "ffn(dim=0)",
     "ffn(dim=500)", "ffn(ldo=500)", "ffn(out=at(2))", "ffn(act=1)", "ffn(x=None)", "ffn(out=None)", "ffn(n=-1)",
     "ffn(res=at(1) + 4)", "ffn(n=1 << 24, ffn=16384)",
+    "quantize(m=at(2))", "quantize(m=at(2) + 16 * 512)", "quantize(x=at(1) + 16 * 256)", "pack(m=at(2))", "pack(scales=at(2) + 1279)",
+    "pack(m=at(3))", "unpack(m=at(2) + 1264)", "unpack(scales=at(1) + 16 * 256 + 255)", "unpack(scales=at(2))",
+    "matmul_q(out=at(2))", "matmul_q(out=at(2) + 16 * 384 + 252, res=None)", "matmul_q(xq=at(1) + 4 * 5 * 300 - 8 - 8)",
+    "matmul_q(out=at(4))", "matmul(out=at(4) + 19 * 16 * 256, res=None)", "matmul(w=at(1) + 16, res=None)", "gated(out=at(3) + 64)",
+    "gated(out=at(4))", "ffn(out=at(4), res=None)", "ffn(out=at(5) + 256, res=None)", "ffn(out=at(6), res=None)",
 ])
 def test_refusals(standin, call):  # noqa: F811
     assert standin(SETUP + f"result = launched(lambda: {call})") == [-1, 0]
@@ -68,7 +78,8 @@ def test_calls_that_are_taken(standin):  # noqa: F811
     calls = ["matmul(res=None)", "matmul(res=at(1))", "matmul(out=at(2) + 4 * 512, ldo=1024, ldx=1024, res=None)",
              "matmul(x=at(1) + 4 * 304, ldx=816, ldo=816, res=None)", "gated(out=at(2) + 4 * 512, ldo=812, ldx=812)",
              "matmul(res=at(1) + 4 * 5 * 300)", "matmul_q(res=at(1))", "ffn(res=None)", "ffn(res=at(1))", "quantize(type=6)", "pack(type=6)",
-             "unpack()"]
+             "unpack()", "quantize(m=at(2) + 5 * 512 * 4)", "quantize(x=at(1) + 17 * 256)", "pack(scales=at(2) + 1280)",
+             "matmul_q(out=at(2) + 16 * 384 + 256)"]
     body = "result = [launched(f)[0] for f in (" + ", ".join(f"lambda: {c}" for c in calls) + ",)]"
     assert standin(SETUP + body) == [0] * len(calls)
 
@@ -152,3 +163,15 @@ def test_binding_refuses_host_tensors_and_shapes(kq4_cpu):
         kq4_cpu.mx_matmul_q_dev(None, torch.zeros(1, 64), None)
     with pytest.raises(kq4_cpu.KQ4Error, match="expected a 4-bit MX"):
         kq4_cpu.mx_gated_dev(None, torch.zeros(1, 64), None, None)
+    for call in (lambda: kq4_cpu.mx_quantize_dev(None, torch.zeros(1, 64)),
+                 lambda: kq4_cpu.mx_pack_dev(None, torch.zeros(1, 32, dtype=torch.uint8), torch.zeros(1, 2, dtype=torch.uint8))):
+        with pytest.raises(kq4_cpu.KQ4Error, match="expected an MX"):
+            call()
+
+
+def test_the_bindings_first_call_may_be_any():
+    """Without a call before it that loads the library: the binding's own error."""
+    code = ("import sys, torch; sys.path.insert(0, %r)\nimport kq4\n"
+            "try: kq4.logprobs_dev(torch.zeros(2, 8))\nexcept kq4.KQ4Error as e: assert 'device' in str(e), e\nelse: assert 0\n"
+            % os.path.dirname(kq4.__file__))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
