@@ -60,5 +60,12 @@ constexpr int kq4_mx_fmt = TYPE == 4 ? 4 : 2;
 
 KQ4_DEV uint32_t kq4_absbits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// silu(g) * u. exp(-g) may overflow: g / inf is the limit.
-KQ4_DEV float kq4_mx_gate(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u = g / (1 + e^-g) * u, e^-g as 2^(-g log2 e) with the product's rounding put right to first order: off by less
+// than 2^-21 of the result (1 ulp each of exp2 and the reciprocal, half of one each of four others). exp may overflow: g / inf
+// is the limit, and past 200 nothing of it is left either way.
+KQ4_DEV float kq4_mx_gate(float g, float u) {
+  const float a = -__builtin_amdgcn_fmed3f(g, -200.0f, 200.0f), hi = a * 1.44269504f;
+  const float lo = fmaf(a, 1.92596303e-8f, fmaf(a, 1.44269504f, -hi));
+  const float e = __builtin_amdgcn_exp2f(hi) * fmaf(lo, 0.693147181f, 1.0f);
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
