@@ -10,7 +10,10 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 as they lie, a tile one 16-byte load per lane.
 // The activations come the same way from a quantized matrix (FQ = 0), or the workgroup quantizes the fp32 rows into LDS
 // while its first weights are on their way (FQ = 1): one launch instead of two. Loads return in order, so what is needed
-// first is asked for first: the activations before the weights. AHEAD: all loads of a piece are on their way before its
+// first is asked for first: the activations before the weights. What bounds it: the weights' bytes where they are many (one
+// token: 151936 x 2048 27 us, 6.1 TB/s; 2 x 12288 x 4096 gated 11 us, 4.9 TB/s with what starts and ends it), the latency of
+// a piece below (4096 x 4096 4.4 us), the operands' way through the L2 caches for more tokens (64 x 4096 x 12288, 6 bits: 12 us for
+// 132 MB, 11 TB/s). AHEAD: all loads of a piece are on their way before its
 // first product; left alone they alternate with the products in fewer registers. It pays with fewer than 8
 // waves a CU (64 x 4096 x 12288: 12.1 us with, 15.8 without) and costs above (256 x 4096 x 4096: 11.3 with, 10.4 without).
 template <int TYPE, int G, int RT, int TT, int NW, bool FQ, bool AHEAD>
@@ -237,13 +240,19 @@ static int launch_k(const KQ4MxArgs &a, int ncu, hipStream_t s) {
   return tiles * ks < 8L * ncu ? launch<TYPE, G, RT, TT, 4, FQ, true>(a, ks, s) : launch<TYPE, G, RT, TT, 4, FQ, false>(a, ks, s);
 }
 
+// A wave's tile: the smallest with at most 1.75 tiles a CU, as few waves cover a piece's latency badly (128 x 1024 x 1024, 6
+// bits: 3.0 us with 16 rows x 16 tokens, 4.3 with 32 x 32); else the largest, which loads the least (128 x 4096 x 12288: 14.2 with
+// 32 x 64, 19.2 with 32 x 32). One tile of tokens where there are 16 or 32 of them. Within 2.7 % of the best of six tiles
+// (17 to 300 tokens of six matrices).
 template <int TYPE, int G>
 static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
-  if (a.ldx) return a.n <= 16 ? launch_k<TYPE, G, 1, 1, true>(a, ncu, s) : launch_k<TYPE, G, 1, 2, true>(a, ncu, s);
-  if (a.n <= 16) return launch_k<TYPE, G, 1, 1, false>(a, ncu, s);
-  if (a.n <= 32) return launch_k<TYPE, G, 1, 2, false>(a, ncu, s);
+  if (a.ldx) return launch_k<TYPE, G, 1, 1, true>(a, ncu, s);
+  const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
+  auto few = [&](int rt, int tt) { return 4L * ((dw.nt + rt - 1) / rt) * ((dx.nt + tt - 1) / tt) <= 7L * ncu; };
+  if (a.n <= 16 || few(1, 1)) return launch_k<TYPE, G, 1, 1, false>(a, ncu, s);
+  if (a.n <= 32 || few(1, 2)) return launch_k<TYPE, G, 1, 2, false>(a, ncu, s);
   if constexpr (G == 2) return launch_k<TYPE, G, 1, 4, false>(a, ncu, s);
-  else return a.n <= 128 ? launch_k<TYPE, G, 2, 2, false>(a, ncu, s) : launch_k<TYPE, G, 2, 4, false>(a, ncu, s);
+  else return few(2, 2) ? launch_k<TYPE, G, 2, 2, false>(a, ncu, s) : launch_k<TYPE, G, 2, 4, false>(a, ncu, s);
 }
 
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
@@ -253,11 +262,11 @@ int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
 
 // Every workgroup quantizes its tokens' activations, 0.12 us for 1000 elements of each workgroup that its CU runs, against a
 // launch of the quantizer (2.5 to 3.4 us, and as much of the host's time). Worth it up to 32768 elements a CU (4096 x 4096:
-// four tokens 6.4 us against 7.4, eight 8.3 against 7.8 and a launch less, sixteen 12.3 against 7.8), and where the weights
-// take the memory longer than that anyway (151936 x 2048: one token 26 against 38 us, eight 80 against 38).
+// four tokens 6.1 us against 7.4, eight 8.0 against 7.4 and a launch less, sixteen 11.8 against 7.5), and where the weights
+// take the memory longer than that anyway (151936 x 2048: one token 27 against 31.5 us, eight 81 against 34).
 bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
-  const int tiles = n <= 16 ? 1 : 2, tokens = min(n, 16 * tiles), mtiles = (n + 16 * tiles - 1) / (16 * tiles);
+  const int tokens = min(n, 16), mtiles = (n + 15) / 16;
   if (kq4_mx_rows_lds(tokens, d, type) > 64 * 1024) return false;
   const int ks = slices(d, (long)d.nt * mtiles, ncu), tpw = (ks == 8 ? 8 : 4) / ks;
   const double wgs = (double)((d.nt + tpw - 1) / tpw) * mtiles, each = (double)((long)((wgs + ncu - 1) / ncu)) * tokens * cols;
