@@ -15,9 +15,8 @@
 // from registers: 5.9 to 7.0). The matrix unit is busy half of the time at 1.83 to 1.87 of 2.4 GHz: the power that it takes
 // lowers the clock, and 256 x 256 tiles, wave tiles of 128 x 128 and finer turns of loads and products came within 6 % of each
 // other. Short K ends in its outputs: 2048 x 12288 x 4096 gated is 115 us, 94 without its 100 MB of stores, which the
-// workgroups, all in step, send at once. Stores and the residual's loads are non-temporal (one matrix of 2048 x
-// 12288 x 4096 69 -> 58 us, 4096 x 4096 x 12288 with a residual and the quantizer 146.3 -> 143.9; a quantizer that reads the
-// outputs next takes no longer for it); priorities that set a CU's two workgroups apart changed nothing.
+// workgroups, all in step, send at once. Priorities that set a CU's two workgroups apart
+// changed nothing. NT: outputs and residual go past the caches (launch_form has when).
 template <int TYPE, int TI, int TJ, int WM, int WN, int S>
 struct KQ4MxTile {
   static constexpr int NW = WM * WN, BM = 32 * TI * WM, BN = 32 * TJ * WN;
@@ -58,7 +57,7 @@ KQ4_DEV void kq4_mx_load(const kq4_rsrc4 &r, uint32_t v16, uint32_t soff, uint32
   if constexpr (N > 4) kq4_mx_load<N - 4>(r, v16, soff + 4096, to + 4096);
 }
 
-template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC>
+template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC, bool NT>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArgs a, int mtiles, int ntiles, int ksplit, int per) {
   using T = KQ4MxTile<TYPE, TI, TJ, WM, WN, S>;
   constexpr int RG = T::BN / G;                 // output rows of the workgroup
@@ -301,7 +300,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
         for (int e = 0; e < 16; ++e) {
           const float *r = a.res + (size_t)min(t0 + 8 * (e >> 2) + (e & 3), a.n - 1) * a.ldo;
 #pragma unroll
-          for (int j = 0; j < TJ / G; ++j) y[e][j] = __builtin_nontemporal_load(r + min(c0 + 32 * j, a.rows - 1));
+          for (int j = 0; j < TJ / G; ++j) {
+            const float *p = r + min(c0 + 32 * j, a.rows - 1);
+            y[e][j] = NT ? __builtin_nontemporal_load(p) : *p;
+          }
         }
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -316,7 +318,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
         float *o = a.out + (size_t)tok * a.ldo + c0;
         if (inside) {
 #pragma unroll
-          for (int j = 0; j < TJ / G; ++j) __builtin_nontemporal_store(y[e][j], o + 32 * j);
+          for (int j = 0; j < TJ / G; ++j) {
+            if constexpr (NT) __builtin_nontemporal_store(y[e][j], o + 32 * j);
+            else o[32 * j] = y[e][j];
+          }
         } else if (tok < a.n) {
 #pragma unroll
           for (int j = 0; j < TJ / G; ++j)
@@ -364,10 +369,10 @@ __global__ __launch_bounds__(256) void kq4_mx_join_kernel(KQ4MxArgs a, int kspli
   }
 }
 
-template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC>
+template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC, bool NT>
 static int launch(const KQ4MxArgs &a, int ksplit, hipStream_t s) {
   using T = KQ4MxTile<TYPE, TI, TJ, WM, WN, S>;
-  auto *k = kq4_mx_gemm_kernel<TYPE, G, TI, TJ, WM, WN, S, OCC>;
+  auto *k = kq4_mx_gemm_kernel<TYPE, G, TI, TJ, WM, WN, S, OCC, NT>;
   static std::atomic<unsigned long long> done{0};
   hipError_t e = kq4_lds_limit_once(reinterpret_cast<const void *>(k), T::LDS, done);
   if (e != hipSuccess) return (int)e;
@@ -391,11 +396,17 @@ int kq4_mx_split(int kq, int want) {
 
 // Launches that leave a workgroup alone on its CU run it in 8 waves of 64 x 64 with a stage more in its ring, two waves per
 // SIMD as elsewhere two workgroups have (512 x 4096 x 4096: 17.3 us instead of 19.4, of 6 bits 20.0 instead of 23.8).
+// Outputs and residuals of KQ4_MX_PAST_CACHE bytes and more go past the caches (non-temporal: 2048 x 12288 x 4096 of one
+// matrix 69 -> 58 us, 4096 x 12288 x 1024 65 -> 44, with a residual 98 -> 85); the memory side's 256 MB hold smaller ones for
+// what reads them next (1796 x 5127 x 64 with a residual 18 us, non-temporal 28; 2048 x 8192 x 512 17 and 20).
+#define KQ4_MX_PAST_CACHE ((size_t)80 << 20)
 template <int TYPE, int G>
 static int launch_form(const KQ4MxArgs &a, int ksplit, int ncu, hipStream_t s) {
   const long wgs = (long)((a.n + 127) / 128) * ((a.rows + 256 / G - 1) / (256 / G)) * ksplit;
-  if (wgs <= ncu) return launch<TYPE, G, 2, 2, 2, 4, 3, 1>(a, ksplit, s);
-  return launch<TYPE, G, 2, 4, 2, 2, TYPE == 4 ? 3 : 2, 2>(a, ksplit, s);
+  if (wgs <= ncu) return launch<TYPE, G, 2, 2, 2, 4, 3, 1, false>(a, ksplit, s);
+  const size_t bytes = ksplit > 1 || a.q ? 0 : (size_t)a.n * a.rows * (a.res ? 8 : 4);
+  if (bytes >= KQ4_MX_PAST_CACHE) return launch<TYPE, G, 2, 4, 2, 2, TYPE == 4 ? 3 : 2, 2, true>(a, ksplit, s);
+  return launch<TYPE, G, 2, 4, 2, 2, TYPE == 4 ? 3 : 2, 2, false>(a, ksplit, s);
 }
 
 int kq4_launch_mx_gemm(const KQ4MxArgs &a, int type, int ksplit, int ncu, hipStream_t s) {

@@ -231,13 +231,37 @@ static int slices(const KQ4MxDims &dw, long tiles, int ncu) {
   return ks;
 }
 
-template <int TYPE, int G, int RT, int TT, bool FQ>
+// The same where the workgroups quantize the activations: past a tile a CU, workgroups of 8 waves and as many slices as
+// leave one workgroup a CU, so that few of them repeat that work (151936 x 2048, three tokens: 28.8 us with 8 waves of a tile each, 40.8
+// with 4 waves on a tile; 50000 x 1024, one token: 6.6 and 10.3; but 12288 x 4096, one token: 7.7 and 7.3).
+static int fused_slices(const KQ4MxDims &dw, long tiles, int ncu, int &waves) {
+  waves = 8;
+  if (tiles <= ncu) {
+    const int ks = slices(dw, tiles, ncu);
+    if (ks < 8) waves = 4;
+    return ks;
+  }
+  int ks = 4;
+  while (ks > 1 && (ks > dw.kq || tiles * ks > 8L * ncu)) ks /= 2;
+  return ks;
+}
+
+template <int TYPE, int G, int RT, int TT>
 static int launch_k(const KQ4MxArgs &a, int ncu, hipStream_t s) {
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   const long tiles = (long)((dw.nt + RT - 1) / RT) * ((dx.nt + TT - 1) / TT);
   const int ks = slices(dw, tiles, ncu);
-  if (ks == 8) return launch<TYPE, G, RT, TT, 8, FQ, true>(a, ks, s);
-  return tiles * ks < 8L * ncu ? launch<TYPE, G, RT, TT, 4, FQ, true>(a, ks, s) : launch<TYPE, G, RT, TT, 4, FQ, false>(a, ks, s);
+  if (ks == 8) return launch<TYPE, G, RT, TT, 8, false, true>(a, ks, s);
+  return tiles * ks < 8L * ncu ? launch<TYPE, G, RT, TT, 4, false, true>(a, ks, s)
+                               : launch<TYPE, G, RT, TT, 4, false, false>(a, ks, s);
+}
+
+template <int TYPE, int G>
+static int launch_fused(const KQ4MxArgs &a, int ncu, hipStream_t s) {
+  const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols);
+  int waves;
+  const int ks = fused_slices(dw, (long)dw.nt * ((a.n + 15) / 16), ncu, waves);
+  return waves == 8 ? launch<TYPE, G, 1, 1, 8, true, false>(a, ks, s) : launch<TYPE, G, 1, 1, 4, true, false>(a, ks, s);
 }
 
 // A wave's tile: the smallest with at most 1.75 tiles a CU, as few waves cover a piece's latency badly (128 x 1024 x 1024, 6
@@ -246,13 +270,13 @@ static int launch_k(const KQ4MxArgs &a, int ncu, hipStream_t s) {
 // (17 to 300 tokens of six matrices).
 template <int TYPE, int G>
 static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
-  if (a.ldx) return launch_k<TYPE, G, 1, 1, true>(a, ncu, s);
+  if (a.ldx) return launch_fused<TYPE, G>(a, ncu, s);
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   auto few = [&](int rt, int tt) { return 4L * ((dw.nt + rt - 1) / rt) * ((dx.nt + tt - 1) / tt) <= 7L * ncu; };
-  if (a.n <= 16 || few(1, 1)) return launch_k<TYPE, G, 1, 1, false>(a, ncu, s);
-  if (a.n <= 32 || few(1, 2)) return launch_k<TYPE, G, 1, 2, false>(a, ncu, s);
-  if constexpr (G == 2) return launch_k<TYPE, G, 1, 4, false>(a, ncu, s);
-  else return few(2, 2) ? launch_k<TYPE, G, 2, 2, false>(a, ncu, s) : launch_k<TYPE, G, 2, 4, false>(a, ncu, s);
+  if (a.n <= 16 || few(1, 1)) return launch_k<TYPE, G, 1, 1>(a, ncu, s);
+  if (a.n <= 32 || few(1, 2)) return launch_k<TYPE, G, 1, 2>(a, ncu, s);
+  if constexpr (G == 2) return launch_k<TYPE, G, 1, 4>(a, ncu, s);
+  else return few(2, 2) ? launch_k<TYPE, G, 2, 2>(a, ncu, s) : launch_k<TYPE, G, 2, 4>(a, ncu, s);
 }
 
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
@@ -261,14 +285,18 @@ int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
 }
 
 // Every workgroup quantizes its tokens' activations, 0.12 us for 1000 elements of each workgroup that its CU runs, against a
-// launch of the quantizer (2.5 to 3.4 us, and as much of the host's time). Worth it up to 32768 elements a CU (4096 x 4096:
-// four tokens 6.1 us against 7.4, eight 8.0 against 7.4 and a launch less, sixteen 11.8 against 7.5), and where the weights
-// take the memory longer than that anyway (151936 x 2048: one token 27 against 31.5 us, eight 81 against 34).
+// launch of the quantizer (2.5 to 3.4 us, and as much of the host's time). Worth it up to 24576 elements a CU, up to 32768 in
+// launches of a tile a CU, where the host takes the longer (4096 x 4096: four tokens 6.1 us against 7.4, eight 8.1 against 7.5
+// and a launch less, sixteen 11.8 against 7.5; 12288 x 4096, eight tokens: 11.2 against 10.4), up to 8192 where more tokens have wider tiles without it
+// (32 x 4096 x 512: 4.5 against 6.4; 32 x 6144 x 2048: 9.1 against 7.7), and where the weights take
+// the memory longer than that anyway (151936 x 2048: one token 27 us against 31.5, eight 33 against 34, sixteen 46 against 38).
 bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   const int tokens = min(n, 16), mtiles = (n + 15) / 16;
+  const long tiles = (long)d.nt * mtiles;
   if (kq4_mx_rows_lds(tokens, d, type) > 64 * 1024) return false;
-  const int ks = slices(d, (long)d.nt * mtiles, ncu), tpw = (ks == 8 ? 8 : 4) / ks;
-  const double wgs = (double)((d.nt + tpw - 1) / tpw) * mtiles, each = (double)((long)((wgs + ncu - 1) / ncu)) * tokens * cols;
-  return each <= 32768.0 || (n <= 16 && each * 0.12e-3 <= 0.4 * matrices * rows * (double)cols * 0.53 / 6.0e6);
+  int waves;
+  const int ks = fused_slices(d, tiles, ncu, waves), tpw = waves / ks;
+  const double wgs = (double)((d.nt + tpw - 1) / tpw) * mtiles, each = (wgs > ncu ? wgs / ncu : 1.0) * tokens * cols;
+  return each <= (tiles <= ncu ? 32768.0 : n <= 16 ? 24576.0 : 8192.0) || (n <= 16 && each * 0.12e-3 <= 0.4 * matrices * rows * (double)cols * 0.53 / 6.0e6);
 }

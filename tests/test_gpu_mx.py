@@ -151,6 +151,25 @@ def test_every_form(kq4, torch_dev, n, rows, cols, act, form, split):
         check_gated(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act)
 
 
+@pytest.mark.parametrize("act", [4, 6])
+@pytest.mark.parametrize("n,rows,cols", [(3, 6500, 2080), (2, 9001, 1120), (5, 17000, 1056), (17, 2100, 1120), (64, 3100, 544),
+                                         (64, 4100, 1056), (64, 8200, 544), (100, 4000, 4128)])
+def test_every_tile_of_the_rows_kernel(kq4, torch_dev, n, rows, cols, act):
+    """Launches past a tile a CU (256 CUs): activations quantized in workgroups of 8 waves with 4, 2 and 1 of them on a
+    tile; tiles of 16 x 16 to 32 x 64."""
+    with kq4.options(mx_form=1):
+        check_matmul(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act, n % 2, pad_x=4, pad_out=1)
+        check_gated(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act)
+
+
+def test_outputs_past_the_caches(kq4, torch_dev):
+    """Outputs of more than 80 MiB, ragged at both edges."""
+    rng = np.random.default_rng(4)
+    for res in (None, True, "in place"):
+        check_matmul(kq4, torch_dev, rng, 1301, 16500, 96, 4 if res else 6, res, pad_out=3)
+    check_gated(kq4, torch_dev, rng, 1301, 16500, 64, 6)
+
+
 @pytest.mark.parametrize("n", [1, 20, 200])
 @pytest.mark.parametrize("act", [4, 6])
 def test_nan_stays_in_its_token_and_row(kq4, torch_dev, n, act):

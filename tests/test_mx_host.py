@@ -113,12 +113,12 @@ result = [before, after, smaller]
 
 @pytest.mark.parametrize("shape,want", [
     ((1, 4096, 4096, "matmul"), ["rows"]), ((4, 4096, 4096, "matmul"), ["rows"]), ((9, 4096, 4096, "matmul"), ["quantize", "rows"]), ((1, 151936, 2048, "matmul"), ["rows"]),
-    ((8, 151936, 2048, "matmul"), ["quantize", "rows"]),
+    ((8, 151936, 2048, "matmul"), ["rows"]),
     ((16, 151936, 2048, "matmul"), ["quantize", "rows"]), ((64, 4096, 12288, "matmul"), ["quantize", "rows"]),
     ((256, 4096, 4096, "matmul"), ["quantize", "rows"]), ((768, 4096, 4096, "matmul"), ["quantize", "gemm"]),
     ((512, 4096, 12288, "matmul"), ["quantize", "gemm", "join"]), ((4096, 4096, 12288, "matmul"), ["quantize", "gemm"]),
     ((1, 12288, 4096, "gated"), ["rows"]), ((29, 6144, 2048, "gated"), ["quantize", "rows"]),
-    ((2048, 12288, 4096, "gated"), ["quantize", "gemm"]), ((300, 1024, 512, "gated"), ["rows"]),
+    ((2048, 12288, 4096, "gated"), ["quantize", "gemm"]), ((300, 1024, 512, "gated"), ["rows"]), ((40, 1024, 512, "gated"), ["rows"]), ((40, 6144, 2048, "gated"), ["quantize", "rows"]),
     ((1, 4096, 12288, "ffn"), ["rows", "rows"]), ((12, 4096, 12288, "ffn"), ["quantize", "rows", "quantize", "rows"]),
     ((2048, 4096, 12288, "ffn"), ["quantize", "gemm", "gemm"]),
 ])
