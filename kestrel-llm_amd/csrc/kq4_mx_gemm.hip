@@ -425,7 +425,7 @@ size_t kq4_mx_part_bytes(int n, int rows, int matrices, int ksplit) {
 //   K in slices   2.5 for the second launch + the sums written and read at 4.5e6 bytes a microsecond
 // e.g. 4096 x 4096, 6 bits: 256 tokens 10.4 us in the rows kernel against 16.3 (two slices) and 17.8 in the GEMM, 768 26.4 against
 // 22.7 and 19.4; 4096 x 12288, 512 tokens: 31.2 in four slices, 49.8 in one, 48.1 in the rows kernel. Over 396 launches its choices
-// take 1.006 times the best ones (geometric mean), 1.35 times at most.
+// take 1.006 times the best ones (geometric mean), 1.38 times at most.
 KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu, int force_form, int force_split) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   const double outputs = (double)n * rows, products = outputs * cols * matrices;
