@@ -232,7 +232,7 @@ struct KQ4MxArgs {
   long ldx, ldo;         // ldx 0: x is quantized
   int rows, cols, n;
 };
-bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu);   // whether xf is the faster way
+bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu);   // whether ldx > 0 is the faster way
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s);
 // ksplit > 1 (as kq4_mx_split gives it): K in that many slices, each its own sums in part (kq4_mx_part_bytes), added in
 // slice order by a second launch.

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const uint32_t *sp = reinterpret_cast<const uint32_t *>(ws[i] + (uint32_t)q * (wstep[i] * KQ4_MX_STILE)) + lane;
-      p.s[i] = TT == 1 ? __builtin_nontemporal_load(sp) : *sp;   // (several workgroups read them for more tokens)
+      p.s[i] = TT == 1 ? __builtin_nontemporal_load(sp) : *sp;   // (with more tokens other workgroups read them too)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const kq4_v4u *cp =
@@ -266,17 +266,20 @@ static int launch_fused(const KQ4MxArgs &a, int ncu, hipStream_t s) {
 
 // A wave's tile: the smallest with at most 1.75 tiles a CU, as few waves cover a piece's latency badly (128 x 1024 x 1024, 6
 // bits: 3.0 us with 16 rows x 16 tokens, 4.3 with 32 x 32); else the largest, which loads the least (128 x 4096 x 12288: 14.2 with
-// 32 x 64, 19.2 with 32 x 32). One tile of tokens where there are 16 or 32 of them. Within 2.7 % of the best of six tiles
-// (17 to 300 tokens of six matrices).
+// 32 x 64, 19.2 with 32 x 32). One tile of tokens where there are 16 or 32 of them, of 32 rows where rows are many (16 x 151936 x
+// 2048: 35.1 us, of 16 rows 38.7; 32 tokens 48.3 and 56.6; but 16 x 12288 x 4096 8.6 and 8.1). Within 2.7 % of the best of
+// six tiles (17 to 300 tokens of six matrices).
 template <int TYPE, int G>
 static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
   if (a.ldx) return launch_fused<TYPE, G>(a, ncu, s);
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   auto few = [&](int rt, int tt) { return 4L * ((dw.nt + rt - 1) / rt) * ((dx.nt + tt - 1) / tt) <= 7L * ncu; };
+  if constexpr (G == 1)
+    if (a.n <= 16 && dw.nt > 4 * ncu) return launch_k<TYPE, G, 2, 1>(a, ncu, s);
   if (a.n <= 16 || few(1, 1)) return launch_k<TYPE, G, 1, 1>(a, ncu, s);
-  if (a.n <= 32 || few(1, 2)) return launch_k<TYPE, G, 1, 2>(a, ncu, s);
+  if (few(1, 2) || (G == 2 && a.n <= 32)) return launch_k<TYPE, G, 1, 2>(a, ncu, s);
   if constexpr (G == 2) return launch_k<TYPE, G, 1, 4>(a, ncu, s);
-  else return few(2, 2) ? launch_k<TYPE, G, 2, 2>(a, ncu, s) : launch_k<TYPE, G, 2, 4>(a, ncu, s);
+  else return a.n <= 32 || few(2, 2) ? launch_k<TYPE, G, 2, 2>(a, ncu, s) : launch_k<TYPE, G, 2, 4>(a, ncu, s);
 }
 
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
