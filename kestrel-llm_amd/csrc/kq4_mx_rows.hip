@@ -190,21 +190,28 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
           for (int v = 1; v < ks; ++v) acc[i][j] += red[(((wave - slice + v) * W + i) * TT + j) * 64 + lane];
         }
   }
+  const bool by4 = (((uintptr_t)a.out | (uintptr_t)a.res | (uintptr_t)(a.ldo * 4)) & 15) == 0;   // (the four in one access)
 #pragma unroll
   for (int j = 0; j < TT; ++j) {
     const int T = 16 * (m0 + j) + r16;
     if (slice != (j & (ks - 1)) || T >= a.n) continue;
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int r = 0; r < RT; ++r) {
+      const int R = 16 * (t + r) + 4 * g4;
+      const size_t at = (size_t)T * a.ldo + R;
+      kq4_v4f y = acc[r][j];
+      if constexpr (G == 2)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int R = 16 * (t + r) + 4 * g4 + e;
-        if (R >= a.rows) continue;
-        float y = acc[r][j][e];
-        if constexpr (G == 2) y = kq4_mx_gate(y, acc[RT + r][j][e]);
-        const size_t at = (size_t)T * a.ldo + R;
-        a.out[at] = a.res ? y + a.res[at] : y;
+        for (int e = 0; e < 4; ++e) y[e] = kq4_mx_gate(y[e], acc[RT + r][j][e]);
+      if (by4 && R + 4 <= a.rows) {
+        if (a.res) y += *reinterpret_cast<const kq4_v4f *>(a.res + at);
+        *reinterpret_cast<kq4_v4f *>(a.out + at) = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (R + e < a.rows) a.out[at + e] = a.res ? y[e] + a.res[at + e] : y[e];
       }
+    }
   }
 }
 
