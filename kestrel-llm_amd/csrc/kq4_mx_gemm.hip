@@ -420,18 +420,18 @@ size_t kq4_mx_part_bytes(int n, int rows, int matrices, int ksplit) {
 
 // The form by estimated microseconds, fitted to the times of both forms and of 1 to 16 slices over 9 matrices and 24 to 1024
 // tokens:
-//   rows kernel   3 + 1.8 per million outputs + products at 0.75e9 a microsecond (6 bits 0.6e9; gated 0.85e9, 0.66e9)
+//   rows kernel   2.5 + 1.2 per million outputs + products at 0.7e9 a microsecond (6 bits 0.65e9; gated 0.85e9, 0.66e9)
 //   GEMM          6.5 + its stages: 0.38 (6 bits 0.48) for a workgroup alone on its CU, 1.05 a round for two
 //   K in slices   2.5 for the second launch + the sums written and read at 4.5e6 bytes a microsecond
-// e.g. 4096 x 4096, 6 bits: 256 tokens 10.4 us in the rows kernel against 16.3 (two slices) and 17.8 in the GEMM, 768 26.4 against
-// 22.7 and 19.4; 4096 x 12288, 512 tokens: 31.2 in four slices, 49.8 in one, 48.1 in the rows kernel. Over 396 launches its choices
-// take 1.006 times the best ones (geometric mean), 1.33 times at most.
+// e.g. 4096 x 4096, 6 bits: 256 tokens 9.5 us in the rows kernel against 16.3 (two slices) and 17.9 in the GEMM, 768 20.4 against
+// 22.2 and 19.1; 4096 x 12288, 512 tokens: 29.6 in four slices, 50.4 in one, 45.5 in the rows kernel. Over 396 launches its choices
+// take 1.006 times the best ones (geometric mean), 1.32 times at most.
 KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu, int force_form, int force_split) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   const double outputs = (double)n * rows, products = outputs * cols * matrices;
-  const double rate = matrices == 2 ? (type == 4 ? 0.85e9 : 0.66e9) : (type == 4 ? 0.75e9 : 0.6e9);
+  const double rate = matrices == 2 ? (type == 4 ? 0.85e9 : 0.66e9) : (type == 4 ? 0.7e9 : 0.65e9);
   KQ4MxPlan best = {0, 1};
-  double least = 3.0 + 1.8e-6 * outputs + products / rate;
+  double least = 2.5 + 1.2e-6 * outputs + products / rate;
   const double tiles = (double)((n + 127) / 128) * ((rows + 256 / matrices - 1) / (256 / matrices));
   // what is forced is done where its launches have fewer than 2^32 threads
   if (n <= 16 || (force_form == 1 && (double)d.nt * ((n + 15) >> 4) < 1 << 23)) least = 0.0;   // (a token tile: no GEMM)

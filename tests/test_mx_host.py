@@ -113,7 +113,7 @@ result = [before, after, smaller]
 
 @pytest.mark.parametrize("shape,want", [
     ((1, 4096, 4096, "matmul"), ["rows"]), ((4, 4096, 4096, "matmul"), ["rows"]), ((9, 4096, 4096, "matmul"), ["quantize", "rows"]), ((1, 151936, 2048, "matmul"), ["rows"]),
-    ((8, 151936, 2048, "matmul"), ["rows"]),
+    ((6, 151936, 2048, "matmul"), ["rows"]), ((8, 151936, 2048, "matmul"), ["quantize", "rows"]),
     ((16, 151936, 2048, "matmul"), ["quantize", "rows"]), ((64, 4096, 12288, "matmul"), ["quantize", "rows"]),
     ((256, 4096, 4096, "matmul"), ["quantize", "rows"]), ((768, 4096, 4096, "matmul"), ["quantize", "gemm"]),
     ((512, 4096, 12288, "matmul"), ["quantize", "gemm", "join"]), ((4096, 4096, 12288, "matmul"), ["quantize", "gemm"]),
