@@ -239,8 +239,8 @@ static int slices(const KQ4MxDims &dw, long tiles, int ncu) {
 }
 
 // The same where the workgroups quantize the activations: past a tile a CU, workgroups of 8 waves and as many slices as
-// leave one workgroup a CU, so that few of them repeat that work (151936 x 2048, three tokens: 28.8 us with 8 waves of a tile each, 40.8
-// with 4 waves on a tile; 50000 x 1024, one token: 6.6 and 10.3; but 12288 x 4096, one token: 7.7 and 7.3).
+// leave one workgroup a CU, so that few of them repeat that work (151936 x 2048, three tokens: 28.8 us with 8 waves of a
+// tile each, 40.8 with 4 waves on a tile; 50000 x 1024, one token: 6.6 and 10.3; but 12288 x 4096, one token: 7.7 and 7.3).
 static int fused_slices(const KQ4MxDims &dw, long tiles, int ncu, int &waves) {
   waves = 8;
   if (tiles <= ncu) {
@@ -273,9 +273,9 @@ static int launch_fused(const KQ4MxArgs &a, int ncu, hipStream_t s) {
 
 // A wave's tile: the smallest with at most 1.75 tiles a CU, as few waves cover a piece's latency badly (128 x 1024 x 1024, 6
 // bits: 3.0 us with 16 rows x 16 tokens, 4.3 with 32 x 32); else the largest, which loads the least (128 x 4096 x 12288: 14.2 with
-// 32 x 64, 19.2 with 32 x 32). (64 x 32 is as good: better at 6 bits, worse at 4.) One tile of tokens where there are 16 or 32 of them, of 32 rows where rows are many (16 x 151936 x
-// 2048: 30.7 us, of 16 rows 34.8; 32 tokens 41.2 and 49.9; but 16 x 12288 x 4096 8.6 and 8.1). Within 2.8 % of the best of
-// six tiles (17 to 300 tokens of nine matrices).
+// 32 x 64, 19.2 with 32 x 32; 64 x 32 is as good: better at 6 bits, worse at 4). One tile of tokens where there are 16 or 32
+// of them, of 32 rows where rows are many (16 x 151936 x 2048: 30.7 us, of 16 rows 34.8; 32 tokens 41.2 and 49.9; but 16 x
+// 12288 x 4096 8.6 and 8.1). Within 2.8 % of the best of six tiles (17 to 300 tokens of nine matrices).
 template <int TYPE, int G>
 static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
   if (a.ldx) return launch_fused<TYPE, G>(a, ncu, s);
@@ -297,9 +297,9 @@ int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
 // Every workgroup quantizes its tokens' activations, 0.12 us for 1000 elements of each workgroup that its CU runs, against a
 // launch of the quantizer (2.5 to 3.4 us, and as much of the host's time). Worth it up to 24576 elements a CU, up to 32768 in
 // launches of a tile a CU, where the host takes the longer (4096 x 4096: four tokens 6.1 us against 7.4, eight 8.1 against 7.5
-// and a launch less, sixteen 11.8 against 7.5; 12288 x 4096, eight tokens: 11.2 against 10.4), up to 8192 where more tokens have wider tiles without it
-// (32 x 4096 x 512: 4.5 against 6.4; 32 x 6144 x 2048: 9.1 against 7.7), and where the weights take
-// the memory longer than that anyway (151936 x 2048: one token 27 us against 31, four 28 and 30, eight 32 and 30.5).
+// and a launch less, sixteen 11.8 against 7.5; 12288 x 4096, eight tokens: 11.2 against 10.4), up to 8192 where more tokens
+// have wider tiles without it (32 x 4096 x 512: 4.5 against 6.4; 32 x 6144 x 2048: 9.1 against 7.7), and where the weights
+// take the memory longer than that anyway (151936 x 2048: one token 27 us against 31, four 28 and 30, eight 32 and 30.5).
 bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int ncu) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   const int tokens = min(n, 16), mtiles = (n + 15) / 16;
@@ -308,5 +308,6 @@ bool kq4_mx_rows_fused(int n, int rows, int cols, int matrices, int type, int nc
   int waves;
   const int ks = fused_slices(d, tiles, ncu, waves), tpw = waves / ks;
   const double wgs = (double)((d.nt + tpw - 1) / tpw) * mtiles, each = (wgs > ncu ? wgs / ncu : 1.0) * tokens * cols;
-  return each <= (tiles <= ncu ? 32768.0 : n <= 16 ? 24576.0 : 8192.0) || (n <= 16 && each * 0.12e-3 <= 0.3 * matrices * rows * (double)cols * 0.53 / 6.0e6);
+  return each <= (tiles <= ncu ? 32768.0 : n <= 16 ? 24576.0 : 8192.0) ||
+         (n <= 16 && each * 0.12e-3 <= 0.3 * matrices * rows * (double)cols * 0.53 / 6.0e6);
 }
