@@ -999,19 +999,23 @@ def _mx_out(out, residual, n, rows, device):
     return ldo
 
 
-def _mx_n(x, cols):
-    """The rows of x."""
-    if not isinstance(x, _torch.Tensor) or x.dim() != 2:
-        raise KQ4Error(f"x: expected a [n, {cols}] device tensor")
-    return x.shape[0]
+def _mx_x(x, cols, device):
+    """The rows of x and their stride."""
+    if isinstance(x, _torch.Tensor):
+        shape = x.shape
+        if len(shape) == 2:
+            if shape[1] == cols and x.is_contiguous() and x.dtype is _torch.float32 and x.get_device() == device:
+                return shape[0], cols
+            return shape[0], _rows(x, "x", shape[0], cols, device)
+    raise KQ4Error(f"x: expected a [n, {cols}] device tensor")
 
 
 def mx_matmul_dev(out, x, w, act=MX_FP6, residual=None, stream=None):
     """out [n][w.rows] = [residual +] W . x for fp32 x [n][w.cols], quantized to `act` bits on the way."""
     _mx_w(w, "w")
     rows, cols, dev = w.rows, w.cols, w.device
-    n = _mx_n(x, cols)
-    ldx, ldo = _rows(x, "x", n, cols, dev), _mx_out(out, residual, n, rows, dev)
+    n, ldx = _mx_x(x, cols, dev)
+    ldo = _mx_out(out, residual, n, rows, dev)
     _check_here(dev, "w")
     check(_lib.kq4_mx_matmul_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), w.p, rows, cols, n, act,
                                  _stream_ptr(stream)), "kq4_mx_matmul_dev")
@@ -1034,8 +1038,8 @@ def mx_gated_dev(out, x, gate, up, act=MX_FP6, stream=None):
     _mx_w(gate, "gate")
     rows, cols, dev = gate.rows, gate.cols, gate.device
     _mx_w(up, "up", rows, cols, dev)
-    n = _mx_n(x, cols)
-    ldx, ldo = _rows(x, "x", n, cols, dev), _rows(out, "out", n, rows, dev)
+    n, ldx = _mx_x(x, cols, dev)
+    ldo = _rows(out, "out", n, rows, dev)
     _check_here(dev, "gate")
     check(_lib.kq4_mx_gated_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, gate.p, up.p, rows, cols, n, act,
                                 _stream_ptr(stream)), "kq4_mx_gated_dev")
@@ -1047,8 +1051,8 @@ def mx_ffn_dev(out, x, gate, up, down, act=MX_FP6, residual=None, stream=None):
     ffn, dim, dev = gate.rows, gate.cols, gate.device
     _mx_w(up, "up", ffn, dim, dev)
     _mx_w(down, "down", dim, ffn, dev)
-    n = _mx_n(x, dim)
-    ldx, ldo = _rows(x, "x", n, dim, dev), _mx_out(out, residual, n, dim, dev)
+    n, ldx = _mx_x(x, dim, dev)
+    ldo = _mx_out(out, residual, n, dim, dev)
     _check_here(dev, "gate")
     check(_lib.kq4_mx_ffn_dev(out.data_ptr(), ldo, x.data_ptr(), ldx, _tp(residual), gate.p, up.p, down.p, dim, ffn, n,
                               act, _stream_ptr(stream)), "kq4_mx_ffn_dev")
