@@ -12,8 +12,8 @@
 // while its first weights are on their way (FQ = 1): one launch instead of two. Loads return in order, so what is needed
 // first is asked for first: the activations before the weights. What bounds it: the weights' bytes where they are many (one
 // token: 151936 x 2048 27 us, 6.1 TB/s; 2 x 12288 x 4096 gated 11 us, 4.9 TB/s with what starts and ends it), the latency of
-// a piece below (4096 x 4096 4.4 us), the operands' way through the L2 caches for more tokens (64 x 4096 x 12288, 6 bits: 12 us for
-// 132 MB, 11 TB/s). AHEAD: all loads of a piece are on their way before its
+// a piece below (4096 x 4096 4.4 us), the operands' way through the L2 caches for more tokens (64 x 4096 x 12288, 6 bits: 10.6 us for
+// 132 MB, 12 TB/s). AHEAD: all loads of a piece are on their way before its
 // first product; left alone they alternate with the products in fewer registers. It pays with fewer than 8
 // waves a CU (64 x 4096 x 12288: 12.1 us with, 15.8 without) and costs above (256 x 4096 x 4096: 11.3 with, 10.4 without).
 template <int TYPE, int G, int RT, int TT, int NW, bool FQ, bool AHEAD>
