@@ -253,14 +253,17 @@ static int fused_slices(const KQ4MxDims &dw, long tiles, int ncu, int &waves) {
   return ks;
 }
 
-template <int TYPE, int G, int RT, int TT>
+// FEW, MANY: launches of at most a tile a CU, and of 8 waves a CU and more, come here.
+template <int TYPE, int G, int RT, int TT, bool FEW, bool MANY>
 static int launch_k(const KQ4MxArgs &a, int ncu, hipStream_t s) {
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   const long tiles = (long)((dw.nt + RT - 1) / RT) * ((dx.nt + TT - 1) / TT);
   const int ks = slices(dw, tiles, ncu);
-  if (ks == 8) return launch<TYPE, G, RT, TT, 8, false, true>(a, ks, s);
-  return tiles * ks < 8L * ncu ? launch<TYPE, G, RT, TT, 4, false, true>(a, ks, s)
-                               : launch<TYPE, G, RT, TT, 4, false, false>(a, ks, s);
+  if constexpr (FEW)
+    if (ks == 8) return launch<TYPE, G, RT, TT, 8, false, true>(a, ks, s);
+  if constexpr (MANY)
+    if (tiles * ks >= 8L * ncu) return launch<TYPE, G, RT, TT, 4, false, false>(a, ks, s);
+  return launch<TYPE, G, RT, TT, 4, false, true>(a, ks, s);
 }
 
 template <int TYPE, int G>
@@ -282,11 +285,12 @@ static int launch_t(const KQ4MxArgs &a, int ncu, hipStream_t s) {
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   auto few = [&](int rt, int tt) { return 4L * ((dw.nt + rt - 1) / rt) * ((dx.nt + tt - 1) / tt) <= 7L * ncu; };
   if constexpr (G == 1)
-    if (a.n <= 16 && dw.nt > 4 * ncu) return launch_k<TYPE, G, 2, 1>(a, ncu, s);
-  if (a.n <= 16 || few(1, 1)) return launch_k<TYPE, G, 1, 1>(a, ncu, s);
-  if (few(1, 2) || (G == 2 && a.n <= 32)) return launch_k<TYPE, G, 1, 2>(a, ncu, s);
-  if constexpr (G == 2) return launch_k<TYPE, G, 1, 4>(a, ncu, s);
-  else return a.n <= 32 || few(2, 2) ? launch_k<TYPE, G, 2, 2>(a, ncu, s) : launch_k<TYPE, G, 2, 4>(a, ncu, s);
+    if (a.n <= 16 && dw.nt > 4 * ncu) return launch_k<TYPE, G, 2, 1, false, true>(a, ncu, s);
+  if (a.n <= 16 || few(1, 1)) return launch_k<TYPE, G, 1, 1, true, true>(a, ncu, s);
+  if (few(1, 2) || (G == 2 && a.n <= 32)) return launch_k<TYPE, G, 1, 2, true, G == 2>(a, ncu, s);
+  if constexpr (G == 2) return launch_k<TYPE, G, 1, 4, true, true>(a, ncu, s);
+  else if (a.n <= 32 || few(2, 2)) return launch_k<TYPE, G, 2, 2, true, true>(a, ncu, s);
+  else return launch_k<TYPE, G, 2, 4, true, true>(a, ncu, s);
 }
 
 int kq4_launch_mx_rows(const KQ4MxArgs &a, int type, int ncu, hipStream_t s) {
