@@ -351,6 +351,53 @@ def test_graph_and_stream_and_repeats(kq4, torch_dev, n, act):
         other()
 
 
+def test_two_graphs_share_the_workspace(kq4, torch_dev):
+    """Steps of two sizes captured one after the other and replayed in turn, outputs cleared between."""
+    torch = torch_dev
+    steps = [step(kq4, torch, n, 6, seed) for seed, n in enumerate((300, 21))]
+    for run, _, _ in steps:
+        run()
+    torch.cuda.synchronize()
+    want = [[t.clone() for t in outs + [xq]] for _, outs, xq in steps]
+    graphs = []
+    for run, _, _ in steps:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            run(torch.cuda.current_stream())
+    for _ in range(3):
+        for t in [t for _, outs, _ in steps for t in outs]:
+            t.fill_(float("nan"))
+        for g in graphs + graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for (_, outs, xq), w in zip(steps, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs + [xq], w))
+
+
+@pytest.mark.parametrize("n", [1, 9, 40, 300])
+@pytest.mark.parametrize("form", [1, 2])
+def test_rows_behind_the_batch_stay(kq4, torch_dev, n, form):
+    """Outputs and residuals of more rows than x: those behind are not written; x of more rows than
+    a matrix."""
+    torch, rng = torch_dev, np.random.default_rng(n)
+    rows, cols = 260, 544
+    w = [packed(kq4, torch, *R.random_weights(rng, r, c)) for r, c in ((rows, cols), (rows, cols), (cols, 288), (288, cols), (288, cols))]
+    x = up(torch, R.acts(rng, n + 2, cols))
+    small = [torch.empty(n, c, device="cuda") for c in (rows, rows, rows, cols)]
+    large = [torch.full((n + 5, c), 7.0, device="cuda") for c in (rows, rows, rows, cols)]
+    res = up(torch, rng.standard_normal((n + 1, rows)).astype(F32))
+    with kq4.options(mx_form=form):
+        for o in (small, large):
+            xq = kq4.MX(n, cols, 6)
+            kq4.mx_quantize_dev(xq, x)
+            kq4.mx_matmul_dev(o[0], x[:n], w[0], residual=res)
+            kq4.mx_matmul_q_dev(o[1], xq, w[0])
+            kq4.mx_gated_dev(o[2], x[:n], w[0], w[1])
+            kq4.mx_ffn_dev(o[3], x[:n], w[3], w[4], w[2])
+    for a, b in zip(small, large):
+        assert torch.equal(a, b[:n]) and (b[n:] == 7.0).all()
+
+
 @pytest.mark.slow
 def test_matrix_past_32_bits(kq4, torch_dev):
     """A matrix of more than 4 GiB: rows at both ends and across the borders of 2^31 and 2^32 bytes."""
