@@ -17,15 +17,17 @@
 // first product; left alone they alternate with the products in fewer registers. It pays with fewer than 8
 // waves a CU (64 x 4096 x 12288: 12.1 us with, 15.8 without) and costs above (256 x 4096 x 4096: 11.3 with, 10.4 without).
 template <int TYPE, int G, int RT, int TT, int NW, bool FQ, bool AHEAD>
-__global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int ks, int mtiles, int all) {
+__global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int ks, int mtiles, int all, int turn) {
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
   constexpr int W = G * RT;                              // weight tiles of a wave: [matrix][row tile]
-  // XCD x works on a run of row tiles, each against all tokens before the next: its cache reads the weights once
+  // XCD x works on a run of row tiles, each against all tokens before the next: its cache reads the weights once; or
+  // (turn: the row tiles' workgroups) on a run of tokens against all rows, and reads the activations once
   const int xcd = blockIdx.x & 7, q8 = all >> 3, r8 = all & 7;
   const int v = xcd * q8 + (xcd < r8 ? xcd : r8) + (int)(blockIdx.x >> 3);
-  const int t = (v / mtiles * (NW / ks) + wave / ks) * RT, slice = wave % ks, m0 = v % mtiles * TT;
+  const int tw = turn ? v % turn : v / mtiles, m0 = (turn ? v / turn : v % mtiles) * TT;
+  const int t = (tw * (NW / ks) + wave / ks) * RT, slice = wave % ks;
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   uint32_t wstep[W];   // from a tile to the next, in tiles (a row tile's offsets stay below 2^32: cols <= 2^20)
   const uint8_t *w[W], *ws[W];
@@ -222,9 +224,13 @@ template <int TYPE, int G, int RT, int TT, int NW, bool FQ, bool AHEAD>
 static int launch(const KQ4MxArgs &a, int ks, hipStream_t s) {
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   const int tpw = NW / ks * RT, mtiles = (dx.nt + TT - 1) / TT, all = (dw.nt + tpw - 1) / tpw * mtiles;
+  // Tokens outside where the activations are more than the weights and than an XCD's cache of 4 MB: 4096 x 256 x 12288, 6 bits,
+  // 21 us so and 45 with the rows outside; 512 x 128 x 4096 4.5 and 4.0.
+  const size_t xs = kq4_mx_size(dx, TYPE);
+  const bool turn = xs > (4u << 20) && xs > G * kq4_mx_size(dw, 4);
   const size_t red = ks > 1 ? (size_t)NW * G * RT * TT * 1024 : 0, x = FQ ? kq4_mx_rows_lds(min(a.n, 16 * TT), dw, TYPE) : 0;
   hipLaunchKernelGGL((kq4_mx_rows_kernel<TYPE, G, RT, TT, NW, FQ, AHEAD>), dim3((unsigned)all), dim3(64 * NW), red > x ? red : x, s,
-                     a, ks, mtiles, all);
+                     a, ks, mtiles, all, turn ? all / mtiles : 0);
   return (int)hipGetLastError();
 }
 

@@ -153,10 +153,10 @@ def test_every_form(kq4, torch_dev, n, rows, cols, act, form, split):
 
 @pytest.mark.parametrize("act", [4, 6])
 @pytest.mark.parametrize("n,rows,cols", [(3, 6500, 2080), (2, 9001, 1120), (5, 17000, 1056), (17, 2100, 1120), (64, 3100, 544),
-                                         (64, 4100, 1056), (64, 8200, 544), (100, 4000, 4128), (16, 16500, 1120), (30, 8000, 544)])
+                                         (64, 4100, 1056), (64, 8200, 544), (100, 4000, 4128), (16, 16500, 1120), (30, 8000, 544), (1500, 260, 4384), (3007, 33, 2848)])
 def test_every_tile_of_the_rows_kernel(kq4, torch_dev, n, rows, cols, act):
     """Launches past a tile a CU (256 CUs): activations quantized in workgroups of 8 waves with 4, 2 and 1 of them on a
-    tile; tiles of 16 x 16 to 32 x 64, from quantized activations too."""
+    tile; tiles of 16 x 16 to 32 x 64, from quantized activations too; activations past an XCD's cache."""
     with kq4.options(mx_form=1):
         check_matmul(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act, n % 2, pad_x=4, pad_out=1)
         check_matmul(kq4, torch_dev, np.random.default_rng(n), n, rows, cols, act, True, pad_out=2, quantized=True)
