@@ -31,7 +31,7 @@ struct KQ4MxTile {
   static_assert(B % (1024 * NW) == 0 && SLOADS % SPW == 0, "kq4_mx_gemm: runs per wave");
   // the first run of a wave's activations (where there are not as many for each, the last waves bring the last ones)
   static __device__ int first_a(int wave) { return wave * LA < A / 1024 - LA ? wave * LA : A / 1024 - LA; }
-  static_assert(8 * TA % (LA * 1024) == 0 && 8 % LB == 0 && BM % 128 == 0 && BN % 256 == 0, "kq4_mx_gemm: groups");
+  static_assert(8 * TA % (LA * 1024) == 0 && 8 % LB == 0 && BM % 128 == 0 && BN % 128 == 0, "kq4_mx_gemm: groups");
   static_assert(LDS <= 160 * 1024, "kq4_mx_gemm: LDS");
 };
 
@@ -61,6 +61,7 @@ template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC, bool 
 __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArgs a, int mtiles, int ntiles, int ksplit, int per) {
   using T = KQ4MxTile<TYPE, TI, TJ, WM, WN, S>;
   constexpr int RG = T::BN / G;                 // output rows of the workgroup
+  static_assert(RG % 128 == 0, "kq4_mx_gemm: whole groups of rows");
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM, l32 = lane & 31, half = lane >> 5;
@@ -394,16 +395,25 @@ int kq4_mx_split(int kq, int want) {
   return (kq + per - 1) / per;
 }
 
-// Launches that leave a workgroup alone on its CU run it in 8 waves of 64 x 64 with a stage more in its ring, two waves per
-// SIMD as elsewhere two workgroups have (512 x 4096 x 4096: 17.3 us instead of 19.4, of 6 bits 20.0 instead of 23.8).
+// One matrix: tiles of 128 x 128 in 4 waves of 64 x 64, as long as three of them a CU hold the launch, since a stage of few
+// workgroups is all latency and shorter for the smaller tile (512 x 4096 x 4096: 12.7 us, in 128 x 256 18.1; 2400 x 4096 x 4096
+// 30.5 and 34.2; but 4096 x 4096 x 4096, two rounds, 44.0 and 38.6), with the deeper ring up to one and a half a CU (1322 x
+// 2944 x 3744 15.0 against 15.5, but 1800 x 4096 x 4096 26.1 against 24.4). Two matrices, whose tiles of 128 x 128 would not be
+// whole groups of rows: where workgroups are alone on their CUs they have 8 waves of 64 x 64 and a stage more, two waves per
+// SIMD as elsewhere two workgroups have.
 // Outputs and residuals of KQ4_MX_PAST_CACHE bytes and more go past the caches (non-temporal: 2048 x 12288 x 4096 of one
 // matrix 69 -> 58 us, 4096 x 12288 x 1024 65 -> 44, with a residual 98 -> 85); the memory side's 256 MB hold smaller ones for
 // what reads them next (1796 x 5127 x 64 with a residual 18 us, non-temporal 28; 2048 x 8192 x 512 17 and 20).
 #define KQ4_MX_PAST_CACHE ((size_t)80 << 20)
 template <int TYPE, int G>
 static int launch_form(const KQ4MxArgs &a, int ksplit, int ncu, hipStream_t s) {
-  const long wgs = (long)((a.n + 127) / 128) * ((a.rows + 256 / G - 1) / (256 / G)) * ksplit;
-  if (wgs <= ncu) return launch<TYPE, G, 2, 2, 2, 4, 3, 1, false>(a, ksplit, s);
+  const long tiles = (long)((a.n + 127) / 128) * ((a.rows + 127) / 128) * ksplit;
+  if constexpr (G == 1) {
+    if (2 * tiles <= 3L * ncu) return launch<TYPE, 1, 2, 2, 2, 2, TYPE == 4 ? 4 : 3, 2, false>(a, ksplit, s);
+    if (tiles <= 3L * ncu) return launch<TYPE, 1, 2, 2, 2, 2, TYPE == 4 ? 3 : 2, 3, false>(a, ksplit, s);
+  } else {
+    if (tiles <= ncu) return launch<TYPE, 2, 2, 2, 2, 4, 3, 1, false>(a, ksplit, s);
+  }
   const size_t bytes = ksplit > 1 || a.q ? 0 : (size_t)a.n * a.rows * (a.res ? 8 : 4);
   if (bytes >= KQ4_MX_PAST_CACHE) return launch<TYPE, G, 2, 4, 2, 2, TYPE == 4 ? 3 : 2, 2, true>(a, ksplit, s);
   return launch<TYPE, G, 2, 4, 2, 2, TYPE == 4 ? 3 : 2, 2, false>(a, ksplit, s);
@@ -421,18 +431,19 @@ size_t kq4_mx_part_bytes(int n, int rows, int matrices, int ksplit) {
 // The form by estimated microseconds, fitted to the times of both forms and of 1 to 16 slices over 9 matrices and 24 to 1024
 // tokens:
 //   rows kernel   2.5 + 1.2 per million outputs + products at 0.7e9 a microsecond (6 bits 0.65e9; gated 0.85e9, 0.66e9)
-//   GEMM          6.5 + its stages: 0.38 (6 bits 0.48) for a workgroup alone on its CU, 1.05 a round for two
+//   GEMM          6.5 + its stages: of one matrix 0.21 (6 bits 0.265) for a tile a CU, 0.28 (0.32) a tile up to three; of
+//                 two 0.38 (0.48) for a workgroup alone on its CU; 1.05 a round of two beyond
 //   K in slices   2.5 for the second launch + the sums written and read at 4.5e6 bytes a microsecond
-// e.g. 4096 x 4096, 6 bits: 256 tokens 9.5 us in the rows kernel against 16.3 (two slices) and 17.9 in the GEMM, 768 20.4 against
-// 22.2 and 19.1; 4096 x 12288, 512 tokens: 29.6 in four slices, 50.4 in one, 45.5 in the rows kernel. Over 396 launches its choices
-// take 1.006 times the best ones (geometric mean), 1.32 times at most.
+// e.g. 4096 x 4096, 6 bits: 256 tokens 9.4 us in the rows kernel against 13.7 (two slices) and 13.2 in the GEMM, 768 20.5 against
+// 21.7 and 14.7; 4096 x 12288, 512 tokens: 30.0 in two slices, 39.9 in one, 45.4 in the rows kernel. Over 556 launches its choices
+// take 1.005 times the best ones (geometric mean), 1.31 times at most.
 KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu, int force_form, int force_split) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   const double outputs = (double)n * rows, products = outputs * cols * matrices;
   const double rate = matrices == 2 ? (type == 4 ? 0.85e9 : 0.66e9) : (type == 4 ? 0.7e9 : 0.65e9);
   KQ4MxPlan best = {0, 1};
   double least = 2.5 + 1.2e-6 * outputs + products / rate;
-  const double tiles = (double)((n + 127) / 128) * ((rows + 256 / matrices - 1) / (256 / matrices));
+  const double tiles = (double)((n + 127) / 128) * ((rows + 127) / 128);
   // what is forced is done where its launches have fewer than 2^32 threads
   if (n <= 16 || (force_form == 1 && (double)d.nt * ((n + 15) >> 4) < 1 << 23)) least = 0.0;   // (a token tile: no GEMM)
   if (force_form == 2) least = 1e30;
@@ -441,9 +452,13 @@ KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu
     if (force_split > 0 && want > 1) break;
     const int ks = kq4_mx_split(d.kq, force_split > 0 ? force_split : want);
     const double wgs = tiles * ks;
-    if (want > 1 && (ks <= best.ksplit || wgs > 2.0 * ncu || kq4_mx_part_bytes(n, rows, matrices, ks) > KQ4_MX_PART_MAX)) break;
+    if (want > 1 && (ks <= best.ksplit || wgs > (matrices == 1 ? 3.0 : 2.0) * ncu || kq4_mx_part_bytes(n, rows, matrices, ks) > KQ4_MX_PART_MAX)) break;
     const int stages = 4 * ((d.kq + ks - 1) / ks);
-    double us = 6.5 + stages * (wgs <= ncu ? (type == 4 ? 0.38 : 0.48) : 1.05 * (double)(long)((wgs + 2 * ncu - 1) / (2 * ncu)));
+    const double wide = matrices == 1 ? (double)((n + 127) / 128) * ((rows + 255) / 256) * ks : wgs;
+    double us = 1.05 * (double)(long)((wide + 2 * ncu - 1) / (2 * ncu));
+    if (matrices == 2 && wgs <= ncu) us = type == 4 ? 0.38 : 0.48;
+    if (matrices == 1 && wgs <= 3.0 * ncu) us = wgs <= ncu ? (type == 4 ? 0.21 : 0.265) : (type == 4 ? 0.28 : 0.32) * (wgs / ncu);
+    us = 6.5 + stages * us;
     if (ks > 1) us += 2.5 + (ks + 1.5) * matrices * outputs * 4.0 / 4.5e6;
     if (us < least) {
       least = us;

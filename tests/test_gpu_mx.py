@@ -142,7 +142,7 @@ def test_matmul_of_odd_sizes_and_strides(kq4, torch_dev, n, rows, cols, act, qua
 
 
 @pytest.mark.parametrize("act", [4, 6])
-@pytest.mark.parametrize("n,rows,cols", [(1, 130, 544), (16, 300, 2080), (33, 515, 1120), (129, 257, 4096), (300, 600, 1536), (1100, 2100, 544)])
+@pytest.mark.parametrize("n,rows,cols", [(1, 130, 544), (16, 300, 2080), (33, 515, 1120), (129, 257, 4096), (300, 600, 1536), (1100, 2100, 544), (2500, 2300, 160), (2700, 2300, 160), (2700, 5000, 96)])
 @pytest.mark.parametrize("form,split", [(1, 0), (2, 1), (2, 2), (2, 3), (2, 50)])
 def test_every_form(kq4, torch_dev, n, rows, cols, act, form, split):
     """The rows kernel and the GEMM, whole and with K in slices, at sizes of either, with and without a residual."""

@@ -149,7 +149,7 @@ def names(**o):
 result = [names(mx_form=1), names(mx_form=2, mx_split=1), names(mx_split=2), names(mx_split=99), names(mx_form=-1, mx_split=-1)]
 """)
     assert [r[0] for r in res] == [0] * 5
-    assert res[1][1:] == ["gemm 9"] and res[2][1:] == ["gemm 18", "join 300"] and res[3][1:] == ["gemm 27", "join 300"]
+    assert res[1][1:] == ["gemm 15"] and res[2][1:] == ["gemm 30", "join 300"] and res[3][1:] == ["gemm 45", "join 300"]
     assert len(res[0]) == 2 and res[0][1].startswith("rows") and res[4] == res[0]
 
 
