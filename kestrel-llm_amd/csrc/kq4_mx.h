@@ -42,6 +42,26 @@ KQ4_HD size_t kq4_mx_size(const KQ4MxDims &d, int type) {
   return kq4_mx_codes_size(d, type) + (size_t)d.nt * d.kq * KQ4_MX_STILE;
 }
 
+// Runs of 1 KB that the GEMM loads a stage at a time: byte `off` of the code tiles (or the scale tiles) of a column tile's row
+// tiles t0, t0 + 1, ... (t0 a group's first). `at`: where the first stage's lies; `step`: how far on the next stage's is;
+// `bytes`: what the matrix holds from `at` on. A run that starts past the last row tile has no bytes and no step. The range
+// check takes the scalar offset (stages times `step`) from `bytes` before it compares, unsigned: of a run that starts in the
+// matrix every stage's start is in it too, so nothing is taken from less.
+struct KQ4MxRun {
+  long at;
+  uint32_t bytes, step;
+};
+KQ4_HD KQ4MxRun kq4_mx_run(const KQ4MxDims &d, int type, bool scales, int t0, int off) {
+  const int tb = scales ? KQ4_MX_STILE : kq4_mx_tile_bytes(type), t = t0 + off / (8 * tb) * 8, in = off % (8 * tb);
+  const long all = (long)kq4_mx_size(d, type);
+  KQ4MxRun r = {all, 0u, 0u};
+  if (t + in / tb >= d.nt) return r;
+  r.at = (scales ? (long)kq4_mx_codes_size(d, type) : 0) + kq4_mx_first(t, scales ? d.kq : d.kt) * tb + in;
+  r.step = (uint32_t)(kq4_mx_step(t, d.nt) * tb);
+  r.bytes = (uint32_t)(all - r.at < 0x7fffffffL ? all - r.at : 0x7fffffffL);
+  return r;
+}
+
 // In a code tile: the first 16 bytes of row r's block b of 4, and the last 8 of its 24 (6 bits).
 KQ4_HD int kq4_mx_piece(int b, int r) { return 256 * b + 16 * r; }
 KQ4_HD int kq4_mx_rest(int b, int r) { return 1024 + 128 * b + 8 * r; }

@@ -35,11 +35,12 @@ struct KQ4MxTile {
   static_assert(LDS <= 160 * 1024, "kq4_mx_gemm: LDS");
 };
 
-// N runs of 1 KB from offset soff of r to LDS address `to` on: one address register for each four, the rest of it in the
+// N runs of 1 KB from offset soff of r to LDS address `to` on: one address register for them all, the rest of it in the
 // instructions' offset, which counts on both sides.
 template <int N>
 KQ4_DEV void kq4_mx_load(const kq4_rsrc4 &r, uint32_t v16, uint32_t soff, uint32_t to) {
-  if constexpr (N >= 4)
+  static_assert(N >= 1 && N <= 4, "kq4_mx_load: runs");
+  if constexpr (N == 4)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
                  "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds\n\tbuffer_load_dwordx4 %1, %2, %3 offen offset:2048 lds\n\t"
                  "buffer_load_dwordx4 %1, %2, %3 offen offset:%4 lds" ::"s"(to), "v"(v16), "s"(r), "s"(soff), "n"(3 * 1024)
@@ -54,7 +55,6 @@ KQ4_DEV void kq4_mx_load(const kq4_rsrc4 &r, uint32_t v16, uint32_t soff, uint32
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(v16), "s"(r),
                  "s"(soff) : "memory", "m0");
-  if constexpr (N > 4) kq4_mx_load<N - 4>(r, v16, soff + 4096, to + 4096);
 }
 
 template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC, bool NT>
@@ -73,21 +73,16 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
   const int band = v / (8 * ntiles), bm = min(8, mtiles - 8 * band), u = v - band * 8 * ntiles;
   const int m0 = (8 * band + u % bm) * T::BM, n0 = (u / bm) * RG;
 
-  // A matrix' runs from byte `off` of the stage (or of the scales) of the workgroup's rows, which start with row tile t0 (a
-  // group's first): where they lie and how far the next stage's do. Loads past the matrix read zeros.
+  // Where a wave's runs lie (kq4_mx_run) as a buffer that ends with the matrix. Loads past it read zeros; what a run of the last
+  // group holds past its row tiles belongs to rows that are not stored.
   const KQ4MxDims dw = kq4_mx_dims(a.rows, a.cols), dx = kq4_mx_dims(a.n, a.cols);
   const uint8_t *xq = static_cast<const uint8_t *>(a.x);
   auto runs = [](const uint8_t *m, const KQ4MxDims &d, int type, bool scales, int t0, int off, uint32_t &step) {
-    const int tb = scales ? KQ4_MX_STILE : kq4_mx_tile_bytes(type), t = t0 + off / (8 * tb) * 8;
-    const long all = (long)kq4_mx_size(d, type);
-    long at = (scales ? (long)kq4_mx_codes_size(d, type) : 0) + kq4_mx_first(t, scales ? d.kq : d.kt) * tb + off % (8 * tb);
-    if (t >= d.nt || at > all) at = all;
-    step = t < d.nt ? (uint32_t)(kq4_mx_step(t, d.nt) * tb) : 0u;
-    const long left = all - at;
-    kq4_rsrc4 r = kq4_rsrc_at(m + at, (uint32_t)(left < 0x7fffffffL ? left : 0x7fffffffL), 0);
+    const KQ4MxRun u = kq4_mx_run(d, type, scales, t0, off);
+    kq4_rsrc4 r = kq4_rsrc_at(m + u.at, u.bytes, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);   // (the wave's, in scalar registers)
-    step = (uint32_t)__builtin_amdgcn_readfirstlane((int)step);
+    step = (uint32_t)__builtin_amdgcn_readfirstlane((int)u.step);
     return r;
   };
   uint32_t step_a, step_b, step_s[T::SPW];
