@@ -247,11 +247,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
       for (int i = 0; i < TI; ++i) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+        for (int j = 0; j < TJ / 2; ++j) {
+          const kq4_v16f h = kq4_mx_gate<16>(acc[i][j], acc[i][TJ / 2 + j]);
 #pragma unroll
-          for (int j = 0; j < TJ / 2; ++j)
-            buf[(32 * wm + 8 * (e >> 2) + 4 * half + (e & 3)) * LD + 32 * (TJ / 2 * wn + j) + l32] =
-                kq4_mx_gate(acc[i][j][e], acc[i][TJ / 2 + j][e]);
+          for (int e = 0; e < 16; ++e) buf[(32 * wm + 8 * (e >> 2) + 4 * half + (e & 3)) * LD + 32 * (TJ / 2 * wn + j) + l32] = h[e];
+        }
         __syncthreads();
         for (int u = threadIdx.x; u < 32 * WM * 4; u += 64 * T::NW) {
           const int row = u >> 2, b = u & 3, tok = m0 + 32 * (TI * (row >> 5) + i) + (row & 31);
@@ -302,12 +302,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void kq4_mx_gemm_kernel(KQ4MxArg
           }
         }
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int j = 0; j < TJ / G; ++j) {
+        kq4_v16f p = acc[i][j];
+        if constexpr (G == 2) p = kq4_mx_gate<16>(p, acc[i][TJ / 2 + j]);
 #pragma unroll
-        for (int j = 0; j < TJ / G; ++j) {
-          const float p = G == 2 ? kq4_mx_gate(acc[i][j][e], acc[i][G == 2 ? TJ / 2 + j : j][e]) : acc[i][j][e];
-          y[e][j] = RES ? p + y[e][j] : p;
-        }
+        for (int e = 0; e < 16; ++e) y[e][j] = RES ? p[e] + y[e][j] : p[e];
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int tok = t0 + 8 * (e >> 2) + (e & 3);
@@ -357,12 +357,11 @@ __global__ __launch_bounds__(256) void kq4_mx_join_kernel(KQ4MxArgs a, int kspli
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i][g] += s + u < ksplit ? v[i][g][u] : 0.0f;
   }
+  kq4_v4f o = {y[0][0], y[1][0], y[2][0], y[3][0]};
+  if constexpr (G == 2) o = kq4_mx_gate<4>(o, kq4_v4f{y[0][1], y[1][1], y[2][1], y[3][1]});
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (c0 + 256 * i >= a.rows) continue;
-    const float o = G == 2 ? kq4_mx_gate(y[i][0], y[i][G - 1]) : y[i][0];
-    a.out[(size_t)t * a.ldo + c0 + 256 * i] = a.res ? o + res[i] : o;
-  }
+  for (int i = 0; i < 4; ++i)
+    if (c0 + 256 * i < a.rows) a.out[(size_t)t * a.ldo + c0 + 256 * i] = a.res ? o[i] + res[i] : o[i];
 }
 
 template <int TYPE, int G, int TI, int TJ, int WM, int WN, int S, int OCC, bool NT>

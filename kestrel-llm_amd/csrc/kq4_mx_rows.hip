@@ -202,9 +202,7 @@ __global__ __launch_bounds__(64 * NW) void kq4_mx_rows_kernel(KQ4MxArgs a, int k
       const int R = 16 * (t + r) + 4 * g4;
       const size_t at = (size_t)T * a.ldo + R;
       kq4_v4f y = acc[r][j];
-      if constexpr (G == 2)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = kq4_mx_gate(y[e], acc[RT + r][j][e]);
+      if constexpr (G == 2) y = kq4_mx_gate<4>(y, acc[RT + r][j]);
       if (by4 && R + 4 <= a.rows) {
         if (a.res) y += *reinterpret_cast<const kq4_v4f *>(a.res + at);
         *reinterpret_cast<kq4_v4f *>(a.out + at) = y;
