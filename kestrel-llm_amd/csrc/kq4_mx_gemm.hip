@@ -441,6 +441,7 @@ KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu
   // what is forced is done where its launches have fewer than 2^32 threads
   if (n <= 16 || (force_form == 1 && (double)d.nt * ((n + 15) >> 4) < 1 << 23)) least = 0.0;   // (a token tile: no GEMM)
   if (force_form == 2) least = 1e30;
+  force_split = min(force_split, d.kq);
   if (tiles * force_split >= 1 << 23 || (double)((rows + 1023) / 1024) * n >= 1 << 24) force_split = 1;
   for (int want = 1; want <= 16; want *= 2) {
     if (force_split > 0 && want > 1) break;
