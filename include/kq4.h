@@ -514,7 +514,10 @@ size_t kq4_mx_bytes(int rows, int cols, int type);
 /* fp32 rows (row t at x + t * ldx floats; 16-byte aligned, ldx a multiple of 4) into a microscaled
  * matrix of `type` bits that does not overlap them. A block's scale is the least 2^e, e >= -127, for which its largest
  * magnitude over 2^e, rounded to the element's precision, is not above the largest element (so no
- * element is off by more than half a step of its format); an element is the nearest one to x / 2^e,
+ * element is off by more than half a step of its format). The OCP text's own conversion takes the
+ * exponent of the largest magnitude less the format's and lets what does not fit saturate: its scales
+ * are half of these where the magnitude's mantissa is 1.75 (FP6 1.9375) or more. The products take
+ * either's. An element is the nearest one to x / 2^e,
  * ties to even, signs of zeros kept. A block that holds a NaN or infinity gets scale 255, codes 0.
  * This is the activations' way into the products, and the way of fp32 weights into the format. */
 int kq4_mx_quantize_dev(uint8_t *m, const float *x, long ldx, int rows, int cols, int type,
@@ -545,7 +548,8 @@ int kq4_mx_matmul_q_dev(float *out, long ldo, const uint8_t *xq, const float *re
                         const uint8_t *w, int rows, int cols, int n_batch, int act, void *stream);
 
 /* The gated half of a feed-forward block: out = silu(gate . x) * (up . x), silu(g) = g / (1 + e^-g),
- * both projections (4-bit matrices of rows x cols) and the product in one kernel. x, out, act as
+ * both projections (4-bit matrices of rows x cols) and the product in one kernel, silu off by at
+ * most 6 * 2^-24 of itself (10 * 2^-24 below -64), down to the least normal number. x, out, act as
  * for kq4_mx_matmul_dev. */
 int kq4_mx_gated_dev(float *out, long ldo, const float *x, long ldx, const uint8_t *gate,
                      const uint8_t *up, int rows, int cols, int n_batch, int act, void *stream);

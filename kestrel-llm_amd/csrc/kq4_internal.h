@@ -219,8 +219,8 @@ int kq4_launch_logprobs(const float *logits, long ld, int n, int vocab, int n_to
 int kq4_launch_mx_quantize(uint8_t *m, const float *x, long ldx, int rows, int cols, int type, hipStream_t s);
 int kq4_launch_mx_pack(uint8_t *m, uint8_t *codes, uint8_t *scales, int rows, int cols, int type, bool pack,
                        hipStream_t s);
-// (With a kernel's own integers at most 112 bytes: in about every other process a launch with 128 bytes of arguments or
-// more costs the host 0.8 us more, 3.4 against 2.6. So the dimensions in tiles are not among them.)
+// (With a kernel's own integers at most 112 bytes: in most processes a launch with 120 bytes of arguments or more costs the host
+// 0.7 us more, 3.4 against 2.75; profiles/kernel_stats_mx.md. So the dimensions in tiles are not among them.)
 struct KQ4MxArgs {
   const uint8_t *w[2];   // weights; the second one, where there is one, is the gated block's up projection
   const void *x;         // a quantized matrix, or (rows kernel) fp32 rows that it quantizes itself, row t at t * ldx floats

@@ -430,7 +430,9 @@ size_t kq4_mx_part_bytes(int n, int rows, int matrices, int ksplit) {
 //   K in slices   2.5 for the second launch + the sums written and read at 4.5e6 bytes a microsecond
 // e.g. 4096 x 4096, 6 bits: 256 tokens 9.4 us in the rows kernel against 13.7 (two slices) and 13.2 in the GEMM, 768 20.5 against
 // 21.7 and 14.7; 4096 x 12288, 512 tokens: 30.0 in two slices, 39.9 in one, 45.4 in the rows kernel. Over 556 launches its choices
-// take 1.005 times the best ones (geometric mean), 1.31 times at most.
+// take 1.005 times the best ones (geometric mean), 1.31 times at most: gated pairs of 65 to 127 tokens past a tile a CU, whose second
+// tile of 64 tokens the rows kernel works on whole, where the estimate counts tokens (100 x 12288 x 4096, 6 bits: estimated 19.2 us,
+// 29.9, in two slices of the GEMM 22.9).
 KQ4MxPlan kq4_mx_plan(int n, int rows, int cols, int matrices, int type, int ncu, int force_form, int force_split) {
   const KQ4MxDims d = kq4_mx_dims(rows, cols);
   const double outputs = (double)n * rows, products = outputs * cols * matrices;
