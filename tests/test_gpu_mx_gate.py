@@ -102,3 +102,15 @@ def test_gate_of_infinite_sums(kq4, torch_dev, form, split, n):
         kq4.mx_gated_dev(out, x, gate, u)
     got = out.cpu().numpy()
     assert (got[:, 0] == np.inf).all() and np.isnan(got[:, 1]).all()
+
+
+@pytest.mark.parametrize("form,split,n", FORMS)
+def test_gate_is_the_same_beside_far_ones(kq4, torch_dev, form, split, n):
+    """A gate's bits do not go with its neighbours': the same gates with every seventh or none of them past 64."""
+    g = np.random.default_rng(n).uniform(-64, 64, 2100).astype(F32)
+    mixed = g.copy()
+    mixed[::7] = np.where(np.arange(300) % 2, 3e5, -70)
+    with kq4.options(mx_form=form, mx_split=split):
+        alone, beside = gates(kq4, torch_dev, g, 0, n, 6)[1], gates(kq4, torch_dev, mixed, 0, n, 6)[1]
+    kept = np.arange(2100) % 7 != 0
+    np.testing.assert_array_equal(alone.view(np.int32)[kept], beside.view(np.int32)[kept])
